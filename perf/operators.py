@@ -107,7 +107,7 @@ def draw(rng):
         while m * n * k > 8192 * 14336 * 7168:
             m = max(1, m // 2)
         case = _product("", m, n, k, bias=rng.random() < 0.3, column=column,
-                        dtype=rng.choice(["bf16", "bf16", "fp16", "fp32"]))
+                        dtype=rng.choice(["bf16", "bf16", "fp16"]))
     else:
         rows = _log_int(rng, 1, 8192)
         cols = _log_int(rng, 64, 16384)
