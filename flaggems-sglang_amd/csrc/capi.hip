@@ -945,6 +945,36 @@ static void* device_scratch() {
   return ptrs[dev];
 }
 
+// ------------------------------------------------------ dense operators ---
+// What the norm and the gated activation check alike.
+static int check_row_operator(int64_t rows, int64_t cols, int dtype, int quant, bool none_ok,
+                              const void* q, const float* scales) {
+  if (rows < 0 || cols < 1) return fail(FGS_EINVAL, "rows >= 0 and cols >= 1 required");
+  if (dtype != FGS_DTYPE_BF16 && dtype != FGS_DTYPE_FP16 && dtype != FGS_DTYPE_FP32)
+    return fail(FGS_EINVAL, "unknown element type");
+  if (!none_ok && quant != FGS_QUANT_FP8_GROUP && quant != FGS_QUANT_INT8_TOKEN)
+    return fail(FGS_EINVAL, "unknown quantisation");
+  if (cols > kRowMaxCols)
+    return fail(FGS_EUNSUPPORTED, "rows of more than " + std::to_string(kRowMaxCols) + " columns");
+  if (rows > 0x7fffffff) return fail(FGS_EUNSUPPORTED, "too many rows for a grid");
+  if (rows > 0 && quant != FGS_QUANT_NONE && (!q || !scales))
+    return fail(FGS_EINVAL, "null pointer argument");
+  if (quant == FGS_QUANT_NONE && (q || scales))
+    return fail(FGS_EINVAL, "q and scales need a quantisation");
+  if (reinterpret_cast<uintptr_t>(scales) % 4)
+    return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  return FGS_OK;
+}
+
+static int check_block_sizes(int64_t m, int64_t n, int64_t k, int32_t flags) {
+  if (m < 0 || n < 1 || k < 1) return fail(FGS_EINVAL, "m >= 0, n >= 1 and k >= 1 required");
+  if (k % 16) return fail(FGS_EUNSUPPORTED, "k must be a multiple of 16");
+  if (n > kBlockMaxN || k > kBlockMaxK || m > kBlockMaxM)
+    return fail(FGS_EUNSUPPORTED, "sizes too large for the kernels' grids");
+  if (!block_gemm_flags_ok(flags)) return fail(FGS_EINVAL, "unknown flags");
+  return FGS_OK;
+}
+
 }  // namespace fgs
 
 using namespace fgs;
@@ -1394,6 +1424,146 @@ int32_t fgs_moe_routing_to_topk(const float* gate_scal, const int32_t* gather_sr
   return launch_routing_order(gate_scal, gather_src, expt_hist, numel, num_experts, 1, numel,
                               nullptr, nullptr, nullptr, topk_ids, topk_weights,
                               as_stream(stream));
+}
+
+int32_t fgs_moe_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                         int64_t residual_stride, const void* weight, int32_t dtype,
+                         int32_t weight_dtype, float eps, float weight_offset, int64_t rows,
+                         int64_t cols, void* norm_out, void* residual_out,
+                         int64_t residual_out_stride, int32_t quant, void* q, float* scales,
+                         int64_t scale_row_stride, int64_t scale_col_stride, void* stream) {
+  int rc = check_row_operator(rows, cols, dtype, quant, quant == FGS_QUANT_NONE, q, scales);
+  if (rc) return rc;
+  if (weight_dtype != dtype && weight_dtype != FGS_DTYPE_FP32)
+    return fail(FGS_EUNSUPPORTED, "the weight must be of x's type or fp32");
+  if (!weight || (rows > 0 && !x)) return fail(FGS_EINVAL, "null pointer argument");
+  if (rows > 0 && residual && !residual_out)
+    return fail(FGS_EINVAL, "residual_out is needed with a residual");
+  if (rows > 0 && !norm_out && !q && !residual)
+    return fail(FGS_EINVAL, "no output was asked for");
+  // a row of the output may not overlap the next one; rows that are read may
+  if (rows > 1 && (x_stride < 0 || (residual && (residual_stride < 0 ||
+                                                 residual_out_stride < cols))))
+    return fail(FGS_EINVAL, "row strides must be >= 0, residual_out's >= cols");
+  const uintptr_t es = dtype == FGS_DTYPE_FP32 ? 4 : 2;
+  const uintptr_t wes = weight_dtype == FGS_DTYPE_FP32 ? 4 : 2;
+  for (const void* t : {x, residual, static_cast<const void*>(norm_out),
+                        static_cast<const void*>(residual_out)})
+    if (reinterpret_cast<uintptr_t>(t) % es)
+      return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(weight) % wes)
+    return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  RmsNormParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.res_out = residual ? residual_out : nullptr;
+  p.norm = norm_out;
+  p.q = static_cast<uint8_t*>(q);
+  p.scales = scales;
+  p.rows = rows;
+  p.cols = cols;
+  p.x_stride = x_stride;
+  p.res_stride = residual_stride;
+  p.res_out_stride = residual_out_stride;
+  p.s_row = scale_row_stride;
+  p.s_col = scale_col_stride;
+  p.eps = eps;
+  p.offset = weight_offset;
+  p.quant = quant;
+  return launch_rms_norm(p, dtype, weight_dtype, as_stream(stream));
+}
+
+int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtype, int64_t rows,
+                                   int64_t n, int32_t gelu, int32_t quant, void* q,
+                                   float* scales, int64_t scale_row_stride,
+                                   int64_t scale_col_stride, void* stream) {
+  int rc = check_row_operator(rows, n, dtype, quant, false, q, scales);
+  if (rc) return rc;
+  if (rows > 0 && !x) return fail(FGS_EINVAL, "null pointer argument");
+  if (rows > 1 && x_stride < 0) return fail(FGS_EINVAL, "row strides must be >= 0");
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == FGS_DTYPE_FP32 ? 4 : 2))
+    return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  GatedQuantParams p{};
+  p.x = x;
+  p.q = static_cast<uint8_t*>(q);
+  p.scales = scales;
+  p.rows = rows;
+  p.n = n;
+  p.x_stride = x_stride;
+  p.s_row = scale_row_stride;
+  p.s_col = scale_col_stride;
+  p.quant = quant;
+  p.act = gelu ? kActGelu : kActSilu;
+  return launch_gated_quant(p, dtype, as_stream(stream));
+}
+
+int64_t fgs_moe_fp8_block_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t flags) {
+  if (check_block_sizes(m, n, k, flags)) return -1;
+  return m == 0 ? 0 : block_gemm_workspace(block_gemm_plan(m, n, k, flags), m, n);
+}
+
+int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,
+                                          char* buf, int32_t len) {
+  int rc = check_block_sizes(m, n, k, flags);
+  if (rc) return rc;
+  if (!buf || len < 1) return fail(FGS_EINVAL, "buf must hold at least one byte");
+  const std::string s = m == 0 ? "none" : block_gemm_name(block_gemm_plan(m, n, k, flags));
+  const size_t used = std::min(s.size(), static_cast<size_t>(len - 1));
+  memcpy(buf, s.data(), used);
+  buf[used] = 0;
+  return FGS_OK;
+}
+
+int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scale,
+                                 int64_t as_row_stride, int64_t as_col_stride, const void* w,
+                                 int64_t ldw, const float* w_scale, const void* bias,
+                                 int32_t bias_dtype, int64_t m, int64_t n, int64_t k,
+                                 int32_t out_dtype, int32_t flags, void* workspace,
+                                 int64_t ws_bytes, void* out, int64_t ldo, void* stream) {
+  int rc = check_block_sizes(m, n, k, flags);
+  if (rc) return rc;
+  for (int t : {out_dtype, bias ? bias_dtype : out_dtype})
+    if (t != FGS_DTYPE_BF16 && t != FGS_DTYPE_FP16 && t != FGS_DTYPE_FP32)
+      return fail(FGS_EINVAL, "unknown element type");
+  if (out_dtype == FGS_DTYPE_FP32)
+    return fail(FGS_EUNSUPPORTED, "the output must be bf16 or fp16");
+  if (m == 0) return FGS_OK;
+  if (!a || !a_scale || !w || !w_scale || !out) return fail(FGS_EINVAL, "null pointer argument");
+  if ((m > 1 && (lda < 0 || lda % 16)) || (n > 1 && (ldw < 0 || ldw % 16)) ||
+      reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(w) % 16)
+    return fail(FGS_EUNSUPPORTED, "rows of a and w must be 16-byte aligned");
+  if (m > 1 && ldo < n) return fail(FGS_EINVAL, "ldo must be >= n");
+  if (reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
+      reinterpret_cast<uintptr_t>(out) % 2 ||
+      reinterpret_cast<uintptr_t>(bias) % (bias_dtype == FGS_DTYPE_FP32 ? 4 : 2))
+    return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  const BlockGemmPlan plan = block_gemm_plan(m, n, k, flags);
+  const int64_t need = block_gemm_workspace(plan, m, n);
+  if (need > 0 && (!workspace || ws_bytes < need))
+    return fail(FGS_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes");
+  if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(FGS_EINVAL, "workspace must be 256-byte aligned");
+  BlockGemmParams p{};
+  p.a = static_cast<const uint8_t*>(a);
+  p.a_scale = a_scale;
+  p.w = static_cast<const uint8_t*>(w);
+  p.w_scale = w_scale;
+  p.bias = bias;
+  p.out = out;
+  p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  p.lda = m > 1 ? lda : k;
+  p.ldw = n > 1 ? ldw : k;
+  p.ldo = m > 1 ? ldo : n;
+  p.as_row = as_row_stride;
+  p.as_col = as_col_stride;
+  p.out_dtype = out_dtype;
+  p.bias_dtype = bias_dtype;
+  p.kblocks = static_cast<int32_t>((k + 127) / 128);
+  return launch_block_gemm(p, plan, as_stream(stream));
 }
 
 }  // extern "C"

@@ -178,32 +178,6 @@ __global__ __launch_bounds__(256) void moe_sum_partials_kernel(
 }
 
 // --------------------------------------------------------- quantisers ---
-// x / scale correctly rounded for a finite scale, from inv = 1 / scale
-// (correctly rounded, one division for all of a scale's values): Markstein's
-// scheme (P. Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000 processor", IBM J. Res. Dev. 1990): x * inv is within two ulps,
-// one residual step brings it within one, and a second from there, with a
-// correctly rounded reciprocal, gives the rounded quotient (and, with x's
-// sign, its signed zero). Six FMA-rate instructions in place of a division's
-// ten and its reciprocal; the quantisers were bound by those. Exact where the
-// residuals are: a quotient small enough for one to lose bits rounds to code 0
-// either way.
-__device__ __forceinline__ float quotient(float x, float scale, float inv) {
-  float q = x * inv;
-  q = __builtin_fmaf(__builtin_fmaf(-scale, q, x), inv, q);
-  q = __builtin_fmaf(__builtin_fmaf(-scale, q, x), inv, q);
-  return __builtin_copysignf(q, x);
-}
-
-// The scale for quotient's residuals: itself, or zero for an infinite one (an
-// infinity in the row or group), with which a finite x gives its signed zero
-// and an infinity NaN, as the division does. (With a division as the other
-// branch, per value: int8, 20000 rows of 128 columns 10.2 us, 7.3 so, 1024 of
-// 8192 12.6 and 9.9, one of 14336 6.0 and 5.2; divisions alone 8.1, 11.4, 5.7.)
-__device__ __forceinline__ float residual_scale(float scale) {
-  return scale < INFINITY ? scale : 0.f;
-}
-
 // The row of x a quantiser's work item `i` takes: i, or the padded row given
 // for it (-1: none).
 __device__ __forceinline__ int64_t quant_row(const int32_t* row_of, int64_t i,

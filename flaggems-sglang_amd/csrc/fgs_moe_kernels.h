@@ -208,4 +208,66 @@ void wide_plan_request(bool gemm1, const GemmParams& p, int row_blocks, WidePlan
 // Ints of tile-plan workspace the 4-wave GEMM1 uses (gemm_wide.hip).
 int64_t wide_plan_words();
 
+// ---- dense operators around the routed experts ----
+// Most columns the row operators hold in registers (norm_quant.hip).
+constexpr int64_t kRowMaxCols = 65536;
+
+// Root-mean-square norm; strides in elements, `residual` / `norm` / `q` null:
+// off. The norm and code rows are contiguous.
+struct RmsNormParams {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* res_out;
+  void* norm;
+  uint8_t* q;
+  float* scales;
+  int64_t rows, cols;
+  int64_t x_stride, res_stride, res_out_stride;
+  int64_t s_row, s_col;  // strides of the scales over rows / column groups
+  float eps, offset;
+  int32_t quant;
+};
+int launch_rms_norm(const RmsNormParams& p, int dtype, int weight_dtype, hipStream_t stream);
+
+// Gated activation with an 8-bit output: x [rows, 2 n] -> q [rows, n].
+struct GatedQuantParams {
+  const void* x;
+  uint8_t* q;
+  float* scales;
+  int64_t rows, n, x_stride;
+  int64_t s_row, s_col;
+  int32_t quant, act;
+};
+int launch_gated_quant(const GatedQuantParams& p, int dtype, hipStream_t stream);
+
+// Block-scaled e4m3 product out[m, n] = sum_k a[m, k] w[n, k] with the scales
+// of its 128-wide k blocks (block_gemm.hip).
+struct BlockGemmParams {
+  const uint8_t* a;
+  const float* a_scale;
+  const uint8_t* w;
+  const float* w_scale;  // [ceil(n / 128), ceil(k / 128)], contiguous
+  const void* bias;      // [n] or null
+  void* out;
+  int64_t m, n, k;
+  int64_t lda, ldw, ldo;  // row strides in elements
+  int64_t as_row, as_col; // strides of a_scale over rows / k blocks
+  int32_t out_dtype, bias_dtype;
+  int32_t kblocks;
+  float* part;           // workspace (block_gemm_workspace bytes)
+};
+constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 24;
+// The kernel a product of these sizes runs.
+enum : int { kBlockStream = 0 };
+struct BlockGemmPlan {
+  int form;
+  int mt;  // streaming: 16-token tiles of a workgroup
+};
+BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags);
+bool block_gemm_flags_ok(int32_t flags);
+int64_t block_gemm_workspace(const BlockGemmPlan& plan, int64_t m, int64_t n);
+std::string block_gemm_name(const BlockGemmPlan& plan);
+int launch_block_gemm(const BlockGemmParams& p, const BlockGemmPlan& plan, hipStream_t stream);
+
 }  // namespace fgs

@@ -1,0 +1,295 @@
+// Row operators around the dense 8-bit products: the root-mean-square norm
+// with the residual's addition and an output in 16 / 32 and / or 8 bits, and
+// the gated activation with an output in 8 bits.
+//
+// Both hold a row's values in registers in fp32 (8 consecutive ones a vector,
+// NV vectors a thread), so every input is read once whatever the outputs are:
+// they are bound by memory, or by one load-reduce-store latency where rows
+// are few. A 128-column group of the e4m3 scales is 16 neighbouring lanes, so
+// its largest value is four DPP moves.
+#include <algorithm>
+#include <string>
+
+#include "dense_common.h"
+
+namespace fgs {
+
+constexpr int kRowThreads = 1024;   // most threads a row gets
+constexpr int kRowVecs = 8;         // most vectors a thread holds
+static_assert(kRowMaxCols == 8 * kRowThreads * kRowVecs, "columns a workgroup holds");
+
+// Sum / maximum over the workgroup's waves (`red` has a word a wave).
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum_f32(v);
+  const int nw = blockDim.x / 64;
+  if (nw == 1) return v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < nw; ++i) s += red[i];
+  return s;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+  v = wave_max_u32(v);
+  const int nw = blockDim.x / 64;
+  if (nw == 1) return v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint32_t s = 0;
+  for (int i = 0; i < nw; ++i) s = max(s, red[i]);
+  return s;
+}
+
+// ------------------------------------------------------------------- norm ---
+// h = x + residual; n = h / sqrt(mean(h^2) + eps) * (weight + offset), all in
+// fp32: the residual output is h rounded once, the norm output n rounded once,
+// and the 8-bit codes and scales come from the unrounded n.
+// WAVE: a wave takes a row (4 a workgroup), else the workgroup one row.
+template <int TY, int WTY, bool VEC, bool WAVE, bool RES, int NV>
+__global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
+    const RmsNormParams p) {
+  __shared__ float red_sum[kRowThreads / 64];
+  __shared__ uint32_t red_max[kRowThreads / 64];
+  const int tid = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const int threads = WAVE ? 64 : blockDim.x;
+  const int64_t row = WAVE ? blockIdx.x * int64_t{4} + (threadIdx.x >> 6) : blockIdx.x;
+  if (WAVE && row >= p.rows) return;
+  auto col = [&](int v) { return (static_cast<int64_t>(v) * threads + tid) * 8; };
+
+  // every load of the row first, the weight's among them
+  Vec8<TY, VEC> x[NV], r[RES ? NV : 1];
+  Vec8<WTY, VEC> w[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = col(v);
+    x[v].zero();
+    w[v].zero();
+    if constexpr (RES) r[v].zero();
+    if (c < p.cols) {
+      x[v].load(p.x, row * p.x_stride + c, p.cols - c);
+      if constexpr (RES) r[v].load(p.residual, row * p.res_stride + c, p.cols - c);
+      w[v].load(p.weight, c, p.cols - c);
+    }
+  }
+  float h[NV][8];
+  float sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      h[v][j] = x[v][j];
+      if constexpr (RES) h[v][j] += r[v][j];
+      sum = __builtin_fmaf(h[v][j], h[v][j], sum);
+    }
+    if constexpr (RES) {
+      const int64_t c = col(v);
+      if (c < p.cols) store8<TY, VEC>(p.res_out, row * p.res_out_stride + c, p.cols - c, h[v]);
+    }
+  }
+  sum = WAVE ? wave_sum_f32(sum) : block_sum(sum, red_sum);
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.cols) + p.eps);
+
+  uint32_t amax = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = col(v);
+    // columns past the row: 0, whatever rstd is
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      h[v][j] = c + (VEC ? 0 : j) < p.cols ? h[v][j] * rstd * (w[v][j] + p.offset) : 0.f;
+    if (p.norm && c < p.cols) store8<TY, VEC>(p.norm, row * p.cols + c, p.cols - c, h[v]);
+    if (p.quant == FGS_QUANT_FP8_GROUP) {
+      const float scale = scale_of(row_max(abs_bits8(h[v])), 448.f);
+      if (c < p.cols) {
+        store_codes<VEC>(p.q + row * p.cols + c, p.cols - c, codes_fp8(h[v], scale));
+        if ((tid & 15) == 0) p.scales[row * p.s_row + (c >> 7) * p.s_col] = scale;
+      }
+    } else if (p.quant == FGS_QUANT_INT8_TOKEN) {
+      amax = max(amax, abs_bits8(h[v]));
+    }
+  }
+  if (p.quant != FGS_QUANT_INT8_TOKEN) return;
+  amax = WAVE ? wave_max_u32(amax) : block_max(amax, red_max);
+  const float scale = scale_of(amax, 127.f);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = (static_cast<int64_t>(v) * threads + tid) * 8;
+    if (c < p.cols)
+      store_codes<VEC>(p.q + row * p.cols + c, p.cols - c, codes_int8(h[v], scale));
+  }
+  if (tid == 0) p.scales[row * p.s_row] = scale;
+}
+
+// ------------------------------------------------------- gated activation ---
+// v = act(gate) * up in fp32 (gate the row's first n columns, up the other n),
+// quantised unrounded. e4m3: a workgroup takes blockDim * NV * 8 columns of a
+// row (grid y); int8, whose scale is the row's: the whole row.
+// The exact gelu by erfc, which keeps its relative accuracy for negative gates
+// (1 + erf cancels there); a scale may come from such values alone.
+__device__ __forceinline__ float gelu_tail_mul(float g, float u) {
+  return 0.5f * g * erfcf(-0.70710678118654752f * g) * u;
+}
+
+template <int TY, bool VEC, bool WAVE, int NV>
+__global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void gated_quant_kernel(
+    const GatedQuantParams p) {
+  __shared__ uint32_t red_max[kRowThreads / 64];
+  const int tid = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const int threads = WAVE ? 64 : blockDim.x;
+  const int64_t row = WAVE ? blockIdx.x * int64_t{4} + (threadIdx.x >> 6) : blockIdx.x;
+  if (WAVE && row >= p.rows) return;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * threads * NV;
+
+  Vec8<TY, VEC> g[NV], u[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = (first + static_cast<int64_t>(v) * threads + tid) * 8;
+    g[v].zero();
+    u[v].zero();
+    if (c < p.n) {
+      g[v].load(p.x, row * p.x_stride + c, p.n - c);
+      u[v].load(p.x, row * p.x_stride + p.n + c, p.n - c);
+    }
+  }
+  float h[NV][8];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = (first + static_cast<int64_t>(v) * threads + tid) * 8;
+    if (p.act == kActGelu) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[v][j] = gelu_tail_mul(g[v][j], u[v][j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[v][j] = silu_mul(g[v][j], u[v][j]);
+    }
+    if (p.quant == FGS_QUANT_FP8_GROUP) {
+      const float scale = scale_of(row_max(abs_bits8(h[v])), 448.f);
+      if (c < p.n) {
+        store_codes<VEC>(p.q + row * p.n + c, p.n - c, codes_fp8(h[v], scale));
+        if ((tid & 15) == 0) p.scales[row * p.s_row + (c >> 7) * p.s_col] = scale;
+      }
+    } else {
+      amax = max(amax, abs_bits8(h[v]));
+    }
+  }
+  if (p.quant == FGS_QUANT_FP8_GROUP) return;
+  amax = WAVE ? wave_max_u32(amax) : block_max(amax, red_max);
+  const float scale = scale_of(amax, 127.f);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = (static_cast<int64_t>(v) * threads + tid) * 8;
+    if (c < p.n) store_codes<VEC>(p.q + row * p.n + c, p.n - c, codes_int8(h[v], scale));
+  }
+  if (tid == 0) p.scales[row * p.s_row] = scale;
+}
+
+// -------------------------------------------------------------- launchers ---
+namespace {
+
+// Vectors a thread holds and threads of a row of `chunks` vectors: `wave`
+// for a wave a row.
+struct RowShape {
+  bool wave;
+  int nv, threads;
+};
+// Few rows leave CUs idle, so a row takes as many threads as it has vectors;
+// with many, threads hold two vectors (more loads in flight for the same
+// waves), and a row of at most 128 vectors takes one wave and no barrier.
+RowShape row_shape(int64_t rows, int64_t chunks, bool vec) {
+  if (vec && rows >= 1024 && chunks <= 256) return {true, chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4, 256};
+  int nv = 1;
+  while (nv < kRowVecs && chunks > int64_t{kRowThreads} * nv) nv *= 2;
+  if (rows >= 512 && nv < 4 && chunks >= 128 * nv) nv *= 2;
+  const int64_t t = (chunks + nv - 1) / nv;
+  return {false, nv, static_cast<int>((t + 63) / 64 * 64)};
+}
+
+template <class F>
+int with_nv(int nv, F&& f) {
+  switch (nv) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    default: return f(std::integral_constant<int, 8>{});
+  }
+}
+template <class F>
+int with_type(int ty, F&& f) {
+  switch (ty) {
+    case FGS_DTYPE_BF16: return f(std::integral_constant<int, FGS_DTYPE_BF16>{});
+    case FGS_DTYPE_FP16: return f(std::integral_constant<int, FGS_DTYPE_FP16>{});
+    default: return f(std::integral_constant<int, FGS_DTYPE_FP32>{});
+  }
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int64_t elem_bytes(int ty) { return ty == FGS_DTYPE_FP32 ? 4 : 2; }
+
+}  // namespace
+
+int launch_rms_norm(const RmsNormParams& p, int dtype, int weight_dtype, hipStream_t stream) {
+  if (p.rows == 0) return FGS_OK;
+  const int64_t es = elem_bytes(dtype);
+  const bool vec = p.cols % 8 == 0 && aligned16(p.x) && aligned16(p.weight) && aligned16(p.norm) &&
+                   p.x_stride * es % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(p.q) % 8 == 0 &&
+                   (!p.residual || (aligned16(p.residual) && aligned16(p.res_out) &&
+                                    p.res_stride * es % 16 == 0 && p.res_out_stride * es % 16 == 0));
+  const RowShape s = row_shape(p.rows, (p.cols + 7) / 8, vec);
+  const dim3 grid(static_cast<unsigned>(s.wave ? (p.rows + 3) / 4 : p.rows));
+  const int rc = with_type(dtype, [&](auto ty) {
+    constexpr int TY = decltype(ty)::value;
+    auto go = [&](auto wty) {
+      constexpr int WTY = decltype(wty)::value;
+      auto run = [&](auto res) {
+        constexpr bool RES = decltype(res)::value;
+        return with_nv(s.nv, [&](auto nv) {
+          constexpr int NV = decltype(nv)::value;
+          auto kernel = vec ? rms_norm_kernel<TY, WTY, true, false, RES, NV>
+                            : rms_norm_kernel<TY, WTY, false, false, RES, NV>;
+          if constexpr (NV <= 4) {
+            if (s.wave) kernel = rms_norm_kernel<TY, WTY, true, true, RES, NV>;
+          }
+          hipLaunchKernelGGL(kernel, grid, dim3(s.threads), 0, stream, p);
+          return FGS_OK;
+        });
+      };
+      return p.residual ? run(std::true_type{}) : run(std::false_type{});
+    };
+    if (weight_dtype == FGS_DTYPE_FP32) return go(std::integral_constant<int, FGS_DTYPE_FP32>{});
+    return go(ty);
+  });
+  return rc ? rc : check_launch("rms_norm_kernel");
+}
+
+int launch_gated_quant(const GatedQuantParams& p, int dtype, hipStream_t stream) {
+  if (p.rows == 0) return FGS_OK;
+  const bool vec = p.n % 8 == 0 && aligned16(p.x) && p.x_stride * elem_bytes(dtype) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(p.q) % 8 == 0;
+  const int64_t chunks = (p.n + 7) / 8;
+  RowShape s = row_shape(p.rows, chunks, vec);
+  unsigned gy = 1;
+  if (p.quant == FGS_QUANT_FP8_GROUP && !s.wave) {  // groups are apart: narrow workgroups
+    s.nv = 1;
+    s.threads = static_cast<int>(std::min<int64_t>(256, (chunks + 63) / 64 * 64));
+    gy = static_cast<unsigned>((chunks + s.threads - 1) / s.threads);
+  }
+  const dim3 grid(static_cast<unsigned>(s.wave ? (p.rows + 3) / 4 : p.rows), gy);
+  const int rc = with_type(dtype, [&](auto ty) {
+    constexpr int TY = decltype(ty)::value;
+    return with_nv(s.nv, [&](auto nv) {
+      constexpr int NV = decltype(nv)::value;
+      auto kernel =
+          vec ? gated_quant_kernel<TY, true, false, NV> : gated_quant_kernel<TY, false, false, NV>;
+      if constexpr (NV <= 4) {
+        if (s.wave) kernel = gated_quant_kernel<TY, true, true, NV>;
+      }
+      hipLaunchKernelGGL(kernel, grid, dim3(s.threads), 0, stream, p);
+      return FGS_OK;
+    });
+  });
+  return rc ? rc : check_launch("gated_quant_kernel");
+}
+
+}  // namespace fgs

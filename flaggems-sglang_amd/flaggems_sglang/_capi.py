@@ -20,6 +20,14 @@ QMODE_BF16 = 0
 QMODE_FP8_BLOCK = 1
 QMODE_INT8_CHANNEL = 2
 
+DTYPE_BF16 = 0
+DTYPE_FP16 = 1
+DTYPE_FP32 = 2
+
+QUANT_NONE = 0
+QUANT_FP8_GROUP = 1
+QUANT_INT8_TOKEN = 2
+
 SCORING_SOFTMAX = 0
 SCORING_SIGMOID = 1
 
@@ -130,6 +138,25 @@ SIGNATURES = {
          _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _c_void_p, _i64,
          _c_void_p, _c_void_p],
     ),
+    "fgs_moe_rms_norm": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i32, _i32, ctypes.c_float,
+         ctypes.c_float, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _c_void_p,
+         _c_void_p, _i64, _i64, _c_void_p],
+    ),
+    "fgs_moe_silu_and_mul_quant": (
+        _i32,
+        [_c_void_p, _i64, _i32, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p, _i64,
+         _i64, _c_void_p],
+    ),
+    "fgs_moe_fp8_block_matmul": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p,
+         _i32, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i64, _c_void_p, _i64,
+         _c_void_p],
+    ),
+    "fgs_moe_fp8_block_matmul_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "fgs_moe_fp8_block_matmul_schedule": (_i32, [_i64, _i64, _i64, _i32, _c_void_p, _i32]),
     "fgs_moe_profile_enable": (_i32, [_i32]),
     "fgs_moe_profile_read": (_i32, [_c_void_p, _i32]),
 }
@@ -194,4 +221,13 @@ def schedule(m: int, hidden: int, inter: int, num_experts: int, topk: int,
     buf = ctypes.create_string_buffer(96)
     check(load().fgs_moe_schedule(m, hidden, inter, num_experts, topk, qmode, flags,
                                   buf, len(buf)), "schedule")
+    return buf.value.decode()
+
+
+def block_matmul_schedule(m: int, n: int, k: int, flags: int = 0) -> str:
+    """The schedule a block-scaled product of these sizes runs
+    (``fgs_moe_fp8_block_matmul_schedule``)."""
+    buf = ctypes.create_string_buffer(96)
+    check(load().fgs_moe_fp8_block_matmul_schedule(m, n, k, flags, buf, len(buf)),
+          "schedule")
     return buf.value.decode()

@@ -384,6 +384,79 @@ int32_t fgs_moe_fused_int8_channel(const void* x, const void* w13,
                                    int32_t flags, void* workspace,
                                    int64_t ws_bytes, void* out, void* stream);
 
+/* ---- dense operators around the routed experts -------------------------
+ * No reference counterparts (the reference's layer takes its input normalised
+ * and has no 8-bit path, ops/fused_moe.py:170-185): the norm before the
+ * layer, the dense e4m3 products of the shared expert and the projections,
+ * and the shared expert's activation. Element types of these entries: */
+#define FGS_DTYPE_BF16 0
+#define FGS_DTYPE_FP16 1
+#define FGS_DTYPE_FP32 2
+/* and their 8-bit outputs: e4m3fn with a scale per 128 columns of a row (the
+ * last group may be shorter), int8 with a scale per row. The scale of a group
+ * with a NaN is NaN, of one with an infinity infinite (its finite values then
+ * have code 0). */
+#define FGS_QUANT_NONE 0
+#define FGS_QUANT_FP8_GROUP 1
+#define FGS_QUANT_INT8_TOKEN 2
+
+/* Root-mean-square norm, with the residual's addition and an 8-bit output:
+ *   h = f32(x) + f32(residual);  residual_out = h in x's type
+ *   n = h / sqrt(mean(h^2) + eps) * (f32(weight) + weight_offset)
+ *   norm_out = n in x's type;  q, scales from the unrounded n
+ * (scale = max(amax, 1e-10) / 448, q = e4m3fn(n / scale), or / 127, rne).
+ *   x [rows, cols] with row stride x_stride (elements), residual likewise or
+ *   null (then residual_out is unused); residual_out [rows, cols] may be
+ *   residual or x itself; weight [cols] in x's type or fp32
+ *   norm_out [rows, cols] contiguous, or null
+ *   q [rows, cols] contiguous, scales f32 at scales[r * scale_row_stride +
+ *   g * scale_col_stride] (g = column / 128; int8: g = 0), both null for
+ *   FGS_QUANT_NONE
+ * Any cols in [1, 65536] and any alignment to the element size; multiples of
+ * 8 columns and 16-byte aligned rows take whole vectors. */
+int32_t fgs_moe_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                         int64_t residual_stride, const void* weight, int32_t dtype,
+                         int32_t weight_dtype, float eps, float weight_offset, int64_t rows,
+                         int64_t cols, void* norm_out, void* residual_out,
+                         int64_t residual_out_stride, int32_t quant, void* q, float* scales,
+                         int64_t scale_row_stride, int64_t scale_col_stride, void* stream);
+
+/* Gated activation with an 8-bit output: v = act(f32(x[r, c])) *
+ * f32(x[r, n + c]) with act silu, or the exact gelu (gelu != 0), and q,
+ * scales from the unrounded v as above (quant: FP8_GROUP or INT8_TOKEN).
+ *   x [rows, 2n] with row stride x_stride; q [rows, n] contiguous; n in
+ *   [1, 65536] */
+int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtype, int64_t rows,
+                                   int64_t n, int32_t gelu, int32_t quant, void* q,
+                                   float* scales, int64_t scale_row_stride,
+                                   int64_t scale_col_stride, void* stream);
+
+/* Dense e4m3 product with block scales (128x128 of the weights, 1x128 of the
+ * activations), sums in fp32:
+ *   out[i, j] = sum_kb a_scale[i, kb] * w_scale[j / 128, kb] *
+ *               sum_{l in kb} a[i, l] * w[j, l]   (+ bias[j])
+ *   a e4m3fn [m, k] with row stride lda; a_scale f32 at a_scale[i *
+ *   as_row_stride + kb * as_col_stride]; w e4m3fn [n, k] with row stride ldw;
+ *   w_scale f32 [ceil(n / 128), ceil(k / 128)] contiguous; bias [n] of
+ *   bias_dtype, or null; out [m, n] of out_dtype (bf16 or fp16) with row
+ *   stride ldo
+ * The matrix instruction cuts each of eight neighbouring products 13 bits
+ * below the largest one: about 1.5e-5 of a result from normal data.
+ * k a positive multiple of 16, m and n anything; a and w rows 16-byte
+ * aligned. `flags`: 0, or a schedule to use (FGS_BLOCK_*, below).
+ * workspace: fgs_moe_fp8_block_matmul_workspace_bytes() bytes, 256-byte
+ * aligned (may be null where that is 0). */
+int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scale,
+                                 int64_t as_row_stride, int64_t as_col_stride, const void* w,
+                                 int64_t ldw, const float* w_scale, const void* bias,
+                                 int32_t bias_dtype, int64_t m, int64_t n, int64_t k,
+                                 int32_t out_dtype, int32_t flags, void* workspace,
+                                 int64_t ws_bytes, void* out, int64_t ldo, void* stream);
+int64_t fgs_moe_fp8_block_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t flags);
+/* The schedule such a call runs, as text (as fgs_moe_schedule). */
+int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,
+                                          char* buf, int32_t len);
+
 /* Stage timing for benchmarks. No reference counterpart (the reference
  * times the whole op with triton.testing.do_bench,
  * benchmark/performance_utils.py:365-377). While enabled on the calling
