@@ -157,32 +157,397 @@ __global__ __launch_bounds__(KW * 64) void block_gemm_stream_kernel(const BlockG
   }
 }
 
-// ---------------------------------------------------------------- schedule ---
-BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags) {
-  BlockGemmPlan q{};
-  q.form = kBlockStream;
-  q.mt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-  return q;
+// ------------------------------------------------------------ many tokens ---
+// A workgroup of WM x WN waves owns BM tokens x BN weight rows; both operands'
+// rows of a k block (128 bytes each) and the block's scales stream into a ring
+// of STAGES LDS slots by LDS-DMA. A wave keeps its tokens' fragments of a
+// block in registers and takes its weight rows 16 at a time: RT MFMAs, then
+// the 4 RT FMAs of the 16 rows before them.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int WPE_>
+struct BlockCfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+  static constexpr int WPE = WPE_;            // waves a SIMD holds
+  static constexpr int NW = WM * WN;
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
+  static constexpr int SC_OFF = A_BYTES + W_BYTES;
+  static constexpr int STAGE = SC_OFF + NW * 256;  // a float slot per lane
+  static constexpr int LDS = STAGES * STAGE;
+  static constexpr int NLA = BM / 8 / NW, NLW = BN / 8 / NW;  // loads per wave
+  static constexpr int NL = NLA + NLW + 1;
+  static constexpr int RT = BM / WM / 16, CT = BN / WN / 16;  // 16-wide tiles of a wave
+  static_assert(NLA * 8 * NW == BM && NLW * 8 * NW == BN, "whole loads");
+  static_assert(128 % (CT * 16) == 0, "a wave's weight rows lie in one scale block");
+  static_assert(BN % 128 == 0 || 128 % BN == 0, "scale blocks of a tile");
+  static_assert(BM + (BN + 127) / 128 <= NW * 64, "scale slots");
+  static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * NL < 64 && LDS <= 160 * 1024, "ring");
+  static_assert(CT % 2 == 0, "fragment pipeline");
+};
+
+// Position of logical 16-byte chunk c of stage row r: the LDS serves 16 lanes
+// (256 bytes, two rows) of a 16-byte read at a time, and the XOR spreads the
+// 16 rows that lanes 0-15 read at one chunk over all 16 positions.
+__device__ __forceinline__ int swizzled(int r, int c) { return c ^ ((r >> 1) & 7); }
+
+// Workgroup bid runs on XCD bid % 8, which takes the bid / 8-th item of its
+// contiguous eighth; items go split by split, and inside a split in bands of
+// `band` token tiles walked column by column, so an XCD's 32 CUs share a few
+// rows' and columns' operands in its L2.
+__device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int ksplit, int band, int* tm,
+                                           int* tn, int* ks) {
+  const int tiles = nm * nn;
+  const int total = tiles * ksplit;
+  const int per = (total + 7) / 8;
+  const int at = (bid % 8) * per + bid / 8;
+  if (bid / 8 >= per || at >= total) return false;
+  const int s = at / tiles;
+  const int i = at - s * tiles;
+  const int b = i / (band * nn);
+  const int rem = i - b * band * nn;
+  const int rows = min(band, nm - b * band);
+  // (the divisions run on the VALU: back to scalars, so that the loops and the
+  // buffer resources that follow from them are scalar too)
+  *ks = __builtin_amdgcn_readfirstlane(s);
+  *tn = __builtin_amdgcn_readfirstlane(rem / rows);
+  *tm = __builtin_amdgcn_readfirstlane(b * band + rem % rows);
+  return true;
 }
 
-bool block_gemm_flags_ok(int32_t flags) { return flags == 0; }
+template <class C>
+__global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
+    const BlockGemmParams p, int nm, int nn, int ksplit, int band) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  constexpr int RT = C::RT, CT = C::CT, STAGES = C::STAGES;
+  int tm, tn, ks;
+  if (!block_tile(blockIdx.x, nm, nn, ksplit, band, &tm, &tn, &ks)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  const int64_t m0 = static_cast<int64_t>(tm) * C::BM;
+  const int64_t n0 = static_cast<int64_t>(tn) * C::BN;
 
-int64_t block_gemm_workspace(const BlockGemmPlan& q, int64_t m, int64_t n) { return 0; }
+  // this lane's source of each load: row lane / 8, chunk lane % 8, as byte
+  // offsets from the tile's first row (rows past the end read the last one;
+  // their results are not stored)
+  const int lrow = lane >> 3;
+  const int am = static_cast<int>(min<int64_t>(C::BM, p.m - m0)) - 1;  // last rows
+  const int wm_last = static_cast<int>(min<int64_t>(C::BN, p.n - n0)) - 1;
+  const uint32_t lda = static_cast<uint32_t>(p.lda), ldw = static_cast<uint32_t>(p.ldw);
+  uint32_t aoff[C::NLA], woff[C::NLW];
+#pragma unroll
+  for (int i = 0; i < C::NLA; ++i) {
+    const int r = (wave * C::NLA + i) * 8 + lrow;
+    aoff[i] = min(r, am) * lda + swizzled(r, lane & 7) * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < C::NLW; ++i) {
+    const int r = (wave * C::NLW + i) * 8 + lrow;
+    woff[i] = min(r, wm_last) * ldw + swizzled(r, lane & 7) * 16;
+  }
+  // scale slots: a token's each, then the tile's weight blocks'
+  const int slot = wave * 64 + lane;
+  const float* sc_src;
+  int64_t sc_step;
+  if (slot < C::BM) {
+    sc_src = p.a_scale + min<int64_t>(m0 + slot, p.m - 1) * p.as_row;
+    sc_step = p.as_col;
+  } else {
+    const int64_t b = min<int64_t>((n0 >> 7) + slot - C::BM, (p.n - 1) >> 7);
+    sc_src = p.w_scale + b * p.kblocks;
+    sc_step = 1;
+  }
 
-std::string block_gemm_name(const BlockGemmPlan& q) { return "stream mt=" + std::to_string(q.mt); }
+  const int kt0 = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(static_cast<uint32_t>(ks) * p.kblocks / ksplit));
+  const int KT = __builtin_amdgcn_readfirstlane(static_cast<int>(
+                     static_cast<uint32_t>(ks + 1) * p.kblocks / ksplit)) - kt0;
+  sc_src += kt0 * sc_step;
+  const int k_bytes = static_cast<int>(p.k) - kt0 * 128;  // of the split to the row's end
+
+  // The resources start at stage kt's columns and end with the tile's last
+  // row: what a lane would read past that (the last block's chunks past k of
+  // the last row) is not accessed.
+  auto issue = [&](int kt) {
+    uint8_t* base = lds + (kt % STAGES) * C::STAGE;
+    const int64_t koff = static_cast<int64_t>(kt0 + kt) * 128;
+    const uint32_t left = static_cast<uint32_t>(k_bytes - kt * 128);
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.a) + m0 * p.lda + koff, 0, static_cast<int>(am * lda + left),
+        kBufWord3);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.w) + n0 * p.ldw + koff, 0, static_cast<int>(wm_last * ldw + left),
+        kBufWord3);
+#pragma unroll
+    for (int i = 0; i < C::NLA; ++i)
+      lds_dma16_buf(ra, aoff[i], 0, base + (wave * C::NLA + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < C::NLW; ++i)
+      lds_dma16_buf(rw, woff[i], 0, base + C::A_BYTES + (wave * C::NLW + i) * 1024);
+    lds_dma4(sc_src + kt * sc_step, base + C::SC_OFF + wave * 256);
+  };
+  // Stage kt (this wave's loads of it done): where it is the row's last block
+  // and k ends inside it, the chunks past k that this wave loaded become 0.
+  const int ragged = (p.k & 127) && kt0 + KT == p.kblocks ? KT - 1 : -1;
+  auto end_of_k = [&](int kt) {
+    if (kt != ragged) return;
+    uint8_t* base = lds + (kt % STAGES) * C::STAGE + lane * 16;
+    const int live = static_cast<int>(p.k & 127) / 16;
+#pragma unroll
+    for (int i = 0; i < C::NLA; ++i)
+      if (swizzled((wave * C::NLA + i) * 8 + lrow, lane & 7) >= live)
+        *reinterpret_cast<u32x4*>(base + (wave * C::NLA + i) * 1024) = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < C::NLW; ++i)
+      if (swizzled((wave * C::NLW + i) * 8 + lrow, lane & 7) >= live)
+        *reinterpret_cast<u32x4*>(base + C::A_BYTES + (wave * C::NLW + i) * 1024) =
+            u32x4{0, 0, 0, 0};
+    wait_lgkm0();
+  };
+  const int r16 = lane & 15, g = lane >> 4;
+  const int off_lo = r16 * 128 + swizzled(r16, g) * 16;
+  const int off_hi = r16 * 128 + swizzled(r16, g + 4) * 16;
+  const int a_at = wm * RT * 2048, w_at = C::A_BYTES + wn * CT * 2048;
+  auto frag = [&](const uint8_t* at) -> i32x8 {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(at + off_lo);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(at + off_hi);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto scales = [&](const uint8_t* st, float (&s)[RT]) {
+    const float* sc = reinterpret_cast<const float*>(st + C::SC_OFF);
+    const float w = sc[C::BM + wn * CT * 16 / 128];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) s[t] = sc[wm * RT * 16 + t * 16 + r16] * w;
+  };
+
+  f32x4 acc[CT][RT];
+#pragma unroll
+  for (int i = 0; i < CT; ++i)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (s < KT) issue(s);
+  if (KT >= STAGES) wait_vmcnt<(STAGES - 1) * C::NL>();
+  else wait_vmcnt<0>();
+  if (KT == 1) end_of_k(0);
+  wave_barrier_all();
+
+  // Tile j = i * RT + t of a stage (16 weight rows i, 16 tokens t): its MFMA is
+  // issued LAG tiles ahead of its four FMAs, across the stage's end too (`sp`:
+  // the scales of the stage before).
+  constexpr int TILES = CT * RT, LAG = 3;
+  static_assert(TILES > LAG && RT >= 2, "pipeline");
+  i32x8 x[RT], w[2];
+  float s[RT], sp[RT];
+  f32x4 part[LAG + 1];
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  // (the first stage folds LAG zeros in)
+#pragma unroll
+  for (int j = 0; j <= LAG; ++j) part[j] = zero;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    sp[t] = 0.f;
+    x[t] = frag(lds + a_at + t * 2048);
+  }
+  w[0] = frag(lds + w_at);
+  scales(lds, s);
+  auto fold = [&](int j, const float (&f)[RT]) {
+    const int i = j / RT, t = j % RT;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      acc[i][t][v] = __builtin_fmaf(part[j & LAG][v], f[t], acc[i][t][v]);
+  };
+  static_assert((LAG & (LAG + 1)) == 0 && TILES % (LAG + 1) == 0, "part ring");
+  // One stage. The last 16 weight rows' fragment is its last read, so the
+  // slot is free once every wave has it; the next stage's first fragments
+  // replace each token tile's as its last MFMA has been issued.
+  // REST: the stages behind this one, as far as it matters (STAGES: a refill
+  // of the slot among them). The loop's body has no branch: code behind one
+  // would draw the MFMAs before it in.
+  auto stage = [&](int kt, auto rest_c) {
+    constexpr int REST = decltype(rest_c)::value;
+    constexpr bool MORE = REST > 0;
+    constexpr int L = CT - 1;
+    const uint8_t* st = lds + (kt % STAGES) * C::STAGE;
+    const uint8_t* nx = lds + ((kt + 1) % STAGES) * C::STAGE;
+    float sn[RT];
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+      const int i = j / RT, t = j % RT;
+      if (t == 0 && i < L) w[(i + 1) & 1] = frag(st + w_at + (i + 1) * 2048);
+      if constexpr (MORE) {
+        if (i == L && t == 0) {
+          wait_lgkm0();
+          wait_vmcnt<(REST - 1 < STAGES - 2 ? REST - 1 : STAGES - 2) * C::NL>();
+          if constexpr (REST == 1) end_of_k(kt + 1);
+          wave_barrier_all();
+          if constexpr (REST == STAGES) issue(kt + STAGES);
+        }
+      }
+      part[j & LAG] = mfma16_fp8(w[i & 1], x[t], zero);
+      if (j >= LAG) fold(j - LAG, s);
+      else fold(TILES + j - LAG, sp);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MORE) {
+        if (i == L) {
+          x[t] = frag(nx + a_at + t * 2048);
+          if (t == 0) w[0] = frag(nx + w_at);
+          if (t == RT - 1) scales(nx, sn);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sp[t] = s[t];
+    if constexpr (MORE) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t] = sn[t];
+    }
+  };
+  for (int kt = 0; kt + STAGES < KT; ++kt) stage(kt, std::integral_constant<int, STAGES>{});
+  if constexpr (STAGES > 3) {
+    if (KT > 3) stage(KT - 4, std::integral_constant<int, 3>{});
+  }
+  if constexpr (STAGES > 2) {
+    if (KT > 2) stage(KT - 3, std::integral_constant<int, 2>{});
+  }
+  if (KT > 1) stage(KT - 2, std::integral_constant<int, 1>{});
+  stage(KT - 1, std::integral_constant<int, 0>{});
+#pragma unroll
+  for (int j = TILES - LAG; j < TILES; ++j) fold(j, sp);
+
+  // lane: token r16 of each tile, output columns 4 g .. 4 g + 3 of each
+  const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int64_t m = m0 + (wm * RT + t) * 16 + r16;
+    if (m >= p.m) continue;
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+      const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
+      if (n >= p.n) continue;
+      if (ksplit == 1) {
+        write_out(p, m, n, acc[i][t], vec);
+      } else {
+        float* dst = p.part + (static_cast<int64_t>(ks) * p.m + m) * p.n + n;
+        if (p.n % 4 == 0) {
+          *reinterpret_cast<f32x4*>(dst) = acc[i][t];
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (n + v < p.n) dst[v] = acc[i][t][v];
+        }
+      }
+    }
+  }
+}
+
+// out = sum over the k splits in order (+ bias), four columns a thread.
+__global__ __launch_bounds__(256) void block_gemm_sum_kernel(const BlockGemmParams p, int ksplit) {
+  const int64_t n = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const int64_t m = blockIdx.y;
+  if (n >= p.n) return;
+  const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < ksplit; ++s) {
+    const float* src = p.part + (static_cast<int64_t>(s) * p.m + m) * p.n + n;
+    if (p.n % 4 == 0) {
+      v += *reinterpret_cast<const f32x4*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.n) v[i] += src[i];
+    }
+  }
+  write_out(p, m, n, v, vec);
+}
+
+// ---------------------------------------------------------------- schedule ---
+namespace {
+
+// Forms by number (FGS_BLOCK_FORM): streaming with 16, 32, 64 tokens a
+// workgroup, then the tiled configurations.
+constexpr int kStreamForms = 3;
+struct TiledForm {
+  int bm, bn;
+};
+constexpr TiledForm kTiled[] = {{256, 256}, {128, 256}, {128, 128}, {64, 128}};
+constexpr int kTiledForms = sizeof(kTiled) / sizeof(kTiled[0]);
+typedef BlockCfg<256, 256, 4, 2, 2, 2> Cfg256;
+typedef BlockCfg<128, 256, 2, 4, 3, 2> Cfg128x256;
+typedef BlockCfg<128, 128, 2, 2, 2, 2> Cfg128;
+typedef BlockCfg<64, 128, 2, 2, 3, 2> Cfg64;
+constexpr int kMaxSplit = 8;
 
 template <int MT>
-static void stream_launch(const BlockGemmParams& p, hipStream_t stream) {
+void stream_launch(const BlockGemmParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.n + 15) / 16),
                   static_cast<unsigned>((p.m + 16 * MT - 1) / (16 * MT)));
   hipLaunchKernelGGL((block_gemm_stream_kernel<MT, 8>), grid, dim3(512), 0, stream, p);
 }
 
+template <class C>
+int tiled_launch(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
+  static const hipError_t attr = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(block_gemm_tiled_kernel<C>),
+      hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (attr != hipSuccess)
+    return fail(FGS_ELAUNCH, std::string("block_gemm_tiled_kernel: ") + hipGetErrorString(attr));
+  const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
+  const int64_t total = nm * nn * q.ksplit;
+  if (total > 0x7ffffff0) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  hipLaunchKernelGGL((block_gemm_tiled_kernel<C>), dim3(static_cast<unsigned>((total + 7) / 8 * 8)),
+                     dim3(C::NW * 64), C::LDS, stream, p, static_cast<int>(nm),
+                     static_cast<int>(nn), q.ksplit, q.band);
+  return check_launch("block_gemm_tiled_kernel");
+}
+
+}  // namespace
+
+bool block_gemm_flags_ok(int32_t flags) {
+  return flags >= 0 && (flags & 0xff) <= kStreamForms + kTiledForms && (flags >> 8) <= kMaxSplit;
+}
+
+BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags) {
+  BlockGemmPlan q{};
+  q.ksplit = 1;
+  q.band = 4;
+  const int kb = static_cast<int>((k + 127) / 128);
+  if (flags & 0xff) {
+    q.form = (flags & 0xff) - 1;
+  } else {
+    const int64_t big = (m + 255) / 256 * ((n + 255) / 256);
+    q.form = m <= 16 ? 0 : m <= 32 ? 1 : m <= 64 ? 2 : big >= 200 ? 3 : 6;
+  }
+  if (q.form >= kStreamForms && (flags >> 8)) q.ksplit = std::min(flags >> 8, kb);
+  return q;
+}
+
+int64_t block_gemm_workspace(const BlockGemmPlan& q, int64_t m, int64_t n) {
+  return q.ksplit > 1 ? q.ksplit * m * n * 4 : 0;
+}
+
+std::string block_gemm_name(const BlockGemmPlan& q) {
+  if (q.form < kStreamForms) return "stream tokens=" + std::to_string(16 << q.form);
+  const TiledForm& f = kTiled[q.form - kStreamForms];
+  return "tiled " + std::to_string(f.bm) + "x" + std::to_string(f.bn) +
+         (q.ksplit > 1 ? " ksplit=" + std::to_string(q.ksplit) : "");
+}
+
 int launch_block_gemm(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
-  if (q.mt == 1) stream_launch<1>(p, stream);
-  else if (q.mt == 2) stream_launch<2>(p, stream);
-  else stream_launch<4>(p, stream);
-  return check_launch("block_gemm_stream_kernel");
+  int rc = FGS_OK;
+  switch (q.form) {
+    case 0: stream_launch<1>(p, stream); return check_launch("block_gemm_stream_kernel");
+    case 1: stream_launch<2>(p, stream); return check_launch("block_gemm_stream_kernel");
+    case 2: stream_launch<4>(p, stream); return check_launch("block_gemm_stream_kernel");
+    case 3: rc = tiled_launch<Cfg256>(p, q, stream); break;
+    case 4: rc = tiled_launch<Cfg128x256>(p, q, stream); break;
+    case 5: rc = tiled_launch<Cfg128>(p, q, stream); break;
+    default: rc = tiled_launch<Cfg64>(p, q, stream); break;
+  }
+  if (rc || q.ksplit == 1) return rc;
+  const dim3 grid(static_cast<unsigned>((p.n + 1023) / 1024), static_cast<unsigned>(p.m));
+  hipLaunchKernelGGL(block_gemm_sum_kernel, grid, dim3(256), 0, stream, p, q.ksplit);
+  return check_launch("block_gemm_sum_kernel");
 }
 
 }  // namespace fgs

@@ -258,11 +258,11 @@ struct BlockGemmParams {
   float* part;           // workspace (block_gemm_workspace bytes)
 };
 constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 24;
-// The kernel a product of these sizes runs.
-enum : int { kBlockStream = 0 };
+// The kernel a product of these sizes runs (`flags` 0, or FGS_BLOCK_*).
 struct BlockGemmPlan {
   int form;
-  int mt;  // streaming: 16-token tiles of a workgroup
+  int ksplit;  // tiled: k splits, summed by a second kernel
+  int band;    // tiled: token tiles of a raster band
 };
 BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags);
 bool block_gemm_flags_ok(int32_t flags);

@@ -125,13 +125,6 @@ constexpr int tiled_lds_bytes() {
              : tiled_ring_bytes<DT, C, false>();
 }
 
-// 4-byte LDS-DMA load: lane l copies 4 bytes from `src` to byte 4*l of the
-// 256-byte block at `lds_dst`.
-__device__ __forceinline__ void lds_dma4(const void* src, void* lds_dst) {
-  __builtin_amdgcn_global_load_lds(
-      src, (__attribute__((address_space(3))) void*)(lds_dst), 4, 0, 0);
-}
-
 // One tile (row block rb_id of expert e, column tile tile_n, k split ks).
 // COMPACT: the row block's rows from C::BMA on are all padding, and the LDS
 // ring holds C::BMA activation rows per stage in C::STAGES_C slots.

@@ -42,6 +42,24 @@ __device__ __forceinline__ void lds_dma16(const void* src, void* lds_dst) {
       src, (__attribute__((address_space(3))) void*)(lds_dst), 16, 0, 0);
 }
 
+// 4-byte LDS-DMA load: lane l copies 4 bytes from `src` to byte 4*l of the
+// 256-byte block at `lds_dst`.
+__device__ __forceinline__ void lds_dma4(const void* src, void* lds_dst) {
+  __builtin_amdgcn_global_load_lds(
+      src, (__attribute__((address_space(3))) void*)(lds_dst), 4, 0, 0);
+}
+
+// One wave-wide buffer load into LDS: lane l copies 16 bytes from
+// rsrc + voff + soff to byte 16*l of the 1 KiB block at `lds_dst` (uniform).
+__device__ __forceinline__ void lds_dma16_buf(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff,
+                                              int soff, void* lds_dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      rsrc, (__attribute__((address_space(3))) void*)(lds_dst), 16, voff, soff, 0, 0);
+}
+
+// gfx9 buffer resource word 3 for raw 32-bit loads.
+constexpr int kBufWord3 = 0x00020000;
+
 __device__ __forceinline__ void wave_barrier_all() { __builtin_amdgcn_s_barrier(); }
 
 // s_waitcnt lgkmcnt(0): this wave's LDS reads have completed.

@@ -81,16 +81,6 @@ __device__ __forceinline__ int wide_chunk(int r, int c) {
   return c ^ ((r / C::RPL) % C::CPR);
 }
 
-// One wave-wide buffer load into LDS: lane l copies 16 bytes from
-// rsrc + voff + soff to byte 16*l of the 1 KiB block at `lds_dst` (uniform).
-__device__ __forceinline__ void lds_dma16_buf(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff,
-                                              int soff, void* lds_dst) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      rsrc, (__attribute__((address_space(3))) void*)(lds_dst), 16, voff, soff, 0, 0);
-}
-
-// gfx9 buffer resource word 3 for raw 32-bit loads.
-constexpr int kBufWord3 = 0x00020000;
 
 // The d-th tile (0-based) of an XCD's range [lo, hi) of the row-block-major
 // tile numbering (tile = rball * n_ct + ct), walked over groups of gn

@@ -452,6 +452,8 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
                                  int32_t bias_dtype, int64_t m, int64_t n, int64_t k,
                                  int32_t out_dtype, int32_t flags, void* workspace,
                                  int64_t ws_bytes, void* out, int64_t ldo, void* stream);
+#define FGS_BLOCK_FORM(f) ((f) + 1)    /* kernel form f, for measurement and tests */
+#define FGS_BLOCK_KSPLIT(s) ((s) << 8) /* ... in s (at most 8) k splits */
 int64_t fgs_moe_fp8_block_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t flags);
 /* The schedule such a call runs, as text (as fgs_moe_schedule). */
 int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,

@@ -277,6 +277,14 @@ def _operands(gen, m, n, k, device, narrow=False):
     return codes(m), sa, codes(n), sw
 
 
+def _known_form(form):
+    try:
+        _capi.block_matmul_schedule(256, 256, 1024, form + 1)
+    except ValueError:
+        return False
+    return True
+
+
 def _product_ref(a, sa, w, sw, bias=None):
     k, n = a.shape[1], w.shape[0]
     a = a.double() * sa.double().repeat_interleave(128, 1)[:, :k]
@@ -315,6 +323,31 @@ def test_product(gpu, m, n, k):
             refb, magb = _product_ref(a, sa, w, sw, b)
             _check_product(fgs.fp8_block_matmul(a, sa, w, sw, bias=b), refb, magb, k, BF16,
                            narrow)
+
+
+FORMS = [f for f in range(20) if _known_form(f)]
+RAGGED = [(1, 1, 16), (70, 260, 144), (257, 257, 272), (130, 520, 1168), (300, 384, 640),
+          (255, 1000, 128), (513, 130, 400), (64, 640, 2048)]
+
+
+@pytest.mark.parametrize("m,n,k", RAGGED)
+@pytest.mark.parametrize("form", FORMS)
+def test_every_form_of_the_product(gpu, form, m, n, k):
+    """Each kernel on sizes around its tiles' ends, whole and split over k
+    (more splits than blocks are cut to one a block)."""
+    gen = torch.Generator().manual_seed(m * n + k)
+    a, sa, w, sw = _operands(gen, m, n, k, gpu, narrow=True)
+    bias = torch.randn(n, generator=gen).bfloat16().to(gpu)
+    ref, mag = _product_ref(a, sa, w, sw)
+    refb, magb = _product_ref(a, sa, w, sw, bias)
+    for split in (1, 2, 3, 8):
+        flags = (form + 1) | split << 8
+        if split > 1 and "ksplit" not in _capi.block_matmul_schedule(m, n, k, flags):
+            continue
+        got = fgs.fp8_block_matmul(a, sa, w, sw, out_dtype=F16, _flags=flags)
+        _check_product(got, ref, mag, k, F16, narrow=True)
+        got = fgs.fp8_block_matmul(a, sa.t().contiguous().t(), w, sw, bias=bias, _flags=flags)
+        _check_product(got, refb, magb, k, BF16, narrow=True)
 
 
 def _same(x, y):
