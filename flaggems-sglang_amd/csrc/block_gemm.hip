@@ -33,17 +33,16 @@ __device__ __forceinline__ float bias_at(const BlockGemmParams& p, int64_t n) {
                                         : Elem<FGS_DTYPE_FP16>::to_f32(b);
 }
 template <int TY>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (TY == FGS_DTYPE_BF16) return cvt_pk_bf16(lo, hi);
+  else return Elem<TY>::from_f32(lo) | static_cast<uint32_t>(Elem<TY>::from_f32(hi)) << 16;
+}
+template <int TY>
 __device__ __forceinline__ void store4(void* out, int64_t at, f32x4 v, int64_t left, bool vec) {
   typedef typename Elem<TY>::raw raw;
   raw* o = static_cast<raw*>(out) + at;
   if (vec && left >= 4) {
-    if constexpr (TY == FGS_DTYPE_BF16) {
-      *reinterpret_cast<uint2*>(o) = uint2{cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
-    } else {
-      *reinterpret_cast<uint2*>(o) =
-          uint2{Elem<TY>::from_f32(v[0]) | static_cast<uint32_t>(Elem<TY>::from_f32(v[1])) << 16,
-                Elem<TY>::from_f32(v[2]) | static_cast<uint32_t>(Elem<TY>::from_f32(v[3])) << 16};
-    }
+    *reinterpret_cast<uint2*>(o) = uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
     return;
   }
 #pragma unroll
@@ -212,7 +211,9 @@ __device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int ksplit, 
   return true;
 }
 
-template <class C>
+// OUT: the output's type, or fp32 partial sums of a k split.
+constexpr int kOutPartial = FGS_DTYPE_FP32;
+template <class C, int OUT>
 __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     const BlockGemmParams p, int nm, int nn, int ksplit, int band) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -311,11 +312,12 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     const i32x4 hi = *reinterpret_cast<const i32x4*>(at + off_hi);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto scales = [&](const uint8_t* st, float (&s)[RT]) {
+  // a stage's scales: the wave's tokens' and its weight block's
+  auto raw_scales = [&](const uint8_t* st, float (&a)[RT], float& w) {
     const float* sc = reinterpret_cast<const float*>(st + C::SC_OFF);
-    const float w = sc[C::BM + wn * CT * 16 / 128];
+    w = sc[C::BM + wn * CT * 16 / 128];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) s[t] = sc[wm * RT * 16 + t * 16 + r16] * w;
+    for (int t = 0; t < RT; ++t) a[t] = sc[wm * RT * 16 + t * 16 + r16];
   };
 
   f32x4 acc[CT][RT];
@@ -350,12 +352,24 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     x[t] = frag(lds + a_at + t * 2048);
   }
   w[0] = frag(lds + w_at);
-  scales(lds, s);
+  float w_scale0;
+  raw_scales(lds, s, w_scale0);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) s[t] *= w_scale0;
   auto fold = [&](int j, const float (&f)[RT]) {
     const int i = j / RT, t = j % RT;
 #pragma unroll
     for (int v = 0; v < 4; ++v)
       acc[i][t][v] = __builtin_fmaf(part[j & LAG][v], f[t], acc[i][t][v]);
+  };
+  // Nothing of the sums so far is computed behind this point.
+  auto settle = [&]() {
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) asm volatile("" : "+v"(acc[i][t]));
+#pragma unroll
+    for (int j = 0; j <= LAG; ++j) asm volatile("" : "+v"(part[j]));
   };
   static_assert((LAG & (LAG + 1)) == 0 && TILES % (LAG + 1) == 0, "part ring");
   // One stage. The last 16 weight rows' fragment is its last read, so the
@@ -370,7 +384,7 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     constexpr int L = CT - 1;
     const uint8_t* st = lds + (kt % STAGES) * C::STAGE;
     const uint8_t* nx = lds + ((kt + 1) % STAGES) * C::STAGE;
-    float sn[RT];
+    float sn[RT], swn = 0.f;
 #pragma unroll
     for (int j = 0; j < TILES; ++j) {
       const int i = j / RT, t = j % RT;
@@ -379,7 +393,10 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
         if (i == L && t == 0) {
           wait_lgkm0();
           wait_vmcnt<(REST - 1 < STAGES - 2 ? REST - 1 : STAGES - 2) * C::NL>();
-          if constexpr (REST == 1) end_of_k(kt + 1);
+          if constexpr (REST == 1) {
+            settle();  // (behind end_of_k's branch they would spill)
+            end_of_k(kt + 1);
+          }
           wave_barrier_all();
           if constexpr (REST == STAGES) issue(kt + STAGES);
         }
@@ -390,9 +407,9 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (MORE) {
         if (i == L) {
+          if (t == 0) raw_scales(nx, sn, swn);
           x[t] = frag(nx + a_at + t * 2048);
           if (t == 0) w[0] = frag(nx + w_at);
-          if (t == RT - 1) scales(nx, sn);
         }
       }
     }
@@ -400,7 +417,7 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     for (int t = 0; t < RT; ++t) sp[t] = s[t];
     if constexpr (MORE) {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) s[t] = sn[t];
+      for (int t = 0; t < RT; ++t) s[t] = sn[t] * swn;
     }
   };
   for (int kt = 0; kt + STAGES < KT; ++kt) stage(kt, std::integral_constant<int, STAGES>{});
@@ -414,28 +431,70 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   stage(KT - 1, std::integral_constant<int, 0>{});
 #pragma unroll
   for (int j = TILES - LAG; j < TILES; ++j) fold(j, sp);
+  // Matrix instructions write every lane, whatever EXEC holds: the last stage's
+  // may not be moved into the branches of single lanes that store their
+  // results, where they would overwrite registers of the lanes outside.
+  settle();
 
   // lane: token r16 of each tile, output columns 4 g .. 4 g + 3 of each
-  const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
+  if constexpr (OUT == kOutPartial) {
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int64_t m = m0 + (wm * RT + t) * 16 + r16;
-    if (m >= p.m) continue;
+    for (int t = 0; t < RT; ++t) {
+      const int64_t m = m0 + (wm * RT + t) * 16 + r16;
+      if (m >= p.m) continue;
+      float* row = p.part + (static_cast<int64_t>(ks) * p.m + m) * p.part_ld;
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
+        if (n < p.part_ld) *reinterpret_cast<f32x4*>(row + n) = acc[i][t];
+      }
+    }
+  } else {
+    // Through this wave's share of the ring, so that 16 bytes a lane leave as
+    // whole row segments (four columns a lane are 32 bytes of 16 rows each:
+    // 257 x 257 x 272 took 22 us so). A staged row's 16-byte chunks are
+    // XORed with the row: the 16 rows a write covers meet all banks.
+    constexpr int CH = CT * 2;                 // chunks of a row
+    constexpr int ROWS = 64 / CH;              // rows a store instruction covers
+    static_assert(RT * 16 * CH * 16 <= C::LDS / C::NW && 64 % CH == 0, "staging area");
+    wave_barrier_all();  // every wave has read its last fragments
+    uint8_t* stg = lds + wave * (RT * 16 * CH * 16);
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
       const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
-      if (n >= p.n) continue;
-      if (ksplit == 1) {
-        write_out(p, m, n, acc[i][t], vec);
-      } else {
-        float* dst = p.part + (static_cast<int64_t>(ks) * p.m + m) * p.n + n;
-        if (p.n % 4 == 0) {
-          *reinterpret_cast<f32x4*>(dst) = acc[i][t];
-        } else {
+      f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+      if (p.bias) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (n + v < p.n) dst[v] = acc[i][t][v];
-        }
+        for (int v = 0; v < 4; ++v) bias[v] = bias_at(p, min<int64_t>(n + v, p.n - 1));
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const f32x4 v = acc[i][t] + bias;
+        const int c = (2 * i + (g >> 1)) ^ (r16 % CH);
+        *reinterpret_cast<uint2*>(stg + (t * 16 + r16) * (CH * 16) + c * 16 + (g & 1) * 8) =
+            uint2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const bool vec = p.ldo % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    const int64_t n = n0 + wn * CT * 16 + (lane % CH) * 8;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + n;
+#pragma unroll
+    for (int k = 0; k < RT * 16 / ROWS; ++k) {
+      const int row = k * ROWS + lane / CH;
+      const int64_t m = m0 + wm * RT * 16 + row;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * (CH * 16) +
+                                                      ((lane % CH) ^ (row % CH)) * 16);
+      if (m >= p.m) continue;
+      if (vec && n + 8 <= p.n) {
+        *reinterpret_cast<u32x4*>(out + m * p.ldo) = v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < p.n)
+            out[m * p.ldo + j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j & 1)));
       }
     }
   }
@@ -449,14 +508,8 @@ __global__ __launch_bounds__(256) void block_gemm_sum_kernel(const BlockGemmPara
   const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < ksplit; ++s) {
-    const float* src = p.part + (static_cast<int64_t>(s) * p.m + m) * p.n + n;
-    if (p.n % 4 == 0) {
-      v += *reinterpret_cast<const f32x4*>(src);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < p.n) v[i] += src[i];
-    }
+    v += *reinterpret_cast<const f32x4*>(p.part + (static_cast<int64_t>(s) * p.m + m) * p.part_ld +
+                                         n);
   }
   write_out(p, m, n, v, vec);
 }
@@ -485,20 +538,27 @@ void stream_launch(const BlockGemmParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((block_gemm_stream_kernel<MT, 8>), grid, dim3(512), 0, stream, p);
 }
 
-template <class C>
-int tiled_launch(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
+template <class C, int OUT>
+int tiled_launch_out(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
   static const hipError_t attr = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(block_gemm_tiled_kernel<C>),
+      reinterpret_cast<const void*>(block_gemm_tiled_kernel<C, OUT>),
       hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (attr != hipSuccess)
     return fail(FGS_ELAUNCH, std::string("block_gemm_tiled_kernel: ") + hipGetErrorString(attr));
   const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
   const int64_t total = nm * nn * q.ksplit;
   if (total > 0x7ffffff0) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  hipLaunchKernelGGL((block_gemm_tiled_kernel<C>), dim3(static_cast<unsigned>((total + 7) / 8 * 8)),
+  hipLaunchKernelGGL((block_gemm_tiled_kernel<C, OUT>), dim3(static_cast<unsigned>((total + 7) / 8 * 8)),
                      dim3(C::NW * 64), C::LDS, stream, p, static_cast<int>(nm),
                      static_cast<int>(nn), q.ksplit, q.band);
   return check_launch("block_gemm_tiled_kernel");
+}
+
+template <class C>
+int tiled_launch(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
+  if (q.ksplit > 1) return tiled_launch_out<C, kOutPartial>(p, q, stream);
+  if (p.out_dtype == FGS_DTYPE_BF16) return tiled_launch_out<C, FGS_DTYPE_BF16>(p, q, stream);
+  return tiled_launch_out<C, FGS_DTYPE_FP16>(p, q, stream);
 }
 
 }  // namespace
@@ -523,7 +583,7 @@ BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags) {
 }
 
 int64_t block_gemm_workspace(const BlockGemmPlan& q, int64_t m, int64_t n) {
-  return q.ksplit > 1 ? q.ksplit * m * n * 4 : 0;
+  return q.ksplit > 1 ? q.ksplit * m * ((n + 3) / 4 * 4) * 4 : 0;
 }
 
 std::string block_gemm_name(const BlockGemmPlan& q) {

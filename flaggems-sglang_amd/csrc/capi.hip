@@ -1552,6 +1552,7 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
   p.bias = bias;
   p.out = out;
   p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.part_ld = (n + 3) / 4 * 4;
   p.m = m;
   p.n = n;
   p.k = k;

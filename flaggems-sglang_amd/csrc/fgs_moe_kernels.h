@@ -255,7 +255,8 @@ struct BlockGemmParams {
   int64_t as_row, as_col; // strides of a_scale over rows / k blocks
   int32_t out_dtype, bias_dtype;
   int32_t kblocks;
-  float* part;           // workspace (block_gemm_workspace bytes)
+  float* part;            // workspace: fp32 sums [k splits][m][part_ld], part_ld =
+  int64_t part_ld;        // n rounded up to 4
 };
 constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 24;
 // The kernel a product of these sizes runs (`flags` 0, or FGS_BLOCK_*).

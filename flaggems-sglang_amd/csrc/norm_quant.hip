@@ -56,34 +56,41 @@ __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
   if (WAVE && row >= p.rows) return;
   auto col = [&](int v) { return (static_cast<int64_t>(v) * threads + tid) * 8; };
 
-  // every load of the row first, the weight's among them
-  Vec8<TY, VEC> x[NV], r[RES ? NV : 1];
-  Vec8<WTY, VEC> w[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int64_t c = col(v);
-    x[v].zero();
-    w[v].zero();
-    if constexpr (RES) r[v].zero();
-    if (c < p.cols) {
-      x[v].load(p.x, row * p.x_stride + c, p.cols - c);
-      if constexpr (RES) r[v].load(p.residual, row * p.res_stride + c, p.cols - c);
-      w[v].load(p.weight, c, p.cols - c);
-    }
-  }
+  // Every load of the row first, the weight's among them; rows of more than
+  // two vectors a thread in batches and the weight later, to stay in registers.
+  constexpr int BATCH = NV <= 2 ? NV : sizeof(typename Elem<TY>::raw) == 2 && NV == 4 ? 4 : 2;
+  constexpr bool EARLY = NV <= 2;
+  Vec8<WTY, VEC> w[EARLY ? NV : 1];
   float h[NV][8];
   float sum = 0.f;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
+  for (int v0 = 0; v0 < NV; v0 += BATCH) {
+    Vec8<TY, VEC> x[BATCH], r[RES ? BATCH : 1];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[v][j] = x[v][j];
-      if constexpr (RES) h[v][j] += r[v][j];
-      sum = __builtin_fmaf(h[v][j], h[v][j], sum);
+    for (int b = 0; b < BATCH; ++b) {
+      const int64_t c = col(v0 + b);
+      x[b].zero();
+      if constexpr (EARLY) w[b].zero();
+      if constexpr (RES) r[b].zero();
+      if (c < p.cols) {
+        x[b].load(p.x, row * p.x_stride + c, p.cols - c);
+        if constexpr (RES) r[b].load(p.residual, row * p.res_stride + c, p.cols - c);
+        if constexpr (EARLY) w[b].load(p.weight, c, p.cols - c);
+      }
     }
-    if constexpr (RES) {
-      const int64_t c = col(v);
-      if (c < p.cols) store8<TY, VEC>(p.res_out, row * p.res_out_stride + c, p.cols - c, h[v]);
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int v = v0 + b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        h[v][j] = x[b][j];
+        if constexpr (RES) h[v][j] += r[b][j];
+        sum = __builtin_fmaf(h[v][j], h[v][j], sum);
+      }
+      if constexpr (RES) {
+        const int64_t c = col(v);
+        if (c < p.cols) store8<TY, VEC>(p.res_out, row * p.res_out_stride + c, p.cols - c, h[v]);
+      }
     }
   }
   sum = WAVE ? wave_sum_f32(sum) : block_sum(sum, red_sum);
@@ -93,10 +100,15 @@ __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int64_t c = col(v);
+    if constexpr (!EARLY) {
+      w[0].zero();
+      if (c < p.cols) w[0].load(p.weight, c, p.cols - c);
+    }
+    const Vec8<WTY, VEC>& wv = w[EARLY ? v : 0];
     // columns past the row: 0, whatever rstd is
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      h[v][j] = c + (VEC ? 0 : j) < p.cols ? h[v][j] * rstd * (w[v][j] + p.offset) : 0.f;
+      h[v][j] = c + (VEC ? 0 : j) < p.cols ? h[v][j] * rstd * (wv[j] + p.offset) : 0.f;
     if (p.norm && c < p.cols) store8<TY, VEC>(p.norm, row * p.cols + c, p.cols - c, h[v]);
     if (p.quant == FGS_QUANT_FP8_GROUP) {
       const float scale = scale_of(row_max(abs_bits8(h[v])), 448.f);
@@ -140,29 +152,38 @@ __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void gated_quant_kernel(
   if (WAVE && row >= p.rows) return;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * threads * NV;
 
-  Vec8<TY, VEC> g[NV], u[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int64_t c = (first + static_cast<int64_t>(v) * threads + tid) * 8;
-    g[v].zero();
-    u[v].zero();
-    if (c < p.n) {
-      g[v].load(p.x, row * p.x_stride + c, p.n - c);
-      u[v].load(p.x, row * p.x_stride + p.n + c, p.n - c);
-    }
-  }
+  // vectors loaded at once
+  constexpr int BATCH = NV <= 2 ? NV : NV == 8 && TY == FGS_DTYPE_FP32 ? 1 : 2;
   float h[NV][8];
   uint32_t amax = 0;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int64_t c = (first + static_cast<int64_t>(v) * threads + tid) * 8;
+  for (int v0 = 0; v0 < NV; v0 += BATCH) {
+    Vec8<TY, VEC> g[BATCH], u[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int64_t c = (first + static_cast<int64_t>(v0 + b) * threads + tid) * 8;
+      g[b].zero();
+      u[b].zero();
+      if (c < p.n) {
+        g[b].load(p.x, row * p.x_stride + c, p.n - c);
+        u[b].load(p.x, row * p.x_stride + p.n + c, p.n - c);
+      }
+    }
     if (p.act == kActGelu) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[v][j] = gelu_tail_mul(g[v][j], u[v][j]);
+      for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[v0 + b][j] = gelu_tail_mul(g[b][j], u[b][j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[v][j] = silu_mul(g[v][j], u[v][j]);
+      for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[v0 + b][j] = silu_mul(g[b][j], u[b][j]);
     }
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int64_t c = (first + static_cast<int64_t>(v) * threads + tid) * 8;
     if (p.quant == FGS_QUANT_FP8_GROUP) {
       const float scale = scale_of(row_max(abs_bits8(h[v])), 448.f);
       if (c < p.n) {

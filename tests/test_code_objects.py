@@ -96,3 +96,19 @@ def test_quantisers_divide_per_row_only(tmp_path):
             seen.add(n)
             assert code.count("v_div_fixup_f32") <= 2, n
     assert len(seen) > 10
+
+
+def test_products_are_done_before_lanes_branch(tmp_path):
+    """A matrix instruction writes every lane whatever EXEC holds, so the
+    compiler may not move one into the branches of single lanes that store
+    results (it did: registers of the lanes outside were overwritten): in the
+    block-scaled kernels the last one stands before the first store."""
+    seen = 0
+    for obj in _objects(LIB, str(tmp_path)):
+        for n in (n for n, _ in _kernels(obj) if "block_gemm" in n):
+            code = _tool("llvm-objdump", "-d", f"--disassemble-symbols={n}", obj)
+            if "v_mfma" not in code:
+                continue
+            seen += 1
+            assert code.rindex("v_mfma") < code.index("global_store"), n
+    assert seen >= 4
