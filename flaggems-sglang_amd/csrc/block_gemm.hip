@@ -182,6 +182,15 @@ struct BlockCfg {
   static_assert(CT % 2 == 0, "fragment pipeline");
 };
 
+// One wave-wide buffer load into LDS of 4 bytes a lane. (A global load into LDS
+// counts as one that may have gone through LDS: behind one, the compiler waits
+// for every LDS read at once instead of counting them.)
+__device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff,
+                                             void* lds_dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      rsrc, (__attribute__((address_space(3))) void*)(lds_dst), 4, voff, 0, 0, 0);
+}
+
 // Position of logical 16-byte chunk c of stage row r: the LDS serves 16 lanes
 // (256 bytes, two rows) of a 16-byte read at a time, and the XOR spreads the
 // 16 rows that lanes 0-15 read at one chunk over all 16 positions.
@@ -244,24 +253,20 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     const int r = (wave * C::NLW + i) * 8 + lrow;
     woff[i] = min(r, wm_last) * ldw + swizzled(r, lane & 7) * 16;
   }
-  // scale slots: a token's each, then the tile's weight blocks'
-  const int slot = wave * 64 + lane;
-  const float* sc_src;
-  int64_t sc_step;
-  if (slot < C::BM) {
-    sc_src = p.a_scale + min<int64_t>(m0 + slot, p.m - 1) * p.as_row;
-    sc_step = p.as_col;
-  } else {
-    const int64_t b = min<int64_t>((n0 >> 7) + slot - C::BM, (p.n - 1) >> 7);
-    sc_src = p.w_scale + b * p.kblocks;
-    sc_step = 1;
-  }
+  // scale slots: a token's each, then the tile's weight blocks' (a wave's 64
+  // are all the one or the other)
+  static_assert(C::BM % 64 == 0, "scale slots by waves");
+  const bool a_slots = wave < C::BM / 64;
+  const float* sc_base = a_slots ? p.a_scale + m0 * p.as_row : p.w_scale + (n0 >> 7) * p.kblocks;
+  const int64_t sc_step = a_slots ? p.as_col : 1;
+  const int w_block = min<int>(wave * 64 + lane - C::BM, min<int>((C::BN + 127) / 128 - 1, wm_last >> 7));
+  const uint32_t sc_off = a_slots ? min(wave * 64 + lane, am) * static_cast<uint32_t>(p.as_row) * 4
+                                  : max(w_block, 0) * p.kblocks * 4;
 
   const int kt0 = __builtin_amdgcn_readfirstlane(
       static_cast<int>(static_cast<uint32_t>(ks) * p.kblocks / ksplit));
   const int KT = __builtin_amdgcn_readfirstlane(static_cast<int>(
                      static_cast<uint32_t>(ks + 1) * p.kblocks / ksplit)) - kt0;
-  sc_src += kt0 * sc_step;
   const int k_bytes = static_cast<int>(p.k) - kt0 * 128;  // of the split to the row's end
 
   // The resources start at stage kt's columns and end with the tile's last
@@ -283,7 +288,9 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
 #pragma unroll
     for (int i = 0; i < C::NLW; ++i)
       lds_dma16_buf(rw, woff[i], 0, base + C::A_BYTES + (wave * C::NLW + i) * 1024);
-    lds_dma4(sc_src + kt * sc_step, base + C::SC_OFF + wave * 256);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(sc_base) + (kt0 + kt) * sc_step, 0, 0x7fffffff, kBufWord3);
+    lds_dma4_buf(rs, sc_off, base + C::SC_OFF + wave * 256);
   };
   // Stage kt (this wave's loads of it done): where it is the row's last block
   // and k ends inside it, the chunks past k that this wave loaded become 0.
@@ -420,6 +427,8 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
       for (int t = 0; t < RT; ++t) s[t] = sn[t] * swn;
     }
   };
+  // (so that the loop's own reads are all there is to count at its head)
+  wait_lgkm0();
   for (int kt = 0; kt + STAGES < KT; ++kt) stage(kt, std::integral_constant<int, STAGES>{});
   if constexpr (STAGES > 3) {
     if (KT > 3) stage(KT - 4, std::integral_constant<int, 3>{});

@@ -1533,6 +1533,9 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
   if ((m > 1 && (lda < 0 || lda % 16)) || (n > 1 && (ldw < 0 || ldw % 16)) ||
       reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(w) % 16)
     return fail(FGS_EUNSUPPORTED, "rows of a and w must be 16-byte aligned");
+  if ((m > 1 && (lda > kBlockMaxK || as_row_stride < 0 || as_row_stride > kBlockMaxScaleStride)) ||
+      (n > 1 && ldw > kBlockMaxK) || as_col_stride < 0)
+    return fail(FGS_EUNSUPPORTED, "row stride too large (or a negative one)");
   if (m > 1 && ldo < n) return fail(FGS_EINVAL, "ldo must be >= n");
   if (reinterpret_cast<uintptr_t>(a_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
       reinterpret_cast<uintptr_t>(out) % 2 ||
@@ -1559,7 +1562,7 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
   p.lda = m > 1 ? lda : k;
   p.ldw = n > 1 ? ldw : k;
   p.ldo = m > 1 ? ldo : n;
-  p.as_row = as_row_stride;
+  p.as_row = m > 1 ? as_row_stride : 0;
   p.as_col = as_col_stride;
   p.out_dtype = out_dtype;
   p.bias_dtype = bias_dtype;

@@ -258,7 +258,9 @@ struct BlockGemmParams {
   float* part;            // workspace: fp32 sums [k splits][m][part_ld], part_ld =
   int64_t part_ld;        // n rounded up to 4
 };
-constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 24;
+// Sizes and row strides the kernels' 32-bit offsets inside a tile allow.
+constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 22;
+constexpr int64_t kBlockMaxScaleStride = 1 << 20;
 // The kernel a product of these sizes runs (`flags` 0, or FGS_BLOCK_*).
 struct BlockGemmPlan {
   int form;

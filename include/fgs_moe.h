@@ -442,8 +442,8 @@ int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtyp
  *   stride ldo
  * The matrix instruction cuts each of eight neighbouring products 13 bits
  * below the largest one: about 1.5e-5 of a result from normal data.
- * k a positive multiple of 16, m and n anything; a and w rows 16-byte
- * aligned. `flags`: 0, or a schedule to use (FGS_BLOCK_*, below).
+ * k a positive multiple of 16, m, n and k up to 2^22; a and w rows 16-byte
+ * aligned and at most 2^22 apart, a_scale rows at most 2^20. `flags`: 0, or a schedule to use (FGS_BLOCK_*, below).
  * workspace: fgs_moe_fp8_block_matmul_workspace_bytes() bytes, 256-byte
  * aligned (may be null where that is 0). */
 int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scale,

@@ -92,6 +92,10 @@ def _product(**kw):
     (dict(m=1 << 23), -2, "too large"),
     (dict(n=1 << 23), -2, "too large"),
     (dict(k=1 << 25), -2, "too large"),
+    (dict(lda=1 << 23), -2, "stride too large"),
+    (dict(ldw=1 << 23), -2, "stride too large"),
+    (dict(as_row=1 << 21), -2, "stride too large"),
+    (dict(as_col=-1), -2, "stride too large"),
     (dict(flags=1 << 20), -1, "unknown flags"),
     (dict(flags=-1), -1, "unknown flags"),
     (dict(out_dtype=5), -1, "unknown element type"),
