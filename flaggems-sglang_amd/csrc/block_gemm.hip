@@ -16,6 +16,7 @@
 // at any k, against 3e-2 from the operands' own rounding; outputs are therefore
 // 16-bit types, whose step hides it.
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "dense_common.h"
@@ -63,95 +64,178 @@ __device__ __forceinline__ void write_out(const BlockGemmParams& p, int64_t m, i
   else store4<FGS_DTYPE_FP16>(p.out, at, v, left, vec);
 }
 
+// One wave-wide buffer load into LDS of 4 bytes a lane. (A global load into LDS
+// counts as one that may have gone through LDS: behind one, the compiler waits
+// for every LDS read at once instead of counting them.)
+__device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff,
+                                             void* lds_dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      rsrc, (__attribute__((address_space(3))) void*)(lds_dst), 4, voff, 0, 0, 0);
+}
+
+// Position of logical 16-byte chunk c of stage row r: the LDS serves 16 lanes
+// (256 bytes, two rows) of a 16-byte read at a time, and the XOR spreads the
+// 16 rows that lanes 0-15 read at one chunk over all 16 positions.
+__device__ __forceinline__ int swizzled(int r, int c) { return c ^ ((r >> 1) & 7); }
+
 // ------------------------------------------------------------- few tokens ---
-// A workgroup owns 16 weight rows and 16 * MT tokens; its KW waves split the
-// k blocks into contiguous runs and meet in LDS, added in wave order. The
-// operands go from memory to MFMA registers, each wave's loads of STEP blocks
-// in flight before its first product: the form is bound by the weights' bytes.
-template <int MT, int KW>
-__global__ __launch_bounds__(KW * 64) void block_gemm_stream_kernel(const BlockGemmParams p) {
-  constexpr int STEP = MT == 1 ? 8 : MT == 2 ? 4 : 2;
+// A workgroup owns 16 MT tokens x 16 NT weight rows; its KW waves split the k
+// blocks into contiguous runs and meet in LDS at the end, added in wave order.
+// Each wave streams its own blocks -- both operands' rows and the block's
+// scales -- through a ring of SLOTS LDS slots that is its alone, so nothing but
+// its own load counter orders it: the form is bound by the weights' bytes, and
+// the ring keeps enough of them in flight. (Straight from memory into the
+// MFMA's registers, a load's neighbouring lanes lie in 16 different rows, and
+// the address unit takes them one a cycle: 16 tokens 11.7 us at 4096 x 7168.)
+template <int MT_, int NT_, int KW_, int SLOTS_>
+struct SkinnyCfg {
+  static constexpr int MT = MT_, NT = NT_, KW = KW_, SLOTS = SLOTS_;
+  static constexpr int W_AT = MT * 2048, SC_AT = (MT + NT) * 2048;
+  static constexpr int SLOT = SC_AT + 512;  // 64 token scales, the weight block's
+  static constexpr int NL = 2 * (MT + NT) + 2;
+  static constexpr int LDS = KW * SLOTS * SLOT;
+  static_assert(MT <= 4 && 128 % (16 * NT) == 0, "one scale a lane, one weight block");
+  static_assert(SLOTS >= 2 && SLOTS <= 4 && (SLOTS - 1) * NL < 64 && LDS <= 160 * 1024, "ring");
+  static_assert(KW * MT * NT * 1024 <= LDS, "partial sums");
+};
+
+template <class C>
+__global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const BlockGemmParams p) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  constexpr int MT = C::MT, NT = C::NT, SLOTS = C::SLOTS;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16 * NT;
   const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  const int per = (p.kblocks + C::KW - 1) / C::KW;
+  const int kb0 = min(wave * per, p.kblocks);
+  const int count = min(per, p.kblocks - kb0);
+  const int rows_a = static_cast<int>(min<int64_t>(16 * MT, p.m - m0));
+  const int rows_w = static_cast<int>(min<int64_t>(16 * NT, p.n - n0));
+  const uint32_t lda = static_cast<uint32_t>(p.lda), ldw = static_cast<uint32_t>(p.ldw);
 
-  // rows past the end read the last one; their results are not stored
-  const uint8_t* wrow = p.w + min(n0 + r, p.n - 1) * p.ldw;
-  const uint8_t* arow[MT];
-  const float* asrow[MT];
+  // Lane l of a load: row l / 8 of its eight, 16-byte chunk l % 8, at the
+  // chunk's swizzled place. A resource ends with the last row's last column:
+  // rows past it are not accessed (what their slots hold reaches only results
+  // that are not stored), nor is anything behind k in the last row.
+  uint8_t* ring = lds + wave * SLOTS * C::SLOT;
+  const int lrow = lane >> 3;
+  const uint32_t c0 = swizzled(lrow, lane & 7) * 16;  // rows 0-7 of 16; 8-15: chunk ^ 4
+  const uint32_t a0 = lrow * lda, w0 = lrow * ldw;
+  const uint32_t as0 = lane * static_cast<uint32_t>(p.as_row) * 4;
+  auto issue = [&](int i) {
+    uint8_t* slot = ring + (i % SLOTS) * C::SLOT;
+    const int kb = kb0 + i;
+    const uint32_t left = static_cast<uint32_t>(p.k) - kb * 128;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.a) + m0 * p.lda + static_cast<int64_t>(kb) * 128, 0,
+        static_cast<int>((rows_a - 1) * lda + left), kBufWord3);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.w) + n0 * p.ldw + static_cast<int64_t>(kb) * 128, 0,
+        static_cast<int>((rows_w - 1) * ldw + left), kBufWord3);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(p.a_scale) + m0 * p.as_row + kb * p.as_col, 0,
+        static_cast<int>((rows_a - 1) * static_cast<uint32_t>(p.as_row) * 4 + 4), kBufWord3);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(p.w_scale) + (n0 >> 7) * p.kblocks + kb, 0, 4, kBufWord3);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = min(m0 + t * 16 + r, p.m - 1);
-    arow[t] = p.a + m * p.lda;
-    asrow[t] = p.a_scale + m * p.as_row;
-  }
-  const float* ws = p.w_scale + (n0 >> 7) * p.kblocks;
-
-  // lane group g takes the 16-byte chunks g and g + 4 of both operands' rows;
-  // chunks past k are 0 (k is a multiple of 16, so a chunk is in or out)
-  auto chunk = [&](const uint8_t* row, int kb, int c) -> u32x4 {
-    const int64_t k = static_cast<int64_t>(kb) * 128 + c * 16;
-    if (k >= p.k) return u32x4{0, 0, 0, 0};
-    return *reinterpret_cast<const u32x4*>(row + k);
+    for (int j = 0; j < 2 * NT; ++j)
+      lds_dma16_buf(rw, w0 + j * 8 * ldw + (c0 ^ (64 * (j & 1))), 0, slot + C::W_AT + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j)
+      lds_dma16_buf(ra, a0 + j * 8 * lda + (c0 ^ (64 * (j & 1))), 0, slot + j * 1024);
+    lds_dma4_buf(rs, as0, slot + C::SC_AT);
+    lds_dma4_buf(rb, lane * 4, slot + C::SC_AT + 256);
   };
-  auto frag = [](u32x4 lo, u32x4 hi) {
-    i32x8 f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = static_cast<int>(lo[i]);
-      f[4 + i] = static_cast<int>(hi[i]);
-    }
-    return f;
+  auto wait_stages = [&](int n) {  // at most n later blocks in flight
+    if (n >= 3) wait_vmcnt<(SLOTS > 3 ? 3 * C::NL : 0)>();
+    else if (n == 2) wait_vmcnt<(SLOTS > 2 ? 2 * C::NL : 0)>();
+    else if (n == 1) wait_vmcnt<C::NL>();
+    else wait_vmcnt<0>();
   };
 
-  f32x4 acc[MT];
+  const int r = lane & 15, g = lane >> 4;
+  const int off_lo = r * 128 + swizzled(r, g) * 16;
+  const int off_hi = r * 128 + swizzled(r, g + 4) * 16;
+  auto frag = [&](const uint8_t* at) -> i32x8 {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(at + off_lo);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(at + off_hi);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  // ... of the row's last block, of which only `chunks` lie inside k
+  auto cut = [&](i32x8& f, int chunks) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int per = (p.kblocks + KW - 1) / KW;
-  const int end = min(p.kblocks, (wave + 1) * per);
-  for (int kb0 = wave * per; kb0 < end; kb0 += STEP) {
-    u32x4 w[STEP][2], a[STEP][MT][2];
-    float s[STEP][MT];
+    for (int v = 0; v < 4; ++v) {
+      f[v] = g < chunks ? f[v] : 0;
+      f[4 + v] = g + 4 < chunks ? f[4 + v] : 0;
+    }
+  };
+
+  f32x4 acc[NT][MT];
 #pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      const int kb = min(kb0 + i, end - 1);
-      w[i][0] = chunk(wrow, kb, g);
-      w[i][1] = chunk(wrow, kb, g + 4);
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        a[i][t][0] = chunk(arow[t], kb, g);
-        a[i][t][1] = chunk(arow[t], kb, g + 4);
-        s[i][t] = asrow[t][kb * p.as_col] * ws[kb];
-      }
+    for (int t = 0; t < MT; ++t) acc[j][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i)
+    if (i < count) issue(i);
+  for (int i = 0; i < count; ++i) {
+    wait_stages(min(SLOTS - 1, count - 1 - i));
+    const uint8_t* slot = ring + (i % SLOTS) * C::SLOT;
+    i32x8 w[NT], x[MT];
+    float s[MT];
+    const float ws = *reinterpret_cast<const float*>(slot + C::SC_AT + 256);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      s[t] = *reinterpret_cast<const float*>(slot + C::SC_AT + (t * 16 + r) * 4);
+      x[t] = frag(slot + t * 2048);
     }
 #pragma unroll
-    for (int i = 0; i < STEP; ++i) {
-      if (kb0 + i >= end) break;
-      const i32x8 wf = frag(w[i][0], w[i][1]);
+    for (int j = 0; j < NT; ++j) w[j] = frag(slot + C::W_AT + j * 2048);
+    wait_lgkm0();  // the slot is read: refill it
+    if (i + SLOTS < count) issue(i + SLOTS);
+    const int chunks = static_cast<int>(p.k / 16) - (kb0 + i) * 8;
+    if (chunks < 8) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const f32x4 part =
-            mfma16_fp8(wf, frag(a[i][t][0], a[i][t][1]), f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int t = 0; t < MT; ++t) cut(x[t], chunks);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(part[v], s[i][t], acc[t][v]);
-      }
+      for (int j = 0; j < NT; ++j) cut(w[j], chunks);
+    }
+    // the MFMAs of two token tiles ahead of their FMAs
+    f32x4 part[NT][MT];
+#pragma unroll
+    for (int t0 = 0; t0 < MT; t0 += 2) {
+#pragma unroll
+      for (int t = t0; t < t0 + 2 && t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          part[j][t] = mfma16_fp8(w[j], x[t], f32x4{0.f, 0.f, 0.f, 0.f});
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = t0; t < t0 + 2 && t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            acc[j][t][v] = __builtin_fmaf(part[j][t][v], s[t] * ws, acc[j][t][v]);
     }
   }
 
-  __shared__ f32x4 red[KW][MT][64];
+  __syncthreads();  // the rings are done with
+  f32x4* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[(wave * NT * MT + j * MT + t) * 64 + lane] = acc[j][t];
   __syncthreads();
   const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
-  for (int i = threadIdx.x; i < MT * 64; i += KW * 64) {
-    const int t = i >> 6, l = i & 63;
-    f32x4 v = red[0][t][l];
+  for (int i = threadIdx.x; i < NT * MT * 64; i += C::KW * 64) {
+    f32x4 v = red[i];
 #pragma unroll
-    for (int k = 1; k < KW; ++k) v += red[k][t][l];
-    const int64_t m = m0 + t * 16 + (l & 15);
-    const int64_t n = n0 + 4 * (l >> 4);
+    for (int k = 1; k < C::KW; ++k) v += red[k * NT * MT * 64 + i];
+    const int tile = i >> 6, l = i & 63;
+    const int64_t m = m0 + (tile % MT) * 16 + (l & 15);
+    const int64_t n = n0 + (tile / MT) * 16 + 4 * (l >> 4);
     if (m < p.m && n < p.n) write_out(p, m, n, v, vec);
   }
 }
@@ -182,53 +266,33 @@ struct BlockCfg {
   static_assert(CT % 2 == 0, "fragment pipeline");
 };
 
-// One wave-wide buffer load into LDS of 4 bytes a lane. (A global load into LDS
-// counts as one that may have gone through LDS: behind one, the compiler waits
-// for every LDS read at once instead of counting them.)
-__device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff,
-                                             void* lds_dst) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      rsrc, (__attribute__((address_space(3))) void*)(lds_dst), 4, voff, 0, 0, 0);
-}
-
-// Position of logical 16-byte chunk c of stage row r: the LDS serves 16 lanes
-// (256 bytes, two rows) of a 16-byte read at a time, and the XOR spreads the
-// 16 rows that lanes 0-15 read at one chunk over all 16 positions.
-__device__ __forceinline__ int swizzled(int r, int c) { return c ^ ((r >> 1) & 7); }
-
-// Workgroup bid runs on XCD bid % 8, which takes the bid / 8-th item of its
-// contiguous eighth; items go split by split, and inside a split in bands of
-// `band` token tiles walked column by column, so an XCD's 32 CUs share a few
-// rows' and columns' operands in its L2.
-__device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int ksplit, int band, int* tm,
-                                           int* tn, int* ks) {
-  const int tiles = nm * nn;
-  const int total = tiles * ksplit;
+// Workgroup bid runs on XCD bid % 8, which takes the bid / 8-th tile of its
+// contiguous eighth; tiles go in bands of kBand token tiles walked column by
+// column, so an XCD's 32 CUs share a few rows' and columns' operands in its L2.
+constexpr int kBand = 4;
+__device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int* tm, int* tn) {
+  const int total = nm * nn;
   const int per = (total + 7) / 8;
   const int at = (bid % 8) * per + bid / 8;
   if (bid / 8 >= per || at >= total) return false;
-  const int s = at / tiles;
-  const int i = at - s * tiles;
-  const int b = i / (band * nn);
-  const int rem = i - b * band * nn;
-  const int rows = min(band, nm - b * band);
+  const int b = at / (kBand * nn);
+  const int rem = at - b * kBand * nn;
+  const int rows = min(kBand, nm - b * kBand);
   // (the divisions run on the VALU: back to scalars, so that the loops and the
   // buffer resources that follow from them are scalar too)
-  *ks = __builtin_amdgcn_readfirstlane(s);
   *tn = __builtin_amdgcn_readfirstlane(rem / rows);
-  *tm = __builtin_amdgcn_readfirstlane(b * band + rem % rows);
+  *tm = __builtin_amdgcn_readfirstlane(b * kBand + rem % rows);
   return true;
 }
 
-// OUT: the output's type, or fp32 partial sums of a k split.
-constexpr int kOutPartial = FGS_DTYPE_FP32;
+// OUT: the output's type.
 template <class C, int OUT>
 __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
-    const BlockGemmParams p, int nm, int nn, int ksplit, int band) {
+    const BlockGemmParams p, int nm, int nn) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   constexpr int RT = C::RT, CT = C::CT, STAGES = C::STAGES;
-  int tm, tn, ks;
-  if (!block_tile(blockIdx.x, nm, nn, ksplit, band, &tm, &tn, &ks)) return;
+  int tm, tn;
+  if (!block_tile(blockIdx.x, nm, nn, &tm, &tn)) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
@@ -263,19 +327,15 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   const uint32_t sc_off = a_slots ? min(wave * 64 + lane, am) * static_cast<uint32_t>(p.as_row) * 4
                                   : max(w_block, 0) * p.kblocks * 4;
 
-  const int kt0 = __builtin_amdgcn_readfirstlane(
-      static_cast<int>(static_cast<uint32_t>(ks) * p.kblocks / ksplit));
-  const int KT = __builtin_amdgcn_readfirstlane(static_cast<int>(
-                     static_cast<uint32_t>(ks + 1) * p.kblocks / ksplit)) - kt0;
-  const int k_bytes = static_cast<int>(p.k) - kt0 * 128;  // of the split to the row's end
+  const int KT = p.kblocks;
 
   // The resources start at stage kt's columns and end with the tile's last
   // row: what a lane would read past that (the last block's chunks past k of
   // the last row) is not accessed.
   auto issue = [&](int kt) {
     uint8_t* base = lds + (kt % STAGES) * C::STAGE;
-    const int64_t koff = static_cast<int64_t>(kt0 + kt) * 128;
-    const uint32_t left = static_cast<uint32_t>(k_bytes - kt * 128);
+    const int64_t koff = static_cast<int64_t>(kt) * 128;
+    const uint32_t left = static_cast<uint32_t>(static_cast<int>(p.k) - kt * 128);
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(p.a) + m0 * p.lda + koff, 0, static_cast<int>(am * lda + left),
         kBufWord3);
@@ -289,12 +349,12 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     for (int i = 0; i < C::NLW; ++i)
       lds_dma16_buf(rw, woff[i], 0, base + C::A_BYTES + (wave * C::NLW + i) * 1024);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<float*>(sc_base) + (kt0 + kt) * sc_step, 0, 0x7fffffff, kBufWord3);
+        const_cast<float*>(sc_base) + kt * sc_step, 0, 0x7fffffff, kBufWord3);
     lds_dma4_buf(rs, sc_off, base + C::SC_OFF + wave * 256);
   };
   // Stage kt (this wave's loads of it done): where it is the row's last block
   // and k ends inside it, the chunks past k that this wave loaded become 0.
-  const int ragged = (p.k & 127) && kt0 + KT == p.kblocks ? KT - 1 : -1;
+  const int ragged = p.k & 127 ? KT - 1 : -1;
   auto end_of_k = [&](int kt) {
     if (kt != ragged) return;
     uint8_t* base = lds + (kt % STAGES) * C::STAGE + lane * 16;
@@ -446,177 +506,178 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   settle();
 
   // lane: token r16 of each tile, output columns 4 g .. 4 g + 3 of each
-  if constexpr (OUT == kOutPartial) {
+  // Through this wave's share of the ring, so that 16 bytes a lane leave as
+  // whole row segments (four columns a lane are 32 bytes of 16 rows each:
+  // 257 x 257 x 272 took 22 us so). A staged row's 16-byte chunks are
+  // XORed with the row: the 16 rows a write covers meet all banks.
+  constexpr int CH = CT * 2;                 // chunks of a row
+  constexpr int ROWS = 64 / CH;              // rows a store instruction covers
+  static_assert(RT * 16 * CH * 16 <= C::LDS / C::NW && 64 % CH == 0, "staging area");
+  wave_barrier_all();  // every wave has read its last fragments
+  uint8_t* stg = lds + wave * (RT * 16 * CH * 16);
+#pragma unroll
+  for (int i = 0; i < CT; ++i) {
+    const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
+    f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) bias[v] = bias_at(p, min<int64_t>(n + v, p.n - 1));
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int64_t m = m0 + (wm * RT + t) * 16 + r16;
-      if (m >= p.m) continue;
-      float* row = p.part + (static_cast<int64_t>(ks) * p.m + m) * p.part_ld;
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
-        if (n < p.part_ld) *reinterpret_cast<f32x4*>(row + n) = acc[i][t];
-      }
-    }
-  } else {
-    // Through this wave's share of the ring, so that 16 bytes a lane leave as
-    // whole row segments (four columns a lane are 32 bytes of 16 rows each:
-    // 257 x 257 x 272 took 22 us so). A staged row's 16-byte chunks are
-    // XORed with the row: the 16 rows a write covers meet all banks.
-    constexpr int CH = CT * 2;                 // chunks of a row
-    constexpr int ROWS = 64 / CH;              // rows a store instruction covers
-    static_assert(RT * 16 * CH * 16 <= C::LDS / C::NW && 64 % CH == 0, "staging area");
-    wave_barrier_all();  // every wave has read its last fragments
-    uint8_t* stg = lds + wave * (RT * 16 * CH * 16);
-#pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
-      f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-      if (p.bias) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) bias[v] = bias_at(p, min<int64_t>(n + v, p.n - 1));
-      }
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const f32x4 v = acc[i][t] + bias;
-        const int c = (2 * i + (g >> 1)) ^ (r16 % CH);
-        *reinterpret_cast<uint2*>(stg + (t * 16 + r16) * (CH * 16) + c * 16 + (g & 1) * 8) =
-            uint2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const bool vec = p.ldo % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    const int64_t n = n0 + wn * CT * 16 + (lane % CH) * 8;
-    uint16_t* out = static_cast<uint16_t*>(p.out) + n;
-#pragma unroll
-    for (int k = 0; k < RT * 16 / ROWS; ++k) {
-      const int row = k * ROWS + lane / CH;
-      const int64_t m = m0 + wm * RT * 16 + row;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * (CH * 16) +
-                                                      ((lane % CH) ^ (row % CH)) * 16);
-      if (m >= p.m) continue;
-      if (vec && n + 8 <= p.n) {
-        *reinterpret_cast<u32x4*>(out + m * p.ldo) = v;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (n + j < p.n)
-            out[m * p.ldo + j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j & 1)));
-      }
+      const f32x4 v = acc[i][t] + bias;
+      const int c = (2 * i + (g >> 1)) ^ (r16 % CH);
+      *reinterpret_cast<uint2*>(stg + (t * 16 + r16) * (CH * 16) + c * 16 + (g & 1) * 8) =
+          uint2{pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
     }
   }
-}
-
-// out = sum over the k splits in order (+ bias), four columns a thread.
-__global__ __launch_bounds__(256) void block_gemm_sum_kernel(const BlockGemmParams p, int ksplit) {
-  const int64_t n = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-  const int64_t m = blockIdx.y;
-  if (n >= p.n) return;
-  const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 8 == 0;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ksplit; ++s) {
-    v += *reinterpret_cast<const f32x4*>(p.part + (static_cast<int64_t>(s) * p.m + m) * p.part_ld +
-                                         n);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const bool vec = p.ldo % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  const int64_t n = n0 + wn * CT * 16 + (lane % CH) * 8;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + n;
+#pragma unroll
+  for (int k = 0; k < RT * 16 / ROWS; ++k) {
+    const int row = k * ROWS + lane / CH;
+    const int64_t m = m0 + wm * RT * 16 + row;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(stg + row * (CH * 16) +
+                                                    ((lane % CH) ^ (row % CH)) * 16);
+    if (m >= p.m) continue;
+    if (vec && n + 8 <= p.n) {
+      *reinterpret_cast<u32x4*>(out + m * p.ldo) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < p.n)
+          out[m * p.ldo + j] = static_cast<uint16_t>(v[j / 2] >> (16 * (j & 1)));
+    }
   }
-  write_out(p, m, n, v, vec);
 }
 
 // ---------------------------------------------------------------- schedule ---
 namespace {
 
-// Forms by number (FGS_BLOCK_FORM): streaming with 16, 32, 64 tokens a
-// workgroup, then the tiled configurations.
-constexpr int kStreamForms = 3;
-struct TiledForm {
-  int bm, bn;
+// The forms (FGS_BLOCK_FORM(i)): tile in tokens x weight rows; k blocks an
+// iteration takes (the streaming forms' waves take one each); workgroups that
+// run at once; microseconds of an iteration with the chip full, and beside the
+// iterations of a round. Measured at K 7168 and N 4096 (tokens: us): 1: 7.2
+// (form 0), 16: 8.1 (1), 32: 10.7 (2), 64: 11.3 (3; 64 x 32 tiles 15.6), 128:
+// 15.9 (4; 18.6 with 32 x 32), 256: 19.7 (5; 27), 512: 31 (6; 35 with 64 x 64),
+// 1024: 53 (7), 2048: 68 (7; 256 x 256 91), 4096: 110 (8; 128 x 128 125).
+struct Form {
+  int bm, bn, step, at_once;
+  double iter, half, round;  // half: an iteration with half of at_once or fewer
 };
-constexpr TiledForm kTiled[] = {{256, 256}, {128, 256}, {128, 128}, {64, 128}};
-constexpr int kTiledForms = sizeof(kTiled) / sizeof(kTiled[0]);
-typedef BlockCfg<256, 256, 4, 2, 2, 2> Cfg256;
-typedef BlockCfg<128, 256, 2, 4, 3, 2> Cfg128x256;
-typedef BlockCfg<128, 128, 2, 2, 2, 2> Cfg128;
-typedef BlockCfg<64, 128, 2, 2, 3, 2> Cfg64;
-constexpr int kMaxSplit = 8;
+constexpr Form kForms[] = {
+    {16, 16, 8, 512, 1.1, 0.85, 0.5},    {16, 16, 8, 256, 0.75, 0.95, 0.5},
+    {32, 16, 8, 256, 1.05, 0.95, 0.5},   {32, 32, 8, 256, 1.1, 1.1, 0.8},
+    {64, 32, 4, 256, 0.9, 0.9, 1.0},     {64, 64, 4, 256, 1.13, 1.13, 1.4},
+    {64, 128, 1, 512, 0.69, 0.47, 1.8},  {128, 128, 1, 512, 1.04, 0.85, 3.0},
+    {256, 256, 1, 256, 1.8, 1.5, 6.5},
+};
+constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
 
-template <int MT>
-void stream_launch(const BlockGemmParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((p.n + 15) / 16),
-                  static_cast<unsigned>((p.m + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((block_gemm_stream_kernel<MT, 8>), grid, dim3(512), 0, stream, p);
+template <int F>
+struct FormCfg;
+template <> struct FormCfg<0> { typedef SkinnyCfg<1, 1, 8, 2> type; };
+template <> struct FormCfg<1> { typedef SkinnyCfg<1, 1, 8, 4> type; };
+template <> struct FormCfg<2> { typedef SkinnyCfg<2, 1, 8, 2> type; };
+template <> struct FormCfg<3> { typedef SkinnyCfg<2, 2, 8, 2> type; };
+template <> struct FormCfg<4> { typedef SkinnyCfg<4, 2, 4, 3> type; };
+template <> struct FormCfg<5> { typedef SkinnyCfg<4, 4, 4, 2> type; };
+template <> struct FormCfg<6> { typedef BlockCfg<64, 128, 2, 2, 3, 2> type; };
+template <> struct FormCfg<7> { typedef BlockCfg<128, 128, 2, 2, 2, 2> type; };
+template <> struct FormCfg<8> { typedef BlockCfg<256, 256, 4, 2, 2, 2> type; };
+
+// Lets a kernel use more than 64 KiB of LDS, once.
+hipError_t allow_lds(const void* kernel, int bytes) {
+  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <class C, int OUT>
-int tiled_launch_out(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
-  static const hipError_t attr = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(block_gemm_tiled_kernel<C, OUT>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+template <int F>
+int skinny_launch(const BlockGemmParams& p, hipStream_t stream) {
+  typedef typename FormCfg<F>::type C;
+  static_assert(kForms[F].bm == 16 * C::MT && kForms[F].bn == 16 * C::NT && kForms[F].step == C::KW,
+                "form table");
+  static const hipError_t attr =
+      allow_lds(reinterpret_cast<const void*>(block_gemm_skinny_kernel<C>), C::LDS);
+  if (attr != hipSuccess)
+    return fail(FGS_ELAUNCH, std::string("block_gemm_skinny_kernel: ") + hipGetErrorString(attr));
+  const int64_t ny = (p.m + 16 * C::MT - 1) / (16 * C::MT);
+  if (ny > 65535) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  const dim3 grid(static_cast<unsigned>((p.n + 16 * C::NT - 1) / (16 * C::NT)),
+                  static_cast<unsigned>(ny));
+  hipLaunchKernelGGL((block_gemm_skinny_kernel<C>), grid, dim3(C::KW * 64), C::LDS, stream, p);
+  return check_launch("block_gemm_skinny_kernel");
+}
+
+template <int F, int OUT>
+int tiled_launch_out(const BlockGemmParams& p, hipStream_t stream) {
+  typedef typename FormCfg<F>::type C;
+  static_assert(kForms[F].bm == C::BM && kForms[F].bn == C::BN && kForms[F].step == 1, "form table");
+  static const hipError_t attr =
+      allow_lds(reinterpret_cast<const void*>(block_gemm_tiled_kernel<C, OUT>), C::LDS);
   if (attr != hipSuccess)
     return fail(FGS_ELAUNCH, std::string("block_gemm_tiled_kernel: ") + hipGetErrorString(attr));
   const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
-  const int64_t total = nm * nn * q.ksplit;
-  if (total > 0x7ffffff0) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  hipLaunchKernelGGL((block_gemm_tiled_kernel<C, OUT>), dim3(static_cast<unsigned>((total + 7) / 8 * 8)),
-                     dim3(C::NW * 64), C::LDS, stream, p, static_cast<int>(nm),
-                     static_cast<int>(nn), q.ksplit, q.band);
+  if (nm * nn > 0x7ffffff0 / kBand) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  hipLaunchKernelGGL((block_gemm_tiled_kernel<C, OUT>),
+                     dim3(static_cast<unsigned>((nm * nn + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS,
+                     stream, p, static_cast<int>(nm), static_cast<int>(nn));
   return check_launch("block_gemm_tiled_kernel");
 }
-
-template <class C>
-int tiled_launch(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
-  if (q.ksplit > 1) return tiled_launch_out<C, kOutPartial>(p, q, stream);
-  if (p.out_dtype == FGS_DTYPE_BF16) return tiled_launch_out<C, FGS_DTYPE_BF16>(p, q, stream);
-  return tiled_launch_out<C, FGS_DTYPE_FP16>(p, q, stream);
+template <int F>
+int tiled_launch(const BlockGemmParams& p, hipStream_t stream) {
+  return p.out_dtype == FGS_DTYPE_BF16 ? tiled_launch_out<F, FGS_DTYPE_BF16>(p, stream)
+                                       : tiled_launch_out<F, FGS_DTYPE_FP16>(p, stream);
 }
 
 }  // namespace
 
-bool block_gemm_flags_ok(int32_t flags) {
-  return flags >= 0 && (flags & 0xff) <= kStreamForms + kTiledForms && (flags >> 8) <= kMaxSplit;
-}
+bool block_gemm_flags_ok(int32_t flags) { return flags >= 0 && flags <= kNumForms; }
 
-BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags) {
-  BlockGemmPlan q{};
-  q.ksplit = 1;
-  q.band = 4;
-  const int kb = static_cast<int>((k + 127) / 128);
-  if (flags & 0xff) {
-    q.form = (flags & 0xff) - 1;
-  } else {
-    const int64_t big = (m + 255) / 256 * ((n + 255) / 256);
-    q.form = m <= 16 ? 0 : m <= 32 ? 1 : m <= 64 ? 2 : big >= 200 ? 3 : 6;
+// The form with the shortest estimate: rounds of the workgroups that run at
+// once, each its iterations. A form of more tokens than there are reads nothing
+// more for them, so tokens alone rule none out.
+int block_gemm_form(int64_t m, int64_t n, int64_t k, int32_t flags) {
+  if (flags) return flags - 1;
+  const double blocks = static_cast<double>((k + 127) / 128);
+  int best = 0;
+  double best_us = 0;
+  for (int f = 0; f < kNumForms; ++f) {
+    const Form& q = kForms[f];
+    const int64_t wgs = ((m + q.bm - 1) / q.bm) * ((n + q.bn - 1) / q.bn);
+    const int64_t rounds = (wgs + q.at_once - 1) / q.at_once;
+    const double iter = wgs <= q.at_once / 2 ? q.half : q.iter;
+    const double iters = std::ceil(blocks / q.step);
+    const double us = static_cast<double>(rounds) * (iters * iter + q.round);
+    if (f == 0 || us < best_us) {
+      best = f;
+      best_us = us;
+    }
   }
-  if (q.form >= kStreamForms && (flags >> 8)) q.ksplit = std::min(flags >> 8, kb);
-  return q;
+  return best;
 }
 
-int64_t block_gemm_workspace(const BlockGemmPlan& q, int64_t m, int64_t n) {
-  return q.ksplit > 1 ? q.ksplit * m * ((n + 3) / 4 * 4) * 4 : 0;
+std::string block_gemm_name(int form) {
+  const Form& q = kForms[form];
+  return (q.step > 1 ? "stream " : "tiled ") + std::to_string(q.bm) + "x" + std::to_string(q.bn) +
+         (form == 1 ? " deep" : "");
 }
 
-std::string block_gemm_name(const BlockGemmPlan& q) {
-  if (q.form < kStreamForms) return "stream tokens=" + std::to_string(16 << q.form);
-  const TiledForm& f = kTiled[q.form - kStreamForms];
-  return "tiled " + std::to_string(f.bm) + "x" + std::to_string(f.bn) +
-         (q.ksplit > 1 ? " ksplit=" + std::to_string(q.ksplit) : "");
-}
-
-int launch_block_gemm(const BlockGemmParams& p, const BlockGemmPlan& q, hipStream_t stream) {
-  int rc = FGS_OK;
-  switch (q.form) {
-    case 0: stream_launch<1>(p, stream); return check_launch("block_gemm_stream_kernel");
-    case 1: stream_launch<2>(p, stream); return check_launch("block_gemm_stream_kernel");
-    case 2: stream_launch<4>(p, stream); return check_launch("block_gemm_stream_kernel");
-    case 3: rc = tiled_launch<Cfg256>(p, q, stream); break;
-    case 4: rc = tiled_launch<Cfg128x256>(p, q, stream); break;
-    case 5: rc = tiled_launch<Cfg128>(p, q, stream); break;
-    default: rc = tiled_launch<Cfg64>(p, q, stream); break;
+int launch_block_gemm(const BlockGemmParams& p, int form, hipStream_t stream) {
+  switch (form) {
+    case 0: return skinny_launch<0>(p, stream);
+    case 1: return skinny_launch<1>(p, stream);
+    case 2: return skinny_launch<2>(p, stream);
+    case 3: return skinny_launch<3>(p, stream);
+    case 4: return skinny_launch<4>(p, stream);
+    case 5: return skinny_launch<5>(p, stream);
+    case 6: return tiled_launch<6>(p, stream);
+    case 7: return tiled_launch<7>(p, stream);
+    default: return tiled_launch<8>(p, stream);
   }
-  if (rc || q.ksplit == 1) return rc;
-  const dim3 grid(static_cast<unsigned>((p.n + 1023) / 1024), static_cast<unsigned>(p.m));
-  hipLaunchKernelGGL(block_gemm_sum_kernel, grid, dim3(256), 0, stream, p, q.ksplit);
-  return check_launch("block_gemm_sum_kernel");
 }
 
 }  // namespace fgs

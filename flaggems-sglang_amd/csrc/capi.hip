@@ -1498,17 +1498,12 @@ int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtyp
   return launch_gated_quant(p, dtype, as_stream(stream));
 }
 
-int64_t fgs_moe_fp8_block_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t flags) {
-  if (check_block_sizes(m, n, k, flags)) return -1;
-  return m == 0 ? 0 : block_gemm_workspace(block_gemm_plan(m, n, k, flags), m, n);
-}
-
 int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,
                                           char* buf, int32_t len) {
   int rc = check_block_sizes(m, n, k, flags);
   if (rc) return rc;
   if (!buf || len < 1) return fail(FGS_EINVAL, "buf must hold at least one byte");
-  const std::string s = m == 0 ? "none" : block_gemm_name(block_gemm_plan(m, n, k, flags));
+  const std::string s = m == 0 ? "none" : block_gemm_name(block_gemm_form(m, n, k, flags));
   const size_t used = std::min(s.size(), static_cast<size_t>(len - 1));
   memcpy(buf, s.data(), used);
   buf[used] = 0;
@@ -1519,8 +1514,8 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
                                  int64_t as_row_stride, int64_t as_col_stride, const void* w,
                                  int64_t ldw, const float* w_scale, const void* bias,
                                  int32_t bias_dtype, int64_t m, int64_t n, int64_t k,
-                                 int32_t out_dtype, int32_t flags, void* workspace,
-                                 int64_t ws_bytes, void* out, int64_t ldo, void* stream) {
+                                 int32_t out_dtype, int32_t flags, void* out, int64_t ldo,
+                                 void* stream) {
   int rc = check_block_sizes(m, n, k, flags);
   if (rc) return rc;
   for (int t : {out_dtype, bias ? bias_dtype : out_dtype})
@@ -1541,12 +1536,6 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
       reinterpret_cast<uintptr_t>(out) % 2 ||
       reinterpret_cast<uintptr_t>(bias) % (bias_dtype == FGS_DTYPE_FP32 ? 4 : 2))
     return fail(FGS_EINVAL, "tensors must be aligned to their elements");
-  const BlockGemmPlan plan = block_gemm_plan(m, n, k, flags);
-  const int64_t need = block_gemm_workspace(plan, m, n);
-  if (need > 0 && (!workspace || ws_bytes < need))
-    return fail(FGS_EINVAL, "workspace too small: need " + std::to_string(need) + " bytes");
-  if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 256)
-    return fail(FGS_EINVAL, "workspace must be 256-byte aligned");
   BlockGemmParams p{};
   p.a = static_cast<const uint8_t*>(a);
   p.a_scale = a_scale;
@@ -1554,8 +1543,6 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
   p.w_scale = w_scale;
   p.bias = bias;
   p.out = out;
-  p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
-  p.part_ld = (n + 3) / 4 * 4;
   p.m = m;
   p.n = n;
   p.k = k;
@@ -1567,7 +1554,7 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
   p.out_dtype = out_dtype;
   p.bias_dtype = bias_dtype;
   p.kblocks = static_cast<int32_t>((k + 127) / 128);
-  return launch_block_gemm(p, plan, as_stream(stream));
+  return launch_block_gemm(p, block_gemm_form(m, n, k, flags), as_stream(stream));
 }
 
 }  // extern "C"

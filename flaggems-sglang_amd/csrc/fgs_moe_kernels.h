@@ -255,22 +255,15 @@ struct BlockGemmParams {
   int64_t as_row, as_col; // strides of a_scale over rows / k blocks
   int32_t out_dtype, bias_dtype;
   int32_t kblocks;
-  float* part;            // workspace: fp32 sums [k splits][m][part_ld], part_ld =
-  int64_t part_ld;        // n rounded up to 4
 };
 // Sizes and row strides the kernels' 32-bit offsets inside a tile allow.
 constexpr int64_t kBlockMaxM = 1 << 22, kBlockMaxN = 1 << 22, kBlockMaxK = 1 << 22;
 constexpr int64_t kBlockMaxScaleStride = 1 << 20;
-// The kernel a product of these sizes runs (`flags` 0, or FGS_BLOCK_*).
-struct BlockGemmPlan {
-  int form;
-  int ksplit;  // tiled: k splits, summed by a second kernel
-  int band;    // tiled: token tiles of a raster band
-};
-BlockGemmPlan block_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t flags);
+// The form of the kernel a product of these sizes runs (`flags` 0, or
+// FGS_BLOCK_FORM), its description, and the launch.
 bool block_gemm_flags_ok(int32_t flags);
-int64_t block_gemm_workspace(const BlockGemmPlan& plan, int64_t m, int64_t n);
-std::string block_gemm_name(const BlockGemmPlan& plan);
-int launch_block_gemm(const BlockGemmParams& p, const BlockGemmPlan& plan, hipStream_t stream);
+int block_gemm_form(int64_t m, int64_t n, int64_t k, int32_t flags);
+std::string block_gemm_name(int form);
+int launch_block_gemm(const BlockGemmParams& p, int form, hipStream_t stream);
 
 }  // namespace fgs

@@ -152,10 +152,8 @@ SIGNATURES = {
     "fgs_moe_fp8_block_matmul": (
         _i32,
         [_c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p,
-         _i32, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i64, _c_void_p, _i64,
-         _c_void_p],
+         _i32, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i64, _c_void_p],
     ),
-    "fgs_moe_fp8_block_matmul_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "fgs_moe_fp8_block_matmul_schedule": (_i32, [_i64, _i64, _i64, _i32, _c_void_p, _i32]),
     "fgs_moe_profile_enable": (_i32, [_i32]),
     "fgs_moe_profile_read": (_i32, [_c_void_p, _i32]),

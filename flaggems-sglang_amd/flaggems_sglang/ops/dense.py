@@ -320,16 +320,10 @@ def fp8_block_matmul(
     if not given:
         out = a_scale.new_empty(lead + (n,), dtype=out_dtype)
     ldo = out.stride(0) if given and out.ndim == 2 else n
-    lib = _capi.load()
-    ws_ptr = None
-    ws_bytes = lib.fgs_moe_fp8_block_matmul_workspace_bytes(m, n, k, _flags)
-    if ws_bytes > 0:
-        ws = a_scale.new_empty(ws_bytes, dtype=torch.uint8)
-        ws_ptr = ws.data_ptr()
-    _call(index, "fp8_block_matmul", lib.fgs_moe_fp8_block_matmul,
+    _call(index, "fp8_block_matmul", _capi.load().fgs_moe_fp8_block_matmul,
           a.data_ptr(), lda, a_scale.data_ptr(), as_row, as_col, w.data_ptr(), ldw,
           w_scale.data_ptr(), bias_ptr, bias_type, m, n, k, _DTYPES[out_dtype], _flags,
-          ws_ptr, ws_bytes, out.data_ptr(), ldo, _stream_ptr(a))
+          out.data_ptr(), ldo, _stream_ptr(a))
     if given:
         _written(out)
     return out

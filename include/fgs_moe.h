@@ -443,18 +443,16 @@ int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtyp
  * The matrix instruction cuts each of eight neighbouring products 13 bits
  * below the largest one: about 1.5e-5 of a result from normal data.
  * k a positive multiple of 16, m, n and k up to 2^22; a and w rows 16-byte
- * aligned and at most 2^22 apart, a_scale rows at most 2^20. `flags`: 0, or a schedule to use (FGS_BLOCK_*, below).
- * workspace: fgs_moe_fp8_block_matmul_workspace_bytes() bytes, 256-byte
- * aligned (may be null where that is 0). */
+ * aligned and at most 2^22 apart, a_scale rows at most 2^20. `flags`: 0, or
+ * FGS_BLOCK_FORM(f), the kernel form f whatever the sizes (for measurement
+ * and tests). No workspace. */
+#define FGS_BLOCK_FORM(f) ((f) + 1)
 int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scale,
                                  int64_t as_row_stride, int64_t as_col_stride, const void* w,
                                  int64_t ldw, const float* w_scale, const void* bias,
                                  int32_t bias_dtype, int64_t m, int64_t n, int64_t k,
-                                 int32_t out_dtype, int32_t flags, void* workspace,
-                                 int64_t ws_bytes, void* out, int64_t ldo, void* stream);
-#define FGS_BLOCK_FORM(f) ((f) + 1)    /* kernel form f, for measurement and tests */
-#define FGS_BLOCK_KSPLIT(s) ((s) << 8) /* ... in s (at most 8) k splits */
-int64_t fgs_moe_fp8_block_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t flags);
+                                 int32_t out_dtype, int32_t flags, void* out, int64_t ldo,
+                                 void* stream);
 /* The schedule such a call runs, as text (as fgs_moe_schedule). */
 int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,
                                           char* buf, int32_t len);

@@ -77,8 +77,7 @@ def test_activation_refusals(kw, rc, text):
 
 def _product(**kw):
     a = dict(a=P, lda=256, a_scale=P, as_row=2, as_col=1, w=P, ldw=256, w_scale=P, bias=None,
-             bias_dtype=0, m=4, n=512, k=256, out_dtype=0, flags=0, ws=P, ws_bytes=1 << 40,
-             out=P, ldo=512)
+             bias_dtype=0, m=4, n=512, k=256, out_dtype=0, flags=0, out=P, ldo=512)
     a.update(kw)
     rc = _capi.load().fgs_moe_fp8_block_matmul(*a.values(), None)
     return rc, _capi.last_error()
@@ -125,10 +124,21 @@ def test_schedule_text():
     buf = ctypes.create_string_buffer(5)
     assert lib.fgs_moe_fp8_block_matmul_schedule(1, 4096, 7168, 0, buf, 5) == 0
     assert buf.value == b"stre"
-    assert lib.fgs_moe_fp8_block_matmul_workspace_bytes(1, 4096, 100, 0) == -1
-    assert lib.fgs_moe_fp8_block_matmul_workspace_bytes(0, 4096, 7168, 0) == 0
     with pytest.raises(NotImplementedError):
         _capi.block_matmul_schedule(1, 1, 8)
+
+
+@pytest.mark.parametrize("m,n,k,schedule", [
+    (0, 4096, 7168, "none"), (1, 16384, 7168, "stream 16x16"),
+    (16, 4096, 7168, "stream 16x16 deep"), (64, 4096, 7168, "stream 32x32"),
+    (128, 4096, 7168, "stream 64x32"), (256, 4096, 7168, "stream 64x64"),
+    (512, 4096, 7168, "tiled 64x128"), (2048, 4096, 7168, "tiled 128x128"),
+    (4096, 4096, 7168, "tiled 256x256"), (8192, 14336, 7168, "tiled 256x256"),
+])
+def test_schedules(m, n, k, schedule):
+    """The tile of a product by the sizes' estimate (the shapes the estimate
+    was measured on)."""
+    assert _capi.block_matmul_schedule(m, n, k) == schedule
 
 
 def test_cpu_tensors_are_refused():
