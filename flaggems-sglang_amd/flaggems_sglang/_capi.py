@@ -196,6 +196,33 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The extension module of the dense operators' host side (``_host``,
+    csrc/host_ext.cpp), bound (once) to the loaded library."""
+    global _host
+    if _host is None:
+        lib = load()
+        with _lock:
+            if _host is None:
+                import torch  # noqa: F401  (its libraries, which the module links to)
+                try:
+                    from flaggems_sglang import _host as module
+                except ImportError as e:
+                    raise RuntimeError(
+                        f"flaggems_sglang._host did not load ({e}); build it with "
+                        "`make -C flaggems-sglang_amd/csrc` (or __graft_entry__.build())"
+                    ) from e
+                module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                              for name in ("fgs_moe_last_error", "fgs_moe_rms_norm",
+                                           "fgs_moe_silu_and_mul_quant",
+                                           "fgs_moe_fp8_block_matmul")))
+                _host = module
+    return _host
+
+
 def last_error() -> str:
     return load().fgs_moe_last_error().decode()
 
