@@ -329,10 +329,10 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
 
   const int KT = p.kblocks;
 
-  // The resources start at stage kt's columns and end with the tile's last
-  // row: what a lane would read past that (the last block's chunks past k of
-  // the last row) is not accessed.
-  auto issue = [&](int kt) {
+  // Loads [from, to) of stage kt. The resources start at its columns and end
+  // with the tile's last row: what a lane would read past that (the last
+  // block's chunks past k of the last row) is not accessed.
+  auto issue = [&](int kt, int from, int to) {
     uint8_t* base = lds + (kt % STAGES) * C::STAGE;
     const int64_t koff = static_cast<int64_t>(kt) * 128;
     const uint32_t left = static_cast<uint32_t>(static_cast<int>(p.k) - kt * 128);
@@ -342,15 +342,19 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(p.w) + n0 * p.ldw + koff, 0, static_cast<int>(wm_last * ldw + left),
         kBufWord3);
-#pragma unroll
-    for (int i = 0; i < C::NLA; ++i)
-      lds_dma16_buf(ra, aoff[i], 0, base + (wave * C::NLA + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < C::NLW; ++i)
-      lds_dma16_buf(rw, woff[i], 0, base + C::A_BYTES + (wave * C::NLW + i) * 1024);
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<float*>(sc_base) + kt * sc_step, 0, 0x7fffffff, kBufWord3);
-    lds_dma4_buf(rs, sc_off, base + C::SC_OFF + wave * 256);
+#pragma unroll
+    for (int i = 0; i < C::NL; ++i) {
+      if (i < from || i >= to) continue;
+      if (i < C::NLA)
+        lds_dma16_buf(ra, aoff[i], 0, base + (wave * C::NLA + i) * 1024);
+      else if (i < C::NLA + C::NLW)
+        lds_dma16_buf(rw, woff[i - C::NLA], 0,
+                      base + C::A_BYTES + (wave * C::NLW + i - C::NLA) * 1024);
+      else
+        lds_dma4_buf(rs, sc_off, base + C::SC_OFF + wave * 256);
+    }
   };
   // Stage kt (this wave's loads of it done): where it is the row's last block
   // and k ends inside it, the chunks past k that this wave loaded become 0.
@@ -395,7 +399,7 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s)
-    if (s < KT) issue(s);
+    if (s < KT) issue(s, 0, C::NL);
   if (KT >= STAGES) wait_vmcnt<(STAGES - 1) * C::NL>();
   else wait_vmcnt<0>();
   if (KT == 1) end_of_k(0);
@@ -406,6 +410,7 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   // the scales of the stage before).
   constexpr int TILES = CT * RT, LAG = 3;
   static_assert(TILES > LAG && RT >= 2, "pipeline");
+  static_assert(C::NL - RT <= (CT - 1) * RT && RT <= C::NL, "a refill ends before the next barrier");
   i32x8 x[RT], w[2];
   float s[RT], sp[RT];
   f32x4 part[LAG + 1];
@@ -443,10 +448,14 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   // slot is free once every wave has it; the next stage's first fragments
   // replace each token tile's as its last MFMA has been issued.
   // REST: the stages behind this one, as far as it matters (STAGES: a refill
-  // of the slot among them). The loop's body has no branch: code behind one
-  // would draw the MFMAs before it in.
-  auto stage = [&](int kt, auto rest_c) {
+  // of its slot among them; STAGES - 1 and not FIRST: the rest of the refill
+  // that the stage before has begun). The loop's body has no branch: code
+  // behind one would draw the MFMAs before it in. A refill's loads go out one a
+  // tile: all at once, the eight waves' 72 stood before the address unit (16
+  // cycles each) and held every MFMA behind them: 8192^3 450 -> 415 us.
+  auto stage = [&](int kt, auto rest_c, auto first_c) {
     constexpr int REST = decltype(rest_c)::value;
+    constexpr bool FIRST = decltype(first_c)::value;
     constexpr bool MORE = REST > 0;
     constexpr int L = CT - 1;
     const uint8_t* st = lds + (kt % STAGES) * C::STAGE;
@@ -465,12 +474,19 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
             end_of_k(kt + 1);
           }
           wave_barrier_all();
-          if constexpr (REST == STAGES) issue(kt + STAGES);
         }
       }
       part[j & LAG] = mfma16_fp8(w[i & 1], x[t], zero);
       if (j >= LAG) fold(j - LAG, s);
       else fold(TILES + j - LAG, sp);
+      // refills, a load a tile: RT of them behind the barrier, the others at the
+      // next stage's start
+      if constexpr (REST == STAGES) {
+        if (i == L) issue(kt + STAGES, t, t + 1);
+      }
+      if constexpr (REST >= STAGES - 1 && !FIRST) {
+        if (j + RT < C::NL) issue(kt + STAGES - 1, j + RT, j + RT + 1);
+      }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (MORE) {
         if (i == L) {
@@ -489,15 +505,21 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   };
   // (so that the loop's own reads are all there is to count at its head)
   wait_lgkm0();
-  for (int kt = 0; kt + STAGES < KT; ++kt) stage(kt, std::integral_constant<int, STAGES>{});
-  if constexpr (STAGES > 3) {
-    if (KT > 3) stage(KT - 4, std::integral_constant<int, 3>{});
+  const std::false_type later{};
+  int kt = 0;
+  if (kt + STAGES < KT) {
+    stage(kt, std::integral_constant<int, STAGES>{}, std::true_type{});
+    ++kt;
+    for (; kt + STAGES < KT; ++kt) stage(kt, std::integral_constant<int, STAGES>{}, later);
+    // (the refill of the last stage goes on)
+    stage(KT - STAGES, std::integral_constant<int, STAGES - 1>{}, later);
+  } else if (KT >= STAGES) {
+    stage(0, std::integral_constant<int, STAGES - 1>{}, std::true_type{});
   }
   if constexpr (STAGES > 2) {
-    if (KT > 2) stage(KT - 3, std::integral_constant<int, 2>{});
+    if (KT > 1) stage(KT - 2, std::integral_constant<int, 1>{}, std::true_type{});
   }
-  if (KT > 1) stage(KT - 2, std::integral_constant<int, 1>{});
-  stage(KT - 1, std::integral_constant<int, 0>{});
+  stage(KT - 1, std::integral_constant<int, 0>{}, std::true_type{});
 #pragma unroll
   for (int j = TILES - LAG; j < TILES; ++j) fold(j, sp);
   // Matrix instructions write every lane, whatever EXEC holds: the last stage's
@@ -573,8 +595,8 @@ constexpr Form kForms[] = {
     {16, 16, 8, 512, 1.1, 0.85, 0.5},    {16, 16, 8, 256, 0.75, 0.95, 0.5},
     {32, 16, 8, 256, 1.05, 0.95, 0.5},   {32, 32, 8, 256, 1.1, 1.1, 0.8},
     {64, 32, 4, 256, 0.9, 0.9, 1.0},     {64, 64, 4, 256, 1.13, 1.13, 1.4},
-    {64, 128, 1, 512, 0.69, 0.47, 1.8},  {128, 128, 1, 512, 1.04, 0.85, 3.0},
-    {256, 256, 1, 256, 1.8, 1.5, 6.5},
+    {64, 128, 1, 512, 0.65, 0.45, 1.8},  {128, 128, 1, 512, 0.98, 0.80, 3.0},
+    {256, 256, 1, 256, 1.55, 1.35, 6.5},
 };
 constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
 
