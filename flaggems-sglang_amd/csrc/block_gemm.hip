@@ -27,11 +27,26 @@ namespace fgs {
 // ---------------------------------------------------------------- output ---
 // Four neighbouring output columns n .. n + 3 of token m (`left`: columns of
 // them that exist; vec: the row start and n allow one 8-byte store).
-__device__ __forceinline__ float bias_at(const BlockGemmParams& p, int64_t n) {
-  if (p.bias_dtype == FGS_DTYPE_FP32) return static_cast<const float*>(p.bias)[n];
-  const uint16_t b = static_cast<const uint16_t*>(p.bias)[n];
-  return p.bias_dtype == FGS_DTYPE_BF16 ? Elem<FGS_DTYPE_BF16>::to_f32(b)
-                                        : Elem<FGS_DTYPE_FP16>::to_f32(b);
+// The bias of output column n in two steps, so that what lies between covers
+// the load: its bits (columns past the end: the last one's; without a bias 0),
+// then their value. The kernels load the bits before their first load into LDS
+// and count on that order where they wait for those. (Loaded at the end, the
+// bias cost 0.4 to 1.6 us: 333 x 2112 x 1552, 64 x 64 tiles, 9.6 and 11.2.)
+__device__ __forceinline__ uint32_t bias_bits(const BlockGemmParams& p, int64_t n) {
+  uint32_t bits = 0;
+  if (p.bias) {
+    n = min(n, p.n - 1);
+    bits = p.bias_dtype == FGS_DTYPE_FP32 ? static_cast<const uint32_t*>(p.bias)[n]
+                                          : static_cast<const uint16_t*>(p.bias)[n];
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  return bits;
+}
+__device__ __forceinline__ float bias_value(const BlockGemmParams& p, uint32_t bits) {
+  if (p.bias_dtype == FGS_DTYPE_FP32) return __uint_as_float(bits);
+  return p.bias_dtype == FGS_DTYPE_BF16 ? Elem<FGS_DTYPE_BF16>::to_f32(bits)
+                                        : Elem<FGS_DTYPE_FP16>::to_f32(bits);
 }
 template <int TY>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -50,15 +65,10 @@ __device__ __forceinline__ void store4(void* out, int64_t at, f32x4 v, int64_t l
   for (int i = 0; i < 4; ++i)
     if (i < left) o[i] = Elem<TY>::from_f32(v[i]);
 }
-// out[m, n .. n + 3] = v + bias in the output's type.
+// out[m, n .. n + 3] = v in the output's type.
 __device__ __forceinline__ void write_out(const BlockGemmParams& p, int64_t m, int64_t n, f32x4 v,
                                           bool vec) {
   const int64_t left = p.n - n;
-  if (p.bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) v[i] += bias_at(p, n + i);
-  }
   const int64_t at = m * p.ldo + n;
   if (p.out_dtype == FGS_DTYPE_BF16) store4<FGS_DTYPE_BF16>(p.out, at, v, left, vec);
   else store4<FGS_DTYPE_FP16>(p.out, at, v, left, vec);
@@ -78,6 +88,15 @@ __device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, uint32
 // 16 rows that lanes 0-15 read at one chunk over all 16 positions.
 __device__ __forceinline__ int swizzled(int r, int c) { return c ^ ((r >> 1) & 7); }
 
+// Workgroup i of a grid runs on XCD i % 8. Its place in an order that gives each
+// XCD a contiguous eighth of `total`, so that neighbours share an L2. (The grid
+// has no workgroup too many: a check for one, which stands before the other
+// arguments are loaded, cost 0.3 us a call.)
+__device__ __forceinline__ int xcd_order(int i, int total) {
+  const int xcd = i & 7;
+  return xcd * (total >> 3) + min(xcd, total & 7) + (i >> 3);
+}
+
 // ------------------------------------------------------------- few tokens ---
 // A workgroup owns 16 MT tokens x 16 NT weight rows; its KW waves split the k
 // blocks into contiguous runs and meet in LDS at the end, added in wave order.
@@ -95,18 +114,28 @@ struct SkinnyCfg {
   static constexpr int NL = 2 * (MT + NT) + 2;
   static constexpr int LDS = KW * SLOTS * SLOT;
   static_assert(MT <= 4 && 128 % (16 * NT) == 0, "one scale a lane, one weight block");
-  static_assert(SLOTS >= 2 && SLOTS <= 4 && (SLOTS - 1) * NL < 64 && LDS <= 160 * 1024, "ring");
+  static_assert(SLOTS >= 2 && SLOTS <= 4 && (SLOTS - 1) * NL < 64 && LDS + 64 * NT <= 160 * 1024,
+                "ring");
   static_assert(KW * MT * NT * 1024 <= LDS, "partial sums");
 };
 
 template <class C>
-__global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const BlockGemmParams p) {
+__global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const BlockGemmParams p,
+                                                                       int nm, int total) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  __shared__ __attribute__((aligned(16))) float bias[16 * C::NT];
   constexpr int MT = C::MT, NT = C::NT, SLOTS = C::SLOTS;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16 * NT;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  // column by column, so that the tiles that read the same weight rows share an
+  // L2: 333 x 2112 x 1552 (64 x 64 tiles) 8.4 us, 9.5 row by row; one row of
+  // tiles, 1 x 4096 x 7168, 7.35, 7.25 without the division
+  const int at = xcd_order(blockIdx.x, total);
+  const int tn = __builtin_amdgcn_readfirstlane(at / nm), tm = at - tn * nm;
+  const int64_t n0 = static_cast<int64_t>(tn) * 16 * NT;
+  const int64_t m0 = static_cast<int64_t>(tm) * 16 * MT;
+  static_assert(16 * NT <= 64, "the first wave has the bias");
+  const uint32_t my_bias = wave == 0 ? bias_bits(p, n0 + lane) : 0;
   const int per = (p.kblocks + C::KW - 1) / C::KW;
   const int kb0 = min(wave * per, p.kblocks);
   const int count = min(per, p.kblocks - kb0);
@@ -222,6 +251,7 @@ __global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const Blo
   }
 
   __syncthreads();  // the rings are done with
+  if (threadIdx.x < 16 * NT) bias[threadIdx.x] = bias_value(p, my_bias);
   f32x4* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
   for (int j = 0; j < NT; ++j)
@@ -236,6 +266,7 @@ __global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const Blo
     const int tile = i >> 6, l = i & 63;
     const int64_t m = m0 + (tile % MT) * 16 + (l & 15);
     const int64_t n = n0 + (tile / MT) * 16 + 4 * (l >> 4);
+    v += *reinterpret_cast<const f32x4*>(bias + (tile / MT) * 16 + 4 * (l >> 4));
     if (m < p.m && n < p.n) write_out(p, m, n, v, vec);
   }
 }
@@ -262,19 +293,15 @@ struct BlockCfg {
   static_assert(128 % (CT * 16) == 0, "a wave's weight rows lie in one scale block");
   static_assert(BN % 128 == 0 || 128 % BN == 0, "scale blocks of a tile");
   static_assert(BM + (BN + 127) / 128 <= NW * 64, "scale slots");
-  static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * NL < 64 && LDS <= 160 * 1024, "ring");
+  static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * NL < 64 && LDS + 4 * BN <= 160 * 1024,
+                "ring");
   static_assert(CT % 2 == 0, "fragment pipeline");
 };
 
-// Workgroup bid runs on XCD bid % 8, which takes the bid / 8-th tile of its
-// contiguous eighth; tiles go in bands of kBand token tiles walked column by
-// column, so an XCD's 32 CUs share a few rows' and columns' operands in its L2.
+// Tiles go in bands of kBand token tiles walked column by column, so an XCD's 32
+// CUs share a few rows' and columns' operands in its L2.
 constexpr int kBand = 4;
-__device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int* tm, int* tn) {
-  const int total = nm * nn;
-  const int per = (total + 7) / 8;
-  const int at = (bid % 8) * per + bid / 8;
-  if (bid / 8 >= per || at >= total) return false;
+__device__ __forceinline__ void block_tile(int at, int nm, int nn, int* tm, int* tn) {
   const int b = at / (kBand * nn);
   const int rem = at - b * kBand * nn;
   const int rows = min(kBand, nm - b * kBand);
@@ -282,7 +309,6 @@ __device__ __forceinline__ bool block_tile(int bid, int nm, int nn, int* tm, int
   // buffer resources that follow from them are scalar too)
   *tn = __builtin_amdgcn_readfirstlane(rem / rows);
   *tm = __builtin_amdgcn_readfirstlane(b * kBand + rem % rows);
-  return true;
 }
 
 // OUT: the output's type.
@@ -290,14 +316,18 @@ template <class C, int OUT>
 __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
     const BlockGemmParams p, int nm, int nn) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  __shared__ __attribute__((aligned(16))) float tile_biases[C::BN];
   constexpr int RT = C::RT, CT = C::CT, STAGES = C::STAGES;
   int tm, tn;
-  if (!block_tile(blockIdx.x, nm, nn, &tm, &tn)) return;
+  block_tile(xcd_order(blockIdx.x, nm * nn), nm, nn, &tm, &tn);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int64_t m0 = static_cast<int64_t>(tm) * C::BM;
   const int64_t n0 = static_cast<int64_t>(tn) * C::BN;
+
+  static_assert(C::BN <= C::NW * 64 && C::BN % 64 == 0, "a bias a thread");
+  const uint32_t my_bias = wave < C::BN / 64 ? bias_bits(p, n0 + threadIdx.x) : 0;
 
   // this lane's source of each load: row lane / 8, chunk lane % 8, as byte
   // offsets from the tile's first row (rows past the end read the last one;
@@ -535,16 +565,13 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   constexpr int CH = CT * 2;                 // chunks of a row
   constexpr int ROWS = 64 / CH;              // rows a store instruction covers
   static_assert(RT * 16 * CH * 16 <= C::LDS / C::NW && 64 % CH == 0, "staging area");
-  wave_barrier_all();  // every wave has read its last fragments
+  if (threadIdx.x < C::BN) tile_biases[threadIdx.x] = bias_value(p, my_bias);
+  __syncthreads();  // and every wave has read its last fragments
   uint8_t* stg = lds + wave * (RT * 16 * CH * 16);
 #pragma unroll
   for (int i = 0; i < CT; ++i) {
-    const int64_t n = n0 + (wn * CT + i) * 16 + 4 * g;
-    f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) bias[v] = bias_at(p, min<int64_t>(n + v, p.n - 1));
-    }
+    const f32x4 bias =
+        *reinterpret_cast<const f32x4*>(tile_biases + (wn * CT + i) * 16 + 4 * g);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const f32x4 v = acc[i][t] + bias;
@@ -626,11 +653,12 @@ int skinny_launch(const BlockGemmParams& p, hipStream_t stream) {
       allow_lds(reinterpret_cast<const void*>(block_gemm_skinny_kernel<C>), C::LDS);
   if (attr != hipSuccess)
     return fail(FGS_ELAUNCH, std::string("block_gemm_skinny_kernel: ") + hipGetErrorString(attr));
-  const int64_t ny = (p.m + 16 * C::MT - 1) / (16 * C::MT);
-  if (ny > 65535) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  const dim3 grid(static_cast<unsigned>((p.n + 16 * C::NT - 1) / (16 * C::NT)),
-                  static_cast<unsigned>(ny));
-  hipLaunchKernelGGL((block_gemm_skinny_kernel<C>), grid, dim3(C::KW * 64), C::LDS, stream, p);
+  const int64_t nn = (p.n + 16 * C::NT - 1) / (16 * C::NT);
+  const int64_t nm = (p.m + 16 * C::MT - 1) / (16 * C::MT);
+  if (nm * nn > 0x7ffffff0) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  hipLaunchKernelGGL((block_gemm_skinny_kernel<C>), dim3(static_cast<unsigned>(nm * nn)),
+                     dim3(C::KW * 64), C::LDS, stream, p, static_cast<int>(nm),
+                     static_cast<int>(nm * nn));
   return check_launch("block_gemm_skinny_kernel");
 }
 
@@ -643,10 +671,11 @@ int tiled_launch_out(const BlockGemmParams& p, hipStream_t stream) {
   if (attr != hipSuccess)
     return fail(FGS_ELAUNCH, std::string("block_gemm_tiled_kernel: ") + hipGetErrorString(attr));
   const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
-  if (nm * nn > 0x7ffffff0 / kBand) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  if (nm * nn > 0x7fffffff / (2 * kBand))
+    return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
   hipLaunchKernelGGL((block_gemm_tiled_kernel<C, OUT>),
-                     dim3(static_cast<unsigned>((nm * nn + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS,
-                     stream, p, static_cast<int>(nm), static_cast<int>(nn));
+                     dim3(static_cast<unsigned>(nm * nn)), dim3(C::NW * 64), C::LDS, stream, p,
+                     static_cast<int>(nm), static_cast<int>(nn));
   return check_launch("block_gemm_tiled_kernel");
 }
 template <int F>

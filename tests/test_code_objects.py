@@ -2,6 +2,7 @@
 schedule keeps registers in scratch memory, and the quantisers' divisions."""
 
 import os
+import re
 import shutil
 import struct
 import subprocess
@@ -111,4 +112,22 @@ def test_products_are_done_before_lanes_branch(tmp_path):
                 continue
             seen += 1
             assert code.rindex("v_mfma") < code.index("global_store"), n
+    assert seen >= 4
+
+
+def test_loads_into_lds_come_last(tmp_path):
+    """The block-scaled kernels wait for loads into LDS by how many later ones
+    are in flight, so no other load may be issued behind the first of them."""
+    seen = 0
+    for obj in _objects(LIB, str(tmp_path)):
+        for n in (n for n, _ in _kernels(obj) if "block_gemm" in n):
+            code = _tool("llvm-objdump", "-d", f"--disassemble-symbols={n}", obj).splitlines()
+            loads = [i for i, x in enumerate(code)
+                     if re.search(r"\b(global|flat|buffer|scratch)_(load|atomic)", x)]
+            into = [i for i in loads if re.search(r"\blds\b", code[i])]
+            if not into:
+                continue
+            seen += 1
+            assert [i for i in loads if i not in into and i > into[0]] == [], n
+            assert len(into) < len(loads), n  # (the bias)
     assert seen >= 4
