@@ -16,6 +16,7 @@
 // at any k, against 3e-2 from the operands' own rounding; outputs are therefore
 // 16-bit types, whose step hides it.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -639,9 +640,24 @@ template <> struct FormCfg<6> { typedef BlockCfg<64, 128, 2, 2, 3, 2> type; };
 template <> struct FormCfg<7> { typedef BlockCfg<128, 128, 2, 2, 2, 2> type; };
 template <> struct FormCfg<8> { typedef BlockCfg<256, 256, 4, 2, 2, 2> type; };
 
-// Lets a kernel use more than 64 KiB of LDS, once.
-hipError_t allow_lds(const void* kernel, int bytes) {
-  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Launches `kernel` with more than 64 KiB of LDS, which each GPU has to be told
+// of once (`told`: a bit a GPU).
+template <class... P, class... A>
+int launch_wide_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told, int64_t wgs,
+                    int threads, int lds, hipStream_t stream, A... args) {
+  // (the runtime counts a grid in 32-bit threads)
+  if (wgs * threads > 0xffffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  int gpu = 0;
+  hipError_t e = hipGetDevice(&gpu);
+  const uint64_t bit = uint64_t{1} << (gpu & 63);
+  if (e == hipSuccess && (gpu > 63 || !(told.load(std::memory_order_relaxed) & bit))) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess && gpu <= 63) told.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != hipSuccess) return fail(FGS_ELAUNCH, std::string(name) + ": " + hipGetErrorString(e));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), lds, stream, args...);
+  return check_launch(name);
 }
 
 template <int F>
@@ -649,34 +665,23 @@ int skinny_launch(const BlockGemmParams& p, hipStream_t stream) {
   typedef typename FormCfg<F>::type C;
   static_assert(kForms[F].bm == 16 * C::MT && kForms[F].bn == 16 * C::NT && kForms[F].step == C::KW,
                 "form table");
-  static const hipError_t attr =
-      allow_lds(reinterpret_cast<const void*>(block_gemm_skinny_kernel<C>), C::LDS);
-  if (attr != hipSuccess)
-    return fail(FGS_ELAUNCH, std::string("block_gemm_skinny_kernel: ") + hipGetErrorString(attr));
-  const int64_t nn = (p.n + 16 * C::NT - 1) / (16 * C::NT);
+  static std::atomic<uint64_t> told{0};
   const int64_t nm = (p.m + 16 * C::MT - 1) / (16 * C::MT);
-  if (nm * nn > 0x7ffffff0) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  hipLaunchKernelGGL((block_gemm_skinny_kernel<C>), dim3(static_cast<unsigned>(nm * nn)),
-                     dim3(C::KW * 64), C::LDS, stream, p, static_cast<int>(nm),
-                     static_cast<int>(nm * nn));
-  return check_launch("block_gemm_skinny_kernel");
+  const int64_t nn = (p.n + 16 * C::NT - 1) / (16 * C::NT);
+  return launch_wide_lds("block_gemm_skinny_kernel", block_gemm_skinny_kernel<C>, told, nm * nn,
+                         C::KW * 64, C::LDS, stream, p, static_cast<int>(nm),
+                         static_cast<int>(nm * nn));
 }
 
 template <int F, int OUT>
 int tiled_launch_out(const BlockGemmParams& p, hipStream_t stream) {
   typedef typename FormCfg<F>::type C;
   static_assert(kForms[F].bm == C::BM && kForms[F].bn == C::BN && kForms[F].step == 1, "form table");
-  static const hipError_t attr =
-      allow_lds(reinterpret_cast<const void*>(block_gemm_tiled_kernel<C, OUT>), C::LDS);
-  if (attr != hipSuccess)
-    return fail(FGS_ELAUNCH, std::string("block_gemm_tiled_kernel: ") + hipGetErrorString(attr));
+  static std::atomic<uint64_t> told{0};
   const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
-  if (nm * nn > 0x7fffffff / (2 * kBand))
-    return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  hipLaunchKernelGGL((block_gemm_tiled_kernel<C, OUT>),
-                     dim3(static_cast<unsigned>(nm * nn)), dim3(C::NW * 64), C::LDS, stream, p,
-                     static_cast<int>(nm), static_cast<int>(nn));
-  return check_launch("block_gemm_tiled_kernel");
+  return launch_wide_lds("block_gemm_tiled_kernel", block_gemm_tiled_kernel<C, OUT>, told, nm * nn,
+                         C::NW * 64, C::LDS, stream, p, static_cast<int>(nm),
+                         static_cast<int>(nn));
 }
 template <int F>
 int tiled_launch(const BlockGemmParams& p, hipStream_t stream) {

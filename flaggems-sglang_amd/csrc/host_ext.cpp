@@ -62,7 +62,8 @@ Arg tensor_arg(PyObject* o, const char* name, bool optional = false) {
   return {name, &THPVariable_Unpack(o)};
 }
 
-// Every tensor given is on one GPU and needs no gradient; that GPU's index.
+// Every tensor given is on one GPU, holds its values and needs no gradient; that
+// GPU's index.
 int check_inputs(std::initializer_list<Arg> args) {
   const at::Tensor* first = args.begin()->t;
   if (!first->is_cuda())
@@ -75,6 +76,8 @@ int check_inputs(std::initializer_list<Arg> args) {
     if (a.t->device() != first->device())
       refuse(PyExc_RuntimeError, std::string(a.name) + " is on " + a.t->device().str() +
                                      ", not on " + first->device().str());
+    if (a.t->is_neg())  // (its memory holds the values' negatives)
+      refuse(PyExc_NotImplementedError, std::string(a.name) + " is a lazily negated view");
     if (grad && a.t->requires_grad())
       refuse(PyExc_RuntimeError, std::string(a.name) +
                                      " requires a gradient: this operator has no backward pass "

@@ -244,6 +244,12 @@ int with_type(int ty, F&& f) {
   }
 }
 
+// The runtime counts a grid in 32-bit threads.
+int check_grid(const dim3& grid, int threads) {
+  if (static_cast<int64_t>(grid.x) * threads > 0xffffffffll)
+    return fail(FGS_EUNSUPPORTED, "too many rows for a grid");
+  return FGS_OK;
+}
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int64_t elem_bytes(int ty) { return ty == FGS_DTYPE_FP32 ? 4 : 2; }
 
@@ -259,6 +265,7 @@ int launch_rms_norm(const RmsNormParams& p, int dtype, int weight_dtype, hipStre
                                     p.res_stride * es % 16 == 0 && p.res_out_stride * es % 16 == 0));
   const RowShape s = row_shape(p.rows, (p.cols + 7) / 8, vec);
   const dim3 grid(static_cast<unsigned>(s.wave ? (p.rows + 3) / 4 : p.rows));
+  if (const int rc = check_grid(grid, s.threads)) return rc;
   const int rc = with_type(dtype, [&](auto ty) {
     constexpr int TY = decltype(ty)::value;
     auto go = [&](auto wty) {
@@ -302,6 +309,7 @@ int launch_gated_quant(const GatedQuantParams& p, int dtype, hipStream_t stream)
     gy = static_cast<unsigned>((chunks + s.threads - 1) / s.threads);
   }
   const dim3 grid(static_cast<unsigned>(s.wave ? (p.rows + 3) / 4 : p.rows), gy);
+  if (const int rc = check_grid(grid, s.threads)) return rc;
   const int rc = with_type(dtype, [&](auto ty) {
     constexpr int TY = decltype(ty)::value;
     return with_nv(s.nv, [&](auto nv) {

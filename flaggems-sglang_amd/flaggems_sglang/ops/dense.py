@@ -74,7 +74,8 @@ def fused_rms_norm(
     the unrounded ``n``). ``column_major_scales`` lays e4m3 scales out with
     the rows adjacent. ``return_norm``: whether ``n`` comes back in x's type
     (default: where nothing is quantised). ``inplace``: the sum replaces
-    ``residual``'s values and ``residual`` is the residual output.
+    ``residual``'s values and ``residual`` is the residual output (``x`` may be
+    ``residual`` itself, but share no part of its memory otherwise).
 
     A NaN in a row makes its outputs NaN (int8 codes 0, scale NaN). Returns
     ``RMSNormOutput(norm, residual, q, scales)``.
@@ -134,8 +135,10 @@ def fp8_block_matmul(
     number of rows are any. Sums are fp32 (of groups of eight products that the
     matrix instruction aligns to the largest and cuts 13 bits below it),
     ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
-    rounded once to ``out_dtype`` (bf16 or fp16). ``out``: a tensor of that type and shape to write, whose
-    rows may lie apart (2-D).
+    rounded once to ``out_dtype`` (bf16 or fp16). ``out``: a tensor of the
+    result's shape to write and return, whose type counts instead of
+    ``out_dtype``, whose rows may lie apart (2-D) and whose memory none of the
+    inputs shares.
     """
     code = _OUT_DTYPES.get(out_dtype, _capi.DTYPE_FP32)  # (refused there)
     return _capi.host().fp8_block_matmul(a, a_scale, w, w_scale, bias, code, out, _flags)

@@ -26,7 +26,14 @@ EPS = 1e-10
 @torch.no_grad()
 def quantize_fp8_block(w: torch.Tensor, block: int = 128):
     """``[E, R, C]`` float -> (e4m3fn ``[E, R, C]``, fp32 ``[E, R/b, C/b]``).
-    Processed one expert at a time to bound temporary memory."""
+    Processed one expert at a time to bound temporary memory. A dense matrix
+    ``[R, C]`` of any size has ``[ceil(R/b), ceil(C/b)]`` scales; the blocks at
+    its ends are smaller."""
+    if w.dim() == 2:
+        R, C = w.shape
+        q, s = quantize_fp8_block(torch.nn.functional.pad(w, (0, -C % block, 0, -R % block))[None],
+                                  block)
+        return q[0, :R, :C].contiguous(), s[0]
     E, R, C = w.shape
     assert R % block == 0 and C % block == 0, "dims must be multiples of block"
     q = torch.empty((E, R, C), dtype=torch.float8_e4m3fn, device=w.device)

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from flaggems_sglang import _capi, fp8_block_matmul, fused_rms_norm, silu_and_mul_quant
+from flaggems_sglang import _capi, fp8_block_matmul, fused_rms_norm, quant, silu_and_mul_quant
 
 P = 0x1000  # an address no call reads
 
@@ -158,3 +158,50 @@ def test_registered():
 
     for name in ("fused_rms_norm", "silu_and_mul_quant", "fp8_block_matmul"):
         assert flaggems_sglang.get_op(name) is getattr(flaggems_sglang, name)
+
+
+def test_grids_the_runtime_cannot_count():
+    """A grid's threads are counted in 32 bits."""
+    rows = (1 << 31) - 1
+    for rc, msg in (_norm(rows=rows, cols=4096), _norm(rows=rows), _act(rows=rows),
+                    _product(m=1 << 22, n=1 << 22, ldo=1 << 22),
+                    _product(m=1 << 22, n=1 << 14, ldo=1 << 14, flags=1)):
+        assert rc == -2 and "for a grid" in msg
+
+
+def test_host_module_arguments():
+    host = _capi.host()
+    with pytest.raises(TypeError, match="9 arguments expected, got 1"):
+        host.rms_norm(1)
+    with pytest.raises(TypeError, match="a must be a tensor"):
+        fp8_block_matmul(None, None, None, None)
+    with pytest.raises(TypeError, match="residual must be a tensor"):
+        fused_rms_norm(torch.zeros(1, 8), torch.zeros(8), 1e-6, 3)
+    for bad in ("fp4", 1):
+        with pytest.raises(ValueError, match="quantisation"):
+            fused_rms_norm(torch.zeros(1, 8), torch.zeros(8), quant=bad)
+        with pytest.raises(ValueError, match="quantisation"):
+            silu_and_mul_quant(torch.zeros(1, 8), bad)
+    with pytest.raises(ValueError, match="quantisation"):
+        silu_and_mul_quant(torch.zeros(1, 8), None)
+    with pytest.raises(ValueError, match="activation"):
+        silu_and_mul_quant(torch.zeros(1, 8), activation="relu")
+
+
+@pytest.mark.parametrize("r,c", [(128, 256), (1, 16), (300, 208), (129, 128)])
+def test_dense_weights_in_blocks(r, c):
+    """A matrix of any size: each block's scale is its largest magnitude over
+    448, and its codes are its values over that (as an expert's weights)."""
+    w = torch.randn(r, c, generator=torch.Generator().manual_seed(r))
+    q, s = quant.quantize_fp8_block(w)
+    assert q.shape == (r, c) and q.is_contiguous() and s.shape == (-(-r // 128), -(-c // 128))
+    for i in range(s.shape[0]):
+        for j in range(s.shape[1]):
+            b = w[128 * i:128 * i + 128, 128 * j:128 * j + 128]
+            scale = b.abs().max() / 448
+            assert s[i, j] == scale
+            got = q[128 * i:128 * i + 128, 128 * j:128 * j + 128]
+            assert torch.equal(got.float(), (b / scale).to(torch.float8_e4m3fn).float())
+    if r % 128 == 0 and c % 128 == 0:
+        q3, s3 = quant.quantize_fp8_block(w[None])
+        assert torch.equal(q3[0].float(), q.float()) and torch.equal(s3[0], s)

@@ -21,6 +21,8 @@ exponents in one of seven, and six fraction bits) are not cut at all: with them
 the roundings alone are the bound.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -486,3 +488,200 @@ def test_two_streams_at_once(gpu):
                 got.append((fgs.fp8_block_matmul(*args), ref))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in got)
+
+
+# ----------------------------------------------------- calls less ordinary ---
+def test_one_tensor_as_both_inputs(gpu):
+    """The residual is the input itself, replaced in place or not; rows that
+    are one row repeated; weights that lie apart."""
+    gen = torch.Generator().manual_seed(8)
+    for rows, cols in ((3, 200), (1030, 512), (2, 40000)):
+        x = _rand(gen, (rows, cols), BF16, gpu)
+        w = _rand(gen, (cols, 2), BF16, gpu, loud=False)[:, 1]
+        h, n = _norm_ref(x, w, 1e-6, x, 0.0)
+        plain = fgs.fused_rms_norm(x, w, residual=x, quant="int8", return_norm=True)
+        _near(plain.residual, h, HALF[BF16])
+        _near(plain.norm, n, HALF[BF16], TINY[BF16])
+        row = x[:1].expand(rows, cols)
+        flat = fgs.fused_rms_norm(row, w, residual=x)
+        again = fgs.fused_rms_norm(row.contiguous(), w, residual=x)
+        assert _same(flat.norm, again.norm) and _same(flat.residual, again.residual)
+        version = x._version
+        o = fgs.fused_rms_norm(x, w, residual=x, quant="int8", return_norm=True, inplace=True)
+        assert o.residual is x and x._version > version
+        assert all(_same(a, b) for a, b in zip(o, plain))
+
+
+def test_expanded_operands_of_the_product(gpu):
+    gen = torch.Generator().manual_seed(12)
+    for m in (7, 300):
+        a, sa, w, sw = _operands(gen, m, 272, 400, gpu)
+        bias = torch.randn(1, generator=gen).to(gpu).expand(272)
+        got = fgs.fp8_block_matmul(a[:1].expand(m, 400), sa[:1].expand(m, 4), w, sw, bias=bias)
+        ref = fgs.fp8_block_matmul(a[:1].repeat(m, 1), sa[:1].repeat(m, 1), w, sw,
+                                   bias=bias.contiguous())
+        assert _same(got, ref)
+        got = fgs.fp8_block_matmul(a, sa[:, :1].expand(m, 4), w, sw[:1, :1].expand(3, 4))
+        ref = fgs.fp8_block_matmul(a, sa[:, :1].repeat(1, 4), w, sw[:1, :1].repeat(3, 4))
+        assert _same(got, ref)
+
+
+def test_no_rows(gpu):
+    x = torch.zeros(2, 0, 512, dtype=BF16, device=gpu)
+    w = torch.ones(512, device=gpu)
+    for kind in ("fp8", "int8"):
+        o = fgs.fused_rms_norm(x, w, quant=kind, residual=x, inplace=True,
+                               column_major_scales=True)
+        assert o.residual is x and o.q.shape == x.shape
+        assert o.scales.shape == ((2, 0, 4) if kind == "fp8" else (2, 0))
+        q, s = fgs.silu_and_mul_quant(x, kind, column_major_scales=True)
+        assert q.shape == (2, 0, 256) and s.shape == ((2, 0, 2) if kind == "fp8" else (2, 0))
+    q, s = fgs.silu_and_mul_quant(x)
+    weights = torch.zeros(48, 256, device=gpu).to(FP8)
+    out = torch.empty(2, 0, 48, dtype=F16, device=gpu)
+    assert fgs.fp8_block_matmul(q, s, weights, torch.ones(1, 2, device=gpu), out=out) is out
+
+
+def test_refusals_of_gpu_tensors(gpu):
+    gen = torch.Generator().manual_seed(4)
+    x = _rand(gen, (4, 256), F32, gpu)
+    w = torch.ones(256, device=gpu)
+    a, sa, b, sb = _operands(gen, 4, 272, 256, gpu)
+    leaf = x.clone().requires_grad_()
+    for call in (lambda: fgs.fused_rms_norm(leaf, w), lambda: fgs.silu_and_mul_quant(leaf),
+                 lambda: fgs.fused_rms_norm(x, w.clone().requires_grad_()),
+                 lambda: fgs.fused_rms_norm(x, w, residual=leaf, inplace=True),
+                 lambda: fgs.fp8_block_matmul(a, sa, b, sb, bias=torch.ones(
+                     272, device=gpu, requires_grad=True))):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.inference_mode():
+        y = x.clone()
+        assert _same(fgs.fused_rms_norm(y, w, residual=y, inplace=True).residual, x + x)
+    negated = torch.complex(x, x).conj().imag
+    assert negated.is_neg()
+    with pytest.raises(NotImplementedError, match="negated"):
+        fgs.fused_rms_norm(negated, w)
+    with pytest.raises(RuntimeError, match="weight is on cpu"):
+        fgs.fused_rms_norm(x, w.cpu())
+    with pytest.raises(RuntimeError, match="out is on cpu"):
+        fgs.fp8_block_matmul(a, sa, b, sb, out=torch.empty(4, 272, dtype=BF16))
+    for text, kw in (("x's type", dict(weight=w.to(BF16))), ("weight must be", dict(weight=w[:8])),
+                     ("x's shape", dict(residual=x[:2])), ("needs a residual", dict(inplace=True)),
+                     ("no output", dict(return_norm=False))):
+        with pytest.raises(AssertionError, match=text):
+            fgs.fused_rms_norm(**{"x": x, "weight": w, **kw})
+    with pytest.raises(ValueError, match="evenly spaced"):
+        fgs.fused_rms_norm(x, w, residual=x[:1].expand(4, 256), inplace=True)
+    with pytest.raises(ValueError, match="evenly spaced"):
+        fgs.fused_rms_norm(x, w, residual=x.t().contiguous().t(), inplace=True)
+    with pytest.raises(AssertionError, match="gate half"):
+        fgs.silu_and_mul_quant(x[:, :255])
+    with pytest.raises(NotImplementedError, match="65536"):
+        fgs.fused_rms_norm(torch.zeros(1, 65544, device=gpu), torch.ones(65544, device=gpu))
+    for text, args, kw in (
+            ("float8", (a.float(), sa, b, sb), {}), ("must be", (a, sa, b[:, :128], sb), {}),
+            ("a_scale must", (a, sa[:, :1], b, sb), {}), ("w_scale must", (a, sa, b, sb[:2]), {}),
+            ("float32", (a, sa.double(), b, sb), {}), ("bias must", (a, sa, b, sb),
+                                                       dict(bias=torch.ones(271, device=gpu))),
+            ("bfloat16 or float16", (a, sa, b, sb), dict(out_dtype=F32)),
+            ("out must", (a, sa, b, sb), dict(out=torch.empty(4, 271, dtype=BF16, device=gpu)))):
+        with pytest.raises(AssertionError, match=text):
+            fgs.fp8_block_matmul(*args, **kw)
+    for out in (torch.empty(272, 4, dtype=BF16, device=gpu).t(),
+                torch.empty(1, 272, dtype=BF16, device=gpu).expand(4, 272)):
+        with pytest.raises(ValueError, match="out must be adjacent|ldo"):
+            fgs.fp8_block_matmul(a, sa, b, sb, out=out)
+    with pytest.raises(ValueError, match="k >= 1"):
+        fgs.fp8_block_matmul(a[:, :0], sa[:, :0], b[:, :0], sb[:, :0])
+    with pytest.raises(NotImplementedError, match="multiple of 16"):
+        fgs.fp8_block_matmul(a[:, :136], sa, b[:, :136], sb)
+
+
+def test_threads_call_at_once(gpu):
+    """Two Python threads (the calls leave the interpreter's lock), each on a
+    stream of its own, get what one thread gets."""
+    gen = torch.Generator().manual_seed(6)
+    w, topk = _layer(gen, gpu)
+    jobs = []
+    for m in (1, 33):
+        x, residual = (_rand(gen, (m, 512), BF16, gpu) for _ in range(2))
+        jobs.append((x, residual, _run_layer(w, topk, x, residual)[-2]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, residual, ref):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                n = fgs.fused_rms_norm(x, w["norm"], 1e-6, residual, quant="fp8")
+                q, s = fgs.silu_and_mul_quant(
+                    fgs.fp8_block_matmul(n.q, n.scales, w["s13"], w["s13_scale"]))
+                got = fgs.fp8_block_matmul(q, s, w["s2"], w["s2_scale"])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, ref):
+                    wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+# ------------------------------------------------------ offsets past 2^31 ---
+def _picked(rows, cols):
+    """Rows on both sides of element 2^31, and the ends."""
+    edge = 2 ** 31 // cols
+    assert rows > edge + 1
+    return torch.tensor([0, edge - 1, edge, edge + 1, rows - 1])
+
+
+def test_norm_past_31_bits(gpu):
+    rows, cols = 65540, 32768
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    x = torch.randn(rows, cols, device=gpu, dtype=BF16, generator=gen)
+    w = torch.randn(cols, device=gpu, dtype=BF16, generator=gen)
+    at = _picked(rows, cols).to(gpu)
+    h, n = _norm_ref(x[at], w, 1e-6, x[at], 0.0)
+    for kind in ("fp8", "int8"):
+        o = fgs.fused_rms_norm(x, w, residual=x, quant=kind, return_norm=True)
+        _near(o.residual[at], h, HALF[BF16])
+        _near(o.norm[at], n, HALF[BF16], TINY[BF16])
+        _check_codes(o.q.view(torch.uint8)[at].view(o.q.dtype), o.scales[at], n, kind)
+
+
+def test_activation_past_31_bits(gpu):
+    rows, n = 65540, 32768
+    gen = torch.Generator(device=gpu).manual_seed(2)
+    x = torch.randn(rows, 2 * n, device=gpu, dtype=BF16, generator=gen)
+    at = _picked(rows, n).to(gpu)
+    ref = _act_ref(x[at], False)
+    for kind in ("fp8", "int8"):
+        q, s = fgs.silu_and_mul_quant(x, kind)
+        _check_codes(q.view(torch.uint8)[at].view(q.dtype), s[at], ref, kind)
+
+
+@pytest.mark.parametrize("m,n,k,what", [(262149, 32, 8192, "a"), (40000, 65536, 16, "out"),
+                                        (2, 65540, 32768, "w"), (300, 65540, 32768, "w")])
+def test_product_past_31_bits(gpu, m, n, k, what):
+    gen = torch.Generator(device=gpu).manual_seed(m)
+
+    def codes(rows):
+        c = torch.randint(0x38, 0x58, (rows, k), generator=gen, dtype=torch.uint8, device=gpu)
+        c |= torch.randint(0, 2, (rows, k), generator=gen, dtype=torch.uint8, device=gpu) << 7
+        return c.view(FP8)
+    a, w = codes(m), codes(n)
+    sa, sw = (torch.exp2(4 * torch.rand(r, -(-k // 128), generator=gen, device=gpu) - 8)
+              for r in (m, -(-n // 128)))
+    out = fgs.fp8_block_matmul(a, sa, w, sw)
+    rows = _picked(m, k if what == "a" else n).to(gpu) if what != "w" else torch.arange(
+        m, device=gpu)[-64:]
+    cols = _picked(n, k).to(gpu) if what == "w" else torch.arange(n, device=gpu)[-64:]
+    pick_w, pick_sw = w.view(torch.uint8)[cols].view(FP8), sw[cols // 128]
+    pick_a, pick_sa = a.view(torch.uint8)[rows].view(FP8), sa[rows]
+    x = pick_a.double() * pick_sa.double().repeat_interleave(128, 1)[:, :k]
+    y = pick_w.double() * pick_sw.double().repeat_interleave(128, 1)[:, :k]
+    _check_product(out[rows][:, cols], x @ y.t(), x.abs() @ y.abs().t(), k, BF16, narrow=True)
