@@ -115,7 +115,7 @@ struct SkinnyCfg {
   static constexpr int NL = 2 * (MT + NT) + 2;
   static constexpr int LDS = KW * SLOTS * SLOT;
   static_assert(MT <= 4 && 128 % (16 * NT) == 0, "one scale a lane, one weight block");
-  static_assert(SLOTS >= 2 && SLOTS <= 4 && (SLOTS - 1) * NL < 64 && LDS + 64 * NT <= 160 * 1024,
+  static_assert(SLOTS >= 2 && SLOTS <= 3 && (SLOTS - 1) * NL < 64 && LDS + 64 * NT <= 160 * 1024,
                 "ring");
   static_assert(KW * MT * NT * 1024 <= LDS, "partial sums");
 };
@@ -178,8 +178,7 @@ __global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const Blo
     lds_dma4_buf(rb, lane * 4, slot + C::SC_AT + 256);
   };
   auto wait_stages = [&](int n) {  // at most n later blocks in flight
-    if (n >= 3) wait_vmcnt<(SLOTS > 3 ? 3 * C::NL : 0)>();
-    else if (n == 2) wait_vmcnt<(SLOTS > 2 ? 2 * C::NL : 0)>();
+    if (n >= 2) wait_vmcnt<(SLOTS > 2 ? 2 * C::NL : 0)>();
     else if (n == 1) wait_vmcnt<C::NL>();
     else wait_vmcnt<0>();
   };
@@ -294,7 +293,7 @@ struct BlockCfg {
   static_assert(128 % (CT * 16) == 0, "a wave's weight rows lie in one scale block");
   static_assert(BN % 128 == 0 || 128 % BN == 0, "scale blocks of a tile");
   static_assert(BM + (BN + 127) / 128 <= NW * 64, "scale slots");
-  static_assert(STAGES >= 2 && STAGES <= 4 && (STAGES - 1) * NL < 64 && LDS + 4 * BN <= 160 * 1024,
+  static_assert(STAGES >= 2 && (STAGES - 1) * NL < 64 && LDS + 4 * BN <= 160 * 1024,
                 "ring");
   static_assert(CT % 2 == 0, "fragment pipeline");
 };
@@ -547,9 +546,15 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   } else if (KT >= STAGES) {
     stage(0, std::integral_constant<int, STAGES - 1>{}, std::true_type{});
   }
-  if constexpr (STAGES > 2) {
-    if (KT > 1) stage(KT - 2, std::integral_constant<int, 1>{}, std::true_type{});
-  }
+  // the stages behind them, of which fewer than STAGES - 1 are left
+  auto tail = [&](auto self, auto rest_c) {
+    constexpr int REST = decltype(rest_c)::value;
+    if constexpr (REST > 0) {
+      if (KT > REST) stage(KT - 1 - REST, rest_c, std::true_type{});
+      self(self, std::integral_constant<int, REST - 1>{});
+    }
+  };
+  tail(tail, std::integral_constant<int, STAGES - 2>{});
   stage(KT - 1, std::integral_constant<int, 0>{}, std::true_type{});
 #pragma unroll
   for (int j = TILES - LAG; j < TILES; ++j) fold(j, sp);
@@ -611,34 +616,43 @@ namespace {
 // The forms (FGS_BLOCK_FORM(i)): tile in tokens x weight rows; k blocks an
 // iteration takes (the streaming forms' waves take one each); workgroups that
 // run at once; microseconds of an iteration with the chip full, and beside the
-// iterations of a round. Measured at K 7168 and N 4096 (tokens: us): 1: 7.2
-// (form 0), 16: 8.1 (1), 32: 10.7 (2), 64: 11.3 (3; 64 x 32 tiles 15.6), 128:
-// 15.9 (4; 18.6 with 32 x 32), 256: 19.7 (5; 27), 512: 31 (6; 35 with 64 x 64),
-// 1024: 53 (7), 2048: 68 (7; 256 x 256 91), 4096: 110 (8; 128 x 128 125).
+// iterations of a round: fitted to 500 products drawn over m 1 to 8192, n 16 to
+// 16384, k 128 to 16384 (the choice takes 1.3 % more than the best form on 200
+// others).
+// Measured at K 7168 and N 4096, weights not in a cache (tokens: us): 1: 7.3
+// (form 0), 16: 9.1 (0), 32: 10.6 (1; 12.2 with 32 x 32), 64: 11.8 (2; 16.4 with
+// 64 x 32), 128: 15.6 (3; 18.6 with 32 x 32), 256: 20.9 (4; 29 with 64 x 128),
+// 512: 30.4 (5; 36 deep 128 x 128), 1024: 41 (7; 55 with the shallow ring),
+// 2048: 66 (8; 70 with 128 x 128), 4096: 104 (9; 125 with 128 x 256).
+// Between the tiles: an operand passes the L2 once for each tile that shares it
+// (13 TB/s beside the products), so a larger tile is faster until too few are
+// left for the CUs; a CU that has one workgroup of four waves alone waits for
+// each refill, hence the deep ring with eight.
 struct Form {
   int bm, bn, step, at_once;
   double iter, half, round;  // half: an iteration with half of at_once or fewer
 };
 constexpr Form kForms[] = {
-    {16, 16, 8, 512, 1.1, 0.85, 0.5},    {16, 16, 8, 256, 0.75, 0.95, 0.5},
-    {32, 16, 8, 256, 1.05, 0.95, 0.5},   {32, 32, 8, 256, 1.1, 1.1, 0.8},
-    {64, 32, 4, 256, 0.9, 0.9, 1.0},     {64, 64, 4, 256, 1.13, 1.13, 1.4},
-    {64, 128, 1, 512, 0.65, 0.45, 1.8},  {128, 128, 1, 512, 0.98, 0.80, 3.0},
-    {256, 256, 1, 256, 1.55, 1.35, 6.5},
+    {16, 16, 8, 512, 1.07, 0.85, 0.5},    {32, 16, 8, 256, 1.05, 0.95, 0.5},
+    {32, 32, 8, 256, 1.11, 1.03, 0.78},   {64, 32, 4, 256, 0.9, 0.9, 1.0},
+    {64, 64, 4, 256, 1.22, 1.13, 1.62},   {64, 128, 1, 512, 0.73, 0.35, 1.95},
+    {128, 128, 1, 512, 1.03, 0.80, 3.0},  {128, 128, 1, 256, 0.58, 0.66, 3.74},
+    {128, 256, 1, 256, 0.90, 0.84, 5.01}, {256, 256, 1, 256, 1.54, 1.35, 6.53},
 };
 constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
 
 template <int F>
 struct FormCfg;
 template <> struct FormCfg<0> { typedef SkinnyCfg<1, 1, 8, 2> type; };
-template <> struct FormCfg<1> { typedef SkinnyCfg<1, 1, 8, 4> type; };
-template <> struct FormCfg<2> { typedef SkinnyCfg<2, 1, 8, 2> type; };
-template <> struct FormCfg<3> { typedef SkinnyCfg<2, 2, 8, 2> type; };
-template <> struct FormCfg<4> { typedef SkinnyCfg<4, 2, 4, 3> type; };
-template <> struct FormCfg<5> { typedef SkinnyCfg<4, 4, 4, 2> type; };
-template <> struct FormCfg<6> { typedef BlockCfg<64, 128, 2, 2, 3, 2> type; };
-template <> struct FormCfg<7> { typedef BlockCfg<128, 128, 2, 2, 2, 2> type; };
-template <> struct FormCfg<8> { typedef BlockCfg<256, 256, 4, 2, 2, 2> type; };
+template <> struct FormCfg<1> { typedef SkinnyCfg<2, 1, 8, 2> type; };
+template <> struct FormCfg<2> { typedef SkinnyCfg<2, 2, 8, 2> type; };
+template <> struct FormCfg<3> { typedef SkinnyCfg<4, 2, 4, 3> type; };
+template <> struct FormCfg<4> { typedef SkinnyCfg<4, 4, 4, 2> type; };
+template <> struct FormCfg<5> { typedef BlockCfg<64, 128, 2, 2, 3, 2> type; };
+template <> struct FormCfg<6> { typedef BlockCfg<128, 128, 2, 2, 2, 2> type; };
+template <> struct FormCfg<7> { typedef BlockCfg<128, 128, 4, 2, 4, 2> type; };
+template <> struct FormCfg<8> { typedef BlockCfg<128, 256, 2, 4, 3, 2> type; };
+template <> struct FormCfg<9> { typedef BlockCfg<256, 256, 4, 2, 2, 2> type; };
 
 // Launches `kernel` with more than 64 KiB of LDS, which each GPU has to be told
 // of once (`told`: a bit a GPU).
@@ -719,7 +733,7 @@ int block_gemm_form(int64_t m, int64_t n, int64_t k, int32_t flags) {
 std::string block_gemm_name(int form) {
   const Form& q = kForms[form];
   return (q.step > 1 ? "stream " : "tiled ") + std::to_string(q.bm) + "x" + std::to_string(q.bn) +
-         (form == 1 ? " deep" : "");
+         (form == 7 ? " deep" : "");
 }
 
 int launch_block_gemm(const BlockGemmParams& p, int form, hipStream_t stream) {
@@ -729,10 +743,11 @@ int launch_block_gemm(const BlockGemmParams& p, int form, hipStream_t stream) {
     case 2: return skinny_launch<2>(p, stream);
     case 3: return skinny_launch<3>(p, stream);
     case 4: return skinny_launch<4>(p, stream);
-    case 5: return skinny_launch<5>(p, stream);
+    case 5: return tiled_launch<5>(p, stream);
     case 6: return tiled_launch<6>(p, stream);
     case 7: return tiled_launch<7>(p, stream);
-    default: return tiled_launch<8>(p, stream);
+    case 8: return tiled_launch<8>(p, stream);
+    default: return tiled_launch<9>(p, stream);
   }
 }
 

@@ -130,10 +130,12 @@ def test_schedule_text():
 
 @pytest.mark.parametrize("m,n,k,schedule", [
     (0, 4096, 7168, "none"), (1, 16384, 7168, "stream 16x16"),
-    (16, 4096, 7168, "stream 16x16 deep"), (64, 4096, 7168, "stream 32x32"),
-    (128, 4096, 7168, "stream 64x32"), (256, 4096, 7168, "stream 64x64"),
-    (512, 4096, 7168, "tiled 64x128"), (2048, 4096, 7168, "tiled 128x128"),
-    (4096, 4096, 7168, "tiled 256x256"), (8192, 14336, 7168, "tiled 256x256"),
+    (16, 4096, 7168, "stream 16x16"), (32, 4096, 7168, "stream 32x16"),
+    (64, 4096, 7168, "stream 32x32"), (128, 4096, 7168, "stream 64x32"),
+    (256, 4096, 7168, "stream 64x64"), (512, 4096, 7168, "tiled 64x128"),
+    (1024, 4096, 7168, "tiled 128x128 deep"), (2048, 4096, 7168, "tiled 128x256"),
+    (3600, 1828, 384, "tiled 128x128"), (4096, 4096, 7168, "tiled 256x256"),
+    (8192, 14336, 7168, "tiled 256x256"),
 ])
 def test_schedules(m, n, k, schedule):
     """The tile of a product by the sizes' estimate (the shapes the estimate
