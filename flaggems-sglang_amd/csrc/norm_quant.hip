@@ -216,9 +216,12 @@ struct RowShape {
 };
 // Few rows leave CUs idle, so a row takes as many threads as it has vectors;
 // with many, threads hold two vectors (more loads in flight for the same
-// waves), and a row of at most 128 vectors takes one wave and no barrier.
+// waves), and rows of at most 64 vectors take a wave each, four a workgroup
+// (norm with e4m3 output, 4096 x 128: 3.7 us, 4.1 with a workgroup each; two
+// and four vectors a lane lost against workgroups: 4096 x 1024 8.8 / 8.2, 4096 x
+// 2048 15.6 / 13.3).
 RowShape row_shape(int64_t rows, int64_t chunks, bool vec) {
-  if (vec && rows >= 1024 && chunks <= 256) return {true, chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4, 256};
+  if (vec && rows >= 1024 && chunks <= 64) return {true, 1, 256};
   int nv = 1;
   while (nv < kRowVecs && chunks > int64_t{kRowThreads} * nv) nv *= 2;
   if (rows >= 512 && nv < 4 && chunks >= 128 * nv) nv *= 2;
@@ -276,7 +279,7 @@ int launch_rms_norm(const RmsNormParams& p, int dtype, int weight_dtype, hipStre
           constexpr int NV = decltype(nv)::value;
           auto kernel = vec ? rms_norm_kernel<TY, WTY, true, false, RES, NV>
                             : rms_norm_kernel<TY, WTY, false, false, RES, NV>;
-          if constexpr (NV <= 4) {
+          if constexpr (NV == 1) {
             if (s.wave) kernel = rms_norm_kernel<TY, WTY, true, true, RES, NV>;
           }
           hipLaunchKernelGGL(kernel, grid, dim3(s.threads), 0, stream, p);
@@ -316,7 +319,7 @@ int launch_gated_quant(const GatedQuantParams& p, int dtype, hipStream_t stream)
       constexpr int NV = decltype(nv)::value;
       auto kernel =
           vec ? gated_quant_kernel<TY, true, false, NV> : gated_quant_kernel<TY, false, false, NV>;
-      if constexpr (NV <= 4) {
+      if constexpr (NV == 1) {
         if (s.wave) kernel = gated_quant_kernel<TY, true, true, NV>;
       }
       hipLaunchKernelGGL(kernel, grid, dim3(s.threads), 0, stream, p);
