@@ -2,8 +2,8 @@
 // (flaggems_sglang.ops.dense) -- argument checks, output allocation, the
 // current stream, the call into libfgs_moe.so's C ABI. A decode step's kernels
 // take 2 to 8 us and a launch 3.3; the same steps in Python took 9.6 to 13 us a
-// call (a norm with four outputs 13.2, here 7.0), so at one token the host was
-// what a layer waited for.
+// call (a norm with four outputs 13.2, here 5.8; the dispatcher's empty() 7.2),
+// so at one token the host was what a layer waited for.
 //
 // The library's entries come in by address (bind), from the handle that
 // flaggems_sglang._capi has loaded. No C++ exception leaves this file.
@@ -11,9 +11,9 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -96,7 +96,7 @@ int type_code(const at::Tensor& t) {  // FGS_DTYPE_*, -1: none of them
 }
 
 at::Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+  return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
 }
 
 // The rows of a tensor's last dimension: where they are if they lie evenly

@@ -83,7 +83,7 @@ def fused_rms_norm(
     mode = _QUANTS.get(quant)
     if mode is None:
         raise ValueError(f"Unsupported quantisation: {quant}")
-    return RMSNormOutput(*_capi.host().rms_norm(
+    return tuple.__new__(RMSNormOutput, _capi.host().rms_norm(
         x, weight, eps, residual, weight_offset, mode, return_norm, column_major_scales, inplace))
 
 
