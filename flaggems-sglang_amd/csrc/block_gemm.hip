@@ -107,6 +107,7 @@ __device__ __forceinline__ int xcd_order(int i, int total) {
 // the ring keeps enough of them in flight. (Straight from memory into the
 // MFMA's registers, a load's neighbouring lanes lie in 16 different rows, and
 // the address unit takes them one a cycle: 16 tokens 11.7 us at 4096 x 7168.)
+// One token: 4096 x 7168 7.3 us (4.0 TB/s), 14336 x 7168 21.3 (4.8 TB/s).
 template <int MT_, int NT_, int KW_, int SLOTS_>
 struct SkinnyCfg {
   static constexpr int MT = MT_, NT = NT_, KW = KW_, SLOTS = SLOTS_;
@@ -275,8 +276,11 @@ __global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const Blo
 // A workgroup of WM x WN waves owns BM tokens x BN weight rows; both operands'
 // rows of a k block (128 bytes each) and the block's scales stream into a ring
 // of STAGES LDS slots by LDS-DMA. A wave keeps its tokens' fragments of a
-// block in registers and takes its weight rows 16 at a time: RT MFMAs, then
-// the 4 RT FMAs of the 16 rows before them.
+// block in registers and takes its weight rows 16 at a time; an MFMA's four
+// FMAs follow three MFMAs behind it. 256 x 256: 4096 x 4096 x 7168 104 us (2.3
+// PFLOP/s, MFMA 50 % busy, one round of tiles with its fill and epilogue), 8192 x
+// 14336 x 7168 680 (2.5 PFLOP/s, 66 %: the clock falls to 1.7 - 1.9 GHz under
+// random data; zeros run 3.5 PFLOP/s).
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int WPE_>
 struct BlockCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
@@ -353,7 +357,8 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   const bool a_slots = wave < C::BM / 64;
   const float* sc_base = a_slots ? p.a_scale + m0 * p.as_row : p.w_scale + (n0 >> 7) * p.kblocks;
   const int64_t sc_step = a_slots ? p.as_col : 1;
-  const int w_block = min<int>(wave * 64 + lane - C::BM, min<int>((C::BN + 127) / 128 - 1, wm_last >> 7));
+  const int w_block = min<int>(wave * 64 + lane - C::BM,
+                               min<int>((C::BN + 127) / 128 - 1, wm_last >> 7));
   const uint32_t sc_off = a_slots ? min(wave * 64 + lane, am) * static_cast<uint32_t>(p.as_row) * 4
                                   : max(w_block, 0) * p.kblocks * 4;
 
@@ -440,7 +445,8 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   // the scales of the stage before).
   constexpr int TILES = CT * RT, LAG = 3;
   static_assert(TILES > LAG && RT >= 2, "pipeline");
-  static_assert(C::NL - RT <= (CT - 1) * RT && RT <= C::NL, "a refill ends before the next barrier");
+  static_assert(C::NL - RT <= (CT - 1) * RT && RT <= C::NL,
+                "a refill ends before the next barrier");
   i32x8 x[RT], w[2];
   float s[RT], sp[RT];
   f32x4 part[LAG + 1];
@@ -657,8 +663,8 @@ template <> struct FormCfg<9> { typedef BlockCfg<256, 256, 4, 2, 2, 2> type; };
 // Launches `kernel` with more than 64 KiB of LDS, which each GPU has to be told
 // of once (`told`: a bit a GPU).
 template <class... P, class... A>
-int launch_wide_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told, int64_t wgs,
-                    int threads, int lds, hipStream_t stream, A... args) {
+int launch_wide_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told,
+                    int64_t wgs, int threads, int lds, hipStream_t stream, A... args) {
   // (the runtime counts a grid in 32-bit threads)
   if (wgs * threads > 0xffffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
   int gpu = 0;
@@ -690,7 +696,8 @@ int skinny_launch(const BlockGemmParams& p, hipStream_t stream) {
 template <int F, int OUT>
 int tiled_launch_out(const BlockGemmParams& p, hipStream_t stream) {
   typedef typename FormCfg<F>::type C;
-  static_assert(kForms[F].bm == C::BM && kForms[F].bn == C::BN && kForms[F].step == 1, "form table");
+  static_assert(kForms[F].bm == C::BM && kForms[F].bn == C::BN && kForms[F].step == 1,
+                "form table");
   static std::atomic<uint64_t> told{0};
   const int64_t nm = (p.m + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
   return launch_wide_lds("block_gemm_tiled_kernel", block_gemm_tiled_kernel<C, OUT>, told, nm * nn,

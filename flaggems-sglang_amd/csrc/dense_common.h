@@ -83,7 +83,8 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int64_t valid, co
       uint32_t u;
       if constexpr (N == 2) u = __float_as_uint(f[i]);
       else if constexpr (TY == FGS_DTYPE_BF16) u = cvt_pk_bf16(f[2 * i], f[2 * i + 1]);
-      else u = Elem<TY>::from_f32(f[2 * i]) | static_cast<uint32_t>(Elem<TY>::from_f32(f[2 * i + 1])) << 16;
+      else u = Elem<TY>::from_f32(f[2 * i]) |
+               static_cast<uint32_t>(Elem<TY>::from_f32(f[2 * i + 1])) << 16;
       w[i / 4][i % 4] = u;
     }
 #pragma unroll

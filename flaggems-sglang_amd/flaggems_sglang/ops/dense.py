@@ -18,8 +18,9 @@ GPU) is the extension module ``_host``; the arithmetic is in
 has a backward pass: an input that requires a gradient is refused while
 gradients are recorded.
 
-The reference has no counterparts (its layer takes its input normalised, and
-src/flaggems_sglang/ops/fused_moe.py:170-185 rejects every 8-bit mode).
+The reference's fused-MoE path has no counterparts (its layer takes its input
+normalised, and src/flaggems_sglang/ops/fused_moe.py:170-185 rejects every
+8-bit mode).
 """
 
 from __future__ import annotations

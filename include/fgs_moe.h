@@ -385,8 +385,8 @@ int32_t fgs_moe_fused_int8_channel(const void* x, const void* w13,
                                    int64_t ws_bytes, void* out, void* stream);
 
 /* ---- dense operators around the routed experts -------------------------
- * No reference counterparts (the reference's layer takes its input normalised
- * and has no 8-bit path, ops/fused_moe.py:170-185): the norm before the
+ * No counterparts on the reference's path (its layer takes its input
+ * normalised and has no 8-bit mode, ops/fused_moe.py:170-185): the norm before the
  * layer, the dense e4m3 products of the shared expert and the projections,
  * and the shared expert's activation. Element types of these entries: */
 #define FGS_DTYPE_BF16 0
