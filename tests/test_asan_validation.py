@@ -67,3 +67,15 @@ def test_capi_validation_under_asan(asan_setup):
     out = r.stdout + r.stderr
     assert "AddressSanitizer" not in out, out[-4000:]
     assert r.returncode == 0, out[-4000:]
+
+
+def test_dense_validation_under_asan(asan_setup):
+    """The dense operators' entries and form table in the same way."""
+    r = subprocess.run(
+        [sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider",
+         os.path.join(ROOT, "tests", "test_dense_ops.py"), "-k",
+         "refusals or schedule or grids"],
+        cwd=ROOT, env=_child_env(asan_setup), capture_output=True, text=True, timeout=600)
+    out = r.stdout + r.stderr
+    assert "AddressSanitizer" not in out, out[-4000:]
+    assert r.returncode == 0 and "passed" in out, out[-4000:]

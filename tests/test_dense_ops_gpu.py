@@ -206,7 +206,8 @@ def test_norm_of_zeros_nans_and_infinities(gpu, cols):
 
 # -------------------------------------------------------------- activation ---
 ACT_SHAPES = [(1, 2048), (8, 2048), (1, 1), (3, 100), (5, 136), (1025, 64), (1024, 1000),
-              (1026, 768), (600, 2560), (2, 14336), (513, 7168), (1, 65536), (7, 4099)]
+              (1026, 768), (600, 2560), (2, 14336), (513, 7168), (1, 65536), (7, 4099),
+              (1030, 512), (4096, 6144), (4097, 6500), (3, 40000)]
 
 
 def _act_ref(x, gelu):
