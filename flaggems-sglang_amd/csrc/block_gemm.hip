@@ -121,9 +121,12 @@ struct SkinnyCfg {
   static_assert(KW * MT * NT * 1024 <= LDS, "partial sums");
 };
 
+// (Two waves a SIMD also where there is one: with the registers of one the
+// compiler puts products into AGPRs, and a move an FMA takes them out again: 333 x
+// 2112 x 1552 8.4 us, 8.1 so.)
 template <class C>
-__global__ __launch_bounds__(C::KW * 64) void block_gemm_skinny_kernel(const BlockGemmParams p,
-                                                                       int nm, int total) {
+__global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
+    const BlockGemmParams p, int nm, int total) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   __shared__ __attribute__((aligned(16))) float bias[16 * C::NT];
   constexpr int MT = C::MT, NT = C::NT, SLOTS = C::SLOTS;
@@ -627,7 +630,7 @@ namespace {
 // others).
 // Measured at K 7168 and N 4096, weights not in a cache (tokens: us): 1: 7.3
 // (form 0), 16: 9.1 (0), 32: 10.6 (1; 12.2 with 32 x 32), 64: 11.8 (2; 16.4 with
-// 64 x 32), 128: 15.6 (3; 18.6 with 32 x 32), 256: 20.9 (4; 29 with 64 x 128),
+// 64 x 32), 128: 15.6 (3; 18.6 with 32 x 32), 256: 19.5 (4; 29 with 64 x 128),
 // 512: 30.4 (5; 36 deep 128 x 128), 1024: 41 (7; 55 with the shallow ring),
 // 2048: 66 (8; 70 with 128 x 128), 4096: 104 (9; 125 with 128 x 256).
 // Between the tiles: an operand passes the L2 once for each tile that shares it
