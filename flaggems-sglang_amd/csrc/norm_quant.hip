@@ -219,11 +219,12 @@ struct RowShape {
   int nv, threads;
 };
 // Few rows leave CUs idle, so a row takes as many threads as it has vectors;
-// with many, threads hold two vectors (more loads in flight for the same
-// waves), and rows of at most 64 vectors take a wave each, four a workgroup
-// (norm with e4m3 output, 4096 x 128: 3.7 us, 4.1 with a workgroup each; two
-// and four vectors a lane lost against workgroups: 4096 x 1024 8.8 / 8.2, 4096 x
-// 2048 15.6 / 13.3).
+// with many, threads hold two vectors (more loads in flight for the same waves:
+// norm with e4m3 output, 4096 x 7168: 34.8 us, 40.7 with one, 39.6 with four;
+// 1021 x 3584 to int8 8.0, 8.6, 8.4), and rows of at most 64 vectors take a wave
+// each, four a workgroup (norm with e4m3 output, 4096 x 128: 3.7 us, 4.1 with a
+// workgroup each; two and four vectors a lane lost against workgroups: 4096 x
+// 1024 8.8 / 8.2, 4096 x 2048 15.6 / 13.3).
 RowShape row_shape(int64_t rows, int64_t chunks, bool vec) {
   if (vec && rows >= 1024 && chunks <= 64) return {true, 1, 256};
   int nv = 1;
