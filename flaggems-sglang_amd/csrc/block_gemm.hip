@@ -178,6 +178,8 @@ __global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
 #pragma unroll
     for (int j = 0; j < 2 * MT; ++j)
       lds_dma16_buf(ra, a0 + j * 8 * lda + (c0 ^ (64 * (j & 1))), 0, slot + j * 1024);
+    // (rows that lie apart are a cache line a token, which the address unit takes
+    // one a cycle: 128 tokens at 4096 x 7168 18.4 us, 15.5 with adjacent ones)
     lds_dma4_buf(rs, as0, slot + C::SC_AT);
     lds_dma4_buf(rb, lane * 4, slot + C::SC_AT + 256);
   };

@@ -73,7 +73,8 @@ def fused_rms_norm(
     128 columns, ``"int8"``: ``q`` int8 with ``scales [...]`` per row (the
     codes of ``per_token_group_quant_fp8`` / ``per_token_quant_int8``, here of
     the unrounded ``n``). ``column_major_scales`` lays e4m3 scales out with
-    the rows adjacent. ``return_norm``: whether ``n`` comes back in x's type
+    the rows adjacent, which :func:`fp8_block_matmul` reads faster from some
+    dozens of rows on. ``return_norm``: whether ``n`` comes back in x's type
     (default: where nothing is quantised). ``inplace``: the sum replaces
     ``residual``'s values and ``residual`` is the residual output (``x`` may be
     ``residual`` itself, but share no part of its memory otherwise).
@@ -130,7 +131,9 @@ def fp8_block_matmul(
 
     ``a [..., k]`` with ``a_scale [..., ceil(k / 128)]`` (what
     ``per_token_group_quant_fp8``, :func:`fused_rms_norm` and
-    :func:`silu_and_mul_quant` return, row- or column-major), ``w [n, k]``
+    :func:`silu_and_mul_quant` return, row- or column-major: with rows that lie
+    apart a block's scales are a cache line each, 3 to 19 % more time from 64
+    rows on), ``w [n, k]``
     with ``w_scale [ceil(n / 128), ceil(k / 128)]``
     (``quant.quantize_fp8_block``). ``k`` is a multiple of 16, ``n`` and the
     number of rows are any. Sums are fp32 (of groups of eight products that the

@@ -452,6 +452,24 @@ def test_layer_of_routed_and_shared_experts(gpu, m):
     assert torch.equal(out, routed + shared)
 
 
+@pytest.mark.parametrize("m", [1, 33, 300])
+def test_layer_with_adjacent_scales(gpu, m):
+    """The dense half with column-major scales: the bits of row-major ones."""
+    gen = torch.Generator().manual_seed(m + 1)
+    w, _ = _layer(gen, gpu)
+    x, residual = (_rand(gen, (m, 512), BF16, gpu) for _ in range(2))
+    out = []
+    for column in (False, True):
+        n = fgs.fused_rms_norm(x, w["norm"], 1e-6, residual, quant="fp8",
+                               column_major_scales=column)
+        assert n.scales.stride() == ((1, m) if column else (4, 1))
+        h = fgs.fp8_block_matmul(n.q, n.scales, w["s13"], w["s13_scale"])
+        q, s = fgs.silu_and_mul_quant(h, column_major_scales=column)
+        out.append((n.q, n.scales, h, q, s, fgs.fp8_block_matmul(q, s, w["s2"], w["s2_scale"])))
+    for a, b in zip(*out):
+        assert _same(a.contiguous(), b.contiguous())
+
+
 def test_layer_replayed_from_a_graph(gpu):
     """Captured once, replayed several times on new inputs with eager calls
     between; every replay gives the eager bits."""
