@@ -101,7 +101,7 @@ __device__ __forceinline__ int xcd_order(int i, int total) {
 // ------------------------------------------------------------- few tokens ---
 // A workgroup owns 16 MT tokens x 16 NT weight rows; its KW waves split the k
 // blocks into contiguous runs and meet in LDS at the end, added in wave order.
-// Each wave streams its own blocks -- both operands' rows and the block's
+// Each wave streams its own blocks -- both operands' rows and the tokens'
 // scales -- through a ring of SLOTS LDS slots that is its alone, so nothing but
 // its own load counter orders it: the form is bound by the weights' bytes, and
 // the ring keeps enough of them in flight. (Straight from memory into the
@@ -112,8 +112,8 @@ template <int MT_, int NT_, int KW_, int SLOTS_>
 struct SkinnyCfg {
   static constexpr int MT = MT_, NT = NT_, KW = KW_, SLOTS = SLOTS_;
   static constexpr int W_AT = MT * 2048, SC_AT = (MT + NT) * 2048;
-  static constexpr int SLOT = SC_AT + 512;  // 64 token scales, the weight block's
-  static constexpr int NL = 2 * (MT + NT) + 2;
+  static constexpr int SLOT = SC_AT + 256;  // 64 token scales
+  static constexpr int NL = 2 * (MT + NT) + 1;
   static constexpr int LDS = KW * SLOTS * SLOT;
   static_assert(MT <= 4 && 128 % (16 * NT) == 0, "one scale a lane, one weight block");
   static_assert(SLOTS >= 2 && SLOTS <= 3 && (SLOTS - 1) * NL < 64 && LDS + 64 * NT <= 160 * 1024,
@@ -170,8 +170,6 @@ __global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<float*>(p.a_scale) + m0 * p.as_row + kb * p.as_col, 0,
         static_cast<int>((rows_a - 1) * static_cast<uint32_t>(p.as_row) * 4 + 4), kBufWord3);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<float*>(p.w_scale) + (n0 >> 7) * p.kblocks + kb, 0, 4, kBufWord3);
 #pragma unroll
     for (int j = 0; j < 2 * NT; ++j)
       lds_dma16_buf(rw, w0 + j * 8 * ldw + (c0 ^ (64 * (j & 1))), 0, slot + C::W_AT + j * 1024);
@@ -181,7 +179,6 @@ __global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
     // (rows that lie apart are a cache line a token, which the address unit takes
     // one a cycle: 128 tokens at 4096 x 7168 18.4 us, 15.5 with adjacent ones)
     lds_dma4_buf(rs, as0, slot + C::SC_AT);
-    lds_dma4_buf(rb, lane * 4, slot + C::SC_AT + 256);
   };
   auto wait_stages = [&](int n) {  // at most n later blocks in flight
     if (n >= 2) wait_vmcnt<(SLOTS > 2 ? 2 * C::NL : 0)>();
@@ -214,12 +211,19 @@ __global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i)
     if (i < count) issue(i);
+  // The weight block's scale by a scalar load, a block ahead (a load into LDS for
+  // it cost 1 to 3 %: 48 x 7168 x 2048 6.7 us, 6.5 so).
+  typedef const __attribute__((address_space(4))) float* scalars;
+  const scalars w_scales =
+      (scalars)(reinterpret_cast<uintptr_t>(p.w_scale + (n0 >> 7) * p.kblocks + kb0));
+  float ws_next = count > 0 ? w_scales[0] : 0.f;
   for (int i = 0; i < count; ++i) {
     wait_stages(min(SLOTS - 1, count - 1 - i));
     const uint8_t* slot = ring + (i % SLOTS) * C::SLOT;
     i32x8 w[NT], x[MT];
     float s[MT];
-    const float ws = *reinterpret_cast<const float*>(slot + C::SC_AT + 256);
+    const float ws = ws_next;
+    ws_next = w_scales[min(i + 1, count - 1)];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       s[t] = *reinterpret_cast<const float*>(slot + C::SC_AT + (t * 16 + r) * 4);
