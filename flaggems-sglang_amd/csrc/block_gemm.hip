@@ -632,8 +632,8 @@ namespace {
 // iteration takes (the streaming forms' waves take one each); workgroups that
 // run at once; microseconds of an iteration with the chip full, and beside the
 // iterations of a round: fitted to 500 products drawn over m 1 to 8192, n 16 to
-// 16384, k 128 to 16384 (the choice takes 1.3 % more than the best form on 200
-// others).
+// 16384, k 128 to 16384 (the choice takes 1.3 and 0.8 % more than the best form on
+// two sets of 200 others).
 // Measured at K 7168 and N 4096, weights not in a cache (tokens: us): 1: 7.3
 // (form 0), 16: 9.1 (0), 32: 10.6 (1; 12.2 with 32 x 32), 64: 11.8 (2; 16.4 with
 // 64 x 32), 128: 15.6 (3; 18.6 with 32 x 32), 256: 19.5 (4; 29 with 64 x 128),
