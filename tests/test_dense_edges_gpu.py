@@ -1,0 +1,88 @@
+"""The dense operators on inputs at the edges of their ranges.
+
+u = 2^-24, half a step of fp32. The activation's value: exp2 and rcp of the
+hardware are within a step (2 u each), expf within a step too; then come at most
+the correction's product, the sum with 1, the quotient, the product with up and the
+scale's division, 1 u each: 9 u in all, and 1 u more for a code's own quotient.
+"""
+
+import pytest
+import torch
+
+import flaggems_sglang as fgs
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _silu(g, u):
+    g, u = g.double(), u.double()
+    return g * torch.sigmoid(g) * u
+
+
+@pytest.mark.parametrize("lo,hi,up", [(-20.0, 20.0, 3.0), (-86.9, 20.0, 1e15),
+                                      (-100.0, -86.0, 1e34), (80.0, 200.0, 0.5)])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_scale_of_one_gate(gpu, lo, hi, up, kind):
+    """Rows of one value, so a row's scale is its magnitude over the format's
+    largest: the silu's own accuracy from deep negative gates to large ones."""
+    g = torch.linspace(lo, hi, 30011)
+    x = torch.stack([g, torch.full_like(g, up)], 1)
+    top = 448 if kind == "fp8" else 127
+    ref = _silu(x[:, 0], x[:, 1]).abs() / top
+    for copies in (1, 8):  # one by one, and in whole vectors
+        wide = x.repeat_interleave(copies, 1).contiguous().to(gpu)
+        s = fgs.silu_and_mul_quant(wide, kind)[1].reshape(-1).double().cpu()
+        seen = ref * top > 1e-9  # (below, the scale's lower bound)
+        assert int(seen.sum()) > 15000
+        off = (s - ref).abs()[seen] / ref[seen]
+        assert off.max() <= 9 * U, f"{float(off.max()) / U} u"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,n", [(999, 2560), (1500, 250), (2048, 512)])
+def test_int8_codes_of_loud_channels(gpu, rows, n, dtype):
+    """Gates and ups of a few loud channels and of rows of differing norms
+    (gates to about 50): every code is the nearest to its value over the scale
+    but for the value's own roundings."""
+    gen = torch.Generator().manual_seed(rows + n)
+    x = torch.randn(rows, 2 * n, generator=gen)
+    x *= torch.where(torch.rand(2 * n, generator=gen) < 0.01, 8.0, 1.0)
+    x *= 0.5 + torch.rand(rows, 1, generator=gen)
+    x = x.to(dtype)
+    q, s = fgs.silu_and_mul_quant(x.to(gpu), "int8")
+    v = _silu(*x.chunk(2, -1))
+    ref = v.abs().amax(-1).clamp(min=1e-10) / 127
+    s = s.double().cpu()
+    assert ((s - ref).abs() <= 9 * U * ref).all()
+    t = v / s[:, None]
+    off = (q.double().cpu() - t).abs() - (0.5 + 10 * U * t.abs())
+    assert off.max() <= 0, float(off.max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [256, 250])
+def test_activation_of_infinite_gates(gpu, n, dtype):
+    """A gate of +infinity gives infinity, one of -infinity NaN, as the
+    formula's steps; finite ones beyond 87 their values, zero from about -200."""
+    x = torch.ones(6, 2 * n)
+    x[1, 5] = float("inf")
+    x[2, 6] = -float("inf")
+    x[3, 7], x[3, n + 7] = 300.0, -2.0
+    x[4, :n] = -1000.0
+    x[4, 8], x[4, 9] = float("nan"), 88.0
+    x[5, :n] = -200.0
+    x = x.to(dtype).to(gpu)
+    q, s = fgs.silu_and_mul_quant(x)
+    q, s = q.float().cpu(), s.cpu()
+    assert s[1, 0].isinf() and q[1, 5].isnan() and (q[1, 6:128] == 0).all()
+    assert s[2, 0].isnan() and not s[1:3, 1].isnan().any()
+    assert s[3, 0] == torch.tensor(600.0) / 448 and q[3, 7] == -448
+    assert s[4, 0].isnan() and (q[4, 128:] == 0).all()
+    assert (q[5] == 0).all() and (s[5] == torch.tensor(1e-10) / 448).all()
+    q, s = fgs.silu_and_mul_quant(x, "int8")
+    q, s = q.cpu(), s.cpu()
+    assert s[1].isinf() and s[2].isnan() and s[4].isnan() and (q[4] == 0).all()
+    assert s[3] == torch.tensor(600.0) / 127 and q[3, 7] == -127
