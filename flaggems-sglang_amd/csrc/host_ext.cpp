@@ -131,16 +131,37 @@ void* stream_of(int index) {
       .stream();
 }
 
+// The GPU `index` as the current one, and the interpreter's lock given away, for
+// a scope, however it is left.
+struct OnGpu {
+  explicit OnGpu(int index) : was(c10::hip::current_device()), moved(was != index) {
+    if (moved) c10::hip::set_device(static_cast<c10::DeviceIndex>(index));
+  }
+  ~OnGpu() {
+    if (moved) static_cast<void>(c10::hip::SetDevice(static_cast<c10::DeviceIndex>(was)));
+  }
+  OnGpu(const OnGpu&) = delete;
+  const int was;
+  const bool moved;
+};
+struct Unlocked {
+  Unlocked() : state(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state); }
+  Unlocked(const Unlocked&) = delete;
+  PyThreadState* const state;
+};
+
 // Runs a library entry with its GPU current and without the interpreter lock,
-// and raises what it returns.
-template <class F>
-void call(int index, const char* what, F&& f) {
-  const int was = c10::hip::current_device();
-  if (was != index) c10::hip::set_device(static_cast<c10::DeviceIndex>(index));
-  PyThreadState* state = PyEval_SaveThread();
-  const int rc = f();
-  PyEval_RestoreThread(state);
-  if (was != index) c10::hip::set_device(static_cast<c10::DeviceIndex>(was));
+// and raises what it returns. (The arguments are values by then: what asks a
+// tensor for its memory, which may raise, is the caller's expression.)
+template <class... P, class... A>
+void call(int index, const char* what, int32_t (*entry)(P...), A... args) {
+  int32_t rc;
+  {
+    const OnGpu gpu(index);
+    const Unlocked unlocked;
+    rc = entry(args...);
+  }
   if (rc == FGS_OK) return;
   refuse(rc == FGS_EINVAL ? PyExc_ValueError
                           : rc == FGS_EUNSUPPORTED ? PyExc_NotImplementedError : PyExc_RuntimeError,
@@ -186,7 +207,8 @@ float real(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw Raised{};
   return static_cast<float>(v);
 }
-const void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* floats(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
 
 // rms_norm(x, weight, eps, residual, weight_offset, quantisation, return_norm,
 // column_major, inplace) -> (norm, residual, q, scales)
@@ -238,14 +260,9 @@ PyObject* rms_norm(PyObject* const* args) {
   }
   const at::Tensor weight = wa.t->is_contiguous() ? *wa.t : wa.t->contiguous();
   void* stream = stream_of(index);
-  call(index, "fused_rms_norm", [&] {
-    return g_lib.rms_norm(ptr(xr.t), xr.stride, ptr(rr.t), rr.stride, ptr(weight), type,
-                          weight_type, eps, offset, rows, cols, const_cast<void*>(ptr(norm)),
-                          const_cast<void*>(ptr(res_out)), out_stride, mode,
-                          const_cast<void*>(ptr(q)),
-                          static_cast<float*>(const_cast<void*>(ptr(scales.t))), scales.row,
-                          scales.col, stream);
-  });
+  call(index, "fused_rms_norm", g_lib.rms_norm, ptr(xr.t), xr.stride, ptr(rr.t), rr.stride,
+       ptr(weight), type, weight_type, eps, offset, rows, cols, ptr(norm), ptr(res_out), out_stride,
+       mode, ptr(q), floats(scales.t), scales.row, scales.col, stream);
   if (inplace) written(res_out);
   return wrap_all<4>({norm, res_out, q, scales.t});
 }
@@ -269,12 +286,8 @@ PyObject* silu_and_mul_quant(PyObject* const* args) {
       make(shape, mode == FGS_QUANT_INT8_TOKEN ? at::kChar : at::kFloat8_e4m3fn, x);
   const Scales scales = make_scales(x, rows, n, mode, column_major);
   void* stream = stream_of(index);
-  call(index, "silu_and_mul_quant", [&] {
-    return g_lib.silu_and_mul_quant(ptr(xr.t), xr.stride, type, rows, n, gelu, mode,
-                                    const_cast<void*>(ptr(q)),
-                                    static_cast<float*>(const_cast<void*>(ptr(scales.t))),
-                                    scales.row, scales.col, stream);
-  });
+  call(index, "silu_and_mul_quant", g_lib.silu_and_mul_quant, ptr(xr.t), xr.stride, type, rows, n,
+       gelu, mode, ptr(q), floats(scales.t), scales.row, scales.col, stream);
   return wrap_all<2>({q, scales.t});
 }
 
@@ -340,13 +353,10 @@ PyObject* fp8_block_matmul(PyObject* const* args) {
       oa.t ? *oa.t : make(shape, out_type == FGS_DTYPE_BF16 ? at::kBFloat16 : at::kHalf, a);
   const int64_t ldo = oa.t && out.dim() == 2 ? out.stride(0) : n;
   void* stream = stream_of(index);
-  call(index, "fp8_block_matmul", [&] {
-    return g_lib.fp8_block_matmul(
-        ptr(ar.t), ar.stride, static_cast<const float*>(ptr(a_scale)), a_scale.stride(0),
-        a_scale.stride(1), ptr(wr.t), wr.stride, static_cast<const float*>(ptr(w_scale)),
-        ptr(bias), bias.defined() ? type_code(bias) : FGS_DTYPE_FP32, m, n, k, out_type, flags,
-        const_cast<void*>(ptr(out)), ldo, stream);
-  });
+  call(index, "fp8_block_matmul", g_lib.fp8_block_matmul, ptr(ar.t), ar.stride, floats(a_scale),
+       a_scale.stride(0), a_scale.stride(1), ptr(wr.t), wr.stride, floats(w_scale), ptr(bias),
+       bias.defined() ? type_code(bias) : FGS_DTYPE_FP32, m, n, k, out_type, flags, ptr(out), ldo,
+       stream);
   if (oa.t) {
     written(out);
     Py_INCREF(args[6]);

@@ -1,0 +1,109 @@
+"""The dense operators' host module on the CPU: the module's own source built
+for CPU tensors (host_on_cpu.cpp), each test in a process of its own, since
+what it holds against has ended the process."""
+
+import os
+import subprocess
+import sys
+import sysconfig
+import textwrap
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "flaggems-sglang_amd", "csrc")
+TORCH = os.path.dirname(torch.__file__)
+
+PRELUDE = """
+import ctypes, importlib.machinery, importlib.util, sys
+import torch
+path = sys.argv[1]
+loader = importlib.machinery.ExtensionFileLoader("_host", path)
+host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host", loader))
+loader.exec_module(host)
+lib = ctypes.CDLL(path)
+host.bind(*(ctypes.cast(getattr(lib, "host_test_" + name), ctypes.c_void_p).value
+            for name in ("last_error", "rms_norm", "silu_and_mul_quant", "fp8_block_matmul")))
+word = lambda name: ctypes.c_int.in_dll(lib, "host_test_" + name)
+gpu, calls, locked, rc = (word(name) for name in ("gpu", "calls", "locked", "rc"))
+FP8 = torch.float8_e4m3fn
+
+def norm(x, weight=None, residual=None, quant=0, inplace=False):
+    weight = torch.ones(x.shape[-1]) if weight is None else weight
+    return host.rms_norm(x, weight, 1e-6, residual, 0.0, quant, True, False, inplace)
+def act(x):
+    return host.silu_and_mul_quant(x, 1, False, False)
+def product(a=None, sa=None, w=None, sw=None, bias=None, out=None):
+    a = torch.zeros(4, 256).to(FP8) if a is None else a
+    sa = torch.ones(4, 2) if sa is None else sa
+    w = torch.zeros(48, 256).to(FP8) if w is None else w
+    sw = torch.ones(1, 2) if sw is None else sw
+    return host.fp8_block_matmul(a, sa, w, sw, bias, 0, out, 0)
+def refused(call, *kinds, text=""):
+    before = calls.value
+    try:
+        call()
+    except kinds or (RuntimeError,) as e:
+        assert text in str(e), str(e)
+    else:
+        raise AssertionError("not refused")
+    assert gpu.value == 0 and calls.value == before
+x = torch.ones(4, 256)
+"""
+
+
+@pytest.fixture(scope="module")
+def host_on_cpu(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("host") / "_host.so")
+    r = subprocess.run(
+        ["g++", "-O0", "-std=c++17", "-fPIC", "-Wall", "-shared", "-D__HIP_PLATFORM_AMD__=1",
+         "-DUSE_ROCM=1", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,
+         "-isystem", os.path.join(TORCH, "include"),
+         "-isystem", os.path.join(TORCH, "include/torch/csrc/api/include"),
+         "-isystem", sysconfig.get_paths()["include"], "-isystem", "/opt/rocm/include",
+         os.path.join(ROOT, "tests", "host_on_cpu.cpp"), "-o", so, "-L" + os.path.join(TORCH, "lib"),
+         "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"],
+        capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-4000:]
+
+    def run(code):
+        r = subprocess.run([sys.executable, "-c", PRELUDE + textwrap.dedent(code) + "\nprint('ok')",
+                            so], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0 and r.stdout.endswith("ok\n"), (
+            r.returncode, r.stdout[-2000:], r.stderr[-4000:])
+    return run
+
+
+def test_an_entry_runs_without_the_lock(host_on_cpu):
+    host_on_cpu("""
+        for call in (lambda: norm(x), lambda: act(x), product):
+            call()
+        assert (calls.value, locked.value, gpu.value) == (3, 0, 0)
+        rc.value = -2
+        for call in (lambda: norm(x), lambda: act(x), product):
+            try:
+                call()
+            except NotImplementedError as e:
+                assert "the entry's text" in str(e)
+            else:
+                raise AssertionError
+        assert (calls.value, locked.value, gpu.value) == (6, 0, 0)
+    """)
+
+
+def test_transformed_tensors_raise(host_on_cpu):
+    """Tensors of torch.vmap and torch.func have no memory to be asked for: an
+    error, not the end of the process, and the GPU that was current is so again."""
+    host_on_cpu("""
+        for f in (norm, act, lambda t: norm(x, t[0]), lambda t: norm(x, residual=t),
+                  lambda t: product(sa=t[:, :2]), lambda t: product(sw=t[:1, :2]),
+                  lambda t: product(bias=t[0, :48]),
+                  lambda t: product(out=t[:, :48].bfloat16())):
+            refused(lambda: torch.vmap(f)(torch.ones(3, 4, 256)))
+            refused(lambda: torch.func.jvp(f, (x,), (x,)))
+        codes = torch.zeros(3, 4, 256).to(FP8)
+        refused(lambda: torch.vmap(lambda t: product(a=t))(codes))
+        norm(x), act(x), product()
+        assert (calls.value, locked.value, gpu.value) == (3, 0, 0)
+    """)
