@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <ATen/hip/EmptyTensor.h>
@@ -71,6 +72,7 @@ int check_inputs(std::initializer_list<Arg> args) {
                                    " must be a GPU tensor: the fused-MoE kernels run only on the "
                                    "MI355X (no CPU path)");
   const bool grad = c10::GradMode::is_enabled();
+  const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Arg& a : args) {
     if (!a.t) continue;
     if (a.t->device() != first->device())
@@ -82,6 +84,10 @@ int check_inputs(std::initializer_list<Arg> args) {
       refuse(PyExc_RuntimeError, std::string(a.name) +
                                      " requires a gradient: this operator has no backward pass "
                                      "(call it under torch.no_grad())");
+    if (tangents && a.t->_fw_grad(0).defined())
+      refuse(PyExc_RuntimeError, std::string(a.name) +
+                                     " has a forward-mode tangent: this operator has no "
+                                     "forward-mode derivative (give it the primal)");
   }
   return first->get_device();
 }

@@ -15,8 +15,9 @@ The host side (checks of the arguments, allocation of the outputs with the
 torch caching allocator, the call on the current HIP stream of the tensors'
 GPU) is the extension module ``_host``; the arithmetic is in
 ``libfgs_moe.so`` (include/fgs_moe.h). There is no CPU path. None of these
-has a backward pass: an input that requires a gradient is refused while
-gradients are recorded.
+has a backward pass or a forward-mode derivative: an input that requires a
+gradient is refused while gradients are recorded, and so is a dual tensor of
+``torch.autograd.forward_ad``.
 
 The reference's fused-MoE path has no counterparts (its layer takes its input
 normalised, and src/flaggems_sglang/ops/fused_moe.py:170-185 rejects every

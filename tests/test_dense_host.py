@@ -107,3 +107,28 @@ def test_transformed_tensors_raise(host_on_cpu):
         norm(x), act(x), product()
         assert (calls.value, locked.value, gpu.value) == (3, 0, 0)
     """)
+
+
+def test_forward_mode_tangents_are_refused(host_on_cpu):
+    """A dual tensor's tangent would be lost: refused as a leaf that needs a
+    gradient is; its primal, and any tensor with tangents off, is taken."""
+    host_on_cpu("""
+        import torch.autograd.forward_ad as fwAD
+        with fwAD.dual_level():
+            def dual(t):
+                return fwAD.make_dual(t, torch.ones_like(t))
+            d = dual(x)
+            for call in (lambda: norm(d), lambda: act(d), lambda: norm(x, d[0].clone()),
+                         lambda: norm(x, residual=d), lambda: norm(x, residual=d, inplace=True),
+                         lambda: product(sa=dual(torch.ones(4, 2))),
+                         lambda: product(sw=dual(torch.ones(1, 2))),
+                         lambda: product(bias=dual(torch.ones(48))),
+                         lambda: product(out=dual(torch.zeros(4, 48).bfloat16()))):
+                refused(call, text="tangent")
+                with torch.no_grad():  # (which does not turn them off)
+                    refused(call, text="tangent")
+            norm(fwAD.unpack_dual(d).primal), act(x), product()
+            with fwAD._set_fwd_grad_enabled(False):
+                norm(d)
+        assert calls.value == 4
+    """)
