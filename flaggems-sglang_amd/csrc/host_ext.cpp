@@ -10,6 +10,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
@@ -63,6 +64,16 @@ Arg tensor_arg(PyObject* o, const char* name, bool optional = false) {
   return {name, &THPVariable_Unpack(o)};
 }
 
+// Whether all of a tensor's values lie inside its storage. (A freed one's have
+// no address, or only an offset for one, and the library takes a null residual
+// or bias for none.)
+bool in_memory(const at::Tensor& t) {
+  return !t._is_zerotensor() &&
+         t.storage().nbytes() >= at::detail::computeStorageNbytes(t.sizes(), t.strides(),
+                                                                  t.element_size(),
+                                                                  t.storage_offset());
+}
+
 // Every tensor given is on one GPU, holds its values and needs no gradient; that
 // GPU's index.
 int check_inputs(std::initializer_list<Arg> args) {
@@ -78,6 +89,12 @@ int check_inputs(std::initializer_list<Arg> args) {
     if (a.t->device() != first->device())
       refuse(PyExc_RuntimeError, std::string(a.name) + " is on " + a.t->device().str() +
                                      ", not on " + first->device().str());
+    if (!a.t->has_storage())  // (sparse, or inside a transformation)
+      refuse(PyExc_NotImplementedError, std::string(a.name) + " has no storage: this operator takes "
+                                                              "dense tensors, outside torch.func");
+    if (!in_memory(*a.t))
+      refuse(PyExc_RuntimeError,
+             std::string(a.name) + " has no memory for its values (a zero tensor, or freed)");
     if (a.t->is_neg())  // (its memory holds the values' negatives)
       refuse(PyExc_NotImplementedError, std::string(a.name) + " is a lazily negated view");
     if (grad && a.t->requires_grad())

@@ -86,3 +86,28 @@ def test_activation_of_infinite_gates(gpu, n, dtype):
     q, s = q.cpu(), s.cpu()
     assert s[1].isinf() and s[2].isnan() and s[4].isnan() and (q[4] == 0).all()
     assert s[3] == torch.tensor(600.0) / 127 and q[3, 7] == -127
+
+
+def test_tensors_that_cannot_be_taken(gpu):
+    """Inside a transformation, with a tangent, without memory: an error each,
+    before any launch; the process and the calls after them go on."""
+    x = torch.ones(4, 256, dtype=BF16, device=gpu)
+    w = torch.ones(256, dtype=BF16, device=gpu)
+    first = fgs.fused_rms_norm(x, w, residual=x)
+    calls = (lambda t: fgs.fused_rms_norm(t, w).norm, lambda t: fgs.silu_and_mul_quant(t)[1],
+             lambda t: fgs.fused_rms_norm(x, w, residual=t).norm)
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no storage"):
+            torch.vmap(call)(torch.ones(3, 4, 256, dtype=BF16, device=gpu))
+        with pytest.raises(RuntimeError, match="no storage|tangent"):
+            torch.func.jvp(call, (x,), (x,))
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, x)
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(dual)
+        freed = torch.ones(8, 256, dtype=BF16, device=gpu)[4:]
+        freed.untyped_storage().resize_(0)
+        with pytest.raises(RuntimeError, match="no memory"):
+            call(freed)
+    again = fgs.fused_rms_norm(x, w, residual=x)
+    assert torch.equal(again.norm, first.norm) and torch.equal(again.residual, x + x)

@@ -132,3 +132,38 @@ def test_forward_mode_tangents_are_refused(host_on_cpu):
                 norm(d)
         assert calls.value == 4
     """)
+
+
+def test_tensors_without_memory_are_refused(host_on_cpu):
+    """A residual or bias whose memory is gone is not one that was not given, and
+    a view's offset into nothing is no address."""
+    host_on_cpu("""
+        def freed(t, view=lambda t: t):
+            v = view(t)
+            t.untyped_storage().resize_(0)
+            return v
+        zeros = torch._efficientzerotensor
+        half = lambda t: t[t.shape[0] // 2:]
+        for call in (lambda: norm(x, residual=zeros((4, 256))),
+                     lambda: norm(x, residual=freed(torch.ones(4, 256))),
+                     lambda: norm(x, residual=freed(torch.ones(8, 256), half), inplace=True),
+                     lambda: norm(x, freed(torch.ones(512), half)),
+                     lambda: norm(freed(torch.ones(8, 256), half)),
+                     lambda: act(freed(torch.ones(8, 256), half)),
+                     lambda: product(bias=freed(torch.ones(48))),
+                     lambda: product(bias=zeros((48,))),
+                     lambda: product(sa=freed(torch.ones(8, 2), half)),
+                     lambda: product(out=freed(torch.ones(8, 48).bfloat16(), half)),
+                     lambda: product(a=freed(torch.zeros(8, 256).to(FP8), half))):
+            refused(call, text="no memory")
+        short = torch.ones(4, 256)
+        short.untyped_storage().resize_(4 * 1023)
+        refused(lambda: norm(short), text="no memory")
+        for call in (lambda: norm(x.to_sparse()), lambda: act(x.to_sparse_csr()),
+                     lambda: product(bias=torch.ones(48).to_sparse())):
+            refused(call, text="no storage")
+        # no values need none
+        norm(x[:0], residual=freed(torch.ones(0, 256)))
+        norm(x, residual=torch.ones(1, 256).expand(4, 256))
+        assert calls.value == 2
+    """)
