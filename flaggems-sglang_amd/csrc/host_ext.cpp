@@ -233,6 +233,27 @@ float real(PyObject* o) {
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const at::Tensor& t) { return static_cast<float*>(ptr(t)); }
 
+// Rows in memory, in bytes.
+struct Span {
+  const char* at;
+  int64_t rows, stride, bytes;
+  const char* end() const { return at + (rows - 1) * stride + bytes; }
+};
+Span span(const at::Tensor& t, int64_t rows, int64_t cols, int64_t stride) {
+  const int64_t e = t.element_size();
+  return {static_cast<const char*>(ptr(t)), rows, stride * e, cols * e};
+}
+// Whether a value of one may be one of the other. (Columns of one wider tensor,
+// rows the same stride apart, are not; other strides whose ranges cross count as
+// shared.)
+bool shared(const Span& a, const Span& b) {
+  if (a.rows == 0 || b.rows == 0 || a.end() <= b.at || b.end() <= a.at) return false;
+  const int64_t stride = a.rows == 1 ? b.stride : a.stride;
+  if ((a.rows > 1 && b.rows > 1 && a.stride != b.stride) || stride <= 0) return true;
+  const int64_t between = ((b.at - a.at) % stride + stride) % stride;
+  return between < a.bytes || between + b.bytes > stride;
+}
+
 // rms_norm(x, weight, eps, residual, weight_offset, quantisation, return_norm,
 // column_major, inplace) -> (norm, residual, q, scales)
 PyObject* rms_norm(PyObject* const* args) {
@@ -282,6 +303,13 @@ PyObject* rms_norm(PyObject* const* args) {
     scales = make_scales(x, rows, cols, mode, column_major);
   }
   const at::Tensor weight = wa.t->is_contiguous() ? *wa.t : wa.t->contiguous();
+  if (inplace) {
+    const Span to = span(res_out, rows, cols, out_stride), from = span(xr.t, rows, cols, xr.stride);
+    const bool same = to.at == from.at && (rows <= 1 || to.stride == from.stride);
+    if ((!same && shared(to, from)) || shared(to, span(weight, 1, cols, cols)))
+      refuse(PyExc_ValueError, "fused_rms_norm: an inplace residual may be x itself, but share no "
+                               "part of x's or the weight's memory otherwise");
+  }
   void* stream = stream_of(index);
   call(index, "fused_rms_norm", g_lib.rms_norm, ptr(xr.t), xr.stride, ptr(rr.t), rr.stride,
        ptr(weight), type, weight_type, eps, offset, rows, cols, ptr(norm), ptr(res_out), out_stride,
@@ -375,6 +403,14 @@ PyObject* fp8_block_matmul(PyObject* const* args) {
   const at::Tensor out =
       oa.t ? *oa.t : make(shape, out_type == FGS_DTYPE_BF16 ? at::kBFloat16 : at::kHalf, a);
   const int64_t ldo = oa.t && out.dim() == 2 ? out.stride(0) : n;
+  if (oa.t) {
+    const Span to = span(out, m, n, ldo);
+    if (shared(to, span(ar.t, m, k, ar.stride)) || shared(to, span(wr.t, n, k, wr.stride)) ||
+        shared(to, span(a_scale, m, (kb - 1) * a_scale.stride(1) + 1, a_scale.stride(0))) ||
+        shared(to, span(w_scale, 1, w_scale.numel(), w_scale.numel())) ||
+        (bias.defined() && shared(to, span(bias, 1, n, n))))
+      refuse(PyExc_ValueError, "fp8_block_matmul: out shares memory with an input");
+  }
   void* stream = stream_of(index);
   call(index, "fp8_block_matmul", g_lib.fp8_block_matmul, ptr(ar.t), ar.stride, floats(a_scale),
        a_scale.stride(0), a_scale.stride(1), ptr(wr.t), wr.stride, floats(w_scale), ptr(bias),

@@ -78,7 +78,8 @@ def fused_rms_norm(
     dozens of rows on. ``return_norm``: whether ``n`` comes back in x's type
     (default: where nothing is quantised). ``inplace``: the sum replaces
     ``residual``'s values and ``residual`` is the residual output (``x`` may be
-    ``residual`` itself, but share no part of its memory otherwise).
+    ``residual`` itself; an ``x`` or ``weight`` that shares its memory otherwise
+    is refused).
 
     A NaN in a row makes its outputs NaN (int8 codes 0, scale NaN). Returns
     ``RMSNormOutput(norm, residual, q, scales)``.
@@ -142,8 +143,8 @@ def fp8_block_matmul(
     ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
     rounded once to ``out_dtype`` (bf16 or fp16). ``out``: a tensor of the
     result's shape to write and return, whose type counts instead of
-    ``out_dtype``, whose rows may lie apart (2-D) and whose memory none of the
-    inputs shares.
+    ``out_dtype``, whose rows may lie apart (2-D); one that shares memory with
+    an input is refused.
     """
     code = _OUT_DTYPES.get(out_dtype, _capi.DTYPE_FP32)  # (refused there)
     return _capi.host().fp8_block_matmul(a, a_scale, w, w_scale, bias, code, out, _flags)

@@ -111,3 +111,21 @@ def test_tensors_that_cannot_be_taken(gpu):
             call(freed)
     again = fgs.fused_rms_norm(x, w, residual=x)
     assert torch.equal(again.norm, first.norm) and torch.equal(again.residual, x + x)
+
+
+def test_in_place_beside_its_input(gpu):
+    """x and an in-place residual as columns of one wider tensor, and refusals
+    where they overlap."""
+    gen = torch.Generator().manual_seed(2)
+    wide = torch.randn(37, 1024, generator=gen).to(BF16).to(gpu)
+    w = torch.randn(512, generator=gen).to(BF16).to(gpu)
+    x, r = wide[:, :512], wide[:, 512:]
+    ref = fgs.fused_rms_norm(x.contiguous(), w, residual=r.contiguous(), quant="fp8")
+    for bad in (wide[:, 256:768], wide[:, 1:513]):
+        with pytest.raises(ValueError, match="share no part"):
+            fgs.fused_rms_norm(x, w, residual=bad, inplace=True)
+    with pytest.raises(ValueError, match="share no part"):
+        fgs.fused_rms_norm(r[1:], w, residual=r[:36], inplace=True)
+    got = fgs.fused_rms_norm(x, w, residual=r, quant="fp8", inplace=True)
+    assert torch.equal(got.q.view(torch.uint8), ref.q.view(torch.uint8))
+    assert torch.equal(r, ref.residual) and torch.equal(x, wide[:, :512])

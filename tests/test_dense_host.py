@@ -167,3 +167,49 @@ def test_tensors_without_memory_are_refused(host_on_cpu):
         norm(x, residual=torch.ones(1, 256).expand(4, 256))
         assert calls.value == 2
     """)
+
+
+def test_outputs_that_share_an_inputs_memory_are_refused(host_on_cpu):
+    """An in-place residual may be x itself, or columns or rows beside x's; where
+    a row of x is another row's sum the result would depend on their order."""
+    host_on_cpu("""
+        flat = torch.ones(4 * 4096)
+        rows = lambda at, stride=256, n=4, cols=256: flat.as_strided((n, cols), (stride, 1), at)
+        for at, stride in ((256, 256), (1, 256), (768, 256), (255, 256), (0, 512), (100, 300)):
+            refused(lambda: norm(rows(at, stride), residual=rows(0), inplace=True), ValueError,
+                    text="share no part")
+        refused(lambda: norm(rows(0)[:1].expand(4, 256), residual=rows(0), inplace=True),
+                ValueError, text="share no part")
+        refused(lambda: norm(rows(255, 512), residual=rows(0, 512), inplace=True), ValueError,
+                text="share no part")
+        refused(lambda: norm(rows(257, 512), residual=rows(0, 512), inplace=True), ValueError,
+                text="share no part")
+        refused(lambda: norm(rows(8192), rows(300)[0], residual=rows(0), inplace=True), ValueError,
+                text="share no part")
+        for at, stride, n in ((0, 256, 4), (1024, 256, 4), (1024, 300, 4)):
+            norm(rows(at, stride, n), residual=rows(0), inplace=True)
+        for at in (256, 256 + 4 * 512, 511 - 255):  # columns of one wider tensor
+            norm(rows(at, 512), residual=rows(0, 512), inplace=True)
+        norm(rows(0, 512), residual=rows(256, 512), inplace=True)
+        norm(rows(256, 512, 1), residual=rows(0, 512, 1), inplace=True)
+        norm(rows(4, 512, 1), residual=rows(4, 256, 1), inplace=True)
+        norm(rows(0), rows(1024)[0], residual=rows(0), inplace=True)
+        norm(rows(0), rows(0)[0], residual=rows(0))  # (written nowhere)
+        assert calls.value == 11
+
+        m, n, k = 4, 48, 256
+        room = torch.zeros(1 << 16, dtype=torch.uint8)
+        at = lambda b, t, *shape: room[b:b + 2 ** 15].view(t).as_strided(
+            shape, [shape[1], 1] if len(shape) == 2 else [1])
+        out = at(0, torch.bfloat16, m, n)  # 384 bytes
+        for over in (dict(a=at(368, FP8, m, k)), dict(w=at(368, FP8, n, k)),
+                     dict(sa=at(380, torch.float32, m, 2)), dict(sw=at(380, torch.float32, 1, 2)),
+                     dict(bias=at(380, torch.float32, n)),
+                     dict(sa=at(0, torch.float32, 2, m).t())):
+            refused(lambda: product(out=out, **over), ValueError, text="shares memory")
+        product(out=out, a=at(384, FP8, m, k), w=at(2048, FP8, n, k),
+                sa=at(384, torch.float32, 2, m).t(), sw=at(384, torch.float32, 1, 2),
+                bias=at(384, torch.float32, n))
+        product(a=at(0, FP8, m, k), w=at(0, FP8, n, k))  # inputs may be each other's
+        assert calls.value == 13
+    """)
