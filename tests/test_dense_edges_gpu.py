@@ -8,8 +8,11 @@ scale's division, 1 u each: 9 u in all, and 1 u more for a code's own quotient.
 
 import pytest
 import torch
+from test_dense_ops_gpu import _layer, _product_ref, _rand, _run_layer
 
 import flaggems_sglang as fgs
+from flaggems_sglang import testing
+from oracle import moe_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +132,36 @@ def test_in_place_beside_its_input(gpu):
     got = fgs.fused_rms_norm(x, w, residual=r, quant="fp8", inplace=True)
     assert torch.equal(got.q.view(torch.uint8), ref.q.view(torch.uint8))
     assert torch.equal(r, ref.residual) and torch.equal(x, wide[:, :512])
+
+
+@pytest.mark.parametrize("m", [1, 19, 300])
+def test_layer_against_the_oracle(gpu, m):
+    """Both halves of the layer's run: the routed experts, fed with the norm's
+    16-bit output, against the oracle under the bounds of its own tests, and
+    their sum with the 64-bit product of the shared expert (the product's bound,
+    and half a step for the sum). The check sees experts mistaken for their
+    neighbours (planted in the oracle)."""
+    gen = torch.Generator().manual_seed(m + 5)
+    w, topk = _layer(gen, gpu)
+    x, residual = (_rand(gen, (m, 512), BF16, gpu) for _ in range(2))
+    n, h, q, s, routed, shared, out = _run_layer(w, topk, x, residual)
+    tw, ti = fgs.fused_topk(n.norm, n.norm.float() @ w["router"], topk)
+    tol = testing.TOL["fp8"]
+
+    def oracle(ids):
+        ref, mag = moe_ref.fused_moe(n.norm, w["w13"], w["w2"], tw, ids, mode="fp8",
+                                     w1_scale=w["w13_scale"], w2_scale=w["w2_scale"],
+                                     return_mag=True)
+        return ref, mag, *moe_ref.compare(routed, ref, tol["atol"], tol["rtol"], mag)
+
+    ref, mag, ok, max_abs, mean_rel = oracle(ti)
+    assert ok and mean_rel <= tol["mean_rel"], (max_abs, mean_rel)
+    wrong = oracle((ti + 1) % w["w2"].shape[0])
+    assert not wrong[2] and wrong[4] > tol["mean_rel"]
+    dense, terms = _product_ref(q, s, w["s2"], w["s2_scale"])
+    dense, terms = dense.cpu(), terms.cpu()
+    sums = (16 + 2 * 2 + 2) * 2.0 ** -23 + 7 * 2.0 ** -13
+    near = tol["atol"] + tol["rtol"] * mag.double() + 1.01 * sums * terms + 2.0 ** -8 * dense.abs()
+    whole = ref.double() + dense
+    off = (out.double().cpu() - whole).abs() - near - 2.0 ** -8 * (whole.abs() + near)
+    assert off.max() <= 0, float(off.max())
