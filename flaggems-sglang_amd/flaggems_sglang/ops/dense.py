@@ -67,8 +67,9 @@ def fused_rms_norm(
 
     in fp32; each output is rounded once. ``x`` and ``residual`` (of x's
     shape) bf16, fp16 or fp32, ``weight [cols]`` of x's type or fp32;
-    ``weight_offset=1`` for weights stored about zero. ``cols`` up to 65536;
-    multiples of 8 with 16-byte aligned rows run fastest.
+    ``weight_offset=1`` for weights stored about zero. ``cols`` from 1 to 65536;
+    multiples of 8 with 16-byte aligned rows run fastest (4096 x 7168 bf16 with
+    four outputs 45 us, x 7167 163). Fewer than 2^22 rows, of few columns more.
 
     ``quant="fp8"``: ``q`` e4m3fn with ``scales [..., ceil(cols / 128)]`` per
     128 columns, ``"int8"``: ``q`` int8 with ``scales [...]`` per row (the
@@ -103,7 +104,8 @@ def silu_and_mul_quant(
     codes taken from the unrounded fp32 product.
 
     ``activation``: "silu", or "gelu" (exact, erf). ``quant`` and
-    ``column_major_scales`` as for :func:`fused_rms_norm`; ``n`` up to 65536.
+    ``column_major_scales`` as for :func:`fused_rms_norm`; ``n`` from 1 to 65536
+    (odd ones one value a load: 4096 x 7168 31 us, x 7167 76), rows as there.
     Returns ``(q [..., n], scales)``.
     """
     gelu = _ACTIVATIONS.get(activation)
@@ -135,12 +137,13 @@ def fp8_block_matmul(
     ``per_token_group_quant_fp8``, :func:`fused_rms_norm` and
     :func:`silu_and_mul_quant` return, row- or column-major: with rows that lie
     apart a block's scales are a cache line each, 3 to 19 % more time from 64
-    rows on), ``w [n, k]``
-    with ``w_scale [ceil(n / 128), ceil(k / 128)]``
-    (``quant.quantize_fp8_block``). ``k`` is a multiple of 16, ``n`` and the
-    number of rows are any. Sums are fp32 (of groups of eight products that the
-    matrix instruction aligns to the largest and cuts 13 bits below it),
-    ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
+    rows on), ``w [n, k]`` with ``w_scale [ceil(n / 128), ceil(k / 128)]``
+    (``quant.quantize_fp8_block``). ``k`` is a multiple of 16 and ``n`` is at
+    least 1; both and the number of rows (0 among them) go up to 2^22. Sums are
+    fp32, of groups of eight products that the matrix instruction aligns to the
+    largest and cuts 13 bits below it: about 1.5e-5 of a result from normal
+    data, at most 7 * 2^-13 of each group's largest product, also where these
+    cancel. ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
     rounded once to ``out_dtype`` (bf16 or fp16). ``out``: a tensor of the
     result's shape to write and return, whose type counts instead of
     ``out_dtype``, whose rows may lie apart (2-D); one that shares memory with

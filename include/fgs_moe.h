@@ -441,7 +441,8 @@ int32_t fgs_moe_silu_and_mul_quant(const void* x, int64_t x_stride, int32_t dtyp
  *   bias_dtype, or null; out [m, n] of out_dtype (bf16 or fp16) with row
  *   stride ldo
  * The matrix instruction cuts each of eight neighbouring products 13 bits
- * below the largest one: about 1.5e-5 of a result from normal data.
+ * below the largest one: about 1.5e-5 of a result from normal data, at most
+ * 7 * 2^-13 of each eight's largest product (also where these cancel).
  * k a positive multiple of 16, m, n and k up to 2^22; a and w rows 16-byte
  * aligned and at most 2^22 apart, a_scale rows at most 2^20. `flags`: 0, or
  * FGS_BLOCK_FORM(f), the kernel form f whatever the sizes (for measurement
