@@ -29,8 +29,6 @@
 namespace fgs {
 
 // ---------------------------------------------------------------- output ---
-// Four neighbouring output columns n .. n + 3 of token m (`left`: columns of
-// them that exist; vec: the row start and n allow one 8-byte store).
 // The bias of output column n in two steps, so that what lies between covers
 // the load: its bits (columns past the end: the last one's; without a bias 0),
 // then their value. The kernels load the bits before their first load into LDS
@@ -57,6 +55,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (TY == FGS_DTYPE_BF16) return cvt_pk_bf16(lo, hi);
   else return Elem<TY>::from_f32(lo) | static_cast<uint32_t>(Elem<TY>::from_f32(hi)) << 16;
 }
+// Four neighbouring output columns of a token from element `at` on (`left`:
+// columns of them that exist; vec: the address allows one 8-byte store).
 template <int TY>
 __device__ __forceinline__ void store4(void* out, int64_t at, f32x4 v, int64_t left, bool vec) {
   typedef typename Elem<TY>::raw raw;
@@ -581,10 +581,10 @@ __global__ __launch_bounds__(C::NW * 64, C::WPE) void block_gemm_tiled_kernel(
   // results, where they would overwrite registers of the lanes outside.
   settle();
 
-  // lane: token r16 of each tile, output columns 4 g .. 4 g + 3 of each
-  // Through this wave's share of the ring, so that 16 bytes a lane leave as
-  // whole row segments (four columns a lane are 32 bytes of 16 rows each:
-  // 257 x 257 x 272 took 22 us so). A staged row's 16-byte chunks are
+  // A lane holds token r16 of each tile, output columns 4 g .. 4 g + 3. They go
+  // through this wave's share of the ring, so that 16 bytes a lane leave as
+  // whole row segments (stored from here, four columns a lane are 32 bytes of 16
+  // rows each: 257 x 257 x 272 took 22 us). A staged row's 16-byte chunks are
   // XORed with the row: the 16 rows a write covers meet all banks.
   constexpr int CH = CT * 2;                 // chunks of a row
   constexpr int ROWS = 64 / CH;              // rows a store instruction covers
