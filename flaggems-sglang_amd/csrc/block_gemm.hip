@@ -289,9 +289,9 @@ __global__ __launch_bounds__(C::KW * 64, 2) void block_gemm_skinny_kernel(
 // rows of a k block (128 bytes each) and the block's scales stream into a ring
 // of STAGES LDS slots by LDS-DMA. A wave keeps its tokens' fragments of a
 // block in registers and takes its weight rows 16 at a time; an MFMA's four
-// FMAs follow three MFMAs behind it. 256 x 256: 4096 x 4096 x 7168 104 us (2.3
-// PFLOP/s, MFMA 50 % busy, one round of tiles with its fill and epilogue), 8192 x
-// 14336 x 7168 680 (2.5 PFLOP/s, 66 %: the clock falls to 1.7 - 1.9 GHz under
+// FMAs follow three MFMAs behind it. 256 x 256: 4096 x 4096 x 7168 103 us (2.3
+// PFLOP/s, MFMA 53 % busy, one round of tiles with its fill and epilogue), 8192 x
+// 14336 x 7168 658 (2.6 PFLOP/s, 66 %: the clock falls to 1.7 - 1.9 GHz under
 // random data; zeros run 3.5 PFLOP/s).
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int WPE_>
 struct BlockCfg {

@@ -47,7 +47,10 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
 // WAVE: a wave takes a row (4 a workgroup), else the workgroup one row.
 // Bound by memory with many rows: bf16 with residual and all four outputs, 8192
 // x 7168, 97 us (5.5 TB/s); by load, sum and store one after the other with few:
-// 1 x 7168 3.5 us, 61 x 4096 without codes 2.7.
+// 1 x 7168 3.5 us, 61 x 4096 without codes 2.7. Column-major scales leave as
+// single words, each a 32-byte sector of its own: 309 MB written where row-major
+// ones take 295, 97 us and 95 (the product that reads them gains more: its loads).
+// Rows of odd length one value a load: 4096 x 7168 45 us, x 7167 163.
 template <int TY, int WTY, bool VEC, bool WAVE, bool RES, int NV>
 __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
     const RmsNormParams p) {
@@ -142,7 +145,9 @@ __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
 // The exact gelu by erfc, which keeps its relative accuracy for negative gates
 // (1 + erf cancels there), and the silu with the rounding of its exponent's
 // argument made good: a scale may come from such values alone.
-// bf16 to e4m3, 8192 x 14336 118 us (5.0 TB/s), 8 x 2048 2.2 us.
+// bf16 to e4m3, 8192 x 14336 117 us (5.1 TB/s), 8 x 2048 2.1 us; with row-major
+// scales 114 (121 MB written, 147 with column-major ones, a sector each); with
+// gelu 197 and 2.7 (erfc's instructions). 4096 x 7168 31 us, x 7167 76.
 __device__ __forceinline__ float gelu_tail_mul(float g, float u) {
   return 0.5f * g * erfcf(-0.70710678118654752f * g) * u;
 }
