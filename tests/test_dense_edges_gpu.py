@@ -65,6 +65,32 @@ def test_int8_codes_of_loud_channels(gpu, rows, n, dtype):
     assert off.max() <= 0, float(off.max())
 
 
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,n", [(300, 2560), (1500, 250), (4096, 6144)])
+def test_codes_of_loud_channels(gpu, activation, rows, n):
+    """As above to e4m3, and with the exact gelu: its erfc's argument, rounded in
+    its constant and its product, moves a negative gate's value by 2 g^2 u, and
+    erfc itself is taken to be within 64 u."""
+    gen = torch.Generator().manual_seed(rows - n)
+    x = torch.randn(rows, 2 * n, generator=gen)
+    x *= torch.where(torch.rand(2 * n, generator=gen) < 0.01, 8.0, 1.0)
+    x *= 0.5 + torch.rand(rows, 1, generator=gen)
+    x = x.to(BF16)
+    g, u = x.to(gpu).double().chunk(2, -1)
+    if activation == "silu":
+        v, rel = g * torch.sigmoid(g) * u, 10 * U
+    else:
+        v, rel = g * 0.5 * torch.erfc(-g / 2 ** 0.5) * u, (2 * g.clamp(max=0) ** 2 + 74) * U
+    for kind in ("fp8", "int8"):
+        q, s = fgs.silu_and_mul_quant(x.to(gpu), kind, activation=activation)
+        s = s.double().reshape(rows, -1)
+        t = v / s.repeat_interleave(128 if kind == "fp8" else n, 1)[:, :n]
+        half = torch.full_like(t, 0.5) if kind == "int8" else (
+            2.0 ** -4 * t.abs()).clamp(min=2.0 ** -10)
+        off = (q.double() - t).abs() - (half + rel * t.abs())
+        assert off.max() <= 0, float(off.max())
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("n", [256, 250])
 def test_activation_of_infinite_gates(gpu, n, dtype):
