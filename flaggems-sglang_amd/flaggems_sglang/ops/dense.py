@@ -82,7 +82,8 @@ def fused_rms_norm(
     ``residual`` itself; an ``x`` or ``weight`` that shares its memory otherwise
     is refused).
 
-    A NaN in a row makes its outputs NaN (int8 codes 0, scale NaN). Returns
+    A NaN in a row makes its outputs NaN (int8 codes 0, scale NaN); a row whose
+    squares sum past fp32's range (values of about 1e19) becomes zeros. Returns
     ``RMSNormOutput(norm, residual, q, scales)``.
     """
     mode = _QUANTS.get(quant)
@@ -143,7 +144,8 @@ def fp8_block_matmul(
     fp32, of groups of eight products that the matrix instruction aligns to the
     largest and cuts 13 bits below it: about 1.5e-5 of a result from normal
     data, at most 7 * 2^-13 of each group's largest product, also where these
-    cancel. ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
+    cancel. The two scales are multiplied first, in fp32, whose range their
+    product has to stay in. ``bias [n]`` (fp32, bf16 or fp16) is added to them, and the result is
     rounded once to ``out_dtype`` (bf16 or fp16). ``out``: a tensor of the
     result's shape to write and return, whose type counts instead of
     ``out_dtype``, whose rows may lie apart (2-D); one that shares memory with
