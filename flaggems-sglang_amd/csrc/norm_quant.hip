@@ -145,9 +145,10 @@ __global__ __launch_bounds__(WAVE ? 256 : kRowThreads) void rms_norm_kernel(
 // The exact gelu by erfc, which keeps its relative accuracy for negative gates
 // (1 + erf cancels there), and the silu with the rounding of its exponent's
 // argument made good: a scale may come from such values alone.
-// bf16 to e4m3, 8192 x 14336 117 us (5.1 TB/s), 8 x 2048 2.1 us; with row-major
-// scales 114 (121 MB written, 147 with column-major ones, a sector each); with
-// gelu 197 and 2.7 (erfc's instructions). 4096 x 7168 31 us, x 7167 76.
+// bf16 to e4m3, 8192 x 14336 115 us (5.1 TB/s), 8 x 2048 2.1 us, with gelu 190
+// and 2.7 (erfc's instructions). Column-major scales are a 32-byte sector each:
+// 147 MB written, 121 with row-major ones, 114 us and 111. 4096 x 7168 30 us, x
+// 7167 71.
 __device__ __forceinline__ float gelu_tail_mul(float g, float u) {
   return 0.5f * g * erfcf(-0.70710678118654752f * g) * u;
 }
@@ -160,7 +161,7 @@ __device__ __forceinline__ float gelu_tail_mul(float g, float u) {
 // reciprocal. An int8 code is a whole step off where a value lies on the wrong
 // side of a tie: of 40 x 2.6 million codes 3 differ from those of the formula
 // in rounded steps, 13 without it. 999 x 2560 to int8 5.95 us, 5.75 without, 5.5
-// with 2^t alone; e4m3, whose steps do not show it: 8192 x 14336 121, 118, 114.
+// with 2^t alone; e4m3, whose steps do not show it: 8192 x 14336 121, 117, 114.
 // A vector with a gate beyond 87 takes the plain formula, and below -87, where
 // exp(-g) overflows, g exp(g) u in halves: so a gate of +infinity gives
 // infinity, and one of -infinity NaN (infinity times zero).
@@ -360,10 +361,12 @@ int launch_gated_quant(const GatedQuantParams& p, int dtype, hipStream_t stream)
   RowShape s = row_shape(p.rows, chunks, vec);
   unsigned gy = 1;
   // e4m3 groups are apart, so a row takes several workgroups of 256 threads --
-  // but for many wide rows, which read their two halves best as a whole (8192
-  // x 14336 120 -> 110 us, x 7168 58 -> 56; 1024 x 14336 13.6 -> 15.4, 8192 x
-  // 4096 31 -> 32).
-  const bool whole = p.rows >= 4096 && p.n >= 6144;
+  // but for wide rows of more than the 256 MB cache beside the memory holds,
+  // which read their two halves best as a whole (bf16 by parts and whole: 2048 x
+  // 14336 31 and 35 us, 4096 57 and 61, 6000 87 and 84, 8192 118 and 111, 16384
+  // 238 and 213; 8192 x 7168 56 and 54, 52 and 53 where the input was just used;
+  // 32768 x 7168 240 and 205, 16384 x 4096 61 and 61).
+  const bool whole = p.n >= 6144 && p.rows * p.n * 2 * elem_bytes(dtype) > int64_t{256} << 20;
   if (p.quant == FGS_QUANT_FP8_GROUP && !s.wave && !whole) {
     s.nv = 1;
     s.threads = static_cast<int>(std::min<int64_t>(256, (chunks + 63) / 64 * 64));

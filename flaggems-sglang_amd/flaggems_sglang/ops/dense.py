@@ -106,7 +106,7 @@ def silu_and_mul_quant(
 
     ``activation``: "silu", or "gelu" (exact, erf). ``quant`` and
     ``column_major_scales`` as for :func:`fused_rms_norm`; ``n`` from 1 to 65536
-    (odd ones one value a load: 4096 x 7168 31 us, x 7167 76), rows as there.
+    (odd ones one value a load: 4096 x 7168 31 us, x 7167 71), rows as there.
     Returns ``(q [..., n], scales)``.
     """
     gelu = _ACTIVATIONS.get(activation)

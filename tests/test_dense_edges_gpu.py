@@ -191,3 +191,20 @@ def test_layer_against_the_oracle(gpu, m):
     whole = ref.double() + dense
     off = (out.double().cpu() - whole).abs() - near - 2.0 ** -8 * (whole.abs() + near)
     assert off.max() <= 0, float(off.max())
+
+
+@pytest.mark.parametrize("rows,n,dtype", [(11000, 6144, BF16), (10500, 6500, BF16),
+                                          (5500, 14336, BF16), (5600, 6144, F32),
+                                          (2100, 40000, BF16), (1100, 65535, BF16)])
+def test_activation_of_inputs_past_the_cache(gpu, rows, n, dtype):
+    """Wide rows of more than 256 MB take a workgroup each: the bits of the same
+    rows a few hundred at a time."""
+    gen = torch.Generator(device=gpu).manual_seed(rows)
+    x = torch.randn(rows, 2 * n, device=gpu, dtype=dtype, generator=gen)
+    assert x.nbytes > 256 << 20
+    for activation in ("silu", "gelu"):
+        q, s = fgs.silu_and_mul_quant(x, activation=activation, column_major_scales=True)
+        for at in range(0, rows, 700):
+            q2, s2 = fgs.silu_and_mul_quant(x[at:at + 700], activation=activation)
+            assert torch.equal(q[at:at + 700].view(torch.uint8), q2.view(torch.uint8))
+            assert torch.equal(s[at:at + 700], s2)
