@@ -266,4 +266,90 @@ int block_gemm_form(int64_t m, int64_t n, int64_t k, int32_t flags);
 std::string block_gemm_name(int form);
 int launch_block_gemm(const BlockGemmParams& p, int form, hipStream_t stream);
 
+// ---- products of 16-bit matrices and their gradients (linear.hip) ----
+// out[m, n] = sum_r Q[m, r] P[n, r], per group of rows. Forward: Q the tokens'
+// rows, P the weights'; the tokens' gradient: Q dz, P the weights by column; the
+// weights' gradient: Q and P dz and the tokens by column.
+struct LinearParams {
+  const void* q;
+  const void* p;
+  int64_t ldq, ldp;        // row strides in elements
+  int64_t p_group;         // elements between the groups' matrices of P
+  void* out;               // contiguous
+  const void* bias;        // [groups, wide] or null
+  const void* residual;    // or null
+  int64_t ldr;
+  void* z;                 // what the activation is taken of, [rows, wide], or null
+  const int32_t* counts;   // rows of each group, or null: one of all rows
+  int32_t groups, rows;    // rows: of all tokens
+  int32_t red;             // length of the sums (weights' gradient: counts')
+  int32_t m;               // weights' gradient: rows of its output
+  int32_t n;               // columns of the output
+  int32_t act;             // FGS_ACT_*
+};
+enum { kLinearForward = 0, kLinearGated = 1, kLinearDgrad = 2, kLinearWgrad = 3 };
+constexpr int64_t kLinearMaxRows = 1 << 30, kLinearMaxCols = 1 << 20, kLinearMaxStride = 1 << 21;
+bool linear_flags_ok(int32_t flags);
+int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
+                int32_t flags);
+std::string linear_form_name(int mode, int form);
+int launch_linear(const LinearParams& p, int mode, int dtype, int form, hipStream_t stream);
+
+// dz = dout act'(z) (gated: of [gate | up]), values in `dtype`.
+struct LinearActGradParams {
+  const void* dout;
+  int64_t ldd;
+  const void* z;
+  void* dz;
+  int64_t rows, n;
+  int32_t act, gated;
+};
+int launch_linear_act_grad(const LinearActGradParams& p, int dtype, hipStream_t stream);
+// Sums of dz's rows by group.
+struct LinearBiasGradParams {
+  const void* dz;
+  int64_t ldd;
+  const int32_t* counts;
+  int32_t groups, rows;
+  int64_t n;
+  float* part;  // [parts, groups, n] where parts > 1
+  int32_t parts;
+  void* out;
+};
+int linear_bias_parts(int64_t groups, int64_t rows, int64_t n);
+int launch_linear_bias_grad(const LinearBiasGradParams& p, int dtype, hipStream_t stream);
+
+// ---- tokens sorted by expert and back (permute.hip) ----
+struct PermuteParams {
+  const uint8_t* x;       // [m] rows of `bytes`, x_stride bytes apart
+  int64_t x_stride, bytes, m;
+  int32_t topk, experts;
+  const int32_t* ids;     // [m, topk], or null: the order is given
+  const int32_t* place;   // with ids: each slot's row, those of no expert last
+  int32_t* row_of_slot;   // [m, topk], -1: none (with ids: written)
+  int32_t* slot_of_row;   // [m * topk], likewise
+  uint8_t* rows;          // [m * topk, bytes]
+};
+int launch_permute(const PermuteParams& p, hipStream_t stream);
+struct UnpermuteParams {
+  const void* rows;  // [n_rows, cols], ld apart
+  int64_t ld, n_rows, cols, m;
+  int32_t topk;
+  const int32_t* row_of_slot;
+  const float* weights;  // [m, topk], or null: ones
+  void* out;             // [m, cols]; null: the gradients
+  const void* dout;      // [m, cols], ldd apart
+  int64_t ldd;
+  const int32_t* slot_of_row;
+  void* drows;      // [n_rows, cols] or null
+  float* dweights;  // [m, topk] or null
+};
+int launch_unpermute(const UnpermuteParams& p, int dtype, hipStream_t stream);
+
+// dlogits of topk_gating's weights (gating.hip).
+int launch_topk_gating_grad(const void* logits, bool bf16_in, int64_t m, int num_experts, int topk,
+                            bool sigmoid, bool renormalize, const float* weights,
+                            const int32_t* ids, const float* dweights, void* dlogits,
+                            hipStream_t stream);
+
 }  // namespace fgs

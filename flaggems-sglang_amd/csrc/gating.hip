@@ -159,4 +159,99 @@ int launch_topk_gating(const void* logits, bool bf16_in, int64_t m,
   return check_launch("topk_gating_kernel");
 }
 
+// The weights' gradient, a wave a token. With w the weights, d their gradient and
+// D = sum d w over the picks:
+//   softmax                dl[j] = p[j] ([j picked] d - D), p of all logits
+//   softmax, renormalised  dl[pick] = w (d - D): w is the picks' own softmax
+//   sigmoid                dl[pick] = d w (1 - w)
+//   sigmoid, renormalised  dl[pick] = (d - D) w (1 - s), s = sigmoid(l), w = s / sum s
+// and 0 elsewhere. Lane r holds pick r; every lane looks its experts up among them.
+template <int VPL>
+__global__ __launch_bounds__(256) void topk_gating_grad_kernel(
+    const void* __restrict__ logits, int bf16_in, int64_t m, int num_experts, int topk, int sigmoid,
+    int renormalize, const float* __restrict__ weights, const int32_t* __restrict__ ids,
+    const float* __restrict__ dweights, void* __restrict__ dlogits) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  if (row >= m) return;  // whole wave
+  const int64_t base = row * num_experts;
+  auto logit = [&](int e) {
+    return bf16_in ? bf16_bits_to_f32(static_cast<const uint16_t*>(logits)[base + e])
+                   : static_cast<const float*>(logits)[base + e];
+  };
+  const bool pick = lane < topk;
+  const int id = pick ? ids[row * topk + lane] : -1;
+  const float w = pick ? weights[row * topk + lane] : 0.f;
+  const float d = pick ? dweights[row * topk + lane] : 0.f;
+  auto add = [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  };
+  const float D = __uint_as_float(wave_reduce(__float_as_uint(pick ? d * w : 0.f), add));
+
+  // what the picks add to their experts, and the factor of p that all get
+  float mine = 0.f;
+  if (sigmoid) {
+    const float s = renormalize && pick ? 1.f / (1.f + __expf(-logit(id))) : w;
+    mine = renormalize ? (d - D) * w * (1.f - s) : d * w * (1.f - w);
+  } else {
+    mine = renormalize ? w * (d - D) : d * w;
+  }
+  float v[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) v[i] = 0.f;
+  if (!sigmoid && !renormalize) {
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = i * 64 + lane;
+      v[i] = e < num_experts ? logit(e) : -INFINITY;
+      mx = fmaxf(mx, v[i]);
+    }
+    mx = __uint_as_float(wave_reduce(__float_as_uint(mx), [](uint32_t a, uint32_t b) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      v[i] = i * 64 + lane < num_experts ? __expf(v[i] - mx) : 0.f;
+      sum += v[i];
+    }
+    sum = __uint_as_float(wave_reduce(__float_as_uint(sum), add));
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] *= -D / sum;
+  }
+  for (int r = 0; r < topk; ++r) {
+    const int at = __builtin_amdgcn_readlane(id, r);
+    const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), r));
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] += at == i * 64 + lane ? g : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = i * 64 + lane;
+    if (e >= num_experts) continue;
+    if (bf16_in) static_cast<uint16_t*>(dlogits)[base + e] = f32_to_bf16_bits(v[i]);
+    else static_cast<float*>(dlogits)[base + e] = v[i];
+  }
+}
+
+int launch_topk_gating_grad(const void* logits, bool bf16_in, int64_t m, int num_experts, int topk,
+                            bool sigmoid, bool renormalize, const float* weights,
+                            const int32_t* ids, const float* dweights, void* dlogits,
+                            hipStream_t stream) {
+  if (m == 0) return FGS_OK;
+  const dim3 grid(static_cast<unsigned>((m + 3) / 4));
+  const int vpl = (num_experts + 63) / 64;
+#define FGS_GATING_GRAD_CASE(V)                                                            \
+  hipLaunchKernelGGL(topk_gating_grad_kernel<V>, grid, dim3(256), 0, stream, logits,       \
+                     bf16_in ? 1 : 0, m, num_experts, topk, sigmoid ? 1 : 0,               \
+                     renormalize ? 1 : 0, weights, ids, dweights, dlogits)
+  if (vpl <= 1) FGS_GATING_GRAD_CASE(1);
+  else if (vpl <= 2) FGS_GATING_GRAD_CASE(2);
+  else if (vpl <= 4) FGS_GATING_GRAD_CASE(4);
+  else if (vpl <= 8) FGS_GATING_GRAD_CASE(8);
+  else FGS_GATING_GRAD_CASE(16);
+#undef FGS_GATING_GRAD_CASE
+  return check_launch("topk_gating_grad_kernel");
+}
+
 }  // namespace fgs

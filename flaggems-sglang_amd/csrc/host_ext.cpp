@@ -1,6 +1,7 @@
 // Python module `flaggems_sglang._host`: the host side of the dense operators
-// (flaggems_sglang.ops.dense) -- argument checks, output allocation, the
-// current stream, the call into libfgs_moe.so's C ABI. A decode step's kernels
+// (flaggems_sglang.ops.dense) and of the routed layer's steps (host_steps.h) --
+// argument checks, output allocation, the current stream, the call into
+// libfgs_moe.so's C ABI. A decode step's kernels
 // take 2 to 8 us and a launch 3.3; the same steps in Python took 9.6 to 13 us a
 // call (a norm with four outputs 13.2, here 5.8; the dispatcher's empty() 7.2),
 // so at one token the host was what a layer waited for.
@@ -17,7 +18,9 @@
 #include <c10/hip/HIPFunctions.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -424,6 +427,8 @@ PyObject* fp8_block_matmul(PyObject* const* args) {
   return wrap(out);
 }
 
+#include "host_steps.h"
+
 // bind(addresses of fgs_moe_last_error, _rms_norm, _silu_and_mul_quant,
 // _fp8_block_matmul)
 PyObject* bind(PyObject* const* args) {
@@ -443,7 +448,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   try {
-    if (F != bind && !g_lib.last_error) refuse(PyExc_RuntimeError, "the library is not bound");
+    if (F != bind && F != bind_steps && !g_lib.last_error) refuse(PyExc_RuntimeError, "the library is not bound");
     return F(args);
   } catch (const Refusal& r) {
     PyErr_SetString(r.type, r.text.c_str());
@@ -464,6 +469,15 @@ PyMethodDef g_methods[] = {
     method<rms_norm, 9>("rms_norm"),
     method<silu_and_mul_quant, 4>("silu_and_mul_quant"),
     method<fp8_block_matmul, 8>("fp8_block_matmul"),
+    method<bind_steps, 12>("bind_steps"),
+    method<permute, 3>("permute"),
+    method<permute_rows, 3>("permute_rows"),
+    method<unpermute, 3>("unpermute"),
+    method<unpermute_grad, 7>("unpermute_grad"),
+    method<topk_gating_grad, 6>("topk_gating_grad"),
+    method<linear, 9>("linear"),
+    method<linear_grad, 11>("linear_grad"),
+    method<foreign_leaf, 1>("foreign_leaf"),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods,

@@ -1,0 +1,470 @@
+// Products of 16-bit matrices with fp32 sums, and their gradients, dense or per
+// group of rows (the experts' of tokens sorted by expert):
+//   out[m, n] = sum_r Q[m, r] P[n, r]
+//   forward    Q = x    [rows, k],      P = w[e] [n, k]
+//   dx         Q = dz   [rows, n],      P = w[e] by column, [k, n]
+//   dw[e]      Q = dz   by column,      P = x by column, r over the group's rows
+// An operand whose sums run along its rows ("along") is staged in LDS as rows of
+// 64 sums' values; one whose sums run across rows ("across") as 64 rows of the
+// tile's columns, which the LDS reads transpose on the way to the registers
+// (ds_read_b64_tr_b16): no transposed copy is ever made.
+#include <algorithm>
+#include <atomic>
+#include <string>
+
+#include "linear_common.h"
+
+namespace fgs {
+
+// ------------------------------------------------------------------ tiles ---
+// A workgroup of 2 x 2 waves owns a T x T tile; a wave (T / 2)^2 of it in
+// 32x32x16 MFMAs, P as the row operand: a lane's results are then runs of four
+// adjacent output columns of one output row. Stages of 64 sums stream into an LDS
+// ring by buffer loads: P's slots are three, Q's two, so that P is in flight a
+// stage longer. What lies outside an operand -- rows past the tile's, sums past
+// the end -- is outside its buffer resource or sent there: such loads write zeros
+// to LDS (measured), so a sum's tail adds 0 * 0 whatever memory holds there.
+template <int T_>
+struct LinearTile {
+  static constexpr int T = T_;
+  static constexpr int NB = T / 64;           // 32-wide blocks of a wave, each way
+  static constexpr int NL = T / 32;           // loads of a wave per operand and stage
+  static constexpr int SLOT = T * 128;        // bytes
+  static constexpr int LDS = 5 * SLOT;        // Q: slots 0, 1; P: 2, 3, 4
+  static constexpr int STAGING = SLOT;        // a wave's part in the epilogue
+  static_assert(4 * STAGING <= LDS && STAGING >= 32 * (T / 2) * 4, "a block of fp32 per wave");
+};
+
+// Four rows of 16 values in LDS, a row to 16 lanes, column by column: lane i of 16
+// gives the address of four values of row i / 4, from column 4 (i % 4) on, and has
+// the four of column i. (__restrict__: with no scope of its own the compiler takes
+// the read for one of the bytes that the loads in flight will write, and waits for
+// all of those first.)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* LdsWords;
+__device__ __forceinline__ s16x4 read_transposed(LdsWords __restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+}
+
+// Offset that no buffer resource here reaches.
+constexpr uint32_t kOutside = 0x80000000u;
+
+// Where lane l's 16 bytes of the wave's load i come from, in bytes from the
+// stage's origin (`along`: row r of the tile, swizzled chunk of its 128 bytes;
+// `across`: row of the 64, swizzled chunk of its 2T bytes).
+// Along: the LDS serves 16 lanes of a 16-byte read at a time, whose 16 rows share
+// a chunk; the XOR by r / 2 spreads them over the 16 places of two rows.
+// Across: a transposing read of 16 lanes takes 32 bytes of four consecutive rows;
+// the XOR by 2 (row % 4) on 32-byte granules spreads two such reads over 256 bytes.
+template <class C, bool ACROSS>
+struct Feed {
+  uint32_t off[C::NL];
+  uint32_t c0;  // along: byte in the row of even loads; odd ones: ^ 64
+
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld_bytes) {
+    const uint32_t ld = static_cast<uint32_t>(ld_bytes);
+    if constexpr (ACROSS) {
+      constexpr int LPR = C::T / 8;      // lanes a row takes
+      constexpr int RPL = 64 / LPR;      // rows a load covers
+      const int sub = lane / LPR, chunk = lane % LPR;
+#pragma unroll
+      for (int i = 0; i < C::NL; ++i) {
+        const int k = (wave * C::NL + i) * RPL + sub;
+        const int granule = (chunk >> 1) ^ (2 * (k & 3));
+        off[i] = k * ld + granule * 32 + (chunk & 1) * 16;
+      }
+      c0 = 0;
+    } else {
+      const int r8 = lane >> 3;
+      c0 = ((lane & 7) ^ (r8 >> 1)) * 16;
+#pragma unroll
+      for (int i = 0; i < C::NL; ++i) {
+        const int r = (wave * C::NL + i) * 8 + r8;
+        off[i] = r * ld + (c0 ^ ((i & 1) * 64));
+      }
+    }
+  }
+};
+
+template <int TY, int MODE, int ACT, class C>
+__global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams p) {
+  typedef Mma16<TY> M;
+  typedef typename M::Frag Frag;
+  typedef typename Elem<TY>::raw raw;
+  constexpr bool QA = MODE == kLinearWgrad;                          // Q across
+  constexpr bool PA = MODE == kLinearWgrad || MODE == kLinearDgrad;  // P across
+  constexpr bool GATED = MODE == kLinearGated;
+  constexpr bool FORWARD = MODE == kLinearForward || GATED;
+  constexpr int T = C::T, NB = C::NB, NL = C::NL, SLOT = C::SLOT;
+  constexpr int TN = GATED ? T / 2 : T;  // output columns of a tile
+  constexpr int P_AT = 2 * SLOT;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // ---- the tile. Workgroup b runs on XCD b % 8; each XCD takes a contiguous
+  // eighth of the tiles, which go in bands of four columns, row by row, so that
+  // the tiles an XCD's 32 CUs have at a time share rows and columns in its L2.
+  const int n_ct = (p.n + TN - 1) / TN;
+  const GroupScan scan{p.counts, p.groups, p.rows};
+  const int n_rt = QA ? (p.m + T - 1) / T
+                      : p.counts ? scan.tiles(T) : (p.rows + T - 1) / T;
+  const int total = (QA ? p.groups : 1) * n_rt * n_ct;
+  const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3;
+  if (pos >= (total >> 3) + (xcd < (total & 7))) return;
+  int at = xcd * (total >> 3) + min(xcd, total & 7) + pos;
+  int e = 0;
+  if (QA) {
+    e = at / (n_rt * n_ct);
+    at -= e * n_rt * n_ct;
+  }
+  constexpr int BAND = 4;
+  const int band = at / (n_rt * BAND);
+  const int cols = min(BAND, n_ct - band * BAND);
+  at -= band * n_rt * BAND;
+  const int rt = __builtin_amdgcn_readfirstlane(at / cols);
+  const int ct = __builtin_amdgcn_readfirstlane(band * BAND + at % cols);
+  e = __builtin_amdgcn_readfirstlane(e);
+  // rows of Q: [first, first + nrows) of the tile (across: of the group's sums)
+  int first, nrows;
+  if (!p.counts) {
+    first = QA ? 0 : rt * T;
+    nrows = QA ? p.rows : min(T, p.rows - first);
+  } else if (QA) {
+    scan.range(e, &first, &nrows);
+  } else {
+    scan.tile(rt, T, &e, &first, &nrows);
+  }
+  e = __builtin_amdgcn_readfirstlane(e);
+  first = __builtin_amdgcn_readfirstlane(first);
+  nrows = __builtin_amdgcn_readfirstlane(nrows);
+  const bool none = !QA && e >= (p.counts ? p.groups : 1);  // rows of no group
+  const int red = QA ? nrows : none ? 0 : p.red;
+  const int KT = (red + 63) / 64;
+
+  // ---- operands. A stage's resource begins at the stage and ends with its last
+  // value: `along`, with the tile's last row's last sum; `across`, with the last
+  // row's last column.
+  const int64_t ldq = p.ldq * 2, ldp = p.ldp * 2;
+  const uint8_t* q0 = static_cast<const uint8_t*>(p.q) +
+                      (QA ? first * ldq + static_cast<int64_t>(rt) * T * 2 : first * ldq);
+  const uint8_t* p0 = static_cast<const uint8_t*>(p.p) + (QA ? first * ldp : e * p.p_group * 2) +
+                      (PA ? static_cast<int64_t>(ct) * T * 2 : static_cast<int64_t>(ct) * TN * ldp);
+  if (none) p0 = static_cast<const uint8_t*>(p.p);
+  const int prows = PA ? 0 : min(TN, p.n - ct * TN);
+  Feed<C, QA> fq;
+  Feed<C, PA> fp;
+  fq.init(wave, lane, ldq);
+  fp.init(wave, lane, ldp);
+  if constexpr (GATED) {
+    // The tile's rows of P by 32: gate, up, gate, up ... of the same columns; the
+    // up rows' resource starts n rows further on.
+    const int r8 = lane >> 3;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r = (wave * NL + i) * 8 + r8;
+      fp.off[i] = ((r >> 6) * 32 + (r & 31)) * static_cast<uint32_t>(ldp) +
+                  (fp.c0 ^ ((i & 1) * 64));
+    }
+  }
+  auto resource = [](const uint8_t* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base), 0, static_cast<int>(bytes > 0 ? bytes : 0), kBufWord3);
+  };
+  auto feed = [&](auto across_c, const auto& f, const uint8_t* base, int64_t ld, int rows,
+                  int width, int s, uint8_t* dst, bool up) {
+    constexpr bool ACROSS = decltype(across_c)::value;
+    if constexpr (ACROSS) {
+      const int left = min(64, red - s * 64);
+      const __amdgpu_buffer_rsrc_t r = resource(
+          base + static_cast<int64_t>(s) * 64 * ld,
+          left > 0 ? (left - 1) * ld + width * 2 : 0);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) lds_dma16_buf(r, f.off[i], 0, dst + i * 1024);
+    } else {
+      const int left = (red - s * 64) * 2;  // bytes of sums from here on
+      const uint8_t* b = base + static_cast<int64_t>(s) * 128;
+      const int64_t bytes = left > 0 && rows > 0 ? (rows - 1) * ld + left : 0;
+      const __amdgpu_buffer_rsrc_t r = resource(b, bytes);
+      const __amdgpu_buffer_rsrc_t ru = resource(up ? b + p.n * ld : b, bytes);
+      const bool in0 = static_cast<int>(f.c0) < left, in1 = static_cast<int>(f.c0 ^ 64) < left;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const bool is_up = up && (((wave * NL + i) >> 2) & 1);
+        const uint32_t o = ((i & 1) ? in1 : in0) ? f.off[i] : kOutside;
+        if (is_up) lds_dma16_buf(ru, o, 0, dst + i * 1024);
+        else lds_dma16_buf(r, o, 0, dst + i * 1024);
+      }
+    }
+  };
+  auto feed_q = [&](int s, int slot) {
+    feed(std::integral_constant<bool, QA>{}, fq, q0, ldq, nrows, p.m - rt * T, s,
+         lds + slot + wave * NL * 1024, false);
+  };
+  auto feed_p = [&](int s, int slot) {
+    feed(std::integral_constant<bool, PA>{}, fp, p0, ldp, prows, p.n - ct * T, s,
+         lds + P_AT + slot + wave * NL * 1024, GATED);
+  };
+
+  // ---- fragments: 32 rows x 16 sums, eight sums a lane. Q's blocks of a wave are
+  // the tile's blocks 2i + wm, so that both halves share a short tile's rows.
+  const int h = lane >> 5;
+  int along[4];  // by 16 sums
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+    along[kk] = (lane & 31) * 128 + (((2 * kk + h) ^ ((lane >> 1) & 7)) * 16);
+  int across[4];  // by block % 4: lane's row and 8 bytes
+  const int a4 = (lane >> 2) & 3;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    across[b] = (8 * h + a4) * (2 * T) + (b ^ a4) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  auto read = [&](auto across_c, int slot, int block, int kk) -> Frag {
+    if constexpr (decltype(across_c)::value) {
+      const uint8_t* a = lds + slot + across[block & 3] + (block >> 2) * 256 + kk * 16 * 2 * T;
+      const s16x4 lo = read_transposed((LdsWords)(a));
+      const s16x4 hi = read_transposed((LdsWords)(a + 4 * 2 * T));
+      return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      return *reinterpret_cast<const Frag*>(lds + slot + block * 32 * 128 + along[kk]);
+    }
+  };
+  f32x16 acc[NB][NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+  Frag fa[2][NB], fb[2][NB];
+  auto read_frags = [&](int oq, int op, int kk, Frag (&a)[NB], Frag (&b)[NB]) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      a[i] = read(std::integral_constant<bool, QA>{}, oq, 2 * i + wm, kk);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      b[j] = read(std::integral_constant<bool, PA>{}, P_AT + op, wn * NB + j, kk);
+  };
+  auto mma = [&](const Frag (&a)[NB], const Frag (&b)[NB]) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = M::mma32(b[j], a[i], acc[i][j]);
+  };
+
+  // ---- main loop. Stage s lives in Q's slot s % 2 and P's slot s % 3. The
+  // barrier before its last 16 sums publishes stage s + 1 (every wave has waited
+  // for its own loads of it) and frees stage s's slots; P's loads of stage s + 2 go
+  // out during its first 16 sums, Q's after that barrier.
+  auto next_q = [](int o) { return SLOT - o; };
+  auto next_p = [](int o) { return o == 2 * SLOT ? 0 : o + SLOT; };
+  auto prev_p = [](int o) { return o == 0 ? 2 * SLOT : o - SLOT; };
+  auto stage = [&](int s, int oq, int op, auto refill_c) {
+    constexpr bool REFILL = decltype(refill_c)::value;
+#pragma unroll
+    for (int kk = 0; kk < 3; ++kk) {
+      read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+      if (REFILL && kk == 0) feed_p(s + 2, prev_p(op));
+      mma(fa[kk & 1], fb[kk & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_lgkm0();
+    wait_vmcnt<REFILL ? NL : 0>();
+    wave_barrier_all();
+    read_frags(next_q(oq), next_p(op), 0, fa[0], fb[0]);
+    if constexpr (REFILL) feed_q(s + 2, oq);
+    mma(fa[1], fb[1]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (KT > 0) {
+    feed_q(0, 0);
+    feed_p(0, 0);
+    feed_q(1, SLOT);
+    feed_p(1, SLOT);
+    wait_vmcnt<2 * NL>();
+    wave_barrier_all();
+    read_frags(0, 0, 0, fa[0], fb[0]);
+    int s = 0, oq = 0, op = 0;
+    for (; s + 2 < KT; ++s, oq = next_q(oq), op = next_p(op)) stage(s, oq, op, std::true_type{});
+    if (s + 1 < KT) {
+      stage(s, oq, op, std::false_type{});
+      oq = next_q(oq);
+      op = next_p(op);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 3; ++kk) {
+      read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+      mma(fa[kk & 1], fb[kk & 1]);
+    }
+    mma(fa[1], fb[1]);
+  }
+  wait_vmcnt<0>();
+  wait_lgkm0();
+  wave_barrier_all();  // the ring is done with
+
+  // ---- epilogue: 32 output rows at a time through the wave's part of LDS, in
+  // fp32, so that they leave as whole runs of a row and the bias, the activation
+  // and the residual are taken eight columns at a time, before the only rounding.
+  constexpr int WN = 32 * NB;                // staged columns of a wave
+  constexpr int OC = GATED ? WN / 2 : WN;    // output columns
+  constexpr int LPR = OC / 8, RPP = 64 / LPR, NP = 32 / RPP;
+  constexpr int CH = WN / 4;                 // 16-byte chunks of a staged row
+  float* stg = reinterpret_cast<float*>(lds + wave * C::STAGING);
+  const int lr = lane / LPR, lc = lane % LPR;
+  const int col = ct * TN + wn * OC + lc * 8;
+  const bool col_in = col < p.n;
+  const int wide = GATED ? 2 * p.n : p.n;
+  // staged column of the lane's first value (gated: the gate's; up 32 on)
+  const int sc = GATED ? (lc >> 2) * 64 + (lc & 3) * 8 : lc * 8;
+  float bias[GATED ? 2 : 1][8];
+#pragma unroll
+  for (int g = 0; g < (GATED ? 2 : 1); ++g)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[g][j] = 0.f;
+  if (FORWARD && p.bias && !none && col_in) {
+#pragma unroll
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+      const raw* b = static_cast<const raw*>(p.bias) + static_cast<int64_t>(e) * wide + g * p.n + col;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bias[g][j] = Elem<TY>::to_f32(b[j]);
+    }
+  }
+  raw* out = static_cast<raw*>(p.out);
+  // (the weights' gradient: rows of the group's matrix)
+  const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
+  const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
+  auto chunk_at = [](int r, int c) { return r * CH * 4 + ((c ^ (r & 15)) & (CH - 1)) * 4; };
+  static_for<NB>([&](auto i_c) {
+    constexpr int i = decltype(i_c)::value;
+    const int b0 = (2 * i + wm) * 32;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(stg + chunk_at(lane & 31, j * 8 + 2 * g + h)) =
+            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
+                  acc[i][j][4 * g + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    Vec8<TY, true> res[NP];
+    if (FORWARD && p.residual) {
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const int r = b0 + k * RPP + lr;
+        if (r < rows_in && col_in) res[k].load(p.residual, (row0 + r) * p.ldr + col, 8);
+      }
+    }
+    static_for<NP>([&](auto k_c) {
+      constexpr int k = decltype(k_c)::value;
+      const int r = b0 + k * RPP + lr, sr = k * RPP + lr;
+      if (r >= rows_in || !col_in) return;
+      float v[8], u[8];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(stg + chunk_at(sr, sc / 4 + c));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * c + j] = x[j] + bias[0][4 * c + j];
+        if constexpr (GATED) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(stg + chunk_at(sr, sc / 4 + 8 + c));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u[4 * c + j] = y[j] + bias[1][4 * c + j];
+        }
+      }
+      const int64_t o = (row0 + r) * p.n + col;
+      if constexpr (FORWARD) {
+        if (p.z) {
+          const int64_t zo = (row0 + r) * wide + col;
+          store8<TY, true>(p.z, zo, 8, v);
+          if constexpr (GATED) store8<TY, true>(p.z, zo + p.n, 8, u);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = none ? 0.f : linear_act<ACT>(v[j]);
+          if constexpr (GATED) v[j] = none ? 0.f : v[j] * u[j];
+          if (p.residual) v[j] += res[k][j];
+        }
+      }
+      store8<TY, true>(out, o, 8, v);
+    });
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  });
+}
+
+// ---------------------------------------------------------------- schedule ---
+namespace {
+
+template <class... P, class... A>
+int launch_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told, int64_t wgs,
+               int threads, int lds, hipStream_t stream, A... args) {
+  if (wgs * threads > 0xffffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  int gpu = 0;
+  hipError_t e = hipGetDevice(&gpu);
+  const uint64_t bit = uint64_t{1} << (gpu & 63);
+  if (e == hipSuccess && (gpu > 63 || !(told.load(std::memory_order_relaxed) & bit))) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess && gpu <= 63) told.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != hipSuccess) return fail(FGS_ELAUNCH, std::string(name) + ": " + hipGetErrorString(e));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), lds, stream, args...);
+  return check_launch(name);
+}
+
+template <int TY, int MODE, int ACT, int T>
+int launch_tile(const LinearParams& p, hipStream_t stream) {
+  typedef LinearTile<T> C;
+  static std::atomic<uint64_t> told{0};
+  const int64_t tn = MODE == kLinearGated ? T / 2 : T;
+  const int64_t nc = (p.n + tn - 1) / tn;
+  const int64_t nr = MODE == kLinearWgrad
+                         ? static_cast<int64_t>(p.groups) * ((p.m + T - 1) / T)
+                         : (static_cast<int64_t>(p.rows) + T - 1) / T + (p.counts ? p.groups : 0);
+  if (nr * nc > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  const int64_t wgs = (nr * nc + 7) / 8 * 8;
+  return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told, wgs, 256, C::LDS,
+                    stream, p);
+}
+template <int TY, int MODE, int ACT>
+int launch_form(const LinearParams& p, int form, hipStream_t stream) {
+  if (form == 0) return launch_tile<TY, MODE, ACT, 128>(p, stream);
+  return launch_tile<TY, MODE, ACT, 256>(p, stream);
+}
+template <int TY>
+int launch_type(const LinearParams& p, int mode, int form, hipStream_t stream) {
+  if (mode == kLinearDgrad) return launch_form<TY, kLinearDgrad, FGS_ACT_NONE>(p, form, stream);
+  if (mode == kLinearWgrad) return launch_form<TY, kLinearWgrad, FGS_ACT_NONE>(p, form, stream);
+  return with_act(p.act, [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    return mode == kLinearGated ? launch_form<TY, kLinearGated, ACT>(p, form, stream)
+                                : launch_form<TY, kLinearForward, ACT>(p, form, stream);
+  });
+}
+
+}  // namespace
+
+bool linear_flags_ok(int32_t flags) { return flags >= 0 && flags <= 2; }
+
+// 0: 128 x 128 tiles, 1: 256 x 256.
+int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
+                int32_t flags) {
+  if (flags) return flags - 1;
+  const int64_t wide = n * (mode == kLinearGated ? 2 : 1);
+  const int64_t tall = mode == kLinearWgrad ? m * groups : rows;
+  return tall * wide >= int64_t{256} * 256 * 256 && (mode == kLinearWgrad || rows / groups >= 256)
+             ? 1 : 0;
+}
+
+std::string linear_form_name(int mode, int form) {
+  return form == 0 ? "tiled 128x128" : "tiled 256x256";
+}
+
+int launch_linear(const LinearParams& p, int mode, int dtype, int form, hipStream_t stream) {
+  return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, mode, form, stream)
+                                 : launch_type<FGS_DTYPE_FP16>(p, mode, form, stream);
+}
+
+}  // namespace fgs

@@ -28,6 +28,11 @@ QUANT_NONE = 0
 QUANT_FP8_GROUP = 1
 QUANT_INT8_TOKEN = 2
 
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_SILU = 2
+ACT_GELU = 3
+
 SCORING_SOFTMAX = 0
 SCORING_SIGMOID = 1
 
@@ -46,6 +51,9 @@ NOALLOC_SCRATCH_BYTES = 64 << 20  # FGS_NOALLOC_SCRATCH_BYTES
 def flag_tile(cfg: int) -> int:
     """Schedule flag forcing tiled configuration ``cfg`` (FGS_FLAG_TILE)."""
     return ((cfg + 1) & 0x7) << 12
+
+
+LINEAR_FORMS = 2  # FGS_LINEAR_FORM(0 ..): 128 x 128 tiles, 256 x 256
 
 LIB_NAME = "libfgs_moe.so"
 
@@ -155,6 +163,56 @@ SIGNATURES = {
          _i32, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i64, _c_void_p],
     ),
     "fgs_moe_fp8_block_matmul_schedule": (_i32, [_i64, _i64, _i64, _i32, _c_void_p, _i32]),
+    "fgs_moe_topk_gating_grad": (
+        _i32, [_c_void_p, _i32, _i64, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p,
+               _c_void_p, _c_void_p, _c_void_p]
+    ),
+    "fgs_moe_permute_workspace_bytes": (_i64, [_i64, _i32]),
+    "fgs_moe_permute": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i64, _c_void_p, _i32, _i32, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p],
+    ),
+    "fgs_moe_permute_rows": (
+        _i32, [_c_void_p, _i64, _i64, _i64, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p]
+    ),
+    "fgs_moe_unpermute": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _i32, _i64, _i32, _c_void_p,
+         _c_void_p],
+    ),
+    "fgs_moe_unpermute_grad": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _i32, _i64, _i32, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "fgs_moe_linear": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p,
+         _i32, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "fgs_moe_linear_act_grad": (
+        _i32, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i32, _i32, _i32, _c_void_p, _c_void_p]
+    ),
+    "fgs_moe_linear_input_grad": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i32, _i64, _i64, _i64, _i32,
+         _i32, _c_void_p, _c_void_p],
+    ),
+    "fgs_moe_linear_weight_grad": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i32, _i64, _i64, _i64, _i32, _i32,
+         _c_void_p, _c_void_p],
+    ),
+    "fgs_moe_linear_bias_grad_workspace_bytes": (_i64, [_i32, _i64, _i64]),
+    "fgs_moe_linear_bias_grad": (
+        _i32,
+        [_c_void_p, _i64, _c_void_p, _i32, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p,
+         _c_void_p],
+    ),
+    "fgs_moe_linear_schedule": (
+        _i32, [_i32, _i32, _i64, _i64, _i64, _i32, _i32, _c_void_p, _i32]
+    ),
     "fgs_moe_profile_enable": (_i32, [_i32]),
     "fgs_moe_profile_read": (_i32, [_c_void_p, _i32]),
 }
@@ -196,12 +254,17 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+# the entries that the steps' host side calls, in the order of its bind_steps
+_STEPS = ("permute_workspace_bytes", "permute", "permute_rows", "unpermute", "unpermute_grad",
+          "topk_gating_grad", "linear", "linear_act_grad", "linear_input_grad",
+          "linear_weight_grad", "linear_bias_grad_workspace_bytes", "linear_bias_grad")
+
 _host = None
 
 
 def host():
-    """The extension module of the dense operators' host side (``_host``,
-    csrc/host_ext.cpp), bound (once) to the loaded library."""
+    """The extension module of the dense operators' and the layer's steps' host
+    side (``_host``, csrc/host_ext.cpp), bound (once) to the loaded library."""
     global _host
     if _host is None:
         lib = load()
@@ -215,10 +278,14 @@ def host():
                         f"flaggems_sglang._host did not load ({e}); build it with "
                         "`make -C flaggems-sglang_amd/csrc` (or __graft_entry__.build())"
                     ) from e
-                module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                              for name in ("fgs_moe_last_error", "fgs_moe_rms_norm",
-                                           "fgs_moe_silu_and_mul_quant",
-                                           "fgs_moe_fp8_block_matmul")))
+
+                def addresses(*names):
+                    return (ctypes.cast(getattr(lib, "fgs_moe_" + name), ctypes.c_void_p).value
+                            for name in names)
+
+                module.bind(*addresses("last_error", "rms_norm", "silu_and_mul_quant",
+                                       "fp8_block_matmul"))
+                module.bind_steps(*addresses(*_STEPS))
                 _host = module
     return _host
 
@@ -255,4 +322,14 @@ def block_matmul_schedule(m: int, n: int, k: int, flags: int = 0) -> str:
     buf = ctypes.create_string_buffer(96)
     check(load().fgs_moe_fp8_block_matmul_schedule(m, n, k, flags, buf, len(buf)),
           "schedule")
+    return buf.value.decode()
+
+
+def linear_schedule(rows: int, n: int, k: int, groups: int = 1, gated: bool = False,
+                    which: str = "forward", flags: int = 0) -> str:
+    """The schedule a product of these sizes runs (``fgs_moe_linear_schedule``);
+    ``which``: "forward", "input" or "weight" (the gradients)."""
+    buf = ctypes.create_string_buffer(96)
+    check(load().fgs_moe_linear_schedule(("forward", "input", "weight").index(which), groups, rows,
+                                         n, k, gated, flags, buf, len(buf)), "schedule")
     return buf.value.decode()

@@ -22,8 +22,10 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from flaggems_sglang import _capi
+from flaggems_sglang.ops._autograd import needs_gradient
 
 logger = logging.getLogger(__name__)
 
@@ -262,7 +264,8 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     experts ranked by logit (ties: lower id), weights = their scores,
     renormalised to sum 1 when ``renormalize``. Returns ``(topk_weights f32
     [M, topk], topk_ids int32 [M, topk])`` -- the routing the reference's
-    tests build with torch ops (tests/test_fused_moe.py:37-41)."""
+    tests build with torch ops (tests/test_fused_moe.py:37-41). The weights'
+    gradient goes to ``gating_output``."""
     _require_gpu("gating_output", gating_output)
     assert gating_output.ndim == 2, "gating_output must be [M, E]"
     assert hidden_states.shape[0] == gating_output.shape[0], "token count mismatch"
@@ -275,6 +278,12 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     logits = gating_output
     if logits.dtype not in (torch.float32, torch.bfloat16):
         logits = logits.float()
+    if needs_gradient("fused_topk", logits):
+        return _FusedTopk.apply(logits, topk, bool(renormalize), scoring)
+    return _topk_gating(logits, topk, renormalize, scoring)
+
+
+def _topk_gating(logits, topk, renormalize, scoring):
     logits = logits.contiguous()
     M, E = logits.shape
     w = torch.empty((M, topk), dtype=torch.float32, device=logits.device)
@@ -287,6 +296,25 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
         "fused_topk",
     )
     return w, ids
+
+
+class _FusedTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, renormalize, scoring):
+        w, ids = _topk_gating(logits, topk, renormalize, scoring)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, w, ids)
+        ctx.how = scoring, renormalize
+        return w, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dw, _):
+        if dw is None:
+            return None, None, None, None
+        logits, w, ids = ctx.saved_tensors
+        return _capi.host().topk_gating_grad(logits, w, ids, dw, *ctx.how), None, None, None
 
 
 # ------------------------------------------------------------ small ops ---

@@ -458,6 +458,111 @@ int32_t fgs_moe_fp8_block_matmul(const void* a, int64_t lda, const float* a_scal
 int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32_t flags,
                                           char* buf, int32_t len);
 
+/* ---- the routed layer's steps, with gradients ---------------------------
+ * The reference runs the layer as one call without gradients
+ * (ops/fused_moe.py:149-232); these are its steps for a program that trains it or
+ * sends tokens to other GPUs between them. Activations of the products: */
+#define FGS_ACT_NONE 0
+#define FGS_ACT_RELU 1
+#define FGS_ACT_SILU 2
+#define FGS_ACT_GELU 3 /* exact (erf) */
+
+/* Gradient of fgs_moe_topk_gating's weights: dlogits [m, num_experts] (of
+ * logits' type) from the weights and ids that it returned for these logits and
+ * dweights f32 [m, topk]. */
+int32_t fgs_moe_topk_gating_grad(const void* logits, int32_t logits_bf16, int64_t m,
+                                 int32_t num_experts, int32_t topk, int32_t scoring,
+                                 int32_t renormalize, const float* topk_weights,
+                                 const int32_t* topk_ids, const float* dweights, void* dlogits,
+                                 void* stream);
+
+/* Tokens sorted by expert: rows[p] = x[s / topk] for the slot s in place p of the
+ * slots sorted by expert, then by slot.
+ *   x: m rows of row_bytes (any element type), x_stride bytes apart
+ *   topk_ids int32 [m, topk]; ids outside [0, num_experts) (slots of other GPUs'
+ *   experts) come behind the last expert's, as rows of zeros
+ *   rows [m * topk] of row_bytes, contiguous; counts int32 [num_experts]
+ *   row_of_slot int32 [m, topk]: the slot's row, -1 for slots of no expert here
+ *   slot_of_row int32 [m * topk]: its inverse, -1 for the rows behind
+ * Of the values in [0, num_experts) no order depends on atomics. num_experts <=
+ * 1022. Workspace: fgs_moe_permute_workspace_bytes, 256-byte aligned, this call's
+ * alone until it has run. */
+int64_t fgs_moe_permute_workspace_bytes(int64_t numel, int32_t num_experts);
+int32_t fgs_moe_permute(const void* x, int64_t x_stride, int64_t m, int64_t row_bytes,
+                        const int32_t* topk_ids, int32_t topk, int32_t num_experts, void* rows,
+                        int32_t* counts, int32_t* row_of_slot, int32_t* slot_of_row,
+                        void* workspace, int64_t ws_bytes, void* stream);
+/* The same rows by an order that fgs_moe_permute has made. */
+int32_t fgs_moe_permute_rows(const void* x, int64_t x_stride, int64_t m, int64_t row_bytes,
+                             const int32_t* row_of_slot, int32_t topk, const int32_t* slot_of_row,
+                             void* rows, void* stream);
+
+/* Rows back to tokens: out[t] = sum_k w[t, k] rows[row_of_slot[t, k]], in fp32 from
+ * k = 0 on. Slots whose row lies outside [0, n_rows) add nothing, whatever their
+ * weight. topk_weights f32 [m, topk] or null (ones); rows [n_rows, cols] of dtype
+ * with row stride ld; out [m, cols] contiguous. */
+int32_t fgs_moe_unpermute(const void* rows, int64_t ld, int64_t n_rows,
+                          const int32_t* row_of_slot, const float* topk_weights, int64_t m,
+                          int32_t topk, int64_t cols, int32_t dtype, void* out, void* stream);
+/* Its gradients: drows[row_of_slot[t, k]] = w[t, k] dout[t], 0 for rows whose
+ * slot_of_row is negative ([n_rows, cols] contiguous, or null), and dweights[t, k] =
+ * <dout[t], rows[row_of_slot[t, k]]>, 0 for slots without a row (f32 [m, topk], or
+ * null). The order is one that fgs_moe_permute has made: a row that two slots name
+ * has either's gradient. */
+int32_t fgs_moe_unpermute_grad(const void* dout, int64_t ldd, const void* rows, int64_t ld,
+                               int64_t n_rows, const int32_t* row_of_slot,
+                               const int32_t* slot_of_row, const float* topk_weights, int64_t m,
+                               int32_t topk, int64_t cols, int32_t dtype, void* drows,
+                               float* dweights, void* stream);
+
+/* Products of bf16 or fp16 matrices with fp32 sums, dense or by group of rows:
+ *   v = x[i] . w[e][j] + bias[e][j]
+ *   out[i, j] = act(v_j) + residual[i, j]                      (wide = n)
+ *   out[i, j] = act(v_j) * v_{n + j} + residual[i, j]          (gated: wide = 2 n)
+ * rounded once to dtype; z (or null) [rows, wide] gets v.
+ *   x [rows, k] with row stride ldx; w [groups][wide, k] with row stride ldw and
+ *   w_group_stride elements between the groups' matrices; bias [groups, wide] or
+ *   null; residual [rows, n] with row stride ldr, or null; out [rows, n] contiguous
+ *   counts int32 [groups] on the device: the rows of each group, which follow each
+ *   other from row 0 on (negative ones count as 0, and what passes the last row is
+ *   cut); rows behind the last group's have no product (out = residual, or 0; their
+ *   z is not defined). Null: one matrix for all rows.
+ * n and k multiples of 8, up to 2^20; up to 2^30 rows and 4096 groups; rows of x, w,
+ * residual 16-byte aligned and at most 2^21 elements apart. No workspace. `flags`:
+ * 0, or FGS_LINEAR_FORM(f), the kernel form f whatever the sizes (for measurement
+ * and tests). */
+#define FGS_LINEAR_FORM(f) ((f) + 1)
+int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                       int64_t w_group_stride, const void* bias, const void* residual,
+                       int64_t ldr, const int32_t* counts, int32_t groups, int64_t rows,
+                       int64_t n, int64_t k, int32_t dtype, int32_t act, int32_t gated,
+                       int32_t flags, void* z, void* out, void* stream);
+/* Its gradients. dz [rows, wide] contiguous, of v (rows behind the last group's: of
+ * whatever z holds there; the two entries below leave them out): */
+int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const void* z, int64_t rows,
+                                int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
+                                void* stream);
+/* dx [rows, k] = dz[i] w[e], contiguous (rows behind the last group's: 0), */
+int32_t fgs_moe_linear_input_grad(const void* dz, int64_t ldz, const void* w, int64_t ldw,
+                                  int64_t w_group_stride, const int32_t* counts, int32_t groups,
+                                  int64_t rows, int64_t wide, int64_t k, int32_t dtype,
+                                  int32_t flags, void* dx, void* stream);
+/* dw [groups][wide, k] = sum over the group's rows of dz[i]^T x[i], contiguous, */
+int32_t fgs_moe_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx,
+                                   const int32_t* counts, int32_t groups, int64_t rows,
+                                   int64_t wide, int64_t k, int32_t dtype, int32_t flags,
+                                   void* dw, void* stream);
+/* dbias [groups, wide] = sum over the group's rows of dz[i]; workspace
+ * fgs_moe_linear_bias_grad_workspace_bytes (0: none), 16-byte aligned. */
+int64_t fgs_moe_linear_bias_grad_workspace_bytes(int32_t groups, int64_t rows, int64_t wide);
+int32_t fgs_moe_linear_bias_grad(const void* dz, int64_t ldz, const int32_t* counts,
+                                 int32_t groups, int64_t rows, int64_t wide, int32_t dtype,
+                                 void* workspace, int64_t ws_bytes, void* dbias, void* stream);
+/* The schedule of a product, as text (as fgs_moe_schedule): `pass` 0 the forward
+ * one, 1 the input's gradient, 2 the weights'. */
+int32_t fgs_moe_linear_schedule(int32_t pass, int32_t groups, int64_t rows, int64_t n, int64_t k,
+                                int32_t gated, int32_t flags, char* buf, int32_t len);
+
 /* Stage timing for benchmarks. No reference counterpart (the reference
  * times the whole op with triton.testing.do_bench,
  * benchmark/performance_utils.py:365-377). While enabled on the calling
