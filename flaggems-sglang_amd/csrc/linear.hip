@@ -31,8 +31,8 @@ struct LinearTile {
   static constexpr int NL = T / 32;           // loads of a wave per operand and stage
   static constexpr int SLOT = T * 128;        // bytes
   static constexpr int LDS = 5 * SLOT;        // Q: slots 0, 1; P: 2, 3, 4
-  static constexpr int STAGING = SLOT;        // a wave's part in the epilogue
-  static_assert(4 * STAGING <= LDS && STAGING >= 32 * (T / 2) * 4, "a block of fp32 per wave");
+  static constexpr int STAGING = T * T / 2;   // a wave's part in the epilogue, 16 bits
+  static_assert(4 * STAGING <= LDS, "staging");
 };
 
 // Four rows of 16 values in LDS, a row to 16 lanes, column by column: lane i of 16
@@ -144,6 +144,26 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   const int red = QA ? nrows : none ? 0 : p.red;
   const int KT = (red + 63) / 64;
 
+  // ---- the bias, where the accumulators start: its loads go out before the
+  // stages'.
+  constexpr int WN = 32 * NB;              // columns of a wave's accumulators
+  constexpr int OC = GATED ? WN / 2 : WN;  // ... of its output
+  const int col0 = ct * TN + wn * OC;
+  const int wide = GATED ? 2 * p.n : p.n;
+  const int h = lane >> 5;
+  uint2 bias[NB][4];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bias[j][g] = uint2{0, 0};
+      const int c = col0 + (GATED ? j >> 1 : j) * 32 + 8 * g + 4 * h;
+      if (FORWARD && p.bias && !none && c < p.n)
+        __builtin_memcpy(&bias[j][g],
+                         static_cast<const raw*>(p.bias) + static_cast<int64_t>(e) * wide + c +
+                             (GATED && (j & 1) ? p.n : 0), 8);
+    }
+
   // ---- operands. A stage's resource begins at the stage and ends with its last
   // value: `along`, with the tile's last row's last sum; `across`, with the last
   // row's last column.
@@ -210,7 +230,6 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 
   // ---- fragments: 32 rows x 16 sums, eight sums a lane. Q's blocks of a wave are
   // the tile's blocks 2i + wm, so that both halves share a short tile's rows.
-  const int h = lane >> 5;
   int along[4];  // by 16 sums
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
@@ -231,12 +250,6 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     }
   };
   f32x16 acc[NB][NB];
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
   Frag fa[2][NB], fb[2][NB];
   auto read_frags = [&](int oq, int op, int kk, Frag (&a)[NB], Frag (&b)[NB]) {
 #pragma unroll
@@ -253,6 +266,23 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
       for (int j = 0; j < NB; ++j) acc[i][j] = M::mma32(b[j], a[i], acc[i][j]);
   };
 
+  // The order of a step's instructions: the next step's LDS reads behind the first
+  // MFMAs, then the loads (0 or NL) one between each pair of MFMAs.
+  constexpr int NM = NB * NB, NR = NB * ((QA ? 2 : 1) + (PA ? 2 : 1));
+  auto order = [&](auto loads_c) {
+    constexpr int LOADS = decltype(loads_c)::value;
+    constexpr int PER = (NR + NM / 2 - 1) / (NM / 2);  // reads behind an MFMA
+    constexpr int RM = (NR + PER - 1) / PER;           // MFMAs with reads
+    static_for<RM>([&](auto) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    });
+    static_for<LOADS>([&](auto) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    });
+  };
+
   // ---- main loop. Stage s lives in Q's slot s % 2 and P's slot s % 3. The
   // barrier before its last 16 sums publishes stage s + 1 (every wave has waited
   // for its own loads of it) and frees stage s's slots; P's loads of stage s + 2 go
@@ -267,6 +297,8 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
       read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
       if (REFILL && kk == 0) feed_p(s + 2, prev_p(op));
       mma(fa[kk & 1], fb[kk & 1]);
+      if (REFILL && kk == 0) order(std::integral_constant<int, NL>{});
+      else order(std::integral_constant<int, 0>{});
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_lgkm0();
@@ -275,6 +307,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     read_frags(next_q(oq), next_p(op), 0, fa[0], fb[0]);
     if constexpr (REFILL) feed_q(s + 2, oq);
     mma(fa[1], fb[1]);
+    order(std::integral_constant<int, REFILL ? NL : 0>{});
     __builtin_amdgcn_sched_barrier(0);
   };
   if (KT > 0) {
@@ -282,6 +315,19 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     feed_p(0, 0);
     feed_q(1, SLOT);
     feed_p(1, SLOT);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t w = t < 2 ? bias[j][g].x : bias[j][g].y;
+        const float v = FORWARD ? Elem<TY>::to_f32(static_cast<raw>(w >> (16 * (t & 1)))) : 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i][j][4 * g + t] = v;
+      }
+  if (KT > 0) {
     wait_vmcnt<2 * NL>();
     wave_barrier_all();
     read_frags(0, 0, 0, fa[0], fb[0]);
@@ -303,95 +349,117 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   wait_lgkm0();
   wave_barrier_all();  // the ring is done with
 
-  // ---- epilogue: 32 output rows at a time through the wave's part of LDS, in
-  // fp32, so that they leave as whole runs of a row and the bias, the activation
-  // and the residual are taken eight columns at a time, before the only rounding.
-  constexpr int WN = 32 * NB;                // staged columns of a wave
-  constexpr int OC = GATED ? WN / 2 : WN;    // output columns
-  constexpr int LPR = OC / 8, RPP = 64 / LPR, NP = 32 / RPP;
-  constexpr int CH = WN / 4;                 // 16-byte chunks of a staged row
-  float* stg = reinterpret_cast<float*>(lds + wave * C::STAGING);
-  const int lr = lane / LPR, lc = lane % LPR;
-  const int col = ct * TN + wn * OC + lc * 8;
-  const bool col_in = col < p.n;
-  const int wide = GATED ? 2 * p.n : p.n;
-  // staged column of the lane's first value (gated: the gate's; up 32 on)
-  const int sc = GATED ? (lc >> 2) * 64 + (lc & 3) * 8 : lc * 8;
-  float bias[GATED ? 2 : 1][8];
-#pragma unroll
-  for (int g = 0; g < (GATED ? 2 : 1); ++g)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bias[g][j] = 0.f;
-  if (FORWARD && p.bias && !none && col_in) {
-#pragma unroll
-    for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-      const raw* b = static_cast<const raw*>(p.bias) + static_cast<int64_t>(e) * wide + g * p.n + col;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) bias[g][j] = Elem<TY>::to_f32(b[j]);
-    }
-  }
-  raw* out = static_cast<raw*>(p.out);
+  // ---- epilogue. Activation and residual are taken in fp32 in the accumulators'
+  // layout (a gate and its up value are two registers of a lane), then
+  // rounded; the wave's whole part goes through LDS in 16 bits so that it leaves as
+  // runs of a row, 16 bytes a lane. The residual comes in the same way first. (In
+  // fp32, 32 rows at a time, with the arithmetic on the way out: a tile took 6 us
+  // more.)
+  uint8_t* stg = lds + wave * C::STAGING;
   // (the weights' gradient: rows of the group's matrix)
   const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
   const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
-  auto chunk_at = [](int r, int c) { return r * CH * 4 + ((c ^ (r & 15)) & (CH - 1)) * 4; };
-  static_for<NB>([&](auto i_c) {
-    constexpr int i = decltype(i_c)::value;
-    const int b0 = (2 * i + wm) * 32;
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(stg + chunk_at(lane & 31, j * 8 + 2 * g + h)) =
-            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
-                  acc[i][j][4 * g + 3]};
+  // Eight bytes s of staged row r of COLS columns: the XOR spreads a column of
+  // 32 rows over all banks. Sixteen bytes are two of them, swapped in some rows.
+  auto place = [](auto cols_c, int r, int s) {
+    constexpr int W8 = decltype(cols_c)::value / 4, RPL = 32 / W8;
+    return r * W8 * 8 + (s ^ ((r / RPL) & (W8 - 1))) * 8;
+  };
+  auto sync = [] {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    Vec8<TY, true> res[NP];
-    if (FORWARD && p.residual) {
+  };
+  // f(staged row, output row in the tile, 16-byte chunk) for the wave's part, a
+  // chunk a lane; the tile's rows 64 i + 32 wm + r are the staged rows 32 i + r.
+  auto runs = [&](auto cols_c, auto&& f) {
+    constexpr int LPR = decltype(cols_c)::value / 8, RPP = 64 / LPR;
+    const int lr = lane / LPR, lc = lane % LPR;
+#pragma unroll 8
+    for (int k = 0; k < WN / RPP; ++k) {
+      const int sr = k * RPP + lr;
+      f(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc);
+    }
+  };
+  auto store = [&](auto cols_c, void* to, int64_t ld, int64_t at0) {
+    constexpr int COLS = decltype(cols_c)::value, RPL = 128 / COLS;
+    sync();
+    runs(cols_c, [&](int sr, int r, int c) {
+      u32x4 v = *reinterpret_cast<const u32x4*>(stg + (place(cols_c, sr, 2 * c) & ~15));
+      if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+      if (r < rows_in && col0 + c * 8 < p.n)
+        *reinterpret_cast<u32x4*>(static_cast<raw*>(to) + at0 + (row0 + r) * ld + col0 + c * 8) = v;
+    });
+    sync();
+  };
+  auto pack4 = [](const float (&v)[4]) {
+    return uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
+  };
+  const int r32 = lane & 31;
+  constexpr std::integral_constant<int, OC> out_cols{};
+  if (FORWARD && p.z) {
+    // (gated: the gates, then the ups)
+    static_for<GATED ? 2 : 1>([&](auto half_c) {
+      constexpr int HALF = decltype(half_c)::value;
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const int r = b0 + k * RPP + lr;
-        if (r < rows_in && col_in) res[k].load(p.residual, (row0 + r) * p.ldr + col, 8);
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = HALF; j < NB; j += GATED ? 2 : 1)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
+                                acc[i][j][4 * g + 3]};
+            *reinterpret_cast<uint2*>(
+                stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h)) = pack4(v);
+          }
+      store(out_cols, p.z, wide, HALF * p.n);
+    });
+  }
+  if (FORWARD && p.residual) {
+    runs(out_cols, [&](int sr, int r, int c) {
+      u32x4 v{0, 0, 0, 0};
+      if (r < rows_in && col0 + c * 8 < p.n)
+        v = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
+                                            (row0 + r) * p.ldr + col0 + c * 8);
+      if ((sr / (128 / OC)) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+      *reinterpret_cast<u32x4*>(stg + (place(out_cols, sr, 2 * c) & ~15)) = v;
+    });
+    sync();
+  }
+  const bool has_residual = FORWARD && p.residual;
+  // (rows of no group: sums of nothing, whose activations are 0)
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; j += GATED ? 2 : 1) {
+      auto at = [&](int g) {
+        return reinterpret_cast<uint2*>(
+            stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
+      };
+      uint2 res[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        res[g] = FORWARD ? *at(g) : uint2{0, 0};  // (without a residual: what the ring left)
+        res[g].x = has_residual ? res[g].x : 0;
+        res[g].y = has_residual ? res[g].y : 0;
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          v[t] = acc[i][j][4 * g + t];
+          if constexpr (FORWARD) {
+            v[t] = linear_act<ACT>(v[t]);
+            if constexpr (GATED) v[t] *= acc[i][j + 1][4 * g + t];
+            v[t] += Elem<TY>::to_f32(
+                static_cast<raw>((t < 2 ? res[g].x : res[g].y) >> (16 * (t & 1))));
+          }
+        }
+        *at(g) = pack4(v);
       }
     }
-    static_for<NP>([&](auto k_c) {
-      constexpr int k = decltype(k_c)::value;
-      const int r = b0 + k * RPP + lr, sr = k * RPP + lr;
-      if (r >= rows_in || !col_in) return;
-      float v[8], u[8];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(stg + chunk_at(sr, sc / 4 + c));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * c + j] = x[j] + bias[0][4 * c + j];
-        if constexpr (GATED) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(stg + chunk_at(sr, sc / 4 + 8 + c));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) u[4 * c + j] = y[j] + bias[1][4 * c + j];
-        }
-      }
-      const int64_t o = (row0 + r) * p.n + col;
-      if constexpr (FORWARD) {
-        if (p.z) {
-          const int64_t zo = (row0 + r) * wide + col;
-          store8<TY, true>(p.z, zo, 8, v);
-          if constexpr (GATED) store8<TY, true>(p.z, zo + p.n, 8, u);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = none ? 0.f : linear_act<ACT>(v[j]);
-          if constexpr (GATED) v[j] = none ? 0.f : v[j] * u[j];
-          if (p.residual) v[j] += res[k][j];
-        }
-      }
-      store8<TY, true>(out, o, 8, v);
-    });
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  });
+  store(out_cols, p.out, p.n, 0);
 }
 
 // ---------------------------------------------------------------- schedule ---

@@ -133,6 +133,13 @@ struct GroupScan {
   }
 };
 
+// Two values of a 16-bit type in a word.
+template <int TY>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (TY == FGS_DTYPE_BF16) return cvt_pk_bf16(lo, hi);
+  return Elem<TY>::from_f32(lo) | static_cast<uint32_t>(Elem<TY>::from_f32(hi)) << 16;
+}
+
 // ------------------------------------------------------------- activations ---
 // erfc(x) / exp(-x^2) for x >= 0 as t times a polynomial in t = 1 / (1 + x / 2),
 // fitted to scaled erfc at Chebyshev nodes over x in [0, 10.5] (least squares of
