@@ -19,20 +19,37 @@ namespace fgs {
 // ------------------------------------------------------------------ tiles ---
 // A workgroup of 2 x 2 waves owns a T x T tile; a wave (T / 2)^2 of it in
 // 32x32x16 MFMAs, P as the row operand: a lane's results are then runs of four
-// adjacent output columns of one output row. Stages of 64 sums stream into an LDS
-// ring by buffer loads: P's slots are three, Q's two, so that P is in flight a
-// stage longer. What lies outside an operand -- rows past the tile's, sums past
-// the end -- is outside its buffer resource or sent there: such loads write zeros
-// to LDS (measured), so a sum's tail adds 0 * 0 whatever memory holds there.
-template <int T_>
+// adjacent output columns of one output row. Stages of KB sums stream into an LDS
+// ring by buffer loads. What lies outside an operand -- rows past the tile's, sums
+// past the end, stages behind the last -- is outside its buffer resource or sent
+// there: such loads write zeros to LDS (measured), so a sum's tail adds 0 * 0
+// whatever memory holds there.
+// KB 32: five slots for each operand, loads four stages ahead; KB 64: two for Q and
+// three for P, two ahead. The longer way ahead covers an L2 miss, which a stage's
+// first reader in an XCD always has; but a row of 32 sums is half a cache line, and
+// the second request for it costs more than is won where both operands run along
+// their rows. (8192^3, KB 32 / 64, MFMA busy: dw 785 / 823 us, 80 / 67 %; dx 801 / 838;
+// forward 852 / 834. The clock falls from 1.8 to 1.56 GHz as the MFMAs get busier.)
+template <int T_, int KB_>
 struct LinearTile {
   static constexpr int T = T_;
+  static constexpr int KB = KB_;              // sums a stage
+  static constexpr int KK = KB / 16;          // MFMA steps
   static constexpr int NB = T / 64;           // 32-wide blocks of a wave, each way
-  static constexpr int NL = T / 32;           // loads of a wave per operand and stage
-  static constexpr int SLOT = T * 128;        // bytes
-  static constexpr int LDS = 5 * SLOT;        // Q: slots 0, 1; P: 2, 3, 4
+  static constexpr int SLOT = T * KB * 2;     // bytes of an operand's stage
+  static constexpr int NL = SLOT / 4096;      // loads of a wave per operand and stage
+  static constexpr int Q_SLOTS = KB == 32 ? 5 : 2, P_SLOTS = KB == 32 ? 5 : 3;
+  static constexpr int P_AT = Q_SLOTS * SLOT;
+  static constexpr int LDS = (Q_SLOTS + P_SLOTS) * SLOT;
   static constexpr int STAGING = T * T / 2;   // a wave's part in the epilogue, 16 bits
-  static_assert(4 * STAGING <= LDS, "staging");
+  static_assert(KB == 32 || KB == 64, "main loops");
+  static_assert(4 * STAGING <= LDS && LDS <= 160 * 1024, "LDS");
+  // Place of 16-byte chunk c of row r of KB sums: the LDS serves 16 lanes of a
+  // 16-byte read at a time, whose 16 rows share a chunk; the XOR spreads them over
+  // the places of the rows that 256 bytes hold.
+  static __device__ __forceinline__ int chunk(int r, int c) {
+    return c ^ ((r / (128 / KB)) & (KB / 8 - 1));
+  }
 };
 
 // Four rows of 16 values in LDS, a row to 16 lanes, column by column: lane i of 16
@@ -50,18 +67,19 @@ __device__ __forceinline__ s16x4 read_transposed(LdsWords __restrict__ at) {
 constexpr uint32_t kOutside = 0x80000000u;
 
 // Where lane l's 16 bytes of the wave's load i come from, in bytes from the
-// stage's origin (`along`: row r of the tile, swizzled chunk of its 128 bytes;
-// `across`: row of the 64, swizzled chunk of its 2T bytes).
-// Along: the LDS serves 16 lanes of a 16-byte read at a time, whose 16 rows share
-// a chunk; the XOR by r / 2 spreads them over the 16 places of two rows.
+// stage's origin (`along`: row r of the tile, swizzled chunk of its sums; `across`:
+// row of the stage's sums, swizzled chunk of its T columns).
 // Across: a transposing read of 16 lanes takes 32 bytes of four consecutive rows;
 // the XOR by 2 (row % 4) on 32-byte granules spreads two such reads over 256 bytes.
 template <class C, bool ACROSS>
 struct Feed {
   uint32_t off[C::NL];
-  uint32_t c0;  // along: byte in the row of even loads; odd ones: ^ 64
+  int c0;  // along: byte in the row of even loads; odd ones: ^ flip
+  static constexpr int FLIP = C::KB == 64 ? 64 : 0;
 
-  __device__ __forceinline__ void init(int wave, int lane, int64_t ld_bytes) {
+  // row(i): the operand's row, from the tile's first, of the tile's row i
+  template <class R>
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld_bytes, R&& row) {
     const uint32_t ld = static_cast<uint32_t>(ld_bytes);
     if constexpr (ACROSS) {
       constexpr int LPR = C::T / 8;      // lanes a row takes
@@ -75,13 +93,11 @@ struct Feed {
       }
       c0 = 0;
     } else {
-      const int r8 = lane >> 3;
-      c0 = ((lane & 7) ^ (r8 >> 1)) * 16;
+      constexpr int LPR = C::KB / 8, RPL = 64 / LPR;
+      c0 = C::chunk(lane / LPR, lane % LPR) * 16;
 #pragma unroll
-      for (int i = 0; i < C::NL; ++i) {
-        const int r = (wave * C::NL + i) * 8 + r8;
-        off[i] = r * ld + (c0 ^ ((i & 1) * 64));
-      }
+      for (int i = 0; i < C::NL; ++i)
+        off[i] = row((wave * C::NL + i) * RPL + lane / LPR) * ld + (c0 ^ ((i & 1) * FLIP));
     }
   }
 };
@@ -97,7 +113,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   constexpr bool FORWARD = MODE == kLinearForward || GATED;
   constexpr int T = C::T, NB = C::NB, NL = C::NL, SLOT = C::SLOT;
   constexpr int TN = GATED ? T / 2 : T;  // output columns of a tile
-  constexpr int P_AT = 2 * SLOT;
+  constexpr int P_AT = C::P_AT, KB = C::KB;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63;
@@ -142,7 +158,9 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   nrows = __builtin_amdgcn_readfirstlane(nrows);
   const bool none = !QA && e >= (p.counts ? p.groups : 1);  // rows of no group
   const int red = QA ? nrows : none ? 0 : p.red;
-  const int KT = (red + 63) / 64;
+  // (a stage of zeros where there are no sums: the accumulators then come from the
+  // loop alone, not from a choice that the compiler would make in VGPRs)
+  const int KT = max(1, (red + KB - 1) / KB);
 
   // ---- the bias, where the accumulators start: its loads go out before the
   // stages'.
@@ -176,44 +194,38 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   const int prows = PA ? 0 : min(TN, p.n - ct * TN);
   Feed<C, QA> fq;
   Feed<C, PA> fp;
-  fq.init(wave, lane, ldq);
-  fp.init(wave, lane, ldp);
-  if constexpr (GATED) {
-    // The tile's rows of P by 32: gate, up, gate, up ... of the same columns; the
-    // up rows' resource starts n rows further on.
-    const int r8 = lane >> 3;
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = (wave * NL + i) * 8 + r8;
-      fp.off[i] = ((r >> 6) * 32 + (r & 31)) * static_cast<uint32_t>(ldp) +
-                  (fp.c0 ^ ((i & 1) * 64));
-    }
-  }
-  auto resource = [](const uint8_t* base, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(base), 0, static_cast<int>(bytes > 0 ? bytes : 0), kBufWord3);
+  // (gated: the tile's rows of P by 32: gate, up, gate, up ... of the same columns; the
+  // up rows' resource starts n rows further on)
+  fq.init(wave, lane, ldq, [](int r) { return r; });
+  fp.init(wave, lane, ldp, [](int r) { return GATED ? (r >> 6) * 32 + (r & 31) : r; });
+  // `bytes` of them, none unless left > 0. (By a mask: with a branch, which the
+  // compiler makes of a choice here, a stage's instructions cannot be ordered: the
+  // products stood still for the LDS reads, 8 % more time.)
+  auto resource = [](const uint8_t* base, int bytes, int left) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0,
+                                             bytes & ~((left - 1) >> 31), kBufWord3);
   };
   auto feed = [&](auto across_c, const auto& f, const uint8_t* base, int64_t ld, int rows,
                   int width, int s, uint8_t* dst, bool up) {
     constexpr bool ACROSS = decltype(across_c)::value;
+    const int ld32 = static_cast<int>(ld);
     if constexpr (ACROSS) {
-      const int left = min(64, red - s * 64);
-      const __amdgpu_buffer_rsrc_t r = resource(
-          base + static_cast<int64_t>(s) * 64 * ld,
-          left > 0 ? (left - 1) * ld + width * 2 : 0);
+      const int left = red - s * KB;
+      const __amdgpu_buffer_rsrc_t r =
+          resource(base + static_cast<int64_t>(s) * KB * ld,
+                   (min(KB, left) - 1) * ld32 + width * 2, left);
 #pragma unroll
       for (int i = 0; i < NL; ++i) lds_dma16_buf(r, f.off[i], 0, dst + i * 1024);
     } else {
-      const int left = (red - s * 64) * 2;  // bytes of sums from here on
-      const uint8_t* b = base + static_cast<int64_t>(s) * 128;
-      const int64_t bytes = left > 0 && rows > 0 ? (rows - 1) * ld + left : 0;
-      const __amdgpu_buffer_rsrc_t r = resource(b, bytes);
-      const __amdgpu_buffer_rsrc_t ru = resource(up ? b + p.n * ld : b, bytes);
-      const bool in0 = static_cast<int>(f.c0) < left, in1 = static_cast<int>(f.c0 ^ 64) < left;
+      const int left = (red - s * KB) * 2;  // bytes of sums from here on
+      const uint8_t* b = base + static_cast<int64_t>(s) * (KB * 2);
+      const int bytes = (rows - 1) * ld32 + left;
+      const __amdgpu_buffer_rsrc_t r = resource(b, bytes, left);
+      const __amdgpu_buffer_rsrc_t ru = resource(up ? b + p.n * ld : b, bytes, left);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const bool is_up = up && (((wave * NL + i) >> 2) & 1);
-        const uint32_t o = ((i & 1) ? in1 : in0) ? f.off[i] : kOutside;
+        const bool is_up = up && (((wave * NL + i) * (512 / KB) >> 5) & 1);
+        const uint32_t o = (f.c0 ^ ((i & 1) * f.FLIP)) < left ? f.off[i] : kOutside;
         if (is_up) lds_dma16_buf(ru, o, 0, dst + i * 1024);
         else lds_dma16_buf(r, o, 0, dst + i * 1024);
       }
@@ -230,10 +242,10 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 
   // ---- fragments: 32 rows x 16 sums, eight sums a lane. Q's blocks of a wave are
   // the tile's blocks 2i + wm, so that both halves share a short tile's rows.
-  int along[4];  // by 16 sums
+  int along[C::KK];  // by 16 sums
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk)
-    along[kk] = (lane & 31) * 128 + (((2 * kk + h) ^ ((lane >> 1) & 7)) * 16);
+  for (int kk = 0; kk < C::KK; ++kk)
+    along[kk] = (lane & 31) * (KB * 2) + C::chunk(lane & 31, 2 * kk + h) * 16;
   int across[4];  // by block % 4: lane's row and 8 bytes
   const int a4 = (lane >> 2) & 3;
 #pragma unroll
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
       const s16x4 hi = read_transposed((LdsWords)(a + 4 * 2 * T));
       return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const Frag*>(lds + slot + block * 32 * 128 + along[kk]);
+      return *reinterpret_cast<const Frag*>(lds + slot + block * 32 * KB * 2 + along[kk]);
     }
   };
   f32x16 acc[NB][NB];
@@ -267,54 +279,38 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   };
 
   // The order of a step's instructions: the next step's LDS reads behind the first
-  // MFMAs, then the loads (0 or NL) one between each pair of MFMAs.
+  // MFMAs, then the loads (0 or NL) spread over the others.
   constexpr int NM = NB * NB, NR = NB * ((QA ? 2 : 1) + (PA ? 2 : 1));
   auto order = [&](auto loads_c) {
     constexpr int LOADS = decltype(loads_c)::value;
-    constexpr int PER = (NR + NM / 2 - 1) / (NM / 2);  // reads behind an MFMA
-    constexpr int RM = (NR + PER - 1) / PER;           // MFMAs with reads
+    // MFMAs for the reads
+    constexpr int MR = LOADS > 0 && NM - LOADS > NM / 2 ? NM - LOADS : NM / 2;
+    constexpr int PER = (NR + MR - 1) / MR, RM = (NR + PER - 1) / PER;
+    constexpr int LPM = LOADS ? (LOADS + NM - RM - 1) / (NM - RM) : 1;
     static_for<RM>([&](auto) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     });
-    static_for<LOADS>([&](auto) {
-      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    static_for<(LOADS + LPM - 1) / LPM>([&](auto) {
+      __builtin_amdgcn_sched_group_barrier(0x020, LPM, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     });
   };
 
-  // ---- main loop. Stage s lives in Q's slot s % 2 and P's slot s % 3. The
-  // barrier before its last 16 sums publishes stage s + 1 (every wave has waited
-  // for its own loads of it) and frees stage s's slots; P's loads of stage s + 2 go
-  // out during its first 16 sums, Q's after that barrier.
-  auto next_q = [](int o) { return SLOT - o; };
-  auto next_p = [](int o) { return o == 2 * SLOT ? 0 : o + SLOT; };
-  auto prev_p = [](int o) { return o == 0 ? 2 * SLOT : o - SLOT; };
-  auto stage = [&](int s, int oq, int op, auto refill_c) {
-    constexpr bool REFILL = decltype(refill_c)::value;
+  // ---- main loop. Stage s lives in slot s % SLOTS of each ring. The barrier before its
+  // last 16 sums publishes stage s + 1 (every wave has waited for its own loads of it)
+  // and frees stage s's slots. P's loads of stage s + AHEAD go out during the first 16
+  // sums, into the slot of stage s - 1; Q's after the barrier, into stage s - 1's
+  // (five slots) or s's own (two).
+  constexpr int AHEAD = KB == 32 ? 4 : 2;
+  constexpr std::integral_constant<int, NL> loads{};
+  constexpr std::integral_constant<int, 0> no_loads{};
+  auto next_q = [](int o) { return o == (C::Q_SLOTS - 1) * SLOT ? 0 : o + SLOT; };
+  auto next_p = [](int o) { return o == (C::P_SLOTS - 1) * SLOT ? 0 : o + SLOT; };
 #pragma unroll
-    for (int kk = 0; kk < 3; ++kk) {
-      read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
-      if (REFILL && kk == 0) feed_p(s + 2, prev_p(op));
-      mma(fa[kk & 1], fb[kk & 1]);
-      if (REFILL && kk == 0) order(std::integral_constant<int, NL>{});
-      else order(std::integral_constant<int, 0>{});
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    wait_lgkm0();
-    wait_vmcnt<REFILL ? NL : 0>();
-    wave_barrier_all();
-    read_frags(next_q(oq), next_p(op), 0, fa[0], fb[0]);
-    if constexpr (REFILL) feed_q(s + 2, oq);
-    mma(fa[1], fb[1]);
-    order(std::integral_constant<int, REFILL ? NL : 0>{});
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  if (KT > 0) {
-    feed_q(0, 0);
-    feed_p(0, 0);
-    feed_q(1, SLOT);
-    feed_p(1, SLOT);
+  for (int s = 0; s < AHEAD; ++s) {
+    feed_p(s, s * SLOT);
+    feed_q(s, s * SLOT);
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j)
@@ -327,24 +323,35 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 #pragma unroll
         for (int i = 0; i < NB; ++i) acc[i][j][4 * g + t] = v;
       }
-  if (KT > 0) {
-    wait_vmcnt<2 * NL>();
-    wave_barrier_all();
-    read_frags(0, 0, 0, fa[0], fb[0]);
-    int s = 0, oq = 0, op = 0;
-    for (; s + 2 < KT; ++s, oq = next_q(oq), op = next_p(op)) stage(s, oq, op, std::true_type{});
-    if (s + 1 < KT) {
-      stage(s, oq, op, std::false_type{});
-      oq = next_q(oq);
-      op = next_p(op);
-    }
+  wait_vmcnt<2 * (AHEAD - 1) * NL>();
+  wave_barrier_all();
+  read_frags(0, 0, 0, fa[0], fb[0]);
+  int oq = 0, op = 0, to_q = AHEAD % C::Q_SLOTS * SLOT, to_p = AHEAD % C::P_SLOTS * SLOT, s = 0;
+  do {
 #pragma unroll
-    for (int kk = 0; kk < 3; ++kk) {
+    for (int kk = 0; kk + 1 < C::KK; ++kk) {
       read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+      if (kk == 0) feed_p(s + AHEAD, to_p);
       mma(fa[kk & 1], fb[kk & 1]);
+      if (kk == 0) order(loads);
+      else order(no_loads);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    wait_lgkm0();
+    // behind stage s + 1's loads: those of the stages to s + AHEAD - 1, and P's
+    wait_vmcnt<(2 * (AHEAD - 2) + 1) * NL>();
+    wave_barrier_all();
+    __builtin_amdgcn_sched_barrier(0);
+    oq = next_q(oq);
+    op = next_p(op);
+    read_frags(oq, op, 0, fa[0], fb[0]);
+    feed_q(s + AHEAD, to_q);
+    to_q = next_q(to_q);
+    to_p = next_p(to_p);
     mma(fa[1], fb[1]);
-  }
+    order(loads);
+    __builtin_amdgcn_sched_barrier(0);
+  } while (++s < KT);
   wait_vmcnt<0>();
   wait_lgkm0();
   wave_barrier_all();  // the ring is done with
@@ -395,6 +402,9 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   auto pack4 = [](const float (&v)[4]) {
     return uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
   };
+  // (Accumulators stay where they are until they are used: otherwise the compiler
+  // reads all of them into VGPRs ahead, more than there are.)
+  auto keep = [](f32x16& a) { asm volatile("" : "+a"(a)); };
   const int r32 = lane & 31;
   constexpr std::integral_constant<int, OC> out_cols{};
   if (FORWARD && p.z) {
@@ -404,7 +414,8 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = HALF; j < NB; j += GATED ? 2 : 1)
+        for (int j = HALF; j < NB; j += GATED ? 2 : 1) {
+          keep(acc[i][j]);
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
@@ -412,6 +423,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
             *reinterpret_cast<uint2*>(
                 stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h)) = pack4(v);
           }
+        }
       store(out_cols, p.z, wide, HALF * p.n);
     });
   }
@@ -436,6 +448,8 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
         return reinterpret_cast<uint2*>(
             stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
       };
+      keep(acc[i][j]);
+      if constexpr (GATED) keep(acc[i][j + 1]);
       uint2 res[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -484,7 +498,7 @@ int launch_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& to
 
 template <int TY, int MODE, int ACT, int T>
 int launch_tile(const LinearParams& p, hipStream_t stream) {
-  typedef LinearTile<T> C;
+  typedef LinearTile<T, T == 256 && (MODE == kLinearDgrad || MODE == kLinearWgrad) ? 32 : 64> C;
   static std::atomic<uint64_t> told{0};
   const int64_t tn = MODE == kLinearGated ? T / 2 : T;
   const int64_t nc = (p.n + tn - 1) / tn;
