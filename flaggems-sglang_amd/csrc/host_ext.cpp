@@ -20,7 +20,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
@@ -170,9 +171,12 @@ struct OnGpu {
   const int was;
   const bool moved;
 };
+// (A backward pass comes without the lock.)
 struct Unlocked {
-  Unlocked() : state(PyEval_SaveThread()) {}
-  ~Unlocked() { PyEval_RestoreThread(state); }
+  Unlocked() : state(PyGILState_Check() ? PyEval_SaveThread() : nullptr) {}
+  ~Unlocked() {
+    if (state) PyEval_RestoreThread(state);
+  }
   Unlocked(const Unlocked&) = delete;
   PyThreadState* const state;
 };
@@ -469,12 +473,11 @@ PyMethodDef g_methods[] = {
     method<rms_norm, 9>("rms_norm"),
     method<silu_and_mul_quant, 4>("silu_and_mul_quant"),
     method<fp8_block_matmul, 8>("fp8_block_matmul"),
-    method<bind_steps, 12>("bind_steps"),
-    method<permute, 3>("permute"),
-    method<permute_rows, 3>("permute_rows"),
-    method<unpermute, 3>("unpermute"),
-    method<unpermute_grad, 7>("unpermute_grad"),
-    method<topk_gating_grad, 6>("topk_gating_grad"),
+    method<bind_steps, 13>("bind_steps"),
+    method<permute, 4>("permute"),
+    method<permute_rows, 4>("permute_rows"),
+    method<unpermute, 5>("unpermute"),
+    method<topk_gating, 4>("topk_gating"),
     method<linear, 9>("linear"),
     method<linear_grad, 11>("linear_grad"),
     method<foreign_leaf, 1>("foreign_leaf"),

@@ -7,6 +7,7 @@ struct StepsLibrary {
   decltype(&fgs_moe_permute_rows) permute_rows;
   decltype(&fgs_moe_unpermute) unpermute;
   decltype(&fgs_moe_unpermute_grad) unpermute_grad;
+  decltype(&fgs_moe_topk_gating) topk_gating;
   decltype(&fgs_moe_topk_gating_grad) topk_gating_grad;
   decltype(&fgs_moe_linear) linear;
   decltype(&fgs_moe_linear_act_grad) linear_act_grad;
@@ -49,14 +50,18 @@ void check_order(const at::Tensor& row_of_slot, const at::Tensor* slot_of_row) {
           "slot_of_row must be int32 [rows]");
 }
 
-// permute(x, topk_ids, num_experts) -> (rows, counts, row_of_slot, slot_of_row)
-PyObject* permute(PyObject* const* args) {
-  const Arg xa = tensor_arg(args[0], "x"), ia = tensor_arg(args[1], "topk_ids");
-  const int index = check_inputs({xa, ia});
-  const int64_t experts = whole(args[2]);
-  const at::Tensor& x = *xa.t;
+void check_movable(const at::Tensor& x) {
   require(x.dim() == 2 && x.size(1) > 0, "x must be [tokens, cols]");
   require(movable(x.scalar_type()), "x must be of a 8- to 64-bit integer or a 8- to 32-bit float type");
+}
+
+struct Permuted {
+  at::Tensor rows, counts, row_of_slot, slot_of_row;
+};
+Permuted permute_of(const Arg& xa, const Arg& ia, int64_t experts) {
+  const int index = check_inputs({xa, ia});
+  const at::Tensor& x = *xa.t;
+  check_movable(x);
   require(ia.t->dim() == 2 && ia.t->size(0) == x.size(0) && ia.t->size(1) > 0 &&
               ia.t->scalar_type() == at::kInt,
           "topk_ids must be int32 [tokens, topk]");
@@ -65,28 +70,22 @@ PyObject* permute(PyObject* const* args) {
   const int64_t m = x.size(0), topk = ia.t->size(1), slots = m * topk, size = x.element_size();
   const Rows xr = rows_of(x, x.size(1));
   const at::Tensor ids = contiguous(*ia.t);
-  const at::Tensor rows = make({slots, x.size(1)}, x.scalar_type(), x);
-  const at::Tensor counts = make({experts}, at::kInt, x);
-  const at::Tensor row_of_slot = make({m, topk}, at::kInt, x);
-  const at::Tensor slot_of_row = make({slots}, at::kInt, x);
   const int64_t need = g_steps.permute_workspace_bytes(slots, static_cast<int32_t>(experts));
   if (need < 0) refuse(PyExc_NotImplementedError, "moe_permute: more than 2^30 slots");
+  const Permuted p{make({slots, x.size(1)}, x.scalar_type(), x), make({experts}, at::kInt, x),
+                   make({m, topk}, at::kInt, x), make({slots}, at::kInt, x)};
   const at::Tensor ws = bytes_for(need, x);
   void* stream = stream_of(index);
   call(index, "moe_permute", g_steps.permute, ptr(xr.t), xr.stride * size, m, x.size(1) * size,
-       ints(ids), static_cast<int32_t>(topk), static_cast<int32_t>(experts), ptr(rows),
-       ints_out(counts), ints_out(row_of_slot), ints_out(slot_of_row), ptr(ws), need, stream);
-  return wrap_all<4>({rows, counts, row_of_slot, slot_of_row});
+       ints(ids), static_cast<int32_t>(topk), static_cast<int32_t>(experts), ptr(p.rows),
+       ints_out(p.counts), ints_out(p.row_of_slot), ints_out(p.slot_of_row), ptr(ws), need, stream);
+  return p;
 }
 
-// permute_rows(x, row_of_slot, slot_of_row) -> rows
-PyObject* permute_rows(PyObject* const* args) {
-  const Arg xa = tensor_arg(args[0], "x"), ra = tensor_arg(args[1], "row_of_slot"),
-            sa = tensor_arg(args[2], "slot_of_row");
+at::Tensor permute_rows_of(const Arg& xa, const Arg& ra, const Arg& sa) {
   const int index = check_inputs({xa, ra, sa});
   const at::Tensor& x = *xa.t;
-  require(x.dim() == 2 && x.size(1) > 0, "x must be [tokens, cols]");
-  require(movable(x.scalar_type()), "x must be of a 8- to 64-bit integer or a 8- to 32-bit float type");
+  check_movable(x);
   check_order(*ra.t, sa.t);
   require(ra.t->size(0) == x.size(0) && sa.t->size(0) == ra.t->numel(),
           "the order is one of other tokens");
@@ -98,7 +97,7 @@ PyObject* permute_rows(PyObject* const* args) {
   call(index, "moe_permute", g_steps.permute_rows, ptr(xr.t), xr.stride * size, x.size(0),
        x.size(1) * size, ints(row_of_slot), static_cast<int32_t>(row_of_slot.size(1)),
        ints(slot_of_row), ptr(rows), stream);
-  return wrap(rows);
+  return rows;
 }
 
 void check_weights(const Arg& wa, const at::Tensor& row_of_slot) {
@@ -106,10 +105,7 @@ void check_weights(const Arg& wa, const at::Tensor& row_of_slot) {
           "topk_weights must be float32 [tokens, topk]");
 }
 
-// unpermute(rows, row_of_slot, topk_weights) -> out
-PyObject* unpermute(PyObject* const* args) {
-  const Arg ra = tensor_arg(args[0], "rows"), oa = tensor_arg(args[1], "row_of_slot"),
-            wa = tensor_arg(args[2], "topk_weights", true);
+at::Tensor unpermute_of(const Arg& ra, const Arg& oa, const Arg& wa) {
   const int index = check_inputs({ra, oa, wa});
   const at::Tensor& rows = *ra.t;
   const int type = type_code(rows);
@@ -125,17 +121,14 @@ PyObject* unpermute(PyObject* const* args) {
   void* stream = stream_of(index);
   call(index, "moe_unpermute", g_steps.unpermute, ptr(rr.t), rr.stride, rows.size(0), ints(order),
        floats(weights), m, static_cast<int32_t>(order.size(1)), cols, type, ptr(out), stream);
-  return wrap(out);
+  return out;
 }
 
-// unpermute_grad(dout, rows, row_of_slot, slot_of_row, topk_weights, with_drows,
-// with_dweights) -> (drows, dweights); rows may be None without dweights
-PyObject* unpermute_grad(PyObject* const* args) {
-  const Arg da = tensor_arg(args[0], "dout"), ra = tensor_arg(args[1], "rows", true),
-            oa = tensor_arg(args[2], "row_of_slot"), sa = tensor_arg(args[3], "slot_of_row"),
-            wa = tensor_arg(args[4], "topk_weights", true);
+// (drows, dweights), those asked for; rows only for dweights.
+std::array<at::Tensor, 2> unpermute_grad_of(const Arg& da, const Arg& ra, const Arg& oa,
+                                            const Arg& sa, const Arg& wa, bool with_drows,
+                                            bool with_dweights) {
   const int index = check_inputs({da, ra, oa, sa, wa});
-  const bool with_drows = truth(args[5]), with_dweights = truth(args[6]);
   const at::Tensor& dout = *da.t;
   const int type = type_code(dout);
   require(type >= 0, "dout must be bfloat16, float16 or float32");
@@ -162,19 +155,38 @@ PyObject* unpermute_grad(PyObject* const* args) {
   call(index, "moe_unpermute", g_steps.unpermute_grad, ptr(dr.t), dr.stride, ptr(rr.t), rr.stride,
        n_rows, ints(order), ints(slot_of_row), floats(weights), m,
        static_cast<int32_t>(order.size(1)), cols, type, ptr(drows), floats(dweights), stream);
-  return wrap_all<2>({drows, dweights});
+  return {drows, dweights};
 }
 
-// topk_gating_grad(logits, weights, ids, dweights, scoring, renormalize) -> dlogits
-PyObject* topk_gating_grad(PyObject* const* args) {
-  const Arg la = tensor_arg(args[0], "logits"), wa = tensor_arg(args[1], "weights"),
-            ia = tensor_arg(args[2], "ids"), da = tensor_arg(args[3], "dweights");
-  const int index = check_inputs({la, wa, ia, da});
-  const int32_t scoring = static_cast<int32_t>(whole(args[4]));
-  const bool renormalize = truth(args[5]);
-  const at::Tensor& l = *la.t;
+// ----------------------------------------------------------------- router ---
+void check_logits(const at::Tensor& l, int64_t topk) {
   require(l.dim() == 2 && (l.scalar_type() == at::kFloat || l.scalar_type() == at::kBFloat16),
           "logits must be float32 or bfloat16 [tokens, experts]");
+  if (topk < 0 || topk > 64) refuse(PyExc_ValueError, "fused_topk: topk must be in [1, 64]");
+}
+
+// (weights, ids)
+std::array<at::Tensor, 2> topk_gating_of(const Arg& la, int64_t topk, int32_t scoring,
+                                         bool renormalize) {
+  const int index = check_inputs({la});
+  const at::Tensor& l = *la.t;
+  check_logits(l, topk);
+  const at::Tensor logits = contiguous(l);
+  const at::Tensor weights = make({l.size(0), topk}, at::kFloat, l);
+  const at::Tensor ids = make({l.size(0), topk}, at::kInt, l);
+  void* stream = stream_of(index);
+  call(index, "fused_topk", g_steps.topk_gating, ptr(logits),
+       static_cast<int32_t>(l.scalar_type() == at::kBFloat16), l.size(0),
+       static_cast<int32_t>(l.size(1)), static_cast<int32_t>(topk), scoring,
+       static_cast<int32_t>(renormalize), floats(weights), ints_out(ids), stream);
+  return {weights, ids};
+}
+
+at::Tensor topk_gating_grad_of(const Arg& la, const Arg& wa, const Arg& ia, const Arg& da,
+                               int32_t scoring, bool renormalize) {
+  const int index = check_inputs({la, wa, ia, da});
+  const at::Tensor& l = *la.t;
+  check_logits(l, 0);
   require(ia.t->dim() == 2 && ia.t->size(0) == l.size(0) && ia.t->scalar_type() == at::kInt,
           "ids must be int32 [tokens, topk]");
   require(wa.t->sizes() == ia.t->sizes() && da.t->sizes() == ia.t->sizes() &&
@@ -188,7 +200,7 @@ PyObject* topk_gating_grad(PyObject* const* args) {
        static_cast<int32_t>(l.scalar_type() == at::kBFloat16), l.size(0),
        static_cast<int32_t>(l.size(1)), static_cast<int32_t>(ids.size(1)), scoring,
        static_cast<int32_t>(renormalize), floats(weights), ints(ids), floats(d), ptr(out), stream);
-  return wrap(out);
+  return out;
 }
 
 // --------------------------------------------------------------- products ---
@@ -241,19 +253,20 @@ at::Tensor flat(const at::Tensor& x, int64_t rows, int64_t cols) {
   return x.dim() == 2 ? x : x.reshape({rows, cols});
 }
 
-// linear(x, weight, counts, bias, act, gated, residual, with_z, flags) -> (out, z)
-PyObject* linear(PyObject* const* args) {
-  const Arg xa = tensor_arg(args[0], "x"), wa = tensor_arg(args[1], "weight"),
-            ca = tensor_arg(args[2], "counts", true), ba = tensor_arg(args[3], "bias", true),
-            ra = tensor_arg(args[6], "residual", true);
+struct LinearHow {
+  int32_t act;
+  bool gated;
+  int32_t flags;
+};
+
+// (out, z)
+std::array<at::Tensor, 2> linear_of(const Arg& xa, const Arg& wa, const Arg& ca, const Arg& ba,
+                                    const Arg& ra, LinearHow how, bool with_z) {
   const int index = check_inputs({xa, wa, ca, ba, ra});
-  const int32_t act = static_cast<int32_t>(whole(args[4]));
-  const bool gated = truth(args[5]), with_z = truth(args[7]);
-  const int32_t flags = static_cast<int32_t>(whole(args[8]));
   const at::Tensor &x = *xa.t, &w = *wa.t;
   const LinearSizes s = check_product(x, w, ca);
-  require(!gated || s.wide % 2 == 0, "a gated weight must hold gate rows and up rows");
-  const int64_t n = gated ? s.wide / 2 : s.wide;
+  require(!how.gated || s.wide % 2 == 0, "a gated weight must hold gate rows and up rows");
+  const int64_t n = how.gated ? s.wide / 2 : s.wide;
   at::DimVector shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
   at::Tensor bias;
@@ -277,32 +290,26 @@ PyObject* linear(PyObject* const* args) {
   void* stream = stream_of(index);
   call(index, ca.t ? "grouped_linear" : "fused_linear", g_steps.linear, ptr(xm.t), xm.row,
        ptr(wm.t), wm.row, wm.group, ptr(bias), ptr(res.t), res.row, ints(counts),
-       static_cast<int32_t>(s.groups), s.rows, n, s.k, static_cast<int32_t>(type_code(x)), act,
-       static_cast<int32_t>(gated), flags, ptr(z), ptr(out), stream);
-  return wrap_all<2>({out, z});
+       static_cast<int32_t>(s.groups), s.rows, n, s.k, static_cast<int32_t>(type_code(x)),
+       how.act, static_cast<int32_t>(how.gated), how.flags, ptr(z), ptr(out), stream);
+  return {out, z};
 }
 
-// linear_grad(dout, x, weight, counts, z, act, gated, with_dx, with_dweight,
-// with_dbias, flags) -> (dx, dweight, dbias)
-PyObject* linear_grad(PyObject* const* args) {
-  const Arg da = tensor_arg(args[0], "dout"), xa = tensor_arg(args[1], "x"),
-            wa = tensor_arg(args[2], "weight"), ca = tensor_arg(args[3], "counts", true),
-            za = tensor_arg(args[4], "z", true);
+// (dx, dweight, dbias), those asked for
+std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg& wa,
+                                         const Arg& ca, const Arg& za, LinearHow how,
+                                         bool with_dx, bool with_dw, bool with_db) {
   const int index = check_inputs({da, xa, wa, ca, za});
-  const int32_t act = static_cast<int32_t>(whole(args[5]));
-  const bool gated = truth(args[6]), with_dx = truth(args[7]), with_dw = truth(args[8]),
-             with_db = truth(args[9]);
-  const int32_t flags = static_cast<int32_t>(whole(args[10]));
   const at::Tensor &x = *xa.t, &w = *wa.t;
   const char* what = ca.t ? "grouped_linear" : "fused_linear";
   const LinearSizes s = check_product(x, w, ca);
-  require(!gated || s.wide % 2 == 0, "a gated weight must hold gate rows and up rows");
-  const int64_t n = gated ? s.wide / 2 : s.wide;
+  require(!how.gated || s.wide % 2 == 0, "a gated weight must hold gate rows and up rows");
+  const int64_t n = how.gated ? s.wide / 2 : s.wide;
   at::DimVector shape(x.sizes().begin(), x.sizes().end());
   shape.back() = n;
   require(da.t->sizes() == shape && da.t->scalar_type() == x.scalar_type(),
           "dout must be of the output's shape and type");
-  require(za.t || (act == FGS_ACT_NONE && !gated), "an activation's gradient needs z");
+  require(za.t || (how.act == FGS_ACT_NONE && !how.gated), "an activation's gradient needs z");
   require(!za.t || (za.t->dim() == 2 && za.t->size(0) == s.rows && za.t->size(1) == s.wide &&
                     za.t->scalar_type() == x.scalar_type() && za.t->is_contiguous()),
           "z must be [rows, n] of x's type, contiguous");
@@ -312,8 +319,8 @@ PyObject* linear_grad(PyObject* const* args) {
   Matrix dz = matrix(flat(*da.t, s.rows, n), s.rows, n);
   if (za.t) {
     const at::Tensor t = make({s.rows, s.wide}, x.scalar_type(), x);
-    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, ptr(*za.t), s.rows, n, type, act,
-         static_cast<int32_t>(gated), ptr(t), stream);
+    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, ptr(*za.t), s.rows, n, type,
+         how.act, static_cast<int32_t>(how.gated), ptr(t), stream);
     dz = {t, s.wide, 0};
   }
   at::Tensor dx, dw, db;
@@ -321,13 +328,13 @@ PyObject* linear_grad(PyObject* const* args) {
     const Matrix wm = matrix(w, s.wide, s.k);
     dx = make(x.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_input_grad, ptr(dz.t), dz.row, ptr(wm.t), wm.row, wm.group,
-         ints(counts), groups, s.rows, s.wide, s.k, type, flags, ptr(dx), stream);
+         ints(counts), groups, s.rows, s.wide, s.k, type, how.flags, ptr(dx), stream);
   }
   if (with_dw) {
     const Matrix xm = matrix(flat(x, s.rows, s.k), s.rows, s.k);
     dw = make(w.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_weight_grad, ptr(dz.t), dz.row, ptr(xm.t), xm.row,
-         ints(counts), groups, s.rows, s.wide, s.k, type, flags, ptr(dw), stream);
+         ints(counts), groups, s.rows, s.wide, s.k, type, how.flags, ptr(dw), stream);
   }
   if (with_db) {
     const int64_t need = g_steps.linear_bias_grad_workspace_bytes(groups, s.rows, s.wide);
@@ -336,7 +343,238 @@ PyObject* linear_grad(PyObject* const* args) {
     call(index, what, g_steps.linear_bias_grad, ptr(dz.t), dz.row, ints(counts), groups, s.rows,
          s.wide, type, ptr(ws), need, ptr(db), stream);
   }
-  return wrap_all<3>({dx, dw, db});
+  return {dx, dw, db};
+}
+
+// -------------------------------------------------------------- gradients ---
+// The operators as autograd functions. (As Python ones a forward and backward call
+// of the router took 75 us, 8 of them the GPU's.)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+Arg optional_arg(const at::Tensor& t, const char* name) { return {name, t.defined() ? &t : nullptr}; }
+// (An undefined tensor is no argument of an autograd function; an absent optional one has
+// no place among its edges either.)
+std::optional<at::Tensor> given(const Arg& a) {
+  return a.t ? std::optional<at::Tensor>(*a.t) : std::nullopt;
+}
+at::Tensor or_undefined(const std::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); }
+
+// A backward pass: `f` of gradients that are there, without gradients of its own;
+// where a derivative of the result is asked for (create_graph), taking it raises.
+template <class F>
+variable_list backward_of(const char* what, const variable_list& grads, size_t count, F&& f) {
+  variable_list out(count);
+  if (!grads[0].defined()) return out;
+  const bool again = c10::GradMode::is_enabled();
+  {
+    const at::AutoGradMode off(false);
+    try {
+      f(out);
+    } catch (const Refusal& r) {  // (as what the engine hands on to the caller)
+      TORCH_CHECK(false, r.text);
+    }
+  }
+  if (!again) return out;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " has no second derivative", static_cast<int64_t>(count));
+  variable_list defined;
+  for (const at::Tensor& t : out) defined.push_back(t);
+  return (*error)(std::move(defined));
+}
+
+struct PermuteFunction : torch::autograd::Function<PermuteFunction> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids,
+                               int64_t experts) {
+    const Permuted p = permute_of({"x", &x}, {"topk_ids", &ids}, experts);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({p.counts, p.row_of_slot, p.slot_of_row});
+    ctx->save_for_backward({p.row_of_slot});
+    return {p.rows, p.counts, p.row_of_slot, p.slot_of_row};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return backward_of("moe_permute", grads, 3, [&](variable_list& out) {
+      const at::Tensor order = ctx->get_saved_variables()[0];
+      out[0] = unpermute_of({"rows", &grads[0]}, {"row_of_slot", &order}, {"topk_weights", nullptr});
+    });
+  }
+};
+
+struct PermuteRowsFunction : torch::autograd::Function<PermuteRowsFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& row_of_slot,
+                            const at::Tensor& slot_of_row) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({row_of_slot});
+    return permute_rows_of({"x", &x}, {"row_of_slot", &row_of_slot}, {"slot_of_row", &slot_of_row});
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return backward_of("moe_permute", grads, 3, [&](variable_list& out) {
+      const at::Tensor order = ctx->get_saved_variables()[0];
+      out[0] = unpermute_of({"rows", &grads[0]}, {"row_of_slot", &order}, {"topk_weights", nullptr});
+    });
+  }
+};
+
+struct UnpermuteFunction : torch::autograd::Function<UnpermuteFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows,
+                            const std::optional<at::Tensor>& given_weights,
+                            const at::Tensor& row_of_slot, const at::Tensor& slot_of_row,
+                            bool with_dweights) {
+    const at::Tensor weights = or_undefined(given_weights);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({with_dweights ? rows : at::Tensor(), weights, row_of_slot, slot_of_row});
+    return unpermute_of({"rows", &rows}, {"row_of_slot", &row_of_slot},
+                        optional_arg(weights, "topk_weights"));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return backward_of("moe_unpermute", grads, 5, [&](variable_list& out) {
+      const variable_list saved = ctx->get_saved_variables();
+      const auto g = unpermute_grad_of(
+          {"dout", &grads[0]}, optional_arg(saved[0], "rows"), {"row_of_slot", &saved[2]},
+          {"slot_of_row", &saved[3]}, optional_arg(saved[1], "topk_weights"),
+          ctx->needs_input_grad(0), saved[0].defined() && ctx->needs_input_grad(1));
+      out[0] = g[0];
+      out[1] = g[1];
+    });
+  }
+};
+
+struct TopkFunction : torch::autograd::Function<TopkFunction> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, int64_t topk,
+                               int64_t scoring, bool renormalize) {
+    const auto r = topk_gating_of({"gating_output", &logits}, topk, static_cast<int32_t>(scoring),
+                                  renormalize);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({r[1]});
+    ctx->save_for_backward({logits, r[0], r[1]});
+    ctx->saved_data["scoring"] = scoring;
+    ctx->saved_data["renormalize"] = renormalize;
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return backward_of("fused_topk", grads, 4, [&](variable_list& out) {
+      const variable_list saved = ctx->get_saved_variables();
+      out[0] = topk_gating_grad_of({"logits", &saved[0]}, {"weights", &saved[1]}, {"ids", &saved[2]},
+                                   {"dweights", &grads[0]},
+                                   static_cast<int32_t>(ctx->saved_data["scoring"].toInt()),
+                                   ctx->saved_data["renormalize"].toBool());
+    });
+  }
+};
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const std::optional<at::Tensor>& given_bias,
+                            const std::optional<at::Tensor>& given_residual,
+                            const std::optional<at::Tensor>& given_counts, int64_t act, bool gated,
+                            int64_t flags, bool with_z) {
+    const at::Tensor bias = or_undefined(given_bias), residual = or_undefined(given_residual),
+                     counts = or_undefined(given_counts);
+    const LinearHow how{static_cast<int32_t>(act), gated, static_cast<int32_t>(flags)};
+    const auto r = linear_of({"x", &x}, {"weight", &w}, optional_arg(counts, "counts"),
+                             optional_arg(bias, "bias"), optional_arg(residual, "residual"), how,
+                             with_z);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w, counts, r[1]});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["gated"] = gated;
+    ctx->saved_data["flags"] = flags;
+    ctx->saved_data["bias"] = bias.defined();
+    ctx->saved_data["residual"] = residual.defined();
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return backward_of("this product", grads, 9, [&](variable_list& out) {
+      const bool bias = ctx->saved_data["bias"].toBool();
+      const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1),
+                 db = bias && ctx->needs_input_grad(2);
+      if (dx || dw || db) {
+        const variable_list saved = ctx->get_saved_variables();
+        const LinearHow how{static_cast<int32_t>(ctx->saved_data["act"].toInt()),
+                            ctx->saved_data["gated"].toBool(),
+                            static_cast<int32_t>(ctx->saved_data["flags"].toInt())};
+        const auto g = linear_grad_of({"dout", &grads[0]}, {"x", &saved[0]}, {"weight", &saved[1]},
+                                      optional_arg(saved[2], "counts"), optional_arg(saved[3], "z"),
+                                      how, dx, dw, db);
+        for (int i = 0; i < 3; ++i) out[i] = g[i];
+      }
+      if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2 + bias)) out[3] = grads[0];
+    });
+  }
+};
+
+// ------------------------------------------------------------ Python's calls ---
+// permute(x, topk_ids, num_experts, with_grad) -> (rows, counts, row_of_slot,
+// slot_of_row)
+PyObject* permute(PyObject* const* args) {
+  const Arg x = tensor_arg(args[0], "x"), ids = tensor_arg(args[1], "topk_ids");
+  const int64_t experts = whole(args[2]);
+  if (truth(args[3])) {
+    const variable_list r = PermuteFunction::apply(*x.t, *ids.t, experts);
+    return wrap_all<4>({r[0], r[1], r[2], r[3]});
+  }
+  const Permuted p = permute_of(x, ids, experts);
+  return wrap_all<4>({p.rows, p.counts, p.row_of_slot, p.slot_of_row});
+}
+
+// permute_rows(x, row_of_slot, slot_of_row, with_grad) -> rows
+PyObject* permute_rows(PyObject* const* args) {
+  const Arg x = tensor_arg(args[0], "x"), row_of_slot = tensor_arg(args[1], "row_of_slot"),
+            slot_of_row = tensor_arg(args[2], "slot_of_row");
+  if (truth(args[3])) return wrap(PermuteRowsFunction::apply(*x.t, *row_of_slot.t, *slot_of_row.t));
+  return wrap(permute_rows_of(x, row_of_slot, slot_of_row));
+}
+
+// unpermute(rows, row_of_slot, slot_of_row, topk_weights, with_grad) -> out
+PyObject* unpermute(PyObject* const* args) {
+  const Arg rows = tensor_arg(args[0], "rows"), row_of_slot = tensor_arg(args[1], "row_of_slot"),
+            slot_of_row = tensor_arg(args[2], "slot_of_row"),
+            weights = tensor_arg(args[3], "topk_weights", true);
+  if (truth(args[4])) {
+    check_inputs({{"row_of_slot", row_of_slot.t}, {"slot_of_row", slot_of_row.t}});
+    check_order(*row_of_slot.t, slot_of_row.t);
+    return wrap(UnpermuteFunction::apply(*rows.t, given(weights), *row_of_slot.t, *slot_of_row.t,
+                                         weights.t && weights.t->requires_grad()));
+  }
+  return wrap(unpermute_of(rows, row_of_slot, weights));
+}
+
+// topk_gating(logits, topk, scoring, renormalize) -> (weights, ids), with the
+// weights' gradient
+PyObject* topk_gating(PyObject* const* args) {
+  const Arg logits = tensor_arg(args[0], "gating_output");
+  const variable_list r =
+      TopkFunction::apply(*logits.t, whole(args[1]), whole(args[2]), truth(args[3]));
+  return wrap_all<2>({r[0], r[1]});
+}
+
+// linear(x, weight, counts, bias, act, gated, residual, with_grad, flags) -> out
+PyObject* linear(PyObject* const* args) {
+  const Arg x = tensor_arg(args[0], "x"), w = tensor_arg(args[1], "weight"),
+            counts = tensor_arg(args[2], "counts", true), bias = tensor_arg(args[3], "bias", true),
+            residual = tensor_arg(args[6], "residual", true);
+  const LinearHow how{static_cast<int32_t>(whole(args[4])), truth(args[5]),
+                      static_cast<int32_t>(whole(args[8]))};
+  if (!truth(args[7])) return wrap(linear_of(x, w, counts, bias, residual, how, false)[0]);
+  // what the activation is taken of is kept where a gradient goes through it
+  bool through = false;
+  for (const Arg* a : {&x, &w, &bias}) through = through || (a->t && a->t->requires_grad());
+  const bool with_z = through && (how.act != FGS_ACT_NONE || how.gated);
+  return wrap(LinearFunction::apply(*x.t, *w.t, given(bias), given(residual), given(counts),
+                                    static_cast<int64_t>(how.act), how.gated,
+                                    static_cast<int64_t>(how.flags), with_z));
+}
+
+// linear_grad(dout, x, weight, counts, z, act, gated, with_dx, with_dweight,
+// with_dbias, flags) -> (dx, dweight, dbias)
+PyObject* linear_grad(PyObject* const* args) {
+  const Arg dout = tensor_arg(args[0], "dout"), x = tensor_arg(args[1], "x"),
+            w = tensor_arg(args[2], "weight"), counts = tensor_arg(args[3], "counts", true),
+            z = tensor_arg(args[4], "z", true);
+  const LinearHow how{static_cast<int32_t>(whole(args[5])), truth(args[6]),
+                      static_cast<int32_t>(whole(args[10]))};
+  return wrap_all<3>(linear_grad_of(dout, x, w, counts, z, how, truth(args[7]), truth(args[8]),
+                                    truth(args[9])));
 }
 
 // foreign_leaf(tensor) -> whether autograd holds the tensor's gradient node for
@@ -365,12 +603,13 @@ PyObject* bind_steps(PyObject* const* args) {
   set(2, g_steps.permute_rows);
   set(3, g_steps.unpermute);
   set(4, g_steps.unpermute_grad);
-  set(5, g_steps.topk_gating_grad);
-  set(6, g_steps.linear);
-  set(7, g_steps.linear_act_grad);
-  set(8, g_steps.linear_input_grad);
-  set(9, g_steps.linear_weight_grad);
-  set(10, g_steps.linear_bias_grad_workspace_bytes);
-  set(11, g_steps.linear_bias_grad);
+  set(5, g_steps.topk_gating);
+  set(6, g_steps.topk_gating_grad);
+  set(7, g_steps.linear);
+  set(8, g_steps.linear_act_grad);
+  set(9, g_steps.linear_input_grad);
+  set(10, g_steps.linear_weight_grad);
+  set(11, g_steps.linear_bias_grad_workspace_bytes);
+  set(12, g_steps.linear_bias_grad);
   Py_RETURN_NONE;
 }

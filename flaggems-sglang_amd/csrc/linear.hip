@@ -10,6 +10,7 @@
 // (ds_read_b64_tr_b16): no transposed copy is ever made.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <string>
 
 #include "linear_common.h"
@@ -479,32 +480,14 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 // ---------------------------------------------------------------- schedule ---
 namespace {
 
-template <class... P, class... A>
-int launch_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told, int64_t wgs,
-               int threads, int lds, hipStream_t stream, A... args) {
-  if (wgs * threads > 0xffffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  int gpu = 0;
-  hipError_t e = hipGetDevice(&gpu);
-  const uint64_t bit = uint64_t{1} << (gpu & 63);
-  if (e == hipSuccess && (gpu > 63 || !(told.load(std::memory_order_relaxed) & bit))) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e == hipSuccess && gpu <= 63) told.fetch_or(bit, std::memory_order_relaxed);
-  }
-  if (e != hipSuccess) return fail(FGS_ELAUNCH, std::string(name) + ": " + hipGetErrorString(e));
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), lds, stream, args...);
-  return check_launch(name);
-}
-
 template <int TY, int MODE, int ACT, int T>
 int launch_tile(const LinearParams& p, hipStream_t stream) {
   typedef LinearTile<T, T == 256 && (MODE == kLinearDgrad || MODE == kLinearWgrad) ? 32 : 64> C;
   static std::atomic<uint64_t> told{0};
   const int64_t tn = MODE == kLinearGated ? T / 2 : T;
   const int64_t nc = (p.n + tn - 1) / tn;
-  const int64_t nr = MODE == kLinearWgrad
-                         ? static_cast<int64_t>(p.groups) * ((p.m + T - 1) / T)
-                         : (static_cast<int64_t>(p.rows) + T - 1) / T + (p.counts ? p.groups : 0);
+  const int64_t nr = MODE == kLinearWgrad ? static_cast<int64_t>(p.groups) * ((p.m + T - 1) / T)
+                                          : linear_row_tiles(p, T);
   if (nr * nc > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
   const int64_t wgs = (nr * nc + 7) / 8 * 8;
   return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told, wgs, 256, C::LDS,
@@ -512,7 +495,7 @@ int launch_tile(const LinearParams& p, hipStream_t stream) {
 }
 template <int TY, int MODE, int ACT>
 int launch_form(const LinearParams& p, int form, hipStream_t stream) {
-  if (form == 0) return launch_tile<TY, MODE, ACT, 128>(p, stream);
+  if (form == kLinearSmallForms) return launch_tile<TY, MODE, ACT, 128>(p, stream);
   return launch_tile<TY, MODE, ACT, 256>(p, stream);
 }
 template <int TY>
@@ -528,23 +511,78 @@ int launch_type(const LinearParams& p, int mode, int form, hipStream_t stream) {
 
 }  // namespace
 
-bool linear_flags_ok(int32_t flags) { return flags >= 0 && flags <= 2; }
+// The forms (FGS_LINEAR_FORM(i)): tile in rows x weight rows; blocks of 64 sums that an
+// iteration takes (the streaming forms' waves take one each); workgroups that run at
+// once; microseconds of an iteration, of one with half of them or fewer, beside the
+// iterations of a round, and the TB/s at which the weights come: fitted to 590 products
+// of 84 sizes, weights not in a cache (dense: 1 to 2048 rows, n 512 to 14336, k 512 to
+// 7168; 8, 64 and 128 groups, 8 to 16384 rows). The choice takes 1.2 % more than the best
+// form of each, 16 % at most.
+// Measured at n and k 4096 (rows: us): 1: 8.1 (form 0; 36.6 in 128 x 128 tiles), 64: 12.6
+// (2; 37.5), 128: 15.8 (3; 39.9), 256: 19.6 (4; 39.1), 512: 34.7 (4; 38.7), 1024: 41.2 (5; 79
+// in 256 x 256), 2048: 67 (5; 85), 4096: 109 (6; 127).
+struct LinearForm {
+  int bm, bn, step, at_once;
+  double iter, half, round, tbs;
+  const char* name;
+};
+constexpr LinearForm kForms[] = {
+    {16, 16, 8, 512, 0.93, 0.49, 0.74, 5.6, "stream 16x16"},
+    {16, 32, 8, 256, 0.76, 0.73, 0.94, 5.4, "stream 16x32"},
+    {32, 32, 8, 256, 1.14, 0.88, 0.87, 5.8, "stream 32x32"},
+    {64, 32, 4, 256, 0.81, 0.66, 1.06, 8.0, "stream 64x32"},
+    {64, 64, 4, 256, 1.10, 0.99, 1.66, 6.2, "stream 64x64"},
+    {128, 128, 1, 512, 1.01, 0.57, 1.45, 5.6, "tiled 128x128"},
+    {256, 256, 1, 256, 1.38, 1.08, 7.49, 8.0, "tiled 256x256"},
+};
+constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
+static_assert(kNumForms == kLinearSmallForms + 2, "forms");
 
-// 0: 128 x 128 tiles, 1: 256 x 256.
+bool linear_flags_ok(int32_t flags) { return flags >= 0 && flags <= kNumForms; }
+
+// The form with the shortest estimate. Forward: any; the gradients: the tiled ones,
+// which alone read an operand across its rows. (Gated, form 0 is form 1.)
 int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
                 int32_t flags) {
-  if (flags) return flags - 1;
-  const int64_t wide = n * (mode == kLinearGated ? 2 : 1);
-  const int64_t tall = mode == kLinearWgrad ? m * groups : rows;
-  return tall * wide >= int64_t{256} * 256 * 256 && (mode == kLinearWgrad || rows / groups >= 256)
-             ? 1 : 0;
+  const bool forward = mode == kLinearForward || mode == kLinearGated;
+  if (flags) return forward ? flags - 1 : std::max(flags - 1, kLinearSmallForms);
+  const double g = static_cast<double>(groups), r = static_cast<double>(rows);
+  // groups with rows, if rows fall on them evenly; for the weights' gradient all have
+  // an output
+  const double used = groups > 1 ? g * -std::expm1(-r / g) : 1;
+  const double wide = static_cast<double>(n) * (mode == kLinearGated ? 2 : 1);
+  const double sums = mode == kLinearWgrad ? r / g : static_cast<double>(red);
+  const double mb = mode == kLinearWgrad ? g * static_cast<double>(m) * wide * 2e-6
+                                         : used * wide * sums * 2e-6;
+  int best = kNumForms - 1;
+  double best_us = 0;
+  for (int f = kNumForms - 1; f >= (forward ? mode == kLinearGated : kLinearSmallForms); --f) {
+    const LinearForm& q = kForms[f];
+    const double tall = mode == kLinearWgrad ? g * std::ceil(static_cast<double>(m) / q.bm)
+                        : groups > 1         ? std::max(used, r / q.bm + used / 2)
+                                             : std::ceil(r / q.bm);
+    const double wgs = tall * std::ceil(wide / q.bn);
+    const double iters = std::ceil(std::ceil(sums / 64) / q.step);
+    const double iter = wgs <= q.at_once / 2 ? q.half : q.iter;
+    const double look = groups > 1 ? 0.66 * std::ceil(g / 64) : 0;  // for a tile's group
+    const double c = std::ceil(wgs / q.at_once) * (iters * iter + q.round + look);
+    const double w = mb / q.tbs;
+    const double us = c * c * c * c + w * w * w * w;  // (of the two, the longer one counts)
+    if (f == kNumForms - 1 || us < best_us) {
+      best = f;
+      best_us = us;
+    }
+  }
+  return best;
 }
 
 std::string linear_form_name(int mode, int form) {
-  return form == 0 ? "tiled 128x128" : "tiled 256x256";
+  return kForms[mode == kLinearGated && form == 0 ? 1 : form].name;
 }
 
 int launch_linear(const LinearParams& p, int mode, int dtype, int form, hipStream_t stream) {
+  if (form < kLinearSmallForms)
+    return launch_linear_small(p, mode == kLinearGated, dtype, form, stream);
   return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, mode, form, stream)
                                  : launch_type<FGS_DTYPE_FP16>(p, mode, form, stream);
 }

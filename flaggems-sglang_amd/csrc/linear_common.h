@@ -2,6 +2,10 @@
 // element types, the groups of rows, activations.
 #pragma once
 
+#include <algorithm>
+#include <atomic>
+#include <string>
+
 #include "dense_common.h"
 #include "gemm_tiled_common.h"
 
@@ -218,6 +222,37 @@ __device__ __forceinline__ void static_for(F&& f) {
     f(std::integral_constant<int, I>{});
     static_for<N, I + 1>(f);
   }
+}
+
+// ---------------------------------------------------------------- launches ---
+constexpr int kLinearSmallForms = 5;
+int launch_linear_small(const LinearParams& p, bool gated, int dtype, int form,
+                        hipStream_t stream);
+
+// Tiles of bm rows for any division of the rows into the groups and what lies behind
+// them, each of which may end in a tile of its own.
+inline int64_t linear_row_tiles(const LinearParams& p, int bm) {
+  const int64_t rows = p.rows, whole = (rows + bm - 1) / bm;
+  return p.counts ? std::min(rows, whole + p.groups) : whole;
+}
+
+// Launches `kernel` with more than 64 KiB of LDS, which each GPU has to be told
+// of once (`told`: a bit a GPU).
+template <class... P, class... A>
+inline int launch_lds(const char* name, void (*kernel)(P...), std::atomic<uint64_t>& told, int64_t wgs,
+               int threads, int lds, hipStream_t stream, A... args) {
+  if (wgs * threads > 0xffffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  int gpu = 0;
+  hipError_t e = hipGetDevice(&gpu);
+  const uint64_t bit = uint64_t{1} << (gpu & 63);
+  if (e == hipSuccess && (gpu > 63 || !(told.load(std::memory_order_relaxed) & bit))) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess && gpu <= 63) told.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (e != hipSuccess) return fail(FGS_ELAUNCH, std::string(name) + ": " + hipGetErrorString(e));
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(threads), lds, stream, args...);
+  return check_launch(name);
 }
 
 }  // namespace fgs

@@ -53,7 +53,7 @@ def flag_tile(cfg: int) -> int:
     return ((cfg + 1) & 0x7) << 12
 
 
-LINEAR_FORMS = 2  # FGS_LINEAR_FORM(0 ..): 128 x 128 tiles, 256 x 256
+LINEAR_FORMS = 7  # FGS_LINEAR_FORM(0 ..): five streaming ones, 128 x 128 tiles, 256 x 256
 
 LIB_NAME = "libfgs_moe.so"
 
@@ -256,7 +256,7 @@ def load() -> ctypes.CDLL:
 
 # the entries that the steps' host side calls, in the order of its bind_steps
 _STEPS = ("permute_workspace_bytes", "permute", "permute_rows", "unpermute", "unpermute_grad",
-          "topk_gating_grad", "linear", "linear_act_grad", "linear_input_grad",
+          "topk_gating", "topk_gating_grad", "linear", "linear_act_grad", "linear_input_grad",
           "linear_weight_grad", "linear_bias_grad_workspace_bytes", "linear_bias_grad")
 
 _host = None

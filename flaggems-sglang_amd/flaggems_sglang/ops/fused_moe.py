@@ -22,7 +22,6 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flaggems_sglang import _capi
 from flaggems_sglang.ops._autograd import needs_gradient
@@ -279,11 +278,7 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     if logits.dtype not in (torch.float32, torch.bfloat16):
         logits = logits.float()
     if needs_gradient("fused_topk", logits):
-        return _FusedTopk.apply(logits, topk, bool(renormalize), scoring)
-    return _topk_gating(logits, topk, renormalize, scoring)
-
-
-def _topk_gating(logits, topk, renormalize, scoring):
+        return _capi.host().topk_gating(logits, topk, scoring, renormalize)
     logits = logits.contiguous()
     M, E = logits.shape
     w = torch.empty((M, topk), dtype=torch.float32, device=logits.device)
@@ -296,25 +291,6 @@ def _topk_gating(logits, topk, renormalize, scoring):
         "fused_topk",
     )
     return w, ids
-
-
-class _FusedTopk(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, topk, renormalize, scoring):
-        w, ids = _topk_gating(logits, topk, renormalize, scoring)
-        ctx.mark_non_differentiable(ids)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, w, ids)
-        ctx.how = scoring, renormalize
-        return w, ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dw, _):
-        if dw is None:
-            return None, None, None, None
-        logits, w, ids = ctx.saved_tensors
-        return _capi.host().topk_gating_grad(logits, w, ids, dw, *ctx.how), None, None, None
 
 
 # ------------------------------------------------------------ small ops ---

@@ -16,7 +16,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flaggems_sglang import _capi
 from flaggems_sglang.ops._autograd import needs_gradient
@@ -25,37 +24,12 @@ _ACTIVATIONS = {None: _capi.ACT_NONE, "relu": _capi.ACT_RELU, "silu": _capi.ACT_
                 "gelu": _capi.ACT_GELU}
 
 
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, counts, act, gated, flags):
-        # what the activation was taken of is kept, in x's type, where a gradient
-        # goes through it
-        with_z = (act != _capi.ACT_NONE or gated) and any(ctx.needs_input_grad[:3])
-        out, z = _capi.host().linear(x, weight, counts, bias, act, gated, residual, with_z, flags)
-        ctx.save_for_backward(x, weight, counts, z)
-        ctx.how = act, gated, flags
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        x, weight, counts, z = ctx.saved_tensors
-        act, gated, flags = ctx.how
-        needs = ctx.needs_input_grad
-        grads = None, None, None
-        if any(needs[:3]):
-            grads = _capi.host().linear_grad(dout, x, weight, counts, z, act, gated, *needs[:3],
-                                             flags)
-        return (*grads, dout if needs[3] else None, None, None, None, None)
-
-
 def _linear(what, x, weight, counts, bias, activation, gated, residual, flags):
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"Unsupported activation: {activation}")
-    if needs_gradient(what, x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, residual, counts, act, gated, flags)
-    return _capi.host().linear(x, weight, counts, bias, act, gated, residual, False, flags)[0]
+    return _capi.host().linear(x, weight, counts, bias, act, gated, residual,
+                               needs_gradient(what, x, weight, bias, residual), flags)
 
 
 def fused_linear(

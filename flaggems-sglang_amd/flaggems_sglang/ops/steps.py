@@ -23,7 +23,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from flaggems_sglang import _capi
 from flaggems_sglang.ops._autograd import needs_gradient
@@ -38,27 +37,6 @@ class ExpertOrder(NamedTuple):
     counts: torch.Tensor  #: int32 ``[num_experts]``: rows of each expert
     row_of_slot: torch.Tensor  #: int32 ``[tokens, topk]``: -1 for slots without an expert
     slot_of_row: torch.Tensor  #: int32 ``[tokens * topk]``: -1 for the rows behind
-
-
-class _Permute(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, topk_ids, num_experts, order):
-        host = _capi.host()
-        ctx.set_materialize_grads(False)
-        if order is not None:
-            ctx.save_for_backward(order.row_of_slot)
-            return host.permute_rows(x, order.row_of_slot, order.slot_of_row)
-        rows, *made = host.permute(x, topk_ids, num_experts)
-        ctx.mark_non_differentiable(*made)
-        ctx.save_for_backward(made[1])
-        return (rows, *made)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, drows, *_):
-        row_of_slot, = ctx.saved_tensors
-        dx = None if drows is None else _capi.host().unpermute(drows, row_of_slot, None)
-        return dx, None, None, None
 
 
 def moe_permute(
@@ -90,32 +68,13 @@ def moe_permute(
         raise ValueError("moe_permute: needs topk_ids and num_experts, or an order")
     elif topk_ids.dtype == torch.int64:  # (ids past 32 bits stay outside)
         topk_ids = topk_ids.clamp(-1, num_experts).to(torch.int32)
-    if needs_gradient("moe_permute", x):
+    with_grad = needs_gradient("moe_permute", x)
+    if with_grad:
         assert x.dtype in _FLOATS, "x with a gradient must be bfloat16, float16 or float32"
-        made = _Permute.apply(x, topk_ids, num_experts, order)
-    elif order is None:
-        made = _capi.host().permute(x, topk_ids, num_experts)
-    else:
-        made = _capi.host().permute_rows(x, order.row_of_slot, order.slot_of_row)
     if order is not None:
-        return made, order
-    return made[0], tuple.__new__(ExpertOrder, made[1:])
-
-
-class _Unpermute(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, weights, row_of_slot, slot_of_row):
-        with_dweights = weights is not None and ctx.needs_input_grad[1]
-        ctx.save_for_backward(rows if with_dweights else None, weights, row_of_slot, slot_of_row)
-        return _capi.host().unpermute(rows, row_of_slot, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        rows, weights, row_of_slot, slot_of_row = ctx.saved_tensors
-        drows, dweights = _capi.host().unpermute_grad(dout, rows, row_of_slot, slot_of_row, weights,
-                                                      *ctx.needs_input_grad[:2])
-        return drows, dweights, None, None
+        return _capi.host().permute_rows(x, order.row_of_slot, order.slot_of_row, with_grad), order
+    rows, *made = _capi.host().permute(x, topk_ids, num_experts, with_grad)
+    return rows, tuple.__new__(ExpertOrder, made)
 
 
 def moe_unpermute(
@@ -138,9 +97,8 @@ def moe_unpermute(
     assert rows.shape[0] == order.slot_of_row.shape[0], "the order is one of other rows"
     if topk_weights is not None and topk_weights.dtype != torch.float32:
         topk_weights = topk_weights.float()
-    if needs_gradient("moe_unpermute", rows, topk_weights):
-        return _Unpermute.apply(rows, topk_weights, order.row_of_slot, order.slot_of_row)
-    return _capi.host().unpermute(rows, order.row_of_slot, topk_weights)
+    return _capi.host().unpermute(rows, order.row_of_slot, order.slot_of_row, topk_weights,
+                                  needs_gradient("moe_unpermute", rows, topk_weights))
 
 
 __all__ = [
