@@ -15,14 +15,46 @@
 namespace fgs {
 
 // ---------------------------------------------------------------- vectors ---
-// Sixteen bytes (or one value, for rows shorter than that) at any address.
+// Memory words at any address. Rows that are written leave with non-temporal stores:
+// they are not read again before the caches have turned over (8192 tokens of 4 KB to
+// eight rows each 49 us, 52 without).
+typedef uint32_t Unaligned128 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t Unaligned32 __attribute__((aligned(1)));
+template <int W>
+struct WordOf;
+template <>
+struct WordOf<16> {
+  typedef Unaligned128 type;
+};
+template <>
+struct WordOf<4> {
+  typedef Unaligned32 type;
+};
+template <>
+struct WordOf<2> {
+  typedef uint16_t type;
+};
+template <>
+struct WordOf<1> {
+  typedef uint8_t type;
+};
+
+// Sixteen bytes (or one value, for rows shorter than that).
 template <int TY, bool WHOLE>
 struct RowVec {
   typedef typename Elem<TY>::raw raw;
   static constexpr int N = WHOLE ? 16 / sizeof(raw) : 1;
+  typedef typename WordOf<WHOLE ? 16 : sizeof(raw)>::type Word;
   raw v[N];
-  __device__ __forceinline__ void load(const void* p) { __builtin_memcpy(v, p, sizeof(v)); }
-  __device__ __forceinline__ void store(void* p) const { __builtin_memcpy(p, v, sizeof(v)); }
+  __device__ __forceinline__ void load(const void* p) {
+    const Word w = *static_cast<const Word*>(p);
+    __builtin_memcpy(v, &w, sizeof(v));
+  }
+  __device__ __forceinline__ void store(void* p) const {
+    Word w;
+    __builtin_memcpy(&w, v, sizeof(v));
+    __builtin_nontemporal_store(w, static_cast<Word*>(p));
+  }
   __device__ __forceinline__ float operator[](int j) const { return Elem<TY>::to_f32(v[j]); }
   __device__ __forceinline__ void set(int j, float f) { v[j] = Elem<TY>::from_f32(f); }
 };
@@ -35,6 +67,12 @@ __device__ __forceinline__ int64_t vector_at(int64_t i, int64_t n, int N) {
   return i * N + N <= n ? i * N : n - N;
 }
 
+// A value that is the same in all lanes, as a scalar.
+template <bool SAME>
+__device__ __forceinline__ int uniform(int v) {
+  return SAME ? __builtin_amdgcn_readfirstlane(v) : v;
+}
+
 // Threads a token takes: a power of two, at most a workgroup.
 static int token_lanes_log2(int64_t vectors) {
   int l = 0;
@@ -42,37 +80,40 @@ static int token_lanes_log2(int64_t vectors) {
   return l;
 }
 
-constexpr int kAtOnce = 8;  // slots whose rows a thread has in flight
+constexpr int kAtOnce = 8;    // slots whose rows a thread has in flight
+constexpr int kTailRows = 4;  // rows a wave looks at for those without a slot
 
 // ---------------------------------------------------------- tokens -> rows ---
 // rows[row of (t, k)] = x[t] (as bytes). With the ids, the row of a slot that no
 // expert here has is one behind all experts' and gets zeros, and the order's final
 // form is written; without, such a slot has no row (-1), and the workgroups behind
 // the tokens' clear the rows that have no slot.
-template <int W>
+template <int W, bool WAVES>
 __global__ __launch_bounds__(256) void permute_kernel(const PermuteParams p, int lanes_log2,
                                                       int token_wgs) {
-  struct Word {
-    uint8_t b[W];
-  };
+  typedef typename WordOf<W>::type Word;
   const int lanes = 1 << lanes_log2;
+  auto put = [](uint8_t* to, Word v) {
+    __builtin_nontemporal_store(v, reinterpret_cast<Word*>(to));
+  };
   if (static_cast<int>(blockIdx.x) >= token_wgs) {
-    const int64_t row = (blockIdx.x - token_wgs) * int64_t{256 >> lanes_log2} +
-                        (threadIdx.x >> lanes_log2);
-    if (row >= p.m * p.topk || p.slot_of_row[row] >= 0) return;
-    const int64_t i = (threadIdx.x & (lanes - 1)) + blockIdx.y * int64_t{lanes};
-    if (i >= row_vectors(p.bytes, W)) return;
-    const Word zero{};
-    __builtin_memcpy(p.rows + row * p.bytes + vector_at(i, p.bytes, W), &zero, W);
+    const int64_t r0 = ((blockIdx.x - token_wgs) * int64_t{4} + uniform<true>(threadIdx.x >> 6)) *
+                       kTailRows;
+    for (int64_t r = r0; r < min(r0 + kTailRows, p.m * p.topk); ++r) {
+      if (p.slot_of_row[r] >= 0) continue;
+      for (int64_t i = (threadIdx.x & 63) + blockIdx.y * int64_t{64}; i < row_vectors(p.bytes, W);
+           i += gridDim.y * int64_t{64})
+        put(p.rows + r * p.bytes + vector_at(i, p.bytes, W), Word{});
+    }
     return;
   }
-  const int64_t t = blockIdx.x * int64_t{256 >> lanes_log2} + (threadIdx.x >> lanes_log2);
+  const int64_t t = blockIdx.x * int64_t{256 >> lanes_log2} +
+                    uniform<WAVES>(threadIdx.x >> lanes_log2);
   if (t >= p.m) return;
   const int64_t i = (threadIdx.x & (lanes - 1)) + blockIdx.y * int64_t{lanes};
   if (i >= row_vectors(p.bytes, W)) return;
   const int64_t at = vector_at(i, p.bytes, W);
-  Word v;
-  __builtin_memcpy(&v, p.x + t * p.x_stride + at, W);
+  const Word v = *reinterpret_cast<const Word*>(p.x + t * p.x_stride + at);
   for (int k0 = 0; k0 < p.topk; k0 += kAtOnce) {
     int row[kAtOnce], id[kAtOnce];
 #pragma unroll
@@ -92,9 +133,7 @@ __global__ __launch_bounds__(256) void permute_kernel(const PermuteParams p, int
         p.slot_of_row[row[j]] = kept ? static_cast<int32_t>(s) : -1;
       }
       if (!kept && !p.ids) continue;
-      Word o = v;
-      if (!kept) o = Word{};
-      __builtin_memcpy(p.rows + row[j] * p.bytes + at, &o, W);
+      put(p.rows + row[j] * p.bytes + at, kept ? v : Word{});
     }
   }
 }
@@ -105,11 +144,12 @@ static int permute_width(const PermuteParams& p, hipStream_t stream) {
   const int l = token_lanes_log2(vecs);
   const int64_t per = 256 >> l;
   const int64_t tokens = (p.m + per - 1) / per;
-  const int64_t tail = p.ids ? 0 : (p.m * p.topk + per - 1) / per;
+  const int64_t tail = p.ids ? 0 : (p.m * p.topk + 4 * kTailRows - 1) / (4 * kTailRows);
   const int64_t chunks = (vecs + (int64_t{1} << l) - 1) >> l;
   if (tokens + tail > 0xffffffll || chunks > 0xffff)
     return fail(FGS_EUNSUPPORTED, "too many rows or columns for a grid");
-  hipLaunchKernelGGL(permute_kernel<W>,
+  auto kernel = l >= 6 ? permute_kernel<W, true> : permute_kernel<W, false>;
+  hipLaunchKernelGGL(kernel,
                      dim3(static_cast<unsigned>(tokens + tail), static_cast<unsigned>(chunks)),
                      dim3(256), 0, stream, p, l, static_cast<int>(tokens));
   return check_launch("permute_kernel");
@@ -123,12 +163,14 @@ int launch_permute(const PermuteParams& p, hipStream_t stream) {
 // ---------------------------------------------------------- rows -> tokens ---
 // out[t] = sum_k w[t, k] rows[row of (t, k)], in fp32 from k = 0 on; a slot
 // without a row (outside [0, n_rows)) adds nothing, whatever its weight is.
-template <int TY, bool WHOLE, bool WEIGHTS>
+// WAVES: a token has whole waves, so its slots' rows and weights are scalars.
+template <int TY, bool WHOLE, bool WEIGHTS, bool WAVES>
 __global__ __launch_bounds__(256) void unpermute_kernel(const UnpermuteParams p, int lanes_log2) {
   typedef RowVec<TY, WHOLE> V;
   typedef typename V::raw raw;
   const int lanes = 1 << lanes_log2;
-  const int64_t t = blockIdx.x * int64_t{256 >> lanes_log2} + (threadIdx.x >> lanes_log2);
+  const int64_t t = blockIdx.x * int64_t{256 >> lanes_log2} +
+                    uniform<WAVES>(threadIdx.x >> lanes_log2);
   if (t >= p.m) return;
   const int64_t i = (threadIdx.x & (lanes - 1)) + blockIdx.y * int64_t{lanes};
   if (i >= row_vectors(p.cols, V::N)) return;
@@ -171,19 +213,17 @@ __global__ __launch_bounds__(256) void unpermute_grad_kernel(const UnpermutePara
   typedef RowVec<TY, WHOLE> V;
   typedef typename V::raw raw;
   __shared__ float part[4][kAtOnce];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform<true>(threadIdx.x >> 6);
   raw* drows = static_cast<raw*>(p.drows);
   const int64_t vecs = row_vectors(p.cols, V::N);
   if (static_cast<int>(blockIdx.x) >= token_wgs) {
-    // 64 rows a wave: those that have no slot
-    const int64_t r0 = ((blockIdx.x - token_wgs) * int64_t{4} + wave) * 64;
-    uint64_t todo = __ballot(r0 + lane < p.n_rows && p.slot_of_row[r0 + lane] < 0);
+    // kTailRows rows a wave: those that have no slot
+    const int64_t r0 = ((blockIdx.x - token_wgs) * int64_t{4} + wave) * kTailRows;
     V zero;
 #pragma unroll
     for (int c = 0; c < V::N; ++c) zero.set(c, 0.f);
-    while (todo) {
-      const int64_t r = r0 + __ffsll(static_cast<long long>(todo)) - 1;
-      todo &= todo - 1;
+    for (int64_t r = r0; r < min(r0 + kTailRows, p.n_rows); ++r) {
+      if (p.slot_of_row[r] >= 0) continue;
       for (int64_t i = lane; i < vecs; i += 64)
         zero.store(drows + r * p.cols + vector_at(i, p.cols, V::N));
     }
@@ -252,10 +292,10 @@ static int unpermute_width(const UnpermuteParams& p, hipStream_t stream) {
   constexpr int N = RowVec<TY, WHOLE>::N;
   const int64_t vecs = row_vectors(p.cols, N);
   if (!p.out) {
-    // a wave a token, or all four for rows of more than 256 vectors
-    const int waves = vecs > 256 ? 4 : 1;
+    // a vector a lane, with up to four waves a token
+    const int waves = vecs > 128 ? 4 : vecs > 64 ? 2 : 1;
     const int64_t tokens = (p.m * waves + 3) / 4;
-    const int64_t tail = p.drows ? (p.n_rows + 255) / 256 : 0;
+    const int64_t tail = p.drows ? (p.n_rows + 4 * kTailRows - 1) / (4 * kTailRows) : 0;
     if (tokens + tail > 0xffffffll) return fail(FGS_EUNSUPPORTED, "too many rows for a grid");
     if (tokens + tail == 0) return FGS_OK;
     hipLaunchKernelGGL((unpermute_grad_kernel<TY, WHOLE>),
@@ -269,7 +309,10 @@ static int unpermute_width(const UnpermuteParams& p, hipStream_t stream) {
   const int64_t chunks = (vecs + (int64_t{1} << l) - 1) >> l;
   if (tokens > 0xffffffll || chunks > 0xffff)
     return fail(FGS_EUNSUPPORTED, "too many rows or columns for a grid");
-  auto kernel = p.weights ? unpermute_kernel<TY, WHOLE, true> : unpermute_kernel<TY, WHOLE, false>;
+  auto kernel = l >= 6 ? (p.weights ? unpermute_kernel<TY, WHOLE, true, true>
+                                    : unpermute_kernel<TY, WHOLE, false, true>)
+                       : (p.weights ? unpermute_kernel<TY, WHOLE, true, false>
+                                    : unpermute_kernel<TY, WHOLE, false, false>);
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tokens), static_cast<unsigned>(chunks)),
                      dim3(256), 0, stream, p, l);
   return check_launch("unpermute_kernel");
