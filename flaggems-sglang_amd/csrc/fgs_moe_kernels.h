@@ -289,7 +289,7 @@ struct LinearParams {
 };
 enum { kLinearForward = 0, kLinearGated = 1, kLinearDgrad = 2, kLinearWgrad = 3 };
 constexpr int64_t kLinearMaxRows = 1 << 30, kLinearMaxCols = 1 << 20, kLinearMaxStride = 1 << 21;
-bool linear_flags_ok(int32_t flags);
+bool linear_flags_ok(int mode, int32_t flags);
 int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
                 int32_t flags);
 std::string linear_form_name(int mode, int form);

@@ -256,7 +256,8 @@ at::Tensor flat(const at::Tensor& x, int64_t rows, int64_t cols) {
 struct LinearHow {
   int32_t act;
   bool gated;
-  int32_t flags;
+  int32_t flags;  // a byte each of the forward product, the input's gradient, the weights'
+  int32_t of(int pass) const { return (flags >> (8 * pass)) & 0xff; }
 };
 
 // (out, z)
@@ -291,7 +292,7 @@ std::array<at::Tensor, 2> linear_of(const Arg& xa, const Arg& wa, const Arg& ca,
   call(index, ca.t ? "grouped_linear" : "fused_linear", g_steps.linear, ptr(xm.t), xm.row,
        ptr(wm.t), wm.row, wm.group, ptr(bias), ptr(res.t), res.row, ints(counts),
        static_cast<int32_t>(s.groups), s.rows, n, s.k, static_cast<int32_t>(type_code(x)),
-       how.act, static_cast<int32_t>(how.gated), how.flags, ptr(z), ptr(out), stream);
+       how.act, static_cast<int32_t>(how.gated), how.of(0), ptr(z), ptr(out), stream);
   return {out, z};
 }
 
@@ -328,13 +329,13 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
     const Matrix wm = matrix(w, s.wide, s.k);
     dx = make(x.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_input_grad, ptr(dz.t), dz.row, ptr(wm.t), wm.row, wm.group,
-         ints(counts), groups, s.rows, s.wide, s.k, type, how.flags, ptr(dx), stream);
+         ints(counts), groups, s.rows, s.wide, s.k, type, how.of(1), ptr(dx), stream);
   }
   if (with_dw) {
     const Matrix xm = matrix(flat(x, s.rows, s.k), s.rows, s.k);
     dw = make(w.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_weight_grad, ptr(dz.t), dz.row, ptr(xm.t), xm.row,
-         ints(counts), groups, s.rows, s.wide, s.k, type, how.flags, ptr(dw), stream);
+         ints(counts), groups, s.rows, s.wide, s.k, type, how.of(2), ptr(dw), stream);
   }
   if (with_db) {
     const int64_t need = g_steps.linear_bias_grad_workspace_bytes(groups, s.rows, s.wide);

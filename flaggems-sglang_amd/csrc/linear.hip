@@ -53,17 +53,6 @@ struct LinearTile {
   }
 };
 
-// Four rows of 16 values in LDS, a row to 16 lanes, column by column: lane i of 16
-// gives the address of four values of row i / 4, from column 4 (i % 4) on, and has
-// the four of column i. (__restrict__: with no scope of its own the compiler takes
-// the read for one of the bytes that the loads in flight will write, and waits for
-// all of those first.)
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4* LdsWords;
-__device__ __forceinline__ s16x4 read_transposed(LdsWords __restrict__ at) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
-}
-
 // Offset that no buffer resource here reaches.
 constexpr uint32_t kOutside = 0x80000000u;
 
@@ -494,18 +483,17 @@ int launch_tile(const LinearParams& p, hipStream_t stream) {
                     stream, p);
 }
 template <int TY, int MODE, int ACT>
-int launch_form(const LinearParams& p, int form, hipStream_t stream) {
-  if (form == kLinearSmallForms) return launch_tile<TY, MODE, ACT, 128>(p, stream);
-  return launch_tile<TY, MODE, ACT, 256>(p, stream);
+int launch_form(const LinearParams& p, bool large, hipStream_t stream) {
+  return large ? launch_tile<TY, MODE, ACT, 256>(p, stream) : launch_tile<TY, MODE, ACT, 128>(p, stream);
 }
 template <int TY>
-int launch_type(const LinearParams& p, int mode, int form, hipStream_t stream) {
-  if (mode == kLinearDgrad) return launch_form<TY, kLinearDgrad, FGS_ACT_NONE>(p, form, stream);
-  if (mode == kLinearWgrad) return launch_form<TY, kLinearWgrad, FGS_ACT_NONE>(p, form, stream);
+int launch_type(const LinearParams& p, int mode, bool large, hipStream_t stream) {
+  if (mode == kLinearDgrad) return launch_form<TY, kLinearDgrad, FGS_ACT_NONE>(p, large, stream);
+  if (mode == kLinearWgrad) return launch_form<TY, kLinearWgrad, FGS_ACT_NONE>(p, large, stream);
   return with_act(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    return mode == kLinearGated ? launch_form<TY, kLinearGated, ACT>(p, form, stream)
-                                : launch_form<TY, kLinearForward, ACT>(p, form, stream);
+    return mode == kLinearGated ? launch_form<TY, kLinearGated, ACT>(p, large, stream)
+                                : launch_form<TY, kLinearForward, ACT>(p, large, stream);
   });
 }
 
@@ -535,17 +523,37 @@ constexpr LinearForm kForms[] = {
     {128, 128, 1, 512, 1.01, 0.57, 1.45, 5.6, "tiled 128x128"},
     {256, 256, 1, 256, 1.38, 1.08, 7.49, 8.0, "tiled 256x256"},
 };
-constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
-static_assert(kNumForms == kLinearSmallForms + 2, "forms");
+// The gradients', fitted in the same way: of the input, by the weights' columns (1 row at
+// n and k 4096 18.7 us, 34.9 in 128 x 128 tiles; 128: 20.3 and 39.4; 512: 38.0 and 38.7;
+// 68 sizes, 0.4 % more than the best on average), and of the weights (32 sizes).
+constexpr LinearForm kInputForms[] = {
+    {16, 64, 8, 256, 1.36, 1.78, 0.60, 5.2, "stream 16x64"},
+    {32, 64, 4, 256, 0.87, 0.98, 0.88, 5.2, "stream 32x64"},
+    {64, 64, 4, 256, 1.19, 1.17, 1.04, 5.6, "stream 64x64"},
+    {128, 128, 1, 512, 1.07, 0.54, 0.67, 5.8, "tiled 128x128"},
+    {256, 256, 1, 256, 1.35, 1.09, 4.65, 8.0, "tiled 256x256"},
+};
+constexpr LinearForm kWeightForms[] = {
+    {128, 128, 1, 512, 0.98, 0.45, 2.39, 3.8, "tiled 128x128"},
+    {256, 256, 1, 256, 1.50, 1.04, 6.48, 5.1, "tiled 256x256"},
+};
+struct LinearForms {
+  const LinearForm* list;
+  int count;  // the last two: tiles
+};
+LinearForms forms_of(int mode) {
+  if (mode == kLinearDgrad) return {kInputForms, 5};
+  if (mode == kLinearWgrad) return {kWeightForms, 2};
+  return {kForms, 7};
+}
 
-bool linear_flags_ok(int32_t flags) { return flags >= 0 && flags <= kNumForms; }
+bool linear_flags_ok(int mode, int32_t flags) { return flags >= 0 && flags <= forms_of(mode).count; }
 
-// The form with the shortest estimate. Forward: any; the gradients: the tiled ones,
-// which alone read an operand across its rows. (Gated, form 0 is form 1.)
+// The form with the shortest estimate. (Gated, the forward form 0 is form 1.)
 int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
                 int32_t flags) {
-  const bool forward = mode == kLinearForward || mode == kLinearGated;
-  if (flags) return forward ? flags - 1 : std::max(flags - 1, kLinearSmallForms);
+  if (flags) return flags - 1;
+  const LinearForms forms = forms_of(mode);
   const double g = static_cast<double>(groups), r = static_cast<double>(rows);
   // groups with rows, if rows fall on them evenly; for the weights' gradient all have
   // an output
@@ -554,21 +562,21 @@ int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, in
   const double sums = mode == kLinearWgrad ? r / g : static_cast<double>(red);
   const double mb = mode == kLinearWgrad ? g * static_cast<double>(m) * wide * 2e-6
                                          : used * wide * sums * 2e-6;
-  int best = kNumForms - 1;
+  int best = forms.count - 1;
   double best_us = 0;
-  for (int f = kNumForms - 1; f >= (forward ? mode == kLinearGated : kLinearSmallForms); --f) {
-    const LinearForm& q = kForms[f];
+  for (int f = forms.count - 1; f >= (mode == kLinearGated ? 1 : 0); --f) {
+    const LinearForm& q = forms.list[f];
     const double tall = mode == kLinearWgrad ? g * std::ceil(static_cast<double>(m) / q.bm)
                         : groups > 1         ? std::max(used, r / q.bm + used / 2)
                                              : std::ceil(r / q.bm);
     const double wgs = tall * std::ceil(wide / q.bn);
     const double iters = std::ceil(std::ceil(sums / 64) / q.step);
     const double iter = wgs <= q.at_once / 2 ? q.half : q.iter;
-    const double look = groups > 1 ? 0.66 * std::ceil(g / 64) : 0;  // for a tile's group
+    const double look = groups > 1 ? 0.7 * std::ceil(g / 64) : 0;  // for a tile's group
     const double c = std::ceil(wgs / q.at_once) * (iters * iter + q.round + look);
     const double w = mb / q.tbs;
     const double us = c * c * c * c + w * w * w * w;  // (of the two, the longer one counts)
-    if (f == kNumForms - 1 || us < best_us) {
+    if (f == forms.count - 1 || us < best_us) {
       best = f;
       best_us = us;
     }
@@ -577,14 +585,15 @@ int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, in
 }
 
 std::string linear_form_name(int mode, int form) {
-  return kForms[mode == kLinearGated && form == 0 ? 1 : form].name;
+  return forms_of(mode).list[mode == kLinearGated && form == 0 ? 1 : form].name;
 }
 
 int launch_linear(const LinearParams& p, int mode, int dtype, int form, hipStream_t stream) {
-  if (form < kLinearSmallForms)
-    return launch_linear_small(p, mode == kLinearGated, dtype, form, stream);
-  return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, mode, form, stream)
-                                 : launch_type<FGS_DTYPE_FP16>(p, mode, form, stream);
+  const int tiles = forms_of(mode).count - 2;
+  if (form < tiles) return launch_linear_small(p, mode, dtype, form, stream);
+  const bool large = form > tiles;
+  return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, mode, large, stream)
+                                 : launch_type<FGS_DTYPE_FP16>(p, mode, large, stream);
 }
 
 }  // namespace fgs

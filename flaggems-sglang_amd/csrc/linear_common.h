@@ -36,6 +36,17 @@ struct Mma16<FGS_DTYPE_FP16> {
   }
 };
 
+// Four rows of 16 values in LDS, a row to 16 lanes, column by column: lane i of 16
+// gives the address of four values of row i / 4, from column 4 (i % 4) on, and has
+// the four of column i. (__restrict__: with no scope of its own the compiler takes
+// the read for one of the bytes that the loads in flight will write, and waits for
+// all of those first.)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* LdsWords;
+__device__ __forceinline__ s16x4 read_transposed(LdsWords __restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+}
+
 // ---------------------------------------------------------- groups of rows ---
 // Rows come sorted by group: group e has counts[e] of them, from row 0 on.
 // Counts are the device's: a negative one counts as 0, and those that pass the
@@ -225,9 +236,7 @@ __device__ __forceinline__ void static_for(F&& f) {
 }
 
 // ---------------------------------------------------------------- launches ---
-constexpr int kLinearSmallForms = 5;
-int launch_linear_small(const LinearParams& p, bool gated, int dtype, int form,
-                        hipStream_t stream);
+int launch_linear_small(const LinearParams& p, int mode, int dtype, int form, hipStream_t stream);
 
 // Tiles of bm rows for any division of the rows into the groups and what lies behind
 // them, each of which may end in a tile of its own.

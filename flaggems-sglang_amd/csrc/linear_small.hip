@@ -25,7 +25,10 @@ struct LinearSmall {
   static_assert(KW * MT * NT * 1024 <= LDS, "partial sums");
 };
 
-template <int TY, int ACT, bool GATED, class C>
+// INPUT_GRAD: out = x w by w's columns -- a block is 64 of its rows, 128 bytes of each,
+// which the LDS reads transpose on the way to the registers.
+enum { kSmallForward, kSmallGated, kSmallInputGrad };
+template <int TY, int MODE, int ACT, class C>
 __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const LinearParams p, int nm,
                                                                      int total) {
   typedef Mma16<TY> M;
@@ -33,7 +36,9 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
   typedef typename Elem<TY>::raw raw;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   constexpr int MT = C::MT, NT = C::NT, SLOTS = C::SLOTS;
+  constexpr bool GATED = MODE == kSmallGated, ACROSS = MODE == kSmallInputGrad;
   static_assert(!GATED || NT % 2 == 0, "gate and up rows");
+  static_assert(!ACROSS || NT == 4, "128 bytes of a row");
   constexpr int TN = GATED ? 8 * NT : 16 * NT;  // output columns
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -61,7 +66,7 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
   const int ldx = static_cast<int>(p.ldq * 2), ldw = static_cast<int>(p.ldp * 2);
   const uint8_t* x0 = static_cast<const uint8_t*>(p.q) + first * p.ldq * 2;
   const uint8_t* w0 = static_cast<const uint8_t*>(p.p) +
-                      (none ? 0 : (e * p.p_group + n0 * p.ldp) * 2);
+                      (none ? 0 : (e * p.p_group + (ACROSS ? n0 : n0 * p.ldp)) * 2);
 
   // Lane l of a load: row l / 8 of its eight, 16-byte chunk l % 8 at its swizzled
   // place. A resource ends with the last row's last sum; the chunks past the sums' end
@@ -69,6 +74,9 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
   uint8_t* ring = lds + wave * SLOTS * C::SLOT;
   const int lrow = lane >> 3;
   const int c0 = ((lane & 7) ^ (lrow >> 1)) * 16;  // rows 0-7 of 16; 8-15: chunk ^ 4
+  // (across: 32-byte granule g of row r at place g ^ (bit 1 of r, bit 3): a transposing
+  // read takes a granule of four consecutive rows, two of them rows 8 apart at a time)
+  const int wc = ((((lane & 7) >> 1) ^ ((lane >> 4) & 1)) * 32) + (lane & 1) * 16;
   auto issue = [&](int i) {
     uint8_t* slot = ring + (i % SLOTS) * C::SLOT;
     const int kb = kb0 + i;
@@ -78,16 +86,26 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
                                                (r - 1) * ld + left, kBufWord3);
     };
     const __amdgpu_buffer_rsrc_t rx = resource(x0, rows, ldx);
-    const __amdgpu_buffer_rsrc_t rw = resource(w0, cols, ldw);
-    const __amdgpu_buffer_rsrc_t ru = resource(GATED ? w0 + p.n * p.ldp * 2 : w0, cols, ldw);
+    if constexpr (ACROSS) {
+      const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(w0) + kb * int64_t{64} * ldw, 0,
+          (min(64, p.red - kb * 64) - 1) * ldw + (p.n - n0) * 2, kBufWord3);
 #pragma unroll
-    for (int j = 0; j < 2 * NT; ++j) {
-      const int c = c0 ^ (64 * (j & 1));
-      // (gated: 16 gate rows, the 16 up rows of the same columns, ...)
-      const int r = (GATED ? (j >> 2) * 16 + (j & 1) * 8 : j * 8) + lrow;
-      const uint32_t o = c < left ? static_cast<uint32_t>(r * ldw + c) : 0x80000000u;
-      if (GATED && (j & 2)) lds_dma16_buf(ru, o, 0, slot + C::W_AT + j * 1024);
-      else lds_dma16_buf(rw, o, 0, slot + C::W_AT + j * 1024);
+      for (int j = 0; j < 8; ++j)
+        lds_dma16_buf(rw, (j * 8 + lrow) * ldw + (wc ^ (64 * (j & 1))), 0,
+                      slot + C::W_AT + j * 1024);
+    } else {
+      const __amdgpu_buffer_rsrc_t rw = resource(w0, cols, ldw);
+      const __amdgpu_buffer_rsrc_t ru = resource(GATED ? w0 + p.n * p.ldp * 2 : w0, cols, ldw);
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j) {
+        const int c = c0 ^ (64 * (j & 1));
+        // (gated: 16 gate rows, the 16 up rows of the same columns, ...)
+        const int r = (GATED ? (j >> 2) * 16 + (j & 1) * 8 : j * 8) + lrow;
+        const uint32_t o = c < left ? static_cast<uint32_t>(r * ldw + c) : 0x80000000u;
+        if (GATED && (j & 2)) lds_dma16_buf(ru, o, 0, slot + C::W_AT + j * 1024);
+        else lds_dma16_buf(rw, o, 0, slot + C::W_AT + j * 1024);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 2 * MT; ++j) {
@@ -106,6 +124,22 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
   int off[2];
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) off[kk] = r * 128 + (((g + 4 * kk) ^ ((r >> 1) & 7)) * 16);
+
+  int across[ACROSS ? NT : 1];
+  if constexpr (ACROSS)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      across[j] = (8 * g + (r >> 2)) * 128 + (j ^ ((r >> 3) | (g & 1) << 1)) * 32 + (r & 3) * 8;
+  auto weights = [&](const uint8_t* w_slot, int j, int kk) -> Frag {
+    if constexpr (ACROSS) {
+      const uint8_t* a = w_slot + across[j] + kk * 32 * 128;
+      const s16x4 lo = read_transposed((LdsWords)(a));
+      const s16x4 hi = read_transposed((LdsWords)(a + 4 * 128));
+      return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      return *reinterpret_cast<const Frag*>(w_slot + j * 2048 + off[kk]);
+    }
+  };
 
   f32x4 acc[NT][MT];
 #pragma unroll
@@ -126,7 +160,7 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
         x[kk][t] = *reinterpret_cast<const Frag*>(slot + t * 2048 + off[kk]);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        w[kk][j] = *reinterpret_cast<const Frag*>(slot + C::W_AT + j * 2048 + off[kk]);
+        w[kk][j] = weights(slot + C::W_AT, j, kk);
     }
     wait_lgkm0();  // the slot is read: refill it
     if (i + SLOTS < count) issue(i + SLOTS);
@@ -173,12 +207,16 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
     f32x4 v = sum(GATED ? 2 * j * MT + t : tile), u{0.f, 0.f, 0.f, 0.f};
     if constexpr (GATED) u = sum((2 * j + 1) * MT + t);
     if (m >= rows || n >= p.n) continue;
-    if (p.bias && !none) {
+    if (!ACROSS && p.bias && !none) {
       const raw* b = static_cast<const raw*>(p.bias) + static_cast<int64_t>(e) * wide + n;
       four(b, v);
       if constexpr (GATED) four(b + p.n, u);
     }
     const int64_t row = first + m;
+    if constexpr (ACROSS) {
+      put(p.out, row * p.n + n, v);
+      continue;
+    }
     if (p.z) {
       put(p.z, row * wide + n, v);
       if constexpr (GATED) put(p.z, row * wide + p.n + n, u);
@@ -195,49 +233,50 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
 
 namespace {
 
-template <int F>
-struct SmallCfg;
-template <> struct SmallCfg<0> { typedef LinearSmall<1, 1, 8, 2> type; typedef LinearSmall<1, 2, 8, 2> gated; };
-template <> struct SmallCfg<1> { typedef LinearSmall<1, 2, 8, 2> type; typedef LinearSmall<1, 2, 8, 2> gated; };
-template <> struct SmallCfg<2> { typedef LinearSmall<2, 2, 8, 2> type; typedef LinearSmall<2, 2, 8, 2> gated; };
-template <> struct SmallCfg<3> { typedef LinearSmall<4, 2, 4, 3> type; typedef LinearSmall<4, 2, 4, 3> gated; };
-template <> struct SmallCfg<4> { typedef LinearSmall<4, 4, 4, 2> type; typedef LinearSmall<4, 4, 4, 2> gated; };
-
-template <int TY, int ACT, bool GATED, class C>
+template <int TY, int MODE, int ACT, class C>
 int launch_cfg(const LinearParams& p, hipStream_t stream) {
   static std::atomic<uint64_t> told{0};
-  constexpr int BM = 16 * C::MT, TN = (GATED ? 8 : 16) * C::NT;
+  constexpr int BM = 16 * C::MT, TN = (MODE == kSmallGated ? 8 : 16) * C::NT;
   const int64_t nm = linear_row_tiles(p, BM), nn = (p.n + TN - 1) / TN;
   if (nm * nn > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  return launch_lds("linear_small_kernel", linear_small_kernel<TY, ACT, GATED, C>, told, nm * nn,
+  return launch_lds("linear_small_kernel", linear_small_kernel<TY, MODE, ACT, C>, told, nm * nn,
                     C::KW * 64, C::LDS, stream, p, static_cast<int>(nm),
                     static_cast<int>(nm * nn));
 }
-template <int TY, int F>
-int launch_form(const LinearParams& p, bool gated, hipStream_t stream) {
+// CG: the configuration of the gated product
+template <int TY, class C, class CG = C>
+int launch_forward(const LinearParams& p, bool gated, hipStream_t stream) {
   return with_act(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    return gated ? launch_cfg<TY, ACT, true, typename SmallCfg<F>::gated>(p, stream)
-                 : launch_cfg<TY, ACT, false, typename SmallCfg<F>::type>(p, stream);
+    return gated ? launch_cfg<TY, kSmallGated, ACT, CG>(p, stream)
+                 : launch_cfg<TY, kSmallForward, ACT, C>(p, stream);
   });
 }
 template <int TY>
-int launch_type(const LinearParams& p, bool gated, int form, hipStream_t stream) {
+int launch_type(const LinearParams& p, int mode, int form, hipStream_t stream) {
+  if (mode == kLinearDgrad) {
+    switch (form) {
+      case 0: return launch_cfg<TY, kSmallInputGrad, 0, LinearSmall<1, 4, 8, 2>>(p, stream);
+      case 1: return launch_cfg<TY, kSmallInputGrad, 0, LinearSmall<2, 4, 4, 3>>(p, stream);
+      default: return launch_cfg<TY, kSmallInputGrad, 0, LinearSmall<4, 4, 4, 2>>(p, stream);
+    }
+  }
+  const bool gated = mode == kLinearGated;
   switch (form) {
-    case 0: return launch_form<TY, 0>(p, gated, stream);
-    case 1: return launch_form<TY, 1>(p, gated, stream);
-    case 2: return launch_form<TY, 2>(p, gated, stream);
-    case 3: return launch_form<TY, 3>(p, gated, stream);
-    default: return launch_form<TY, 4>(p, gated, stream);
+    case 0: return launch_forward<TY, LinearSmall<1, 1, 8, 2>, LinearSmall<1, 2, 8, 2>>(p, gated, stream);
+    case 1: return launch_forward<TY, LinearSmall<1, 2, 8, 2>>(p, gated, stream);
+    case 2: return launch_forward<TY, LinearSmall<2, 2, 8, 2>>(p, gated, stream);
+    case 3: return launch_forward<TY, LinearSmall<4, 2, 4, 3>>(p, gated, stream);
+    default: return launch_forward<TY, LinearSmall<4, 4, 4, 2>>(p, gated, stream);
   }
 }
 
 }  // namespace
 
-int launch_linear_small(const LinearParams& p, bool gated, int dtype, int form,
+int launch_linear_small(const LinearParams& p, int mode, int dtype, int form,
                         hipStream_t stream) {
-  return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, gated, form, stream)
-                                 : launch_type<FGS_DTYPE_FP16>(p, gated, form, stream);
+  return dtype == FGS_DTYPE_BF16 ? launch_type<FGS_DTYPE_BF16>(p, mode, form, stream)
+                                 : launch_type<FGS_DTYPE_FP16>(p, mode, form, stream);
 }
 
 }  // namespace fgs

@@ -239,7 +239,7 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
   int rc = check_linear(groups, rows, n, k, dtype);
   if (rc) return rc;
   if ((rc = check_act(act))) return rc;
-  if (!linear_flags_ok(flags)) return fail(FGS_EINVAL, "unknown flags");
+  if (!linear_flags_ok(gated ? kLinearGated : kLinearForward, flags)) return fail(FGS_EINVAL, "unknown flags");
   if (!counts && groups != 1) return fail(FGS_EINVAL, "counts are needed for several groups");
   if (rows == 0) return FGS_OK;
   if (!x || !w || !out) return fail(FGS_EINVAL, "null pointer argument");
@@ -302,7 +302,7 @@ int32_t fgs_moe_linear_input_grad(const void* dz, int64_t ldz, const void* w, in
                                   int32_t flags, void* dx, void* stream) {
   int rc = check_linear(groups, rows, wide, k, dtype);
   if (rc) return rc;
-  if (!linear_flags_ok(flags)) return fail(FGS_EINVAL, "unknown flags");
+  if (!linear_flags_ok(kLinearDgrad, flags)) return fail(FGS_EINVAL, "unknown flags");
   if (!counts && groups != 1) return fail(FGS_EINVAL, "counts are needed for several groups");
   if (rows == 0) return FGS_OK;
   if (!dz || !w || !dx) return fail(FGS_EINVAL, "null pointer argument");
@@ -335,7 +335,7 @@ int32_t fgs_moe_linear_weight_grad(const void* dz, int64_t ldz, const void* x, i
                                    void* dw, void* stream) {
   int rc = check_linear(groups, rows, wide, k, dtype);
   if (rc) return rc;
-  if (!linear_flags_ok(flags)) return fail(FGS_EINVAL, "unknown flags");
+  if (!linear_flags_ok(kLinearWgrad, flags)) return fail(FGS_EINVAL, "unknown flags");
   if (!counts && groups != 1) return fail(FGS_EINVAL, "counts are needed for several groups");
   if (!dw || (rows > 0 && (!dz || !x))) return fail(FGS_EINVAL, "null pointer argument");
   if ((rc = check_rows("dz", dz, rows, ldz)) || (rc = check_rows("x", x, rows, ldx)) ||
@@ -397,10 +397,10 @@ int32_t fgs_moe_linear_schedule(int32_t pass, int32_t groups, int64_t rows, int6
   const int64_t wide = gated ? 2 * n : n;
   int rc = check_linear(groups, rows, pass ? wide : n, k, FGS_DTYPE_BF16);
   if (rc) return rc;
-  if (!linear_flags_ok(flags)) return fail(FGS_EINVAL, "unknown flags");
   if (!buf || len < 1) return fail(FGS_EINVAL, "buf must hold at least one byte");
   const int mode = pass == 1 ? kLinearDgrad : pass == 2 ? kLinearWgrad
                                                         : gated ? kLinearGated : kLinearForward;
+  if (!linear_flags_ok(mode, flags)) return fail(FGS_EINVAL, "unknown flags");
   const int form = pass == 1   ? linear_form(mode, groups, rows, 0, k, wide, flags)
                    : pass == 2 ? linear_form(mode, groups, rows, wide, k, rows, flags)
                                : linear_form(mode, groups, rows, 0, n, k, flags);

@@ -53,7 +53,8 @@ def flag_tile(cfg: int) -> int:
     return ((cfg + 1) & 0x7) << 12
 
 
-LINEAR_FORMS = 7  # FGS_LINEAR_FORM(0 ..): five streaming ones, 128 x 128 tiles, 256 x 256
+# FGS_LINEAR_FORM(0 ..) of the forward product, the input's gradient, the weights'
+LINEAR_FORMS = {"forward": 7, "input": 5, "weight": 2}
 
 LIB_NAME = "libfgs_moe.so"
 

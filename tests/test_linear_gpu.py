@@ -10,7 +10,13 @@ from flaggems_sglang import _capi
 
 pytestmark = pytest.mark.gpu
 
-FORMS = range(_capi.LINEAR_FORMS + 1)  # 0: the call's own choice, f + 1: form f
+def flags(form):
+    """Form ``form`` - 1 of each pass, or its last one; 0: the call's own choice."""
+    return sum(min(form, _capi.LINEAR_FORMS[p]) << (8 * i)
+               for i, p in enumerate(("forward", "input", "weight")))
+
+
+FORMS = [flags(f) for f in range(max(_capi.LINEAR_FORMS.values()) + 1)]
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
 
@@ -134,15 +140,14 @@ def test_strides_and_shapes(gpu, form):
     gen = generator(3)
     wide = rand(gen, 90, 200)
     w_wide = rand(gen, 100, 136, scale=0.1)
-    flags = form
     for x, w in [(wide[:, 8:80], w_wide[:72, 64:]), (wide[:, 3:75], w_wide[1:97:2, 5:77]),
                  (wide[:72].t()[8:], w_wide[:72, :72].t()), (wide[:1, :72].expand(40, 72), w_wide[:96, :72])]:
-        a, b = fgs.fused_linear(x, w, _flags=flags), fgs.fused_linear(x.contiguous(), w.contiguous(),
-                                                                    _flags=flags)
+        a, b = fgs.fused_linear(x, w, _flags=form), fgs.fused_linear(x.contiguous(), w.contiguous(),
+                                                                    _flags=form)
         assert torch.equal(a, b)
     x = rand(gen, 2, 3, 5, 64)
     w = rand(gen, 40, 64)
-    out = fgs.fused_linear(x, w, residual=rand(gen, 2, 3, 5, 40), _flags=flags)
+    out = fgs.fused_linear(x, w, residual=rand(gen, 2, 3, 5, 40), _flags=form)
     assert out.shape == (2, 3, 5, 40)
     assert fgs.fused_linear(x[:0], w).shape == (0, 3, 5, 40)
     # stepped groups, and a gradient whose rows all lie at one address
