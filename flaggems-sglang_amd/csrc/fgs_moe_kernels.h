@@ -279,7 +279,7 @@ struct LinearParams {
   const void* bias;        // [groups, wide] or null
   const void* residual;    // or null
   int64_t ldr;
-  void* z;                 // what the activation is taken of, [rows, wide], or null
+  float* z;                // what the activation is taken of, [rows, wide], or null
   const int32_t* counts;   // rows of each group, or null: one of all rows
   int32_t groups, rows;    // rows: of all tokens
   int32_t red;             // length of the sums (weights' gradient: counts')
@@ -299,7 +299,7 @@ int launch_linear(const LinearParams& p, int mode, int dtype, int form, hipStrea
 struct LinearActGradParams {
   const void* dout;
   int64_t ldd;
-  const void* z;
+  const float* z;
   void* dz;
   int64_t rows, n;
   int32_t act, gated;

@@ -287,12 +287,12 @@ std::array<at::Tensor, 2> linear_of(const Arg& xa, const Arg& wa, const Arg& ca,
   const at::Tensor counts = ca.t ? contiguous(*ca.t) : at::Tensor();
   const at::Tensor out = make(shape, x.scalar_type(), x);
   at::Tensor z;
-  if (with_z) z = make({s.rows, s.wide}, x.scalar_type(), x);
+  if (with_z) z = make({s.rows, s.wide}, at::kFloat, x);
   void* stream = stream_of(index);
   call(index, ca.t ? "grouped_linear" : "fused_linear", g_steps.linear, ptr(xm.t), xm.row,
        ptr(wm.t), wm.row, wm.group, ptr(bias), ptr(res.t), res.row, ints(counts),
        static_cast<int32_t>(s.groups), s.rows, n, s.k, static_cast<int32_t>(type_code(x)),
-       how.act, static_cast<int32_t>(how.gated), how.of(0), ptr(z), ptr(out), stream);
+       how.act, static_cast<int32_t>(how.gated), how.of(0), floats(z), ptr(out), stream);
   return {out, z};
 }
 
@@ -312,15 +312,15 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
           "dout must be of the output's shape and type");
   require(za.t || (how.act == FGS_ACT_NONE && !how.gated), "an activation's gradient needs z");
   require(!za.t || (za.t->dim() == 2 && za.t->size(0) == s.rows && za.t->size(1) == s.wide &&
-                    za.t->scalar_type() == x.scalar_type() && za.t->is_contiguous()),
-          "z must be [rows, n] of x's type, contiguous");
+                    za.t->scalar_type() == at::kFloat && za.t->is_contiguous()),
+          "z must be float32 [rows, n], contiguous");
   const int32_t type = static_cast<int32_t>(type_code(x)), groups = static_cast<int32_t>(s.groups);
   const at::Tensor counts = ca.t ? contiguous(*ca.t) : at::Tensor();
   void* stream = stream_of(index);
   Matrix dz = matrix(flat(*da.t, s.rows, n), s.rows, n);
   if (za.t) {
     const at::Tensor t = make({s.rows, s.wide}, x.scalar_type(), x);
-    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, ptr(*za.t), s.rows, n, type,
+    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, floats(*za.t), s.rows, n, type,
          how.act, static_cast<int32_t>(how.gated), ptr(t), stream);
     dz = {t, s.wide, 0};
   }

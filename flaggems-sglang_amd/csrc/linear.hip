@@ -349,19 +349,17 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // ---- epilogue. Activation and residual are taken in fp32 in the accumulators'
   // layout (a gate and its up value are two registers of a lane), then
   // rounded; the wave's whole part goes through LDS in 16 bits so that it leaves as
-  // runs of a row, 16 bytes a lane. The residual comes in the same way first. (In
-  // fp32, 32 rows at a time, with the arithmetic on the way out: a tile took 6 us
-  // more.)
+  // runs of a row, 16 bytes a lane. The residual comes in the same way first; z, which
+  // a gradient is taken at, leaves in fp32 (in 16 bits, its rounding was as large a
+  // part of the gradients' error as their own).
   uint8_t* stg = lds + wave * C::STAGING;
   // (the weights' gradient: rows of the group's matrix)
   const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
   const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
-  // Eight bytes s of staged row r of COLS columns: the XOR spreads a column of
-  // 32 rows over all banks. Sixteen bytes are two of them, swapped in some rows.
-  auto place = [](auto cols_c, int r, int s) {
-    constexpr int W8 = decltype(cols_c)::value / 4, RPL = 32 / W8;
-    return r * W8 * 8 + (s ^ ((r / RPL) & (W8 - 1))) * 8;
-  };
+  // Eight bytes s of staged row r: the XOR spreads a column of 32 rows over all banks.
+  // Sixteen bytes are two of them, swapped in some rows.
+  constexpr int W8 = OC / 4, RPL = 32 / W8;
+  auto place = [](int r, int s) { return r * W8 * 8 + (s ^ ((r / RPL) & (W8 - 1))) * 8; };
   auto sync = [] {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -369,25 +367,14 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   };
   // f(staged row, output row in the tile, 16-byte chunk) for the wave's part, a
   // chunk a lane; the tile's rows 64 i + 32 wm + r are the staged rows 32 i + r.
-  auto runs = [&](auto cols_c, auto&& f) {
-    constexpr int LPR = decltype(cols_c)::value / 8, RPP = 64 / LPR;
+  auto runs = [&](auto&& f) {
+    constexpr int LPR = OC / 8, RPP = 64 / LPR;
     const int lr = lane / LPR, lc = lane % LPR;
 #pragma unroll 8
     for (int k = 0; k < WN / RPP; ++k) {
       const int sr = k * RPP + lr;
       f(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc);
     }
-  };
-  auto store = [&](auto cols_c, void* to, int64_t ld, int64_t at0) {
-    constexpr int COLS = decltype(cols_c)::value, RPL = 128 / COLS;
-    sync();
-    runs(cols_c, [&](int sr, int r, int c) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(stg + (place(cols_c, sr, 2 * c) & ~15));
-      if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
-      if (r < rows_in && col0 + c * 8 < p.n)
-        *reinterpret_cast<u32x4*>(static_cast<raw*>(to) + at0 + (row0 + r) * ld + col0 + c * 8) = v;
-    });
-    sync();
   };
   auto pack4 = [](const float (&v)[4]) {
     return uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
@@ -396,35 +383,44 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // reads all of them into VGPRs ahead, more than there are.)
   auto keep = [](f32x16& a) { asm volatile("" : "+a"(a)); };
   const int r32 = lane & 31;
-  constexpr std::integral_constant<int, OC> out_cols{};
   if (FORWARD && p.z) {
-    // (gated: the gates, then the ups)
-    static_for<GATED ? 2 : 1>([&](auto half_c) {
-      constexpr int HALF = decltype(half_c)::value;
+    // in fp32, 32 rows at a time: chunks of four values, spread over the banks
+    constexpr int CH = WN / 4, RPP = 64 / CH;
+    auto chunk = [&](int r, int c) {
+      return reinterpret_cast<f32x4*>(stg + (r * CH + ((c ^ (r & 15)) & (CH - 1))) * 16);
+    };
+    const int lc = lane % CH;
+    const int zc = col0 + (GATED ? (lc >> 4) * 32 : (lc >> 3) * 32) + (lc & 7) * 4;
+    const int64_t to = zc + (GATED && ((lc >> 3) & 1) ? p.n : 0);
+    static_for<NB>([&](auto i_c) {
+      constexpr int i = decltype(i_c)::value;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int j = 0; j < NB; ++j) {
+        keep(acc[i][j]);
 #pragma unroll
-        for (int j = HALF; j < NB; j += GATED ? 2 : 1) {
-          keep(acc[i][j]);
+        for (int g = 0; g < 4; ++g)
+          *chunk(r32, j * 8 + 2 * g + h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1],
+                                                 acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      }
+      sync();
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
-                                acc[i][j][4 * g + 3]};
-            *reinterpret_cast<uint2*>(
-                stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h)) = pack4(v);
-          }
-        }
-      store(out_cols, p.z, wide, HALF * p.n);
+      for (int k = 0; k < 32 / RPP; ++k) {
+        const int sr = k * RPP + lane / CH, r = i * 64 + wm * 32 + sr;
+        const f32x4 v = *chunk(sr, lc);
+        if (r < rows_in && zc < p.n)
+          *reinterpret_cast<f32x4*>(p.z + (row0 + r) * wide + to) = v;
+      }
+      sync();
     });
   }
   if (FORWARD && p.residual) {
-    runs(out_cols, [&](int sr, int r, int c) {
+    runs([&](int sr, int r, int c) {
       u32x4 v{0, 0, 0, 0};
       if (r < rows_in && col0 + c * 8 < p.n)
         v = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
                                             (row0 + r) * p.ldr + col0 + c * 8);
-      if ((sr / (128 / OC)) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
-      *reinterpret_cast<u32x4*>(stg + (place(out_cols, sr, 2 * c) & ~15)) = v;
+      if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+      *reinterpret_cast<u32x4*>(stg + (place(sr, 2 * c) & ~15)) = v;
     });
     sync();
   }
@@ -436,7 +432,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     for (int j = 0; j < NB; j += GATED ? 2 : 1) {
       auto at = [&](int g) {
         return reinterpret_cast<uint2*>(
-            stg + place(out_cols, i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
+            stg + place(i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
       };
       keep(acc[i][j]);
       if constexpr (GATED) keep(acc[i][j + 1]);
@@ -463,7 +459,13 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
         *at(g) = pack4(v);
       }
     }
-  store(out_cols, p.out, p.n, 0);
+  sync();
+  runs([&](int sr, int r, int c) {
+    u32x4 v = *reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
+    if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+    if (r < rows_in && col0 + c * 8 < p.n)
+      *reinterpret_cast<u32x4*>(static_cast<raw*>(p.out) + (row0 + r) * p.n + col0 + c * 8) = v;
+  });
 }
 
 // ---------------------------------------------------------------- schedule ---

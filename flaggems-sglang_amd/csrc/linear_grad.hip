@@ -15,7 +15,8 @@ __global__ __launch_bounds__(256) void linear_act_grad_kernel(const LinearActGra
   const int64_t r = i / per_row;
   const int64_t c = (i - r * per_row) * 8;
   const int64_t wide = GATED ? 2 * p.n : p.n;
-  Vec8<TY, true> d, g, u;
+  Vec8<TY, true> d;
+  Vec8<FGS_DTYPE_FP32, true> g, u;
   d.load(p.dout, r * p.ldd + c, 8);
   g.load(p.z, r * wide + c, 8);
   if constexpr (GATED) u.load(p.z, r * wide + p.n + c, 8);

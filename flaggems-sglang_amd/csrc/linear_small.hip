@@ -218,8 +218,8 @@ __global__ __launch_bounds__(C::KW * 64, 2) void linear_small_kernel(const Linea
       continue;
     }
     if (p.z) {
-      put(p.z, row * wide + n, v);
-      if constexpr (GATED) put(p.z, row * wide + p.n + n, u);
+      *reinterpret_cast<f32x4*>(p.z + row * wide + n) = v;
+      if constexpr (GATED) *reinterpret_cast<f32x4*>(p.z + row * wide + p.n + n) = u;
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {

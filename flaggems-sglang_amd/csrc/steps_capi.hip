@@ -235,7 +235,7 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
                        int64_t w_group_stride, const void* bias, const void* residual,
                        int64_t ldr, const int32_t* counts, int32_t groups, int64_t rows,
                        int64_t n, int64_t k, int32_t dtype, int32_t act, int32_t gated,
-                       int32_t flags, void* z, void* out, void* stream) {
+                       int32_t flags, float* z, void* out, void* stream) {
   int rc = check_linear(groups, rows, n, k, dtype);
   if (rc) return rc;
   if ((rc = check_act(act))) return rc;
@@ -273,7 +273,7 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
                        as_stream(stream));
 }
 
-int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const void* z, int64_t rows,
+int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, int64_t rows,
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream) {
   int rc = check_linear(1, rows, n, 8, dtype);

@@ -54,10 +54,9 @@ def fused_linear(
     2^20; rows (0 among them) up to 2^30. Operands whose rows are not 16-byte
     aligned, or whose columns are not adjacent, are copied first.
 
-    Gradients go to ``x``, ``weight``, ``bias`` and ``residual``. For them the sums
-    that the activation is taken of are kept in x's type, and so is their gradient:
-    with an activation, x's, weight's and bias's gradients are those of sums rounded
-    so.
+    Gradients go to ``x``, ``weight``, ``bias`` and ``residual``. With an activation,
+    what it is taken of is kept in fp32 for them, and its gradient is rounded to x's
+    type, in which the other gradients' products take it.
     """
     return _linear("fused_linear", x, weight, None, bias, activation, gated, residual, _flags)
 

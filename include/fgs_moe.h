@@ -519,7 +519,7 @@ int32_t fgs_moe_unpermute_grad(const void* dout, int64_t ldd, const void* rows, 
  *   v = x[i] . w[e][j] + bias[e][j]
  *   out[i, j] = act(v_j) + residual[i, j]                      (wide = n)
  *   out[i, j] = act(v_j) * v_{n + j} + residual[i, j]          (gated: wide = 2 n)
- * rounded once to dtype; z (or null) [rows, wide] gets v.
+ * rounded once to dtype; z (or null) f32 [rows, wide] gets v.
  *   x [rows, k] with row stride ldx; w [groups][wide, k] with row stride ldw and
  *   w_group_stride elements between the groups' matrices; bias [groups, wide] or
  *   null; residual [rows, n] with row stride ldr, or null; out [rows, n] contiguous
@@ -536,10 +536,10 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
                        int64_t w_group_stride, const void* bias, const void* residual,
                        int64_t ldr, const int32_t* counts, int32_t groups, int64_t rows,
                        int64_t n, int64_t k, int32_t dtype, int32_t act, int32_t gated,
-                       int32_t flags, void* z, void* out, void* stream);
-/* Its gradients. dz [rows, wide] contiguous, of v (rows behind the last group's: of
+                       int32_t flags, float* z, void* out, void* stream);
+/* Its gradients. dz [rows, wide] contiguous, of v, in dtype (rows behind the last group's: of
  * whatever z holds there; the two entries below leave them out): */
-int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const void* z, int64_t rows,
+int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, int64_t rows,
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream);
 /* dx [rows, k] = dz[i] w[e], contiguous (rows behind the last group's: 0), */

@@ -4,8 +4,8 @@ bounds on how far a kernel may be off that follow from the operators' definition
 * h: half a step of the output's type, once for each rounding;
 * a sum of n products in fp32: each of at most n additions is off by 2^-24 of a
   partial sum, which is at most the sum of the magnitudes;
-* what is kept in 16 bits between the passes (z and dz) is off by h, and that
-  passes on through the derivative of what is taken of it.
+* what is kept between the passes is off by its own rounding (z in fp32, dz by h), and
+  that passes on through the derivative of what is taken of it.
 """
 
 import math
@@ -66,9 +66,9 @@ def product(x, w, bias=None, kind=None, gated=False, residual=None, dout=None):
     if dout is None:
         return out
     d = dout.double()
-    # z is kept rounded: the slope is taken there, off by what |act''| makes of it
+    # z is kept in fp32: the slope is taken there, off by what |act''| makes of it
     if gated:
-        zg, zu = h * z[:, :n].abs() + ez[:, :n], h * u.abs() + ez[:, n:]
+        zg, zu = F32 * z[:, :n].abs() + ez[:, :n], F32 * u.abs() + ez[:, n:]
         dz = torch.cat([d * u * slope, d * a], 1)
         e = torch.cat([d.abs() * (zu * (SLOPE + CURVE[kind] * zg) + u.abs() * CURVE[kind] * zg),
                        d.abs() * SLOPE * zg], 1)
@@ -76,7 +76,7 @@ def product(x, w, bias=None, kind=None, gated=False, residual=None, dout=None):
         e = e + h * (dz.abs() + e)
     elif kind:
         dz = d * slope
-        e = d.abs() * (CURVE[kind] * (h * z.abs() + ez) + fn * SLOPE)
+        e = d.abs() * (CURVE[kind] * (F32 * z.abs() + ez) + fn * SLOPE)
         e = e + h * (dz.abs() + e)
     else:
         dz, e = d, torch.zeros_like(d)
