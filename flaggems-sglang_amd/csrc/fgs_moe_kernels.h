@@ -286,9 +286,12 @@ struct LinearParams {
   int32_t m;               // weights' gradient: rows of its output
   int32_t n;               // columns of the output
   int32_t act;             // FGS_ACT_*
+  int32_t part;            // kLinearWhole ... (linear.hip's)
 };
+enum { kLinearWhole = 0, kLinearCut = 1, kLinearRest = 2 };
 enum { kLinearForward = 0, kLinearGated = 1, kLinearDgrad = 2, kLinearWgrad = 3 };
-constexpr int64_t kLinearMaxRows = 1 << 30, kLinearMaxCols = 1 << 20, kLinearMaxStride = 1 << 21;
+// (two counts of rows add up to less than 2^31)
+constexpr int64_t kLinearMaxRows = (1 << 30) - 1, kLinearMaxCols = 1 << 20, kLinearMaxStride = 1 << 21;
 bool linear_flags_ok(int mode, int32_t flags);
 int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
                 int32_t flags);

@@ -92,6 +92,16 @@ struct Feed {
   }
 };
 
+// Tiles of an XCD, and those of its last round that are cut off: of the 32 CUs at most
+// half have one, and there is a round before it.
+__device__ __host__ __forceinline__ int linear_share(int total, int xcd) {
+  return (total >> 3) + (xcd < (total & 7));
+}
+__device__ __host__ __forceinline__ int linear_rest(int share) {
+  const int rest = share & 31;
+  return share > 32 && rest <= 16 ? rest : 0;
+}
+
 template <int TY, int MODE, int ACT, class C>
 __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams p) {
   typedef Mma16<TY> M;
@@ -113,13 +123,28 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // ---- the tile. Workgroup b runs on XCD b % 8; each XCD takes a contiguous
   // eighth of the tiles, which go in bands of four columns, row by row, so that
   // the tiles an XCD's 32 CUs have at a time share rows and columns in its L2.
-  const int n_ct = (p.n + TN - 1) / TN;
+  // A last round that leaves half of the CUs or more without a tile is cut off
+  // (kLinearCut) and goes to a second launch in quarters, 128 x 128 (kLinearRest): 36
+  // row tiles of 16 columns, 2.25 rounds, k 14336: 975 us in one launch, 932 in two; 4608 x 4096 x 4096
+  // (288 tiles) 215 and 143.
+  const int quarters = T == 128 && p.part == kLinearRest ? 2 : 1;  // a side
+  const int bt = T * quarters, btn = TN * quarters;
+  const int n_ct = (p.n + btn - 1) / btn;
   const GroupScan scan{p.counts, p.groups, p.rows};
-  const int n_rt = QA ? (p.m + T - 1) / T
-                      : p.counts ? scan.tiles(T) : (p.rows + T - 1) / T;
+  const int n_rt = QA ? (p.m + bt - 1) / bt
+                      : p.counts ? scan.tiles(bt) : (p.rows + bt - 1) / bt;
   const int total = (QA ? p.groups : 1) * n_rt * n_ct;
-  const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3;
-  if (pos >= (total >> 3) + (xcd < (total & 7))) return;
+  const int xcd = blockIdx.x & 7;
+  int pos = blockIdx.x >> 3, sub = 0;
+  const int share = linear_share(total, xcd);
+  const int rest = p.part == kLinearWhole ? 0 : linear_rest(share);
+  if (quarters == 2) {
+    sub = pos & 3;
+    pos = share - rest + (pos >> 2);
+    if (pos >= share) return;
+  } else if (pos >= share - rest) {
+    return;
+  }
   int at = xcd * (total >> 3) + min(xcd, total & 7) + pos;
   int e = 0;
   if (QA) {
@@ -130,19 +155,25 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   const int band = at / (n_rt * BAND);
   const int cols = min(BAND, n_ct - band * BAND);
   at -= band * n_rt * BAND;
-  const int rt = __builtin_amdgcn_readfirstlane(at / cols);
-  const int ct = __builtin_amdgcn_readfirstlane(band * BAND + at % cols);
+  int rt = __builtin_amdgcn_readfirstlane(at / cols);
+  const int ct = __builtin_amdgcn_readfirstlane((band * BAND + at % cols) * quarters + (sub & 1));
   e = __builtin_amdgcn_readfirstlane(e);
   // rows of Q: [first, first + nrows) of the tile (across: of the group's sums)
   int first, nrows;
   if (!p.counts) {
-    first = QA ? 0 : rt * T;
-    nrows = QA ? p.rows : min(T, p.rows - first);
+    first = QA ? 0 : rt * bt;
+    nrows = QA ? p.rows : min(bt, p.rows - first);
   } else if (QA) {
     scan.range(e, &first, &nrows);
   } else {
-    scan.tile(rt, T, &e, &first, &nrows);
+    scan.tile(rt, bt, &e, &first, &nrows);
   }
+  rt = rt * quarters + (sub >> 1);
+  if (!QA && quarters == 2) {
+    first += (sub >> 1) * T;
+    nrows = min(T, nrows - (sub >> 1) * T);
+  }
+  if (ct * TN >= p.n || (QA ? rt * T >= p.m : nrows <= 0)) return;  // (quarters may be empty)
   e = __builtin_amdgcn_readfirstlane(e);
   first = __builtin_amdgcn_readfirstlane(first);
   nrows = __builtin_amdgcn_readfirstlane(nrows);
@@ -472,21 +503,33 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 namespace {
 
 template <int TY, int MODE, int ACT, int T>
-int launch_tile(const LinearParams& p, hipStream_t stream) {
+int launch_tile(const LinearParams& p, int64_t wgs, hipStream_t stream) {
   typedef LinearTile<T, T == 256 && (MODE == kLinearDgrad || MODE == kLinearWgrad) ? 32 : 64> C;
   static std::atomic<uint64_t> told{0};
-  const int64_t tn = MODE == kLinearGated ? T / 2 : T;
-  const int64_t nc = (p.n + tn - 1) / tn;
-  const int64_t nr = MODE == kLinearWgrad ? static_cast<int64_t>(p.groups) * ((p.m + T - 1) / T)
-                                          : linear_row_tiles(p, T);
-  if (nr * nc > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
-  const int64_t wgs = (nr * nc + 7) / 8 * 8;
-  return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told, wgs, 256, C::LDS,
-                    stream, p);
+  return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told, wgs, 256,
+                    C::LDS, stream, p);
 }
 template <int TY, int MODE, int ACT>
 int launch_form(const LinearParams& p, bool large, hipStream_t stream) {
-  return large ? launch_tile<TY, MODE, ACT, 256>(p, stream) : launch_tile<TY, MODE, ACT, 128>(p, stream);
+  const int t = large ? 256 : 128, tn = MODE == kLinearGated ? t / 2 : t;
+  const int64_t nc = (p.n + tn - 1) / tn;
+  const int64_t nr = MODE == kLinearWgrad ? static_cast<int64_t>(p.groups) * ((p.m + t - 1) / t)
+                                          : linear_row_tiles(p, t);
+  const int64_t tiles = nr * nc;
+  if (tiles > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  const int64_t wgs = (tiles + 7) / 8 * 8;
+  if (!large) return launch_tile<TY, MODE, ACT, 128>(p, wgs, stream);
+  // how many tiles there are is the device's to know where rows are grouped
+  const bool known = MODE == kLinearWgrad || !p.counts;
+  bool cut = !known && tiles > 256;
+  if (known)
+    for (int xcd = 0; xcd < 8; ++xcd) cut |= linear_rest(linear_share(static_cast<int>(tiles), xcd)) > 0;
+  LinearParams q = p;
+  q.part = cut ? kLinearCut : kLinearWhole;
+  const int rc = launch_tile<TY, MODE, ACT, 256>(q, wgs, stream);
+  if (rc || !cut) return rc;
+  q.part = kLinearRest;
+  return launch_tile<TY, MODE, ACT, 128>(q, 8 * 16 * 4, stream);
 }
 template <int TY>
 int launch_type(const LinearParams& p, int mode, bool large, hipStream_t stream) {
@@ -575,7 +618,13 @@ int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, in
     const double iters = std::ceil(std::ceil(sums / 64) / q.step);
     const double iter = wgs <= q.at_once / 2 ? q.half : q.iter;
     const double look = groups > 1 ? 0.7 * std::ceil(g / 64) : 0;  // for a tile's group
-    const double c = std::ceil(wgs / q.at_once) * (iters * iter + q.round + look);
+    const double round = iters * iter + q.round + look;
+    double rounds = std::ceil(wgs / q.at_once);
+    if (q.bm == 256) {  // (a last round that is cut off: its quarters')
+      const double rest = wgs / q.at_once - std::floor(wgs / q.at_once);
+      if (wgs > q.at_once && rest > 0 && rest <= 0.5) rounds += (rest <= 0.25 ? 0.45 : 0.75) - 1;
+    }
+    const double c = rounds * round;
     const double w = mb / q.tbs;
     const double us = c * c * c * c + w * w * w * w;  // (of the two, the longer one counts)
     if (f == forms.count - 1 || us < best_us) {

@@ -527,7 +527,7 @@ int32_t fgs_moe_unpermute_grad(const void* dout, int64_t ldd, const void* rows, 
  *   other from row 0 on (negative ones count as 0, and what passes the last row is
  *   cut); rows behind the last group's have no product (out = residual, or 0; their
  *   z is not defined). Null: one matrix for all rows.
- * n and k multiples of 8, up to 2^20; up to 2^30 rows and 4096 groups; rows of x, w,
+ * n and k multiples of 8, up to 2^20; fewer than 2^30 rows, up to 4096 groups; rows of x, w,
  * residual 16-byte aligned and at most 2^21 elements apart. No workspace. `flags`:
  * 0, or FGS_LINEAR_FORM(f), the kernel form f whatever the sizes (for measurement
  * and tests). */

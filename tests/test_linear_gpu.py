@@ -274,3 +274,31 @@ def test_other_stream(gpu):
     stream.synchronize()
     for name in want:
         assert torch.equal(got[name], want[name])
+
+
+# (rows, n, k, counts): more than a round of 256 x 256 tiles, the last of which leaves
+# CUs without one: for the forward product and, with n and k swapped, each gradient
+CUT = [(2100, 8200, 72, None), (2304, 8192, 64, None), (2100, 8200, 72, [700, 0, 33, 900, 1, 400]),
+       (2600, 8200, 40, [256] * 9)]
+
+
+@pytest.mark.parametrize("which", ["forward", "gated", "input", "weight"])
+@pytest.mark.parametrize("rows, n, k, counts", CUT)
+def test_last_round_in_quarters(gpu, rows, n, k, counts, which):
+    large = sum(_capi.LINEAR_FORMS[p] << (8 * i) for i, p in enumerate(("forward", "input", "weight")))
+    if which == "input":
+        n, k = k, n
+    if which == "weight":
+        rows, n, k = k, 2104, n
+        counts = None if counts is None else [30, 0, k]  # (cut at the last row)
+    gated = which == "gated"
+    if gated:
+        n = (n // 2 + 7) // 8 * 8
+    groups = None if counts is None else len(counts)
+    t, dout = inputs(rows, n, k, torch.bfloat16, gated, which in ("forward", "gated"), False, groups)
+    on_gpu = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+    options = dict(kind="silu" if gated else None, gated=gated,
+                   dout=dout if which in ("input", "weight") else None)
+    want = ref.product(**t, **options) if counts is None else ref.grouped(**t, counts=counts, **options)
+    got = run(t, on_gpu, options["dout"], activation=options["kind"], gated=gated, _flags=large)
+    compare(got, want)
