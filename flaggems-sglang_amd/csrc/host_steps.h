@@ -378,10 +378,10 @@ variable_list backward_of(const char* what, const variable_list& grads, size_t c
   }
   if (!again) return out;
   const auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string(what) + " has no second derivative", static_cast<int64_t>(count));
-  variable_list defined;
-  for (const at::Tensor& t : out) defined.push_back(t);
-  return (*error)(std::move(defined));
+      std::string(what) + " has no second derivative", 1);
+  for (at::Tensor& t : out)
+    if (t.defined() && !t.is_same(grads[0])) t = (*error)({t.set_requires_grad(true)})[0];
+  return out;
 }
 
 struct PermuteFunction : torch::autograd::Function<PermuteFunction> {

@@ -19,11 +19,11 @@ def needs_gradient(what, *tensors) -> bool:
         return False
     need = False
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if getattr(t, "requires_grad", False):  # (what is no tensor is refused later)
             need = True
     if need and torch.cuda.is_current_stream_capturing():
         for t in tensors:
-            if t is not None and _capi.host().foreign_leaf(t):
+            if isinstance(t, torch.Tensor) and _capi.host().foreign_leaf(t):
                 raise RuntimeError(
                     f"{what}: an earlier graph of this leaf, recorded on another stream, is still "
                     "alive: its backward pass cannot be captured (delete that graph's outputs, or "

@@ -294,3 +294,120 @@ def test_matches_fused_moe(gpu):
     out = fgs.moe_unpermute(fgs.grouped_linear(h, w2, order.counts), order, weights)
     whole = fgs.fused_moe(x, w13, w2, weights, ids)
     assert float((out.double() - whole.double()).norm()) <= 4 * 2.0 ** -8 * float(whole.double().norm())
+
+
+# ---------------------------------------------------------- graphs, streams ---
+def test_graph_of_permute_and_back(gpu):
+    """Captured with dropped slots; every replay of new ids against the eager call."""
+    gen = generator(21)
+    m, topk, experts = 700, 8, 64  # (the alignment's counting kernels, with their scratch)
+    x = torch.randn(m, 72, generator=gen, device="cuda").bfloat16()
+    w = torch.rand(m, topk, generator=gen, device="cuda")
+    ids = make_ids(gen, m, topk, experts, 0.3)
+
+    def step():
+        rows, order = fgs.moe_permute(x, ids, experts)
+        again, _ = fgs.moe_permute(w, order=order)
+        return rows, again, *order, fgs.moe_unpermute(rows, order, w)
+
+    step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        captured = step()
+    for i in range(4):
+        ids.copy_(make_ids(gen, m, topk, experts, 0.25 * i))
+        x.copy_(torch.randn(m, 72, generator=gen, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [c.clone() for c in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
+def test_two_graphs_replay_side_by_side(gpu):
+    """Each capture has its own workspaces."""
+    gen = generator(22)
+    sides = []
+    for seed in (1, 2):
+        x = torch.randn(5000, 64, generator=gen, device="cuda").bfloat16()
+        ids = make_ids(gen, 5000, 2, 16)
+        stream = torch.cuda.Stream()
+        fgs.moe_permute(x, ids, 16)
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            rows, order = fgs.moe_permute(x, ids, 16)
+        sides.append((graph, stream, rows, order, fgs.moe_permute(x, ids, 16), (x, ids)))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream, *_ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, rows, order, (want, want_order), _ in sides:
+            assert torch.equal(rows, want)
+            assert all(torch.equal(a, b) for a, b in zip(order, want_order))
+
+
+def test_capture_beside_an_eager_graph_is_refused(gpu):
+    """A leaf whose eager graph, recorded on another stream, is still alive is refused
+    while a stream is captured; without that graph it is taken."""
+    x = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    w = torch.ones(32, 64, dtype=torch.bfloat16, device="cuda")
+    alive = fgs.fused_linear(x, w)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            with pytest.raises(RuntimeError, match="still alive"):
+                fgs.fused_linear(x, w)
+            out = fgs.fused_linear(x.detach(), w)
+        finally:
+            graph.capture_end()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, alive)
+    del alive
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+        out = fgs.fused_linear(x, w)
+        torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+def test_steps_on_another_stream(gpu):
+    gen = generator(23)
+    x = torch.randn(900, 136, generator=gen, device="cuda").bfloat16()
+    ids = make_ids(gen, 900, 4, 32, 0.2)
+    w = torch.rand(900, 4, generator=gen, device="cuda")
+
+    def step():
+        leaf, lw = x.detach().requires_grad_(), w.detach().requires_grad_()
+        rows, order = fgs.moe_permute(leaf, ids, 32)
+        out = fgs.moe_unpermute(rows, order, lw)
+        return (out.detach(), *torch.autograd.grad(out, (leaf, lw), torch.ones_like(out)))
+
+    want = step()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = step()
+    stream.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_long_rows_and_offsets_past_32_bits(gpu):
+    """More than 2^31 values in rows: 2^17 slots of 2^14 + 8 columns (4.3 GB)."""
+    m, topk, cols = 1 << 14, 8, (1 << 14) + 8
+    x = torch.arange(m, device="cuda", dtype=torch.float32).to(torch.bfloat16)[:, None].expand(m, cols)
+    ids = torch.arange(m * topk, device="cuda", dtype=torch.int32).view(m, topk) % 4
+    rows, order = fgs.moe_permute(x, ids, 4)
+    assert rows.numel() > 1 << 31
+    slots = order.slot_of_row.long()
+    assert torch.equal(rows[:, 0], x[:, 0][slots // topk])
+    assert torch.equal(rows[:, -1], x[:, 0][slots // topk])
+    out = fgs.moe_unpermute(rows, order, torch.full((m, topk), 1 / topk, device="cuda"))
+    assert torch.equal(out[:, 0], x[:, 0]) and torch.equal(out[:, -1], x[:, 0])
