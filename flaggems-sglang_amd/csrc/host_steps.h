@@ -448,17 +448,15 @@ struct TopkFunction : torch::autograd::Function<TopkFunction> {
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({r[1]});
     ctx->save_for_backward({logits, r[0], r[1]});
-    ctx->saved_data["scoring"] = scoring;
-    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["how"] = scoring << 1 | int64_t{renormalize};
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return backward_of("fused_topk", grads, 4, [&](variable_list& out) {
       const variable_list saved = ctx->get_saved_variables();
+      const int64_t how = ctx->saved_data["how"].toInt();
       out[0] = topk_gating_grad_of({"logits", &saved[0]}, {"weights", &saved[1]}, {"ids", &saved[2]},
-                                   {"dweights", &grads[0]},
-                                   static_cast<int32_t>(ctx->saved_data["scoring"].toInt()),
-                                   ctx->saved_data["renormalize"].toBool());
+                                   {"dweights", &grads[0]}, static_cast<int32_t>(how >> 1), how & 1);
     });
   }
 };
@@ -477,29 +475,27 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                              with_z);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, w, counts, r[1]});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["gated"] = gated;
-    ctx->saved_data["flags"] = flags;
-    ctx->saved_data["bias"] = bias.defined();
-    ctx->saved_data["residual"] = residual.defined();
+    // (one entry: each is a look-up by name, 0.4 us)
+    ctx->saved_data["how"] = act | int64_t{gated} << 8 | int64_t{bias.defined()} << 9 |
+                             int64_t{residual.defined()} << 10 | (flags & 0xffffff) << 16;
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return backward_of("this product", grads, 9, [&](variable_list& out) {
-      const bool bias = ctx->saved_data["bias"].toBool();
+      const int64_t saved_how = ctx->saved_data["how"].toInt();
+      const bool bias = saved_how >> 9 & 1, residual = saved_how >> 10 & 1;
       const bool dx = ctx->needs_input_grad(0), dw = ctx->needs_input_grad(1),
                  db = bias && ctx->needs_input_grad(2);
       if (dx || dw || db) {
         const variable_list saved = ctx->get_saved_variables();
-        const LinearHow how{static_cast<int32_t>(ctx->saved_data["act"].toInt()),
-                            ctx->saved_data["gated"].toBool(),
-                            static_cast<int32_t>(ctx->saved_data["flags"].toInt())};
+        const LinearHow how{static_cast<int32_t>(saved_how & 0xff), (saved_how >> 8 & 1) != 0,
+                            static_cast<int32_t>(saved_how >> 16)};
         const auto g = linear_grad_of({"dout", &grads[0]}, {"x", &saved[0]}, {"weight", &saved[1]},
                                       optional_arg(saved[2], "counts"), optional_arg(saved[3], "z"),
                                       how, dx, dw, db);
         for (int i = 0; i < 3; ++i) out[i] = g[i];
       }
-      if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2 + bias)) out[3] = grads[0];
+      if (residual && ctx->needs_input_grad(2 + bias)) out[3] = grads[0];
     });
   }
 };
