@@ -332,8 +332,12 @@ struct PermuteParams {
   int32_t* row_of_slot;   // [m, topk], -1: none (with ids: written)
   int32_t* slot_of_row;   // [m * topk], likewise
   uint8_t* rows;          // [m * topk, bytes]
+  int32_t* counts;        // [experts] (launch_permute_few)
 };
 int launch_permute(const PermuteParams& p, hipStream_t stream);
+// The order and the rows of up to kPermuteFew slots in one launch.
+constexpr int64_t kPermuteFew = 64;
+int launch_permute_few(const PermuteParams& p, hipStream_t stream);
 struct UnpermuteParams {
   const void* rows;  // [n_rows, cols], ld apart
   int64_t ld, n_rows, cols, m;

@@ -138,6 +138,73 @@ __global__ __launch_bounds__(256) void permute_kernel(const PermuteParams p, int
   }
 }
 
+// The same for up to 64 slots, with the order: a decode step's, for which a launch of
+// its own takes as long as the rows do (8 slots of 256 experts, 7168 columns 10.7 us in
+// two launches, 7.4 so). Every wave finds all slots' places, a slot a lane: ballots
+// over the bits of the experts' numbers, most significant first, give the lanes of an
+// equal and of a smaller one.
+template <int W>
+__global__ __launch_bounds__(256) void permute_few_kernel(const PermuteParams p, int lanes_log2,
+                                                          int id_bits) {
+  typedef typename WordOf<W>::type Word;
+  const int lane = threadIdx.x & 63, lanes = 1 << lanes_log2;
+  const int slots = static_cast<int>(p.m) * p.topk;
+  const bool slot = lane < slots;
+  const int id = slot ? p.ids[lane] : -1;
+  const bool kept = id >= 0 && id < p.experts;
+  const int e = kept ? id : p.experts;
+  uint64_t eq = __ballot(slot), lt = 0;
+  for (int b = id_bits - 1; b >= 0; --b) {
+    const bool bit = slot && ((e >> b) & 1);
+    const uint64_t on = __ballot(bit);
+    if (bit) lt |= eq & ~on;
+    eq &= bit ? on : ~on;
+  }
+  const uint64_t below = lane ? ~0ull >> (64 - lane) : 0;
+  const int place = __popcll(lt) + __popcll(eq & below);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) {
+    for (int q = lane; q < p.experts; q += 64) p.counts[q] = 0;
+    __builtin_amdgcn_s_waitcnt(0);  // (the zeros are written before the counts)
+    if (kept && (eq & below) == 0) p.counts[e] = __popcll(eq);
+    if (slot) {
+      p.row_of_slot[lane] = kept ? place : -1;
+      p.slot_of_row[place] = kept ? lane : -1;
+    }
+  }
+  const int t = blockIdx.x * (256 >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  const int64_t i = (threadIdx.x & (lanes - 1)) + blockIdx.y * int64_t{lanes};
+  const bool mine = t < p.m && i < row_vectors(p.bytes, W);
+  const int64_t at = vector_at(i, p.bytes, W);
+  Word v{};
+  if (mine) v = *reinterpret_cast<const Word*>(p.x + t * p.x_stride + at);
+  for (int k = 0; k < p.topk; ++k) {
+    const int from = min(t * p.topk + k, 63);  // (whole waves shuffle)
+    const int64_t row = __shfl(place, from, 64);
+    const bool has = __shfl(static_cast<int>(kept), from, 64);
+    if (mine)
+      __builtin_nontemporal_store(has ? v : Word{},
+                                  reinterpret_cast<Word*>(p.rows + row * p.bytes + at));
+  }
+}
+template <int W>
+static int permute_few(const PermuteParams& p, hipStream_t stream) {
+  const int64_t vecs = row_vectors(p.bytes, W);
+  const int l = token_lanes_log2(vecs);
+  const int per = 256 >> l;
+  int id_bits = 0;
+  while ((1 << id_bits) <= p.experts) ++id_bits;
+  hipLaunchKernelGGL(permute_few_kernel<W>,
+                     dim3(static_cast<unsigned>((p.m + per - 1) / per),
+                          static_cast<unsigned>((vecs + (int64_t{1} << l) - 1) >> l)),
+                     dim3(256), 0, stream, p, l, id_bits);
+  return check_launch("permute_few_kernel");
+}
+int launch_permute_few(const PermuteParams& p, hipStream_t stream) {
+  if (p.bytes >= 16) return permute_few<16>(p, stream);
+  if (p.bytes >= 4) return permute_few<4>(p, stream);
+  return permute_few<1>(p, stream);
+}
+
 template <int W>
 static int permute_width(const PermuteParams& p, hipStream_t stream) {
   const int64_t vecs = row_vectors(p.bytes, W);

@@ -130,9 +130,6 @@ int32_t fgs_moe_permute(const void* x, int64_t x_stride, int64_t m, int64_t row_
   int32_t* classes = reinterpret_cast<int32_t*>(ws + 2 * part);
   int32_t* npp = reinterpret_cast<int32_t*>(ws + 3 * part);
   int32_t* scratch = align_scratch_bytes(numel, num_experts + 1) > 0 ? npp + 64 : nullptr;
-  rc = launch_align(topk_ids, numel, num_experts + 1, 1, sorted, classes, npp, numel,
-                    as_stream(stream), scratch, nullptr, nullptr, num_experts, counts, place);
-  if (rc || numel == 0) return rc;
   PermuteParams p{};
   p.x = static_cast<const uint8_t*>(x);
   p.x_stride = x_stride;
@@ -145,6 +142,11 @@ int32_t fgs_moe_permute(const void* x, int64_t x_stride, int64_t m, int64_t row_
   p.row_of_slot = row_of_slot;
   p.slot_of_row = slot_of_row;
   p.rows = static_cast<uint8_t*>(rows);
+  p.counts = counts;
+  if (numel > 0 && numel <= kPermuteFew) return launch_permute_few(p, as_stream(stream));
+  rc = launch_align(topk_ids, numel, num_experts + 1, 1, sorted, classes, npp, numel,
+                    as_stream(stream), scratch, nullptr, nullptr, num_experts, counts, place);
+  if (rc || numel == 0) return rc;
   return launch_permute(p, as_stream(stream));
 }
 
