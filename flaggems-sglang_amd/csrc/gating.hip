@@ -179,8 +179,9 @@ __global__ __launch_bounds__(256) void topk_gating_grad_kernel(
     return bf16_in ? bf16_bits_to_f32(static_cast<const uint16_t*>(logits)[base + e])
                    : static_cast<const float*>(logits)[base + e];
   };
-  const bool pick = lane < topk;
-  const int id = pick ? ids[row * topk + lane] : -1;
+  int id = lane < topk ? ids[row * topk + lane] : -1;
+  const bool pick = id >= 0 && id < num_experts;  // (an id that is none has no gradient)
+  id = pick ? id : -1;
   const float w = pick ? weights[row * topk + lane] : 0.f;
   const float d = pick ? dweights[row * topk + lane] : 0.f;
   auto add = [](uint32_t a, uint32_t b) {

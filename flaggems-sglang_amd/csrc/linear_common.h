@@ -207,7 +207,7 @@ __device__ __forceinline__ float linear_act_slope(float z, float* slope) {
     return z * phi;
   }
   if constexpr (ACT == FGS_ACT_RELU) {
-    *slope = z > 0.f ? 1.f : 0.f;
+    *slope = z <= 0.f ? 0.f : 1.f;  // (1 of a NaN)
     return z < 0.f ? 0.f : z;
   }
   *slope = 1.f;

@@ -164,7 +164,10 @@ __global__ __launch_bounds__(256) void permute_few_kernel(const PermuteParams p,
   const int place = __popcll(lt) + __popcll(eq & below);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) {
     for (int q = lane; q < p.experts; q += 64) p.counts[q] = 0;
-    __builtin_amdgcn_s_waitcnt(0);  // (the zeros are written before the counts)
+    // the zeros are written before the counts
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (kept && (eq & below) == 0) p.counts[e] = __popcll(eq);
     if (slot) {
       p.row_of_slot[lane] = kept ? place : -1;

@@ -239,7 +239,7 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
                        int64_t n, int64_t k, int32_t dtype, int32_t act, int32_t gated,
                        int32_t flags, float* z, void* out, void* stream) {
   int rc = check_linear(groups, rows, n, k, dtype);
-  if (rc) return rc;
+  if (rc || (gated && (rc = check_linear(groups, rows, 2 * n, k, dtype)))) return rc;
   if ((rc = check_act(act))) return rc;
   if (!linear_flags_ok(gated ? kLinearGated : kLinearForward, flags)) return fail(FGS_EINVAL, "unknown flags");
   if (!counts && groups != 1) return fail(FGS_EINVAL, "counts are needed for several groups");
@@ -279,7 +279,7 @@ int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, i
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream) {
   int rc = check_linear(1, rows, n, 8, dtype);
-  if (rc) return rc;
+  if (rc || (gated && (rc = check_linear(1, rows, 2 * n, 8, dtype)))) return rc;
   if ((rc = check_act(act))) return rc;
   if (rows == 0) return FGS_OK;
   if (!dout || !z || !dz) return fail(FGS_EINVAL, "null pointer argument");
@@ -398,7 +398,7 @@ int32_t fgs_moe_linear_schedule(int32_t pass, int32_t groups, int64_t rows, int6
   if (pass < 0 || pass > 2) return fail(FGS_EINVAL, "pass must be 0, 1 or 2");
   const int64_t wide = gated ? 2 * n : n;
   int rc = check_linear(groups, rows, pass ? wide : n, k, FGS_DTYPE_BF16);
-  if (rc) return rc;
+  if (rc || (rc = check_linear(groups, rows, wide, k, FGS_DTYPE_BF16))) return rc;
   if (!buf || len < 1) return fail(FGS_EINVAL, "buf must hold at least one byte");
   const int mode = pass == 1 ? kLinearDgrad : pass == 2 ? kLinearWgrad
                                                         : gated ? kLinearGated : kLinearForward;

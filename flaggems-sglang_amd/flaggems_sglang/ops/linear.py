@@ -51,7 +51,7 @@ def fused_linear(
     first size, ``residual [..., n]``, all bf16 or all fp16. Sums, activation and
     additions are in fp32, the result is rounded once. ``activation``: None,
     "relu", "silu" or "gelu" (exact, erf). ``n`` and ``k`` are multiples of 8 up to
-    2^20; fewer than 2^30 rows (0 among them). Operands whose rows are not 16-byte
+    2^20 (gated: ``2 n``); fewer than 2^30 rows (0 among them). Operands whose rows are not 16-byte
     aligned, or whose columns are not adjacent, are copied first.
 
     Gradients go to ``x``, ``weight``, ``bias`` and ``residual``. With an activation,

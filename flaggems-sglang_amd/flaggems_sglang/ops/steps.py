@@ -52,7 +52,8 @@ def moe_permute(
 
     ``topk_ids [tokens, topk]`` int32 or int64; ids outside ``[0, num_experts)``
     (experts of other GPUs) come behind the last expert's, as rows of zeros.
-    ``num_experts`` up to 1022, up to 2^30 slots. Or ``order``, as an earlier call
+    ``num_experts`` up to 1022; up to 2^30 slots (gradients and rows by an ``order``:
+    fewer than 2^23 tokens and 2^27 slots, else what their grids can hold). Or ``order``, as an earlier call
     on the same ids returned it: then nothing is sorted again (for the scales of
     8-bit values, say).
 

@@ -469,7 +469,7 @@ int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32
 
 /* Gradient of fgs_moe_topk_gating's weights: dlogits [m, num_experts] (of
  * logits' type) from the weights and ids that it returned for these logits and
- * dweights f32 [m, topk]. */
+ * dweights f32 [m, topk]. (Ids outside [0, num_experts) have no gradient.) */
 int32_t fgs_moe_topk_gating_grad(const void* logits, int32_t logits_bf16, int64_t m,
                                  int32_t num_experts, int32_t topk, int32_t scoring,
                                  int32_t renormalize, const float* topk_weights,
@@ -484,8 +484,9 @@ int32_t fgs_moe_topk_gating_grad(const void* logits, int32_t logits_bf16, int64_
  *   rows [m * topk] of row_bytes, contiguous; counts int32 [num_experts]
  *   row_of_slot int32 [m, topk]: the slot's row, -1 for slots of no expert here
  *   slot_of_row int32 [m * topk]: its inverse, -1 for the rows behind
- * Of the values in [0, num_experts) no order depends on atomics. num_experts <=
- * 1022. Workspace: fgs_moe_permute_workspace_bytes, 256-byte aligned, this call's
+ * No result depends on the order of atomics. num_experts <= 1022; m * topk <= 2^30,
+ * and fewer than 2^23 tokens with fewer than 2^27 slots fit the grids of all entries
+ * here (others are refused where they do not). Workspace: fgs_moe_permute_workspace_bytes, 256-byte aligned, this call's
  * alone until it has run. */
 int64_t fgs_moe_permute_workspace_bytes(int64_t numel, int32_t num_experts);
 int32_t fgs_moe_permute(const void* x, int64_t x_stride, int64_t m, int64_t row_bytes,
@@ -527,7 +528,7 @@ int32_t fgs_moe_unpermute_grad(const void* dout, int64_t ldd, const void* rows, 
  *   other from row 0 on (negative ones count as 0, and what passes the last row is
  *   cut); rows behind the last group's have no product (out = residual, or 0; their
  *   z is not defined). Null: one matrix for all rows.
- * n and k multiples of 8, up to 2^20; fewer than 2^30 rows, up to 4096 groups; rows of x, w,
+ * n and k multiples of 8, n (gated: 2 n) and k up to 2^20; fewer than 2^30 rows, up to 4096 groups; rows of x, w,
  * residual 16-byte aligned and at most 2^21 elements apart. No workspace. `flags`:
  * 0, or FGS_LINEAR_FORM(f), the kernel form f whatever the sizes (for measurement
  * and tests). */

@@ -133,6 +133,18 @@ def test_nan_stays_in_its_row(gpu, form):
     assert torch.equal(got["dw"][:, :103], clean["dw"][:, :103])
 
 
+@pytest.mark.parametrize("kind", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_nan_passes_activations(gpu, kind, gated):
+    """A NaN row reaches its own output and the weights, and no other row."""
+    t, dout = inputs(20, 72, 64, torch.bfloat16, gated, False, False)
+    t["x"][7] = float("nan")
+    got = run(t, dout=dout, activation=kind, gated=gated)
+    assert bool(got["out"][7].isnan().all()) and bool(got["dw"].isnan().all())
+    keep = torch.arange(20, device="cuda") != 7
+    assert bool(got["out"][keep].isfinite().all()) and bool(got["dx"][keep].isfinite().all())
+
+
 @pytest.mark.parametrize("form", FORMS)
 def test_strides_and_shapes(gpu, form):
     """Slices of wider tensors, leading sizes, other strides, offsets that leave

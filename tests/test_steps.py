@@ -89,6 +89,8 @@ DB = dict(dz=P, ldz=32, counts=None, groups=1, rows=4, wide=32, dtype=0, ws=None
     ("linear", LINEAR, dict(k=60), -2, "multiples of 8"),
     ("linear", LINEAR, dict(k=1 << 21), -2, "too large"),
     ("linear", LINEAR, dict(rows=1 << 30), -2, "too large"),
+    ("linear", LINEAR, dict(n=(1 << 19) + 8, gated=1), -2, "too large"),
+    ("linear_act_grad", ACT, dict(n=(1 << 19) + 8, gated=1), -2, "too large"),
     ("linear", LINEAR, dict(groups=4097, counts=P), -2, "too large"),
     ("linear", LINEAR, dict(groups=0, counts=P), -1, "groups >= 1"),
     ("linear", LINEAR, dict(groups=2), -1, "counts are needed"),

@@ -6,6 +6,7 @@ import torch
 
 import flaggems_sglang as fgs
 import steps_ref as ref
+from flaggems_sglang import _capi
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +76,28 @@ def test_permute_other_types(gpu, dtype):
         slots = order.slot_of_row.long()
         raw, got = x.view(torch.uint8), rows.view(torch.uint8)
         assert torch.equal(got, torch.where(slots[:, None] >= 0, raw[slots.clamp(min=0) // 4], 0))
+
+
+@pytest.mark.parametrize("slots", [1, 2, 63, 64, 65])
+@pytest.mark.parametrize("experts", [1, 8, 1022])
+def test_permute_few_slots(gpu, slots, experts):
+    """Up to 64 slots and one more: all of one expert, of none, of the first and the
+    last; rows of 1 to 33 bytes and of several workgroups."""
+    gen = generator(slots, experts)
+    first_last = torch.arange(slots, dtype=torch.int32, device="cuda") % 2 * (experts - 1)
+    stray = torch.where(first_last == 0, first_last, experts)
+    for flat in (torch.zeros_like(first_last), torch.full_like(first_last, -1), first_last, stray):
+        for topk in {1, slots}:
+            ids = flat.view(-1, topk)
+            counts, row_of_slot, slot_of_row = ref.order(ids, experts)
+            at = slot_of_row.long().cuda()
+            for cols in (1, 2, 3, 4, 7, 15, 16, 17, 33, 9001):
+                x = torch.randint(256, (ids.shape[0], cols), generator=gen, device="cuda").byte()
+                rows, order = fgs.moe_permute(x, ids, experts)
+                assert torch.equal(order.counts.cpu(), counts)
+                assert torch.equal(order.row_of_slot.cpu(), row_of_slot)
+                assert torch.equal(order.slot_of_row.cpu(), slot_of_row)
+                assert torch.equal(rows, torch.where(at[:, None] >= 0, x[at.clamp(min=0) // topk], 0))
 
 
 def test_permute_ids_of_64_bits_and_strides(gpu):
@@ -205,6 +228,44 @@ def test_router_gradient(gpu, dtype, m, experts, topk, scoring, renormalize):
     h = ref.half(TYPES[dtype])
     bound = 2.0 ** -14 * mag + 2.0 ** -48 * terms
     ref.close("dlogits", got, want, bound + h * (want.abs() + bound) + ref.tiny(logits, h))
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_router_gradient_of_masked_experts(gpu, scoring, renormalize):
+    """Experts masked with -inf or the type's lowest value, fewer left than are picked,
+    have gradients of 0; a NaN stays in its token's row."""
+    gen = generator(11)
+    logits = torch.randn(6, 70, generator=gen, device="cuda")
+    logits[1, 5:] = float("-inf")
+    logits[2, 3:] = torch.finfo(torch.float32).min
+    logits[3, 17] = float("nan")
+    logits.requires_grad_()
+    d = torch.randn(6, 8, generator=gen, device="cuda")
+    weights, _ = fgs.fused_topk(torch.empty(6, 1, device="cuda"), logits, 8, renormalize, scoring)
+    got, = torch.autograd.grad(weights, logits, d)
+    assert not bool(got[1, 5:].any()) and not bool(got[2, 3:].any())
+    rows = [0, 1, 2, 4, 5]
+    assert bool(got[rows].isfinite().all()) and bool(got[1, :5].any()) and bool(got[2, :3].any())
+    again = logits.detach()[rows].requires_grad_()
+    weights, _ = fgs.fused_topk(torch.empty(5, 1, device="cuda"), again, 8, renormalize, scoring)
+    assert torch.equal(torch.autograd.grad(weights, again, d[rows])[0], got[rows])
+
+
+def test_router_gradient_of_ids_that_are_none(gpu):
+    """The C entry: an id outside the experts has no gradient and reads nothing."""
+    gen = generator(12)
+    logits = torch.randn(4, 16, generator=gen, device="cuda")
+    w, d = torch.rand(2, 4, 2, generator=gen, device="cuda")
+    ids = torch.tensor([[0, -1], [16, 5], [-2 ** 31, 2 ** 31 - 1], [3, 15]], dtype=torch.int32, device="cuda")
+    lib = _capi.load()
+    for scoring in (0, 1):
+        for renormalize in (0, 1):
+            out = torch.full_like(logits, float("nan"))
+            rc = lib.fgs_moe_topk_gating_grad(
+                logits.data_ptr(), 0, 4, 16, 2, scoring, renormalize, w.data_ptr(), ids.data_ptr(),
+                d.data_ptr(), out.data_ptr(), torch.cuda.current_stream().cuda_stream)
+            assert rc == 0 and bool(out.isfinite().all()) and not bool(out[2].any())
 
 
 # ------------------------------------------------------------------ layer ---
