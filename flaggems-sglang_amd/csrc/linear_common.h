@@ -70,17 +70,6 @@ struct GroupScan {
     return e < groups ? min(max(counts[e], 0), rows) : 0;
   }
 
-  // The row behind the last group's.
-  __device__ __forceinline__ int used() const {
-    int base = 0;
-    for (int e0 = 0; e0 < groups; e0 += 64) {
-      int v = count(e0 + (threadIdx.x & 63));
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) v = min(v + __shfl_xor(v, d, 64), rows);
-      base = min(base + v, rows);
-    }
-    return __builtin_amdgcn_readfirstlane(base);
-  }
   // First row and rows of group e.
   __device__ __forceinline__ void range(int e, int* first, int* n) const {
     int base = 0;

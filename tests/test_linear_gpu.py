@@ -314,3 +314,33 @@ def test_last_round_in_quarters(gpu, rows, n, k, counts, which):
     want = ref.product(**t, **options) if counts is None else ref.grouped(**t, counts=counts, **options)
     got = run(t, on_gpu, options["dout"], activation=options["kind"], gated=gated, _flags=large)
     compare(got, want)
+
+
+@pytest.mark.parametrize("which", ["forward", "gated", "input"])
+@pytest.mark.parametrize("rows, counts", [
+    (256 * 18 + 1, None), (256 * 18 + 128, None), (256 * 18 + 129, None), (100, None),
+    (2560, [1, 128, 129, 255, 256, 257, 0, 384, 385, 640]), (2560, [128] * 18 + [100]),
+    (2560, [0, 640, -5, 513, 128]), (2561, [255] * 9 + [385]), (2500, [2200, 400, 100])])
+def test_rows_past_whole_tiles(gpu, rows, counts, which):
+    """More than a round of 256 x 256 tiles: groups (and products) that end in each part
+    of a tile; rows of no group are 0."""
+    large = sum(_capi.LINEAR_FORMS[p] << (8 * i) for i, p in enumerate(("forward", "input", "weight")))
+    wide = 4136 if rows > 256 else 66056
+    n, k = (40, wide) if which == "input" else (wide, 40)
+    gated = which == "gated"
+    if gated:
+        n //= 2
+        n = n // 8 * 8
+    groups = None if counts is None else len(counts)
+    t, dout = inputs(rows, n, k, torch.bfloat16, gated, which != "input", False, groups)
+    on_gpu = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+    options = dict(kind="silu" if gated else None, gated=gated, dout=dout if which == "input" else None)
+    if counts is not None:  # (as the kernels cut them)
+        left, cut = rows, []
+        for c in counts:
+            cut.append(min(max(c, 0), left))
+            left -= cut[-1]
+        counts = cut
+    want = ref.product(**t, **options) if counts is None else ref.grouped(**t, counts=counts, **options)
+    got = run(t, on_gpu, options["dout"], activation=options["kind"], gated=gated, _flags=large)
+    compare(got, want)
