@@ -43,6 +43,7 @@ struct LinearTile {
   static constexpr int P_AT = Q_SLOTS * SLOT;
   static constexpr int LDS = (Q_SLOTS + P_SLOTS) * SLOT;
   static constexpr int STAGING = T * T / 2;   // a wave's part in the epilogue, 16 bits
+  static constexpr bool ROUNDS = KB == 32;    // a workgroup has several tiles
   static_assert(KB == 32 || KB == 64, "main loops");
   static_assert(4 * STAGING <= LDS && LDS <= 160 * 1024, "LDS");
   // Place of 16-byte chunk c of row r of KB sums: the LDS serves 16 lanes of a
@@ -92,6 +93,11 @@ struct Feed {
   }
 };
 
+// The epilogue's staging, which no load in flight writes (__restrict__: as the
+// transposing reads).
+__device__ __forceinline__ void put_staged(uint2* __restrict__ at, uint2 v) { *at = v; }
+__device__ __forceinline__ u32x4 staged(const u32x4* __restrict__ at) { return *at; }
+
 // Tiles of an XCD, and those of its last round that are cut off: of the 32 CUs at most
 // half have one, and there is a round before it.
 __device__ __host__ __forceinline__ int linear_share(int total, int xcd) {
@@ -114,6 +120,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   constexpr int T = C::T, NB = C::NB, NL = C::NL, SLOT = C::SLOT;
   constexpr int TN = GATED ? T / 2 : T;  // output columns of a tile
   constexpr int P_AT = C::P_AT, KB = C::KB;
+  constexpr bool ROUNDS = C::ROUNDS;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63;
@@ -135,18 +142,21 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
                       : p.counts ? scan.tiles(bt) : (p.rows + bt - 1) / bt;
   const int total = (QA ? p.groups : 1) * n_rt * n_ct;
   const int xcd = blockIdx.x & 7;
-  int pos = blockIdx.x >> 3, sub = 0;
   const int share = linear_share(total, xcd);
   const int rest = p.part == kLinearWhole ? 0 : linear_rest(share);
+  int e, rt, ct, first, nrows;  // the tile's: rows of Q [first, first + nrows)
+  // Tile (of the XCD's) pos; false if there is none.
+  auto locate = [&](int pos) -> bool {
+  int sub = 0;
   if (quarters == 2) {
     sub = pos & 3;
     pos = share - rest + (pos >> 2);
-    if (pos >= share) return;
+    if (pos >= share) return false;
   } else if (pos >= share - rest) {
-    return;
+    return false;
   }
   int at = xcd * (total >> 3) + min(xcd, total & 7) + pos;
-  int e = 0;
+  e = 0;
   if (QA) {
     e = at / (n_rt * n_ct);
     at -= e * n_rt * n_ct;
@@ -155,11 +165,10 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   const int band = at / (n_rt * BAND);
   const int cols = min(BAND, n_ct - band * BAND);
   at -= band * n_rt * BAND;
-  int rt = __builtin_amdgcn_readfirstlane(at / cols);
-  const int ct = __builtin_amdgcn_readfirstlane((band * BAND + at % cols) * quarters + (sub & 1));
+  rt = __builtin_amdgcn_readfirstlane(at / cols);
+  ct = __builtin_amdgcn_readfirstlane((band * BAND + at % cols) * quarters + (sub & 1));
   e = __builtin_amdgcn_readfirstlane(e);
-  // rows of Q: [first, first + nrows) of the tile (across: of the group's sums)
-  int first, nrows;
+  // (across: rows of the group's sums)
   if (!p.counts) {
     first = QA ? 0 : rt * bt;
     nrows = QA ? p.rows : min(bt, p.rows - first);
@@ -173,21 +182,37 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     first += (sub >> 1) * T;
     nrows = min(T, nrows - (sub >> 1) * T);
   }
-  if (ct * TN >= p.n || (QA ? rt * T >= p.m : nrows <= 0)) return;  // (quarters may be empty)
   e = __builtin_amdgcn_readfirstlane(e);
   first = __builtin_amdgcn_readfirstlane(first);
   nrows = __builtin_amdgcn_readfirstlane(nrows);
-  const bool none = !QA && e >= (p.counts ? p.groups : 1);  // rows of no group
-  const int red = QA ? nrows : none ? 0 : p.red;
+  return ct * TN < p.n && (QA ? rt * T < p.m : nrows > 0);  // (quarters may be empty)
+  };
+  int pos = blockIdx.x >> 3;
+  if (!locate(pos)) return;
+  bool none;  // rows of no group
+  int red, prows;
+  const uint8_t *q0, *p0;
+  const int64_t ldq = p.ldq * 2, ldp = p.ldp * 2;
+  auto enter = [&] {
+    none = !QA && e >= (p.counts ? p.groups : 1);
+    red = QA ? nrows : none ? 0 : p.red;
+    q0 = static_cast<const uint8_t*>(p.q) +
+         (QA ? first * ldq + static_cast<int64_t>(rt) * T * 2 : first * ldq);
+    p0 = static_cast<const uint8_t*>(p.p) + (QA ? first * ldp : e * p.p_group * 2) +
+         (PA ? static_cast<int64_t>(ct) * T * 2 : static_cast<int64_t>(ct) * TN * ldp);
+    if (none) p0 = static_cast<const uint8_t*>(p.p);
+    prows = PA ? 0 : min(TN, p.n - ct * TN);
+  };
+  enter();
   // (a stage of zeros where there are no sums: the accumulators then come from the
   // loop alone, not from a choice that the compiler would make in VGPRs)
-  const int KT = max(1, (red + KB - 1) / KB);
+  auto stages = [&] { return max(1, (red + KB - 1) / KB); };
 
   // ---- the bias, where the accumulators start: its loads go out before the
   // stages'.
   constexpr int WN = 32 * NB;              // columns of a wave's accumulators
   constexpr int OC = GATED ? WN / 2 : WN;  // ... of its output
-  const int col0 = ct * TN + wn * OC;
+  int col0 = ct * TN + wn * OC;
   const int wide = GATED ? 2 * p.n : p.n;
   const int h = lane >> 5;
   uint2 bias[NB][4];
@@ -206,13 +231,6 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // ---- operands. A stage's resource begins at the stage and ends with its last
   // value: `along`, with the tile's last row's last sum; `across`, with the last
   // row's last column.
-  const int64_t ldq = p.ldq * 2, ldp = p.ldp * 2;
-  const uint8_t* q0 = static_cast<const uint8_t*>(p.q) +
-                      (QA ? first * ldq + static_cast<int64_t>(rt) * T * 2 : first * ldq);
-  const uint8_t* p0 = static_cast<const uint8_t*>(p.p) + (QA ? first * ldp : e * p.p_group * 2) +
-                      (PA ? static_cast<int64_t>(ct) * T * 2 : static_cast<int64_t>(ct) * TN * ldp);
-  if (none) p0 = static_cast<const uint8_t*>(p.p);
-  const int prows = PA ? 0 : min(TN, p.n - ct * TN);
   Feed<C, QA> fq;
   Feed<C, PA> fp;
   // (gated: the tile's rows of P by 32: gate, up, gate, up ... of the same columns; the
@@ -328,11 +346,20 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   constexpr std::integral_constant<int, 0> no_loads{};
   auto next_q = [](int o) { return o == (C::Q_SLOTS - 1) * SLOT ? 0 : o + SLOT; };
   auto next_p = [](int o) { return o == (C::P_SLOTS - 1) * SLOT ? 0 : o + SLOT; };
+  // (ROUNDS: the first PRE stages of a tile go out before the epilogue of the one before)
+  constexpr int PRE = ROUNDS ? 3 : AHEAD;
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) {
+  for (int s = 0; s < PRE; ++s) {
     feed_p(s, s * SLOT);
     feed_q(s, s * SLOT);
   }
+  for (;;) {
+#pragma unroll
+  for (int s = PRE; s < AHEAD; ++s) {
+    feed_p(s, s * SLOT);
+    feed_q(s, s * SLOT);
+  }
+  const int KT = stages();
 #pragma unroll
   for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -383,10 +410,26 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // runs of a row, 16 bytes a lane. The residual comes in the same way first; z, which
   // a gradient is taken at, leaves in fp32 (in 16 bits, its rounding was as large a
   // part of the gradients' error as their own).
-  uint8_t* stg = lds + wave * C::STAGING;
+  uint8_t* stg = lds + (ROUNDS ? (wave >> 1) * P_AT + PRE * SLOT + (wave & 1) * SLOT
+                               : wave * C::STAGING);
   // (the weights' gradient: rows of the group's matrix)
   const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
   const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
+  bool more = false;
+  const int out0 = col0;
+  if constexpr (ROUNDS) {
+    pos += 32;
+    more = locate(pos);
+    if (more) {
+      enter();
+      col0 = ct * TN + wn * OC;
+#pragma unroll
+      for (int s = 0; s < PRE; ++s) {
+        feed_p(s, s * SLOT);
+        feed_q(s, s * SLOT);
+      }
+    }
+  }
   // Eight bytes s of staged row r: the XOR spreads a column of 32 rows over all banks.
   // Sixteen bytes are two of them, swapped in some rows.
   constexpr int W8 = OC / 4, RPL = 32 / W8;
@@ -398,11 +441,12 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   };
   // f(staged row, output row in the tile, 16-byte chunk) for the wave's part, a
   // chunk a lane; the tile's rows 64 i + 32 wm + r are the staged rows 32 i + r.
+  constexpr int PARTS = ROUNDS ? 2 : 1, PB = NB / PARTS;
   auto runs = [&](auto&& f) {
     constexpr int LPR = OC / 8, RPP = 64 / LPR;
     const int lr = lane / LPR, lc = lane % LPR;
 #pragma unroll 8
-    for (int k = 0; k < WN / RPP; ++k) {
+    for (int k = 0; k < WN / PARTS / RPP; ++k) {
       const int sr = k * RPP + lr;
       f(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc);
     }
@@ -427,7 +471,6 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
       constexpr int i = decltype(i_c)::value;
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        keep(acc[i][j]);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *chunk(r32, j * 8 + 2 * g + h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1],
@@ -458,12 +501,15 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   const bool has_residual = FORWARD && p.residual;
   // (rows of no group: sums of nothing, whose activations are 0)
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int part = 0; part < PARTS; ++part) {
+  const int I0 = part * PB;
+#pragma unroll
+  for (int i = I0; i < I0 + PB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; j += GATED ? 2 : 1) {
       auto at = [&](int g) {
         return reinterpret_cast<uint2*>(
-            stg + place(i * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
+            stg + place((i - I0) * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
       };
       keep(acc[i][j]);
       if constexpr (GATED) keep(acc[i][j + 1]);
@@ -487,16 +533,25 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
                 static_cast<raw>((t < 2 ? res[g].x : res[g].y) >> (16 * (t & 1))));
           }
         }
-        *at(g) = pack4(v);
+        if constexpr (ROUNDS) put_staged(at(g), pack4(v));
+        else *at(g) = pack4(v);
       }
     }
   sync();
   runs([&](int sr, int r, int c) {
-    u32x4 v = *reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
+    const u32x4* from = reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
+    u32x4 v = ROUNDS ? staged(from) : *from;
     if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
-    if (r < rows_in && col0 + c * 8 < p.n)
-      *reinterpret_cast<u32x4*>(static_cast<raw*>(p.out) + (row0 + r) * p.n + col0 + c * 8) = v;
+    r += I0 * 64;
+    if (r < rows_in && out0 + c * 8 < p.n)
+      *reinterpret_cast<u32x4*>(static_cast<raw*>(p.out) + (row0 + r) * p.n + out0 + c * 8) = v;
   });
+  if (PARTS > 1) sync();
+  }
+  if (!more) break;
+  wait_lgkm0();
+  wave_barrier_all();  // the staging is done with
+  }
 }
 
 // ---------------------------------------------------------------- schedule ---
@@ -506,8 +561,8 @@ template <int TY, int MODE, int ACT, int T>
 int launch_tile(const LinearParams& p, int64_t wgs, hipStream_t stream) {
   typedef LinearTile<T, T == 256 && (MODE == kLinearDgrad || MODE == kLinearWgrad) ? 32 : 64> C;
   static std::atomic<uint64_t> told{0};
-  return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told, wgs, 256,
-                    C::LDS, stream, p);
+  return launch_lds("linear_tile_kernel", linear_tile_kernel<TY, MODE, ACT, C>, told,
+                    C::ROUNDS ? std::min<int64_t>(wgs, 256) : wgs, 256, C::LDS, stream, p);
 }
 template <int TY, int MODE, int ACT>
 int launch_form(const LinearParams& p, bool large, hipStream_t stream) {
