@@ -348,11 +348,15 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   auto next_p = [](int o) { return o == (C::P_SLOTS - 1) * SLOT ? 0 : o + SLOT; };
   // (ROUNDS: the first PRE stages of a tile go out before the epilogue of the one before)
   constexpr int PRE = ROUNDS ? 3 : AHEAD;
+  constexpr int STORES = ROUNDS ? T * TN / (8 * 256) : 0;  // of a wave
 #pragma unroll
   for (int s = 0; s < PRE; ++s) {
     feed_p(s, s * SLOT);
     feed_q(s, s * SLOT);
   }
+  // (the first tile has no stores before it: the waits that leave room for them would be
+  // too short)
+  if constexpr (ROUNDS) wait_vmcnt<0>();
   for (;;) {
 #pragma unroll
   for (int s = PRE; s < AHEAD; ++s) {
@@ -371,11 +375,13 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 #pragma unroll
         for (int i = 0; i < NB; ++i) acc[i][j][4 * g + t] = v;
       }
-  wait_vmcnt<2 * (AHEAD - 1) * NL>();
+  wait_vmcnt<2 * (AHEAD - 1) * NL + STORES>();
   wave_barrier_all();
   read_frags(0, 0, 0, fa[0], fb[0]);
   int oq = 0, op = 0, to_q = AHEAD % C::Q_SLOTS * SLOT, to_p = AHEAD % C::P_SLOTS * SLOT, s = 0;
-  do {
+  // MORE: vector memory operations that are in flight beside the loads
+  auto stage = [&](auto more_c) {
+    constexpr int MORE = decltype(more_c)::value;
 #pragma unroll
     for (int kk = 0; kk + 1 < C::KK; ++kk) {
       read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
@@ -387,7 +393,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     }
     wait_lgkm0();
     // behind stage s + 1's loads: those of the stages to s + AHEAD - 1, and P's
-    wait_vmcnt<(2 * (AHEAD - 2) + 1) * NL>();
+    wait_vmcnt<(2 * (AHEAD - 2) + 1) * NL + MORE>();
     wave_barrier_all();
     __builtin_amdgcn_sched_barrier(0);
     oq = next_q(oq);
@@ -399,7 +405,17 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     mma(fa[1], fb[1]);
     order(loads);
     __builtin_amdgcn_sched_barrier(0);
-  } while (++s < KT);
+  };
+  // (the loads of the first PRE stages are older than the stores of the tile before)
+  if constexpr (ROUNDS) {
+    const int n = min(KT, PRE - 1);
+    do stage(std::integral_constant<int, STORES>{});
+    while (++s < n);
+  }
+  if (!ROUNDS || s < KT) {
+    do stage(std::integral_constant<int, 0>{});
+    while (++s < KT);
+  }
   wait_vmcnt<0>();
   wait_lgkm0();
   wave_barrier_all();  // the ring is done with
@@ -439,16 +455,26 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
-  // f(staged row, output row in the tile, 16-byte chunk) for the wave's part, a
-  // chunk a lane; the tile's rows 64 i + 32 wm + r are the staged rows 32 i + r.
+  // Both of (staged row, output row in the tile, 16-byte chunk, k) for the wave's part,
+  // a chunk a lane, k of up to eight at a time; the tile's rows 64 i + 32 wm + r are the staged
+  // rows 32 i + r.
   constexpr int PARTS = ROUNDS ? 2 : 1, PB = NB / PARTS;
-  auto runs = [&](auto&& f) {
+  auto runs = [&](auto&& get, auto&& put) {
     constexpr int LPR = OC / 8, RPP = 64 / LPR;
+    constexpr int RUNS = WN / PARTS / RPP, AT = RUNS < 8 ? RUNS : 8;
+    static_assert(RUNS % AT == 0, "runs");
     const int lr = lane / LPR, lc = lane % LPR;
-#pragma unroll 8
-    for (int k = 0; k < WN / PARTS / RPP; ++k) {
-      const int sr = k * RPP + lr;
-      f(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc);
+    for (int k0 = 0; k0 < RUNS; k0 += AT) {
+#pragma unroll
+      for (int k = 0; k < AT; ++k) {
+        const int sr = (k0 + k) * RPP + lr;
+        get(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
+      }
+#pragma unroll
+      for (int k = 0; k < AT; ++k) {
+        const int sr = (k0 + k) * RPP + lr;
+        put(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
+      }
     }
   };
   auto pack4 = [](const float (&v)[4]) {
@@ -488,18 +514,23 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
     });
   }
   if (FORWARD && p.residual) {
-    runs([&](int sr, int r, int c) {
-      u32x4 v{0, 0, 0, 0};
+    u32x4 v[8];
+    runs([&](int, int r, int c, int k) {
+      v[k] = u32x4{0, 0, 0, 0};
       if (r < rows_in && col0 + c * 8 < p.n)
-        v = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
-                                            (row0 + r) * p.ldr + col0 + c * 8);
-      if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
-      *reinterpret_cast<u32x4*>(stg + (place(sr, 2 * c) & ~15)) = v;
+        v[k] = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
+                                               (row0 + r) * p.ldr + col0 + c * 8);
+    }, [&](int sr, int, int c, int k) {
+      if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
+      *reinterpret_cast<u32x4*>(stg + (place(sr, 2 * c) & ~15)) = v[k];
     });
     sync();
   }
   const bool has_residual = FORWARD && p.residual;
   // (rows of no group: sums of nothing, whose activations are 0)
+  // (without a branch, so that every tile has STORES of them: what is outside is dropped)
+  const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+      static_cast<raw*>(p.out) + row0 * p.n + out0, 0, 0x7fffffff, kBufWord3);
 #pragma unroll
   for (int part = 0; part < PARTS; ++part) {
   const int I0 = part * PB;
@@ -538,13 +569,16 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
       }
     }
   sync();
-  runs([&](int sr, int r, int c) {
+  u32x4 v[8];  // (read together: one by one, each store waits for its read)
+  runs([&](int sr, int, int c, int k) {
     const u32x4* from = reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
-    u32x4 v = ROUNDS ? staged(from) : *from;
-    if ((sr / RPL) & 1) v = u32x4{v[2], v[3], v[0], v[1]};
+    v[k] = ROUNDS ? staged(from) : *from;
+  }, [&](int sr, int r, int c, int k) {
+    if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
     r += I0 * 64;
-    if (r < rows_in && out0 + c * 8 < p.n)
-      *reinterpret_cast<u32x4*>(static_cast<raw*>(p.out) + (row0 + r) * p.n + out0 + c * 8) = v;
+    const bool in = r < rows_in && out0 + c * 8 < p.n;
+    __builtin_amdgcn_raw_buffer_store_b128(
+        v[k], to, in ? static_cast<uint32_t>(r * p.n + c * 8) * 2 : kOutside, 0, 0);
   });
   if (PARTS > 1) sync();
   }
