@@ -43,7 +43,9 @@ struct LinearTile {
   static constexpr int P_AT = Q_SLOTS * SLOT;
   static constexpr int LDS = (Q_SLOTS + P_SLOTS) * SLOT;
   static constexpr int STAGING = T * T / 2;   // a wave's part in the epilogue, 16 bits
-  static constexpr bool ROUNDS = KB == 32;    // a workgroup has several tiles
+  // A workgroup has several tiles: only where three stages leave room to stage half a
+  // tile beside them.
+  static constexpr bool ROUNDS = KB == 32;
   static_assert(KB == 32 || KB == 64, "main loops");
   static_assert(4 * STAGING <= LDS && LDS <= 160 * 1024, "LDS");
   // Place of 16-byte chunk c of row r of KB sums: the LDS serves 16 lanes of a
@@ -132,8 +134,12 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   // the tiles an XCD's 32 CUs have at a time share rows and columns in its L2.
   // A last round that leaves half of the CUs or more without a tile is cut off
   // (kLinearCut) and goes to a second launch in quarters, 128 x 128 (kLinearRest): 36
-  // row tiles of 16 columns, 2.25 rounds, k 14336: 975 us in one launch, 932 in two; 4608 x 4096 x 4096
-  // (288 tiles) 215 and 143.
+  // row tiles of 16 columns, 2.25 rounds, k 14336: 975 us in one launch, 932 in two;
+  // 4608 x 4096 x 4096 (288 tiles) 215 and 143.
+  // ROUNDS: a CU's workgroup takes every 32nd of its XCD's tiles. The next tile's first
+  // stages are loaded before a tile is stored, and the stores run on under the first
+  // stages' products (128 groups of 65536 rows, 1536 x 2048: dw 545 us with a workgroup
+  // a tile, 471 so; dx 496 and 476; 8192^3 level).
   const int quarters = T == 128 && p.part == kLinearRest ? 2 : 1;  // a side
   const int bt = T * quarters, btn = TN * quarters;
   const int n_ct = (p.n + btn - 1) / btn;
@@ -147,45 +153,45 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   int e, rt, ct, first, nrows;  // the tile's: rows of Q [first, first + nrows)
   // Tile (of the XCD's) pos; false if there is none.
   auto locate = [&](int pos) -> bool {
-  int sub = 0;
-  if (quarters == 2) {
-    sub = pos & 3;
-    pos = share - rest + (pos >> 2);
-    if (pos >= share) return false;
-  } else if (pos >= share - rest) {
-    return false;
-  }
-  int at = xcd * (total >> 3) + min(xcd, total & 7) + pos;
-  e = 0;
-  if (QA) {
-    e = at / (n_rt * n_ct);
-    at -= e * n_rt * n_ct;
-  }
-  constexpr int BAND = 4;
-  const int band = at / (n_rt * BAND);
-  const int cols = min(BAND, n_ct - band * BAND);
-  at -= band * n_rt * BAND;
-  rt = __builtin_amdgcn_readfirstlane(at / cols);
-  ct = __builtin_amdgcn_readfirstlane((band * BAND + at % cols) * quarters + (sub & 1));
-  e = __builtin_amdgcn_readfirstlane(e);
-  // (across: rows of the group's sums)
-  if (!p.counts) {
-    first = QA ? 0 : rt * bt;
-    nrows = QA ? p.rows : min(bt, p.rows - first);
-  } else if (QA) {
-    scan.range(e, &first, &nrows);
-  } else {
-    scan.tile(rt, bt, &e, &first, &nrows);
-  }
-  rt = rt * quarters + (sub >> 1);
-  if (!QA && quarters == 2) {
-    first += (sub >> 1) * T;
-    nrows = min(T, nrows - (sub >> 1) * T);
-  }
-  e = __builtin_amdgcn_readfirstlane(e);
-  first = __builtin_amdgcn_readfirstlane(first);
-  nrows = __builtin_amdgcn_readfirstlane(nrows);
-  return ct * TN < p.n && (QA ? rt * T < p.m : nrows > 0);  // (quarters may be empty)
+    int sub = 0;
+    if (quarters == 2) {
+      sub = pos & 3;
+      pos = share - rest + (pos >> 2);
+      if (pos >= share) return false;
+    } else if (pos >= share - rest) {
+      return false;
+    }
+    int at = xcd * (total >> 3) + min(xcd, total & 7) + pos;
+    e = 0;
+    if (QA) {
+      e = at / (n_rt * n_ct);
+      at -= e * n_rt * n_ct;
+    }
+    constexpr int BAND = 4;
+    const int band = at / (n_rt * BAND);
+    const int cols = min(BAND, n_ct - band * BAND);
+    at -= band * n_rt * BAND;
+    rt = __builtin_amdgcn_readfirstlane(at / cols);
+    ct = __builtin_amdgcn_readfirstlane((band * BAND + at % cols) * quarters + (sub & 1));
+    e = __builtin_amdgcn_readfirstlane(e);
+    // (across: rows of the group's sums)
+    if (!p.counts) {
+      first = QA ? 0 : rt * bt;
+      nrows = QA ? p.rows : min(bt, p.rows - first);
+    } else if (QA) {
+      scan.range(e, &first, &nrows);
+    } else {
+      scan.tile(rt, bt, &e, &first, &nrows);
+    }
+    rt = rt * quarters + (sub >> 1);
+    if (!QA && quarters == 2) {
+      first += (sub >> 1) * T;
+      nrows = min(T, nrows - (sub >> 1) * T);
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+    first = __builtin_amdgcn_readfirstlane(first);
+    nrows = __builtin_amdgcn_readfirstlane(nrows);
+    return ct * TN < p.n && (QA ? rt * T < p.m : nrows > 0);  // (quarters may be empty)
   };
   int pos = blockIdx.x >> 3;
   if (!locate(pos)) return;
@@ -359,232 +365,232 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
   if constexpr (ROUNDS) wait_vmcnt<0>();
   for (;;) {
 #pragma unroll
-  for (int s = PRE; s < AHEAD; ++s) {
-    feed_p(s, s * SLOT);
-    feed_q(s, s * SLOT);
-  }
-  const int KT = stages();
-#pragma unroll
-  for (int j = 0; j < NB; ++j)
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t w = t < 2 ? bias[j][g].x : bias[j][g].y;
-        const float v = FORWARD ? Elem<TY>::to_f32(static_cast<raw>(w >> (16 * (t & 1)))) : 0.f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i][j][4 * g + t] = v;
-      }
-  wait_vmcnt<2 * (AHEAD - 1) * NL + STORES>();
-  wave_barrier_all();
-  read_frags(0, 0, 0, fa[0], fb[0]);
-  int oq = 0, op = 0, to_q = AHEAD % C::Q_SLOTS * SLOT, to_p = AHEAD % C::P_SLOTS * SLOT, s = 0;
-  // MORE: vector memory operations that are in flight beside the loads
-  auto stage = [&](auto more_c) {
-    constexpr int MORE = decltype(more_c)::value;
-#pragma unroll
-    for (int kk = 0; kk + 1 < C::KK; ++kk) {
-      read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
-      if (kk == 0) feed_p(s + AHEAD, to_p);
-      mma(fa[kk & 1], fb[kk & 1]);
-      if (kk == 0) order(loads);
-      else order(no_loads);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int s = PRE; s < AHEAD; ++s) {
+      feed_p(s, s * SLOT);
+      feed_q(s, s * SLOT);
     }
-    wait_lgkm0();
-    // behind stage s + 1's loads: those of the stages to s + AHEAD - 1, and P's
-    wait_vmcnt<(2 * (AHEAD - 2) + 1) * NL + MORE>();
-    wave_barrier_all();
-    __builtin_amdgcn_sched_barrier(0);
-    oq = next_q(oq);
-    op = next_p(op);
-    read_frags(oq, op, 0, fa[0], fb[0]);
-    feed_q(s + AHEAD, to_q);
-    to_q = next_q(to_q);
-    to_p = next_p(to_p);
-    mma(fa[1], fb[1]);
-    order(loads);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // (the loads of the first PRE stages are older than the stores of the tile before)
-  if constexpr (ROUNDS) {
-    const int n = min(KT, PRE - 1);
-    do stage(std::integral_constant<int, STORES>{});
-    while (++s < n);
-  }
-  if (!ROUNDS || s < KT) {
-    do stage(std::integral_constant<int, 0>{});
-    while (++s < KT);
-  }
-  wait_vmcnt<0>();
-  wait_lgkm0();
-  wave_barrier_all();  // the ring is done with
-
-  // ---- epilogue. Activation and residual are taken in fp32 in the accumulators'
-  // layout (a gate and its up value are two registers of a lane), then
-  // rounded; the wave's whole part goes through LDS in 16 bits so that it leaves as
-  // runs of a row, 16 bytes a lane. The residual comes in the same way first; z, which
-  // a gradient is taken at, leaves in fp32 (in 16 bits, its rounding was as large a
-  // part of the gradients' error as their own).
-  uint8_t* stg = lds + (ROUNDS ? (wave >> 1) * P_AT + PRE * SLOT + (wave & 1) * SLOT
-                               : wave * C::STAGING);
-  // (the weights' gradient: rows of the group's matrix)
-  const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
-  const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
-  bool more = false;
-  const int out0 = col0;
-  if constexpr (ROUNDS) {
-    pos += 32;
-    more = locate(pos);
-    if (more) {
-      enter();
-      col0 = ct * TN + wn * OC;
+    const int KT = stages();
 #pragma unroll
-      for (int s = 0; s < PRE; ++s) {
-        feed_p(s, s * SLOT);
-        feed_q(s, s * SLOT);
-      }
-    }
-  }
-  // Eight bytes s of staged row r: the XOR spreads a column of 32 rows over all banks.
-  // Sixteen bytes are two of them, swapped in some rows.
-  constexpr int W8 = OC / 4, RPL = 32 / W8;
-  auto place = [](int r, int s) { return r * W8 * 8 + (s ^ ((r / RPL) & (W8 - 1))) * 8; };
-  auto sync = [] {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-  // Both of (staged row, output row in the tile, 16-byte chunk, k) for the wave's part,
-  // a chunk a lane, k of up to eight at a time; the tile's rows 64 i + 32 wm + r are the staged
-  // rows 32 i + r.
-  constexpr int PARTS = ROUNDS ? 2 : 1, PB = NB / PARTS;
-  auto runs = [&](auto&& get, auto&& put) {
-    constexpr int LPR = OC / 8, RPP = 64 / LPR;
-    constexpr int RUNS = WN / PARTS / RPP, AT = RUNS < 8 ? RUNS : 8;
-    static_assert(RUNS % AT == 0, "runs");
-    const int lr = lane / LPR, lc = lane % LPR;
-    for (int k0 = 0; k0 < RUNS; k0 += AT) {
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int k = 0; k < AT; ++k) {
-        const int sr = (k0 + k) * RPP + lr;
-        get(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
-      }
-#pragma unroll
-      for (int k = 0; k < AT; ++k) {
-        const int sr = (k0 + k) * RPP + lr;
-        put(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
-      }
-    }
-  };
-  auto pack4 = [](const float (&v)[4]) {
-    return uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
-  };
-  // (Accumulators stay where they are until they are used: otherwise the compiler
-  // reads all of them into VGPRs ahead, more than there are.)
-  auto keep = [](f32x16& a) { asm volatile("" : "+a"(a)); };
-  const int r32 = lane & 31;
-  if (FORWARD && p.z) {
-    // in fp32, 32 rows at a time: chunks of four values, spread over the banks
-    constexpr int CH = WN / 4, RPP = 64 / CH;
-    auto chunk = [&](int r, int c) {
-      return reinterpret_cast<f32x4*>(stg + (r * CH + ((c ^ (r & 15)) & (CH - 1))) * 16);
-    };
-    const int lc = lane % CH;
-    const int zc = col0 + (GATED ? (lc >> 4) * 32 : (lc >> 3) * 32) + (lc & 7) * 4;
-    const int64_t to = zc + (GATED && ((lc >> 3) & 1) ? p.n : 0);
-    static_for<NB>([&](auto i_c) {
-      constexpr int i = decltype(i_c)::value;
-#pragma unroll
-      for (int j = 0; j < NB; ++j) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *chunk(r32, j * 8 + 2 * g + h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1],
-                                                 acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-      }
-      sync();
-#pragma unroll
-      for (int k = 0; k < 32 / RPP; ++k) {
-        const int sr = k * RPP + lane / CH, r = i * 64 + wm * 32 + sr;
-        const f32x4 v = *chunk(sr, lc);
-        if (r < rows_in && zc < p.n)
-          *reinterpret_cast<f32x4*>(p.z + (row0 + r) * wide + to) = v;
-      }
-      sync();
-    });
-  }
-  if (FORWARD && p.residual) {
-    u32x4 v[8];
-    runs([&](int, int r, int c, int k) {
-      v[k] = u32x4{0, 0, 0, 0};
-      if (r < rows_in && col0 + c * 8 < p.n)
-        v[k] = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
-                                               (row0 + r) * p.ldr + col0 + c * 8);
-    }, [&](int sr, int, int c, int k) {
-      if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
-      *reinterpret_cast<u32x4*>(stg + (place(sr, 2 * c) & ~15)) = v[k];
-    });
-    sync();
-  }
-  const bool has_residual = FORWARD && p.residual;
-  // (rows of no group: sums of nothing, whose activations are 0)
-  // (without a branch, so that every tile has STORES of them: what is outside is dropped)
-  const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
-      static_cast<raw*>(p.out) + row0 * p.n + out0, 0, 0x7fffffff, kBufWord3);
-#pragma unroll
-  for (int part = 0; part < PARTS; ++part) {
-  const int I0 = part * PB;
-#pragma unroll
-  for (int i = I0; i < I0 + PB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; j += GATED ? 2 : 1) {
-      auto at = [&](int g) {
-        return reinterpret_cast<uint2*>(
-            stg + place((i - I0) * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
-      };
-      keep(acc[i][j]);
-      if constexpr (GATED) keep(acc[i][j + 1]);
-      uint2 res[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        res[g] = FORWARD ? *at(g) : uint2{0, 0};  // (without a residual: what the ring left)
-        res[g].x = has_residual ? res[g].x : 0;
-        res[g].y = has_residual ? res[g].y : 0;
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float v[4];
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          v[t] = acc[i][j][4 * g + t];
-          if constexpr (FORWARD) {
-            v[t] = linear_act<ACT>(v[t]);
-            if constexpr (GATED) v[t] *= acc[i][j + 1][4 * g + t];
-            v[t] += Elem<TY>::to_f32(
-                static_cast<raw>((t < 2 ? res[g].x : res[g].y) >> (16 * (t & 1))));
-          }
+          const uint32_t w = t < 2 ? bias[j][g].x : bias[j][g].y;
+          const float v = FORWARD ? Elem<TY>::to_f32(static_cast<raw>(w >> (16 * (t & 1)))) : 0.f;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) acc[i][j][4 * g + t] = v;
         }
-        if constexpr (ROUNDS) put_staged(at(g), pack4(v));
-        else *at(g) = pack4(v);
+    wait_vmcnt<2 * (AHEAD - 1) * NL + STORES>();
+    wave_barrier_all();
+    read_frags(0, 0, 0, fa[0], fb[0]);
+    int oq = 0, op = 0, to_q = AHEAD % C::Q_SLOTS * SLOT, to_p = AHEAD % C::P_SLOTS * SLOT, s = 0;
+    // MORE: vector memory operations that are in flight beside the loads
+    auto stage = [&](auto more_c) {
+      constexpr int MORE = decltype(more_c)::value;
+#pragma unroll
+      for (int kk = 0; kk + 1 < C::KK; ++kk) {
+        read_frags(oq, op, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+        if (kk == 0) feed_p(s + AHEAD, to_p);
+        mma(fa[kk & 1], fb[kk & 1]);
+        if (kk == 0) order(loads);
+        else order(no_loads);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_lgkm0();
+      // behind stage s + 1's loads: those of the stages to s + AHEAD - 1, and P's
+      wait_vmcnt<(2 * (AHEAD - 2) + 1) * NL + MORE>();
+      wave_barrier_all();
+      __builtin_amdgcn_sched_barrier(0);
+      oq = next_q(oq);
+      op = next_p(op);
+      read_frags(oq, op, 0, fa[0], fb[0]);
+      feed_q(s + AHEAD, to_q);
+      to_q = next_q(to_q);
+      to_p = next_p(to_p);
+      mma(fa[1], fb[1]);
+      order(loads);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // (the loads of the first PRE stages are older than the stores of the tile before)
+    if constexpr (ROUNDS) {
+      const int n = min(KT, PRE - 1);
+      do stage(std::integral_constant<int, STORES>{});
+      while (++s < n);
+    }
+    if (!ROUNDS || s < KT) {
+      do stage(std::integral_constant<int, 0>{});
+      while (++s < KT);
+    }
+    wait_vmcnt<0>();
+    wait_lgkm0();
+    wave_barrier_all();  // the ring is done with
+
+    // ---- epilogue. Activation and residual are taken in fp32 in the accumulators'
+    // layout (a gate and its up value are two registers of a lane), then
+    // rounded; the wave's whole part goes through LDS in 16 bits so that it leaves as
+    // runs of a row, 16 bytes a lane. The residual comes in the same way first; z, which
+    // a gradient is taken at, leaves in fp32 (in 16 bits, its rounding was as large a
+    // part of the gradients' error as their own).
+    uint8_t* stg = lds + (ROUNDS ? (wave >> 1) * P_AT + PRE * SLOT + (wave & 1) * SLOT
+                                 : wave * C::STAGING);
+    // (the weights' gradient: rows of the group's matrix)
+    const int64_t row0 = QA ? static_cast<int64_t>(e) * p.m + rt * T : first;
+    const int rows_in = QA ? min(T, p.m - rt * T) : nrows;
+    bool more = false;
+    const int out0 = col0;
+    if constexpr (ROUNDS) {
+      pos += 32;
+      more = locate(pos);
+      if (more) {
+        enter();
+        col0 = ct * TN + wn * OC;
+#pragma unroll
+        for (int s = 0; s < PRE; ++s) {
+          feed_p(s, s * SLOT);
+          feed_q(s, s * SLOT);
+        }
       }
     }
-  sync();
-  u32x4 v[8];  // (read together: one by one, each store waits for its read)
-  runs([&](int sr, int, int c, int k) {
-    const u32x4* from = reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
-    v[k] = ROUNDS ? staged(from) : *from;
-  }, [&](int sr, int r, int c, int k) {
-    if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
-    r += I0 * 64;
-    const bool in = r < rows_in && out0 + c * 8 < p.n;
-    __builtin_amdgcn_raw_buffer_store_b128(
-        v[k], to, in ? static_cast<uint32_t>(r * p.n + c * 8) * 2 : kOutside, 0, 0);
-  });
-  if (PARTS > 1) sync();
-  }
-  if (!more) break;
-  wait_lgkm0();
-  wave_barrier_all();  // the staging is done with
+    // Eight bytes s of staged row r: the XOR spreads a column of 32 rows over all banks.
+    // Sixteen bytes are two of them, swapped in some rows.
+    constexpr int W8 = OC / 4, RPL = 32 / W8;
+    auto place = [](int r, int s) { return r * W8 * 8 + (s ^ ((r / RPL) & (W8 - 1))) * 8; };
+    auto sync = [] {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    // Both of (staged row, output row in the tile, 16-byte chunk, k) for the wave's part,
+    // a chunk a lane, k of up to eight at a time; the tile's rows 64 i + 32 wm + r are the staged
+    // rows 32 i + r.
+    constexpr int PARTS = ROUNDS ? 2 : 1, PB = NB / PARTS;
+    auto runs = [&](auto&& get, auto&& put) {
+      constexpr int LPR = OC / 8, RPP = 64 / LPR;
+      constexpr int RUNS = WN / PARTS / RPP, AT = RUNS < 8 ? RUNS : 8;
+      static_assert(RUNS % AT == 0, "runs");
+      const int lr = lane / LPR, lc = lane % LPR;
+      for (int k0 = 0; k0 < RUNS; k0 += AT) {
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+          const int sr = (k0 + k) * RPP + lr;
+          get(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
+        }
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+          const int sr = (k0 + k) * RPP + lr;
+          put(sr, (sr >> 5) * 64 + wm * 32 + (sr & 31), lc, k);
+        }
+      }
+    };
+    auto pack4 = [](const float (&v)[4]) {
+      return uint2{pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3])};
+    };
+    // (Accumulators stay where they are until they are used: otherwise the compiler
+    // reads all of them into VGPRs ahead, more than there are.)
+    auto keep = [](f32x16& a) { asm volatile("" : "+a"(a)); };
+    const int r32 = lane & 31;
+    if (FORWARD && p.z) {
+      // in fp32, 32 rows at a time: chunks of four values, spread over the banks
+      constexpr int CH = WN / 4, RPP = 64 / CH;
+      auto chunk = [&](int r, int c) {
+        return reinterpret_cast<f32x4*>(stg + (r * CH + ((c ^ (r & 15)) & (CH - 1))) * 16);
+      };
+      const int lc = lane % CH;
+      const int zc = col0 + (GATED ? (lc >> 4) * 32 : (lc >> 3) * 32) + (lc & 7) * 4;
+      const int64_t to = zc + (GATED && ((lc >> 3) & 1) ? p.n : 0);
+      static_for<NB>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *chunk(r32, j * 8 + 2 * g + h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1],
+                                                   acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
+        sync();
+#pragma unroll
+        for (int k = 0; k < 32 / RPP; ++k) {
+          const int sr = k * RPP + lane / CH, r = i * 64 + wm * 32 + sr;
+          const f32x4 v = *chunk(sr, lc);
+          if (r < rows_in && zc < p.n)
+            *reinterpret_cast<f32x4*>(p.z + (row0 + r) * wide + to) = v;
+        }
+        sync();
+      });
+    }
+    if (FORWARD && p.residual) {
+      u32x4 v[8];
+      runs([&](int, int r, int c, int k) {
+        v[k] = u32x4{0, 0, 0, 0};
+        if (r < rows_in && col0 + c * 8 < p.n)
+          v[k] = *reinterpret_cast<const u32x4*>(static_cast<const raw*>(p.residual) +
+                                                 (row0 + r) * p.ldr + col0 + c * 8);
+      }, [&](int sr, int, int c, int k) {
+        if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
+        *reinterpret_cast<u32x4*>(stg + (place(sr, 2 * c) & ~15)) = v[k];
+      });
+      sync();
+    }
+    const bool has_residual = FORWARD && p.residual;
+    // (rows of no group: sums of nothing, whose activations are 0)
+    // (without a branch, so that every tile has STORES of them: what is outside is dropped)
+    const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+        static_cast<raw*>(p.out) + row0 * p.n + out0, 0, 0x7fffffff, kBufWord3);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      const int I0 = part * PB;
+#pragma unroll
+      for (int i = I0; i < I0 + PB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; j += GATED ? 2 : 1) {
+          auto at = [&](int g) {
+            return reinterpret_cast<uint2*>(
+                stg + place((i - I0) * 32 + r32, (GATED ? j >> 1 : j) * 8 + 2 * g + h));
+          };
+          keep(acc[i][j]);
+          if constexpr (GATED) keep(acc[i][j + 1]);
+          uint2 res[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            res[g] = FORWARD ? *at(g) : uint2{0, 0};  // (without a residual: what the ring left)
+            res[g].x = has_residual ? res[g].x : 0;
+            res[g].y = has_residual ? res[g].y : 0;
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float v[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              v[t] = acc[i][j][4 * g + t];
+              if constexpr (FORWARD) {
+                v[t] = linear_act<ACT>(v[t]);
+                if constexpr (GATED) v[t] *= acc[i][j + 1][4 * g + t];
+                v[t] += Elem<TY>::to_f32(
+                    static_cast<raw>((t < 2 ? res[g].x : res[g].y) >> (16 * (t & 1))));
+              }
+            }
+            if constexpr (ROUNDS) put_staged(at(g), pack4(v));
+            else *at(g) = pack4(v);
+          }
+        }
+      sync();
+      u32x4 v[8];  // (read together: one by one, each store waits for its read)
+      runs([&](int sr, int, int c, int k) {
+        const u32x4* from = reinterpret_cast<const u32x4*>(stg + (place(sr, 2 * c) & ~15));
+        v[k] = ROUNDS ? staged(from) : *from;
+      }, [&](int sr, int r, int c, int k) {
+        if ((sr / RPL) & 1) v[k] = u32x4{v[k][2], v[k][3], v[k][0], v[k][1]};
+        r += I0 * 64;
+        const bool in = r < rows_in && out0 + c * 8 < p.n;
+        __builtin_amdgcn_raw_buffer_store_b128(
+            v[k], to, in ? static_cast<uint32_t>(r * p.n + c * 8) * 2 : kOutside, 0, 0);
+      });
+      if (PARTS > 1) sync();
+    }
+    if (!more) break;
+    wait_lgkm0();
+    wave_barrier_all();  // the staging is done with
   }
 }
 
@@ -612,7 +618,8 @@ int launch_form(const LinearParams& p, bool large, hipStream_t stream) {
   const bool known = MODE == kLinearWgrad || !p.counts;
   bool cut = !known && tiles > 256;
   if (known)
-    for (int xcd = 0; xcd < 8; ++xcd) cut |= linear_rest(linear_share(static_cast<int>(tiles), xcd)) > 0;
+    for (int xcd = 0; xcd < 8; ++xcd)
+      cut |= linear_rest(linear_share(static_cast<int>(tiles), xcd)) > 0;
   LinearParams q = p;
   q.part = cut ? kLinearCut : kLinearWhole;
   const int rc = launch_tile<TY, MODE, ACT, 256>(q, wgs, stream);
@@ -681,7 +688,9 @@ LinearForms forms_of(int mode) {
   return {kForms, 7};
 }
 
-bool linear_flags_ok(int mode, int32_t flags) { return flags >= 0 && flags <= forms_of(mode).count; }
+bool linear_flags_ok(int mode, int32_t flags) {
+  return flags >= 0 && flags <= forms_of(mode).count;
+}
 
 // The form with the shortest estimate. (Gated, the forward form 0 is form 1.)
 int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, int64_t red,
@@ -713,7 +722,9 @@ int linear_form(int mode, int64_t groups, int64_t rows, int64_t m, int64_t n, in
       const double rest = wgs / q.at_once - std::floor(wgs / q.at_once);
       if (wgs > q.at_once && rest > 0 && rest <= 0.5) rounds += (rest <= 0.25 ? 0.45 : 0.75) - 1;
     }
-    const double c = rounds * round;
+    // (the gradients' workgroups load ahead and store behind from tile to tile)
+    const double saved = q.bm < 256 ? 0 : mode == kLinearWgrad ? 3 : mode == kLinearDgrad ? 2 : 0;
+    const double c = rounds * round - saved * std::max(0.0, rounds - 1);
     const double w = mb / q.tbs;
     const double us = c * c * c * c + w * w * w * w;  // (of the two, the longer one counts)
     if (f == forms.count - 1 || us < best_us) {
