@@ -344,3 +344,23 @@ def test_rows_past_whole_tiles(gpu, rows, counts, which):
     want = ref.product(**t, **options) if counts is None else ref.grouped(**t, counts=counts, **options)
     got = run(t, on_gpu, options["dout"], activation=options["kind"], gated=gated, _flags=large)
     compare(got, want)
+
+
+@pytest.mark.parametrize("which", ["input", "weight"])
+@pytest.mark.parametrize("sums", [8, 64, 72, 136, 520])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_several_tiles_of_a_workgroup(gpu, dtype, sums, which):
+    """The gradients in 256 x 256 tiles, each workgroup with several of them, some of a
+    stage or none: the same bits each time."""
+    large = sum(_capi.LINEAR_FORMS[p] << (8 * i) for i, p in enumerate(("forward", "input", "weight")))
+    if which == "input":
+        rows, n, k, counts = 4700, sums, 8208, [1000, 0, 2000, 257, 1, 1300]  # 142 left over
+    else:
+        rows, n, k, counts = 6 * sums, 1544, 4104, [sums, 0, 3 * sums, 1, sums // 2, sums // 4]
+    t, dout = inputs(rows, n, k, TYPES[dtype], False, False, False, len(counts))
+    on_gpu = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    runs = [run(t, on_gpu, dout, _flags=large) for _ in range(4)]
+    compare(runs[0], ref.grouped(**t, counts=counts, dout=dout))
+    name = "dx" if which == "input" else "dw"
+    for again in runs[1:]:
+        assert torch.equal(again[name], runs[0][name])
