@@ -204,18 +204,20 @@ at::Tensor topk_gating_grad_of(const Arg& la, const Arg& wa, const Arg& ia, cons
 }
 
 // --------------------------------------------------------------- products ---
-// A 16-bit matrix (or several) with adjacent columns and 16-byte aligned rows:
-// where it is, or copied.
+// A 16-bit matrix (or several) with adjacent columns, 16-byte aligned rows and a row
+// stride of at least `least`: where it is, or copied. (Products whose sums run across
+// its rows take a row for the end of the one before it.)
 struct Matrix {
   at::Tensor t;
   int64_t row, group;  // strides
 };
-Matrix matrix(const at::Tensor& t, int64_t rows, int64_t cols) {
+Matrix matrix(const at::Tensor& t, int64_t rows, int64_t cols, int64_t least = 0) {
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && cols % 8 == 0) {
     if (t.is_contiguous()) return {t, cols, rows * cols};
     const int64_t d = t.dim();
     if ((d == 2 || d == 3) && t.stride(d - 1) == 1 &&
-        (rows <= 1 || (t.stride(d - 2) % 8 == 0 && t.stride(d - 2) <= kMaxLinearStride)) &&
+        (rows <= 1 || (t.stride(d - 2) % 8 == 0 && t.stride(d - 2) <= kMaxLinearStride &&
+                       t.stride(d - 2) >= least)) &&
         (d == 2 || t.size(0) <= 1 || t.stride(0) % 8 == 0))
       return {t, rows <= 1 ? cols : t.stride(d - 2), d == 3 ? t.stride(0) : 0};
   }
@@ -317,7 +319,7 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
   const int32_t type = static_cast<int32_t>(type_code(x)), groups = static_cast<int32_t>(s.groups);
   const at::Tensor counts = ca.t ? contiguous(*ca.t) : at::Tensor();
   void* stream = stream_of(index);
-  Matrix dz = matrix(flat(*da.t, s.rows, n), s.rows, n);
+  Matrix dz = matrix(flat(*da.t, s.rows, n), s.rows, n, with_dw && !za.t ? n : 0);
   if (za.t) {
     const at::Tensor t = make({s.rows, s.wide}, x.scalar_type(), x);
     call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, floats(*za.t), s.rows, n, type,
@@ -326,13 +328,13 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
   }
   at::Tensor dx, dw, db;
   if (with_dx) {
-    const Matrix wm = matrix(w, s.wide, s.k);
+    const Matrix wm = matrix(w, s.wide, s.k, s.k);
     dx = make(x.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_input_grad, ptr(dz.t), dz.row, ptr(wm.t), wm.row, wm.group,
          ints(counts), groups, s.rows, s.wide, s.k, type, how.of(1), ptr(dx), stream);
   }
   if (with_dw) {
-    const Matrix xm = matrix(flat(x, s.rows, s.k), s.rows, s.k);
+    const Matrix xm = matrix(flat(x, s.rows, s.k), s.rows, s.k, s.k);
     dw = make(w.sizes(), x.scalar_type(), x);
     call(index, what, g_steps.linear_weight_grad, ptr(dz.t), dz.row, ptr(xm.t), xm.row,
          ints(counts), groups, s.rows, s.wide, s.k, type, how.of(2), ptr(dw), stream);

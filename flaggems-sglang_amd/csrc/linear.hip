@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256, 1) void linear_tile_kernel(const LinearParams 
 
   // ---- operands. A stage's resource begins at the stage and ends with its last
   // value: `along`, with the tile's last row's last sum; `across`, with the last
-  // row's last column.
+  // row's last column (rows lie at least their width apart: check_linear_across).
   Feed<C, QA> fq;
   Feed<C, PA> fp;
   // (gated: the tile's rows of P by 32: gate, up, gate, up ... of the same columns; the
@@ -612,6 +612,7 @@ int launch_form(const LinearParams& p, bool large, hipStream_t stream) {
                                           : linear_row_tiles(p, t);
   const int64_t tiles = nr * nc;
   if (tiles > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  if (const int rc = check_linear_across(p, MODE)) return rc;
   const int64_t wgs = (tiles + 7) / 8 * 8;
   if (!large) return launch_tile<TY, MODE, ACT, 128>(p, wgs, stream);
   // how many tiles there are is the device's to know where rows are grouped

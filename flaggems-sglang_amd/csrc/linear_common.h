@@ -234,6 +234,15 @@ inline int64_t linear_row_tiles(const LinearParams& p, int bm) {
   return p.counts ? std::min(rows, whole + p.groups) : whole;
 }
 
+// Operands whose sums run across their rows: a stage's resource ends with the last
+// row's last column, and the next row has to begin behind that.
+inline int check_linear_across(const LinearParams& p, int mode) {
+  if ((mode == kLinearWgrad && p.ldq < p.m) ||
+      ((mode == kLinearWgrad || mode == kLinearDgrad) && p.ldp < p.n))
+    return fail(FGS_EUNSUPPORTED, "rows that overlap: their stride is less than their width");
+  return FGS_OK;
+}
+
 // Launches `kernel` with more than 64 KiB of LDS, which each GPU has to be told
 // of once (`told`: a bit a GPU).
 template <class... P, class... A>

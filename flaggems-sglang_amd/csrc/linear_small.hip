@@ -239,6 +239,7 @@ int launch_cfg(const LinearParams& p, hipStream_t stream) {
   constexpr int BM = 16 * C::MT, TN = (MODE == kSmallGated ? 8 : 16) * C::NT;
   const int64_t nm = linear_row_tiles(p, BM), nn = (p.n + TN - 1) / TN;
   if (nm * nn > 0x7fffffffll) return fail(FGS_EUNSUPPORTED, "too many tiles for a grid");
+  if (const int rc = MODE == kSmallInputGrad ? check_linear_across(p, kLinearDgrad) : FGS_OK) return rc;
   return launch_lds("linear_small_kernel", linear_small_kernel<TY, MODE, ACT, C>, told, nm * nn,
                     C::KW * 64, C::LDS, stream, p, static_cast<int>(nm),
                     static_cast<int>(nm * nn));

@@ -52,7 +52,8 @@ def fused_linear(
     additions are in fp32, the result is rounded once. ``activation``: None,
     "relu", "silu" or "gelu" (exact, erf). ``n`` and ``k`` are multiples of 8 up to
     2^20 (gated: ``2 n``); fewer than 2^30 rows (0 among them). Operands whose rows are not 16-byte
-    aligned, or whose columns are not adjacent, are copied first.
+    aligned, or whose columns are not adjacent, are copied first, and by the gradients
+    those whose rows overlap (broadcast rows, sliding windows).
 
     Gradients go to ``x``, ``weight``, ``bias`` and ``residual``. With an activation,
     what it is taken of is kept in fp32 for them, and its gradient is rounded to x's

@@ -543,12 +543,14 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
 int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, int64_t rows,
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream);
-/* dx [rows, k] = dz[i] w[e], contiguous (rows behind the last group's: 0), */
+/* dx [rows, k] = dz[i] w[e], contiguous (rows behind the last group's: 0); rows of w at
+ * least k elements apart, */
 int32_t fgs_moe_linear_input_grad(const void* dz, int64_t ldz, const void* w, int64_t ldw,
                                   int64_t w_group_stride, const int32_t* counts, int32_t groups,
                                   int64_t rows, int64_t wide, int64_t k, int32_t dtype,
                                   int32_t flags, void* dx, void* stream);
-/* dw [groups][wide, k] = sum over the group's rows of dz[i]^T x[i], contiguous, */
+/* dw [groups][wide, k] = sum over the group's rows of dz[i]^T x[i], contiguous; rows of
+ * dz at least wide, rows of x at least k elements apart, */
 int32_t fgs_moe_linear_weight_grad(const void* dz, int64_t ldz, const void* x, int64_t ldx,
                                    const int32_t* counts, int32_t groups, int64_t rows,
                                    int64_t wide, int64_t k, int32_t dtype, int32_t flags,
