@@ -275,9 +275,10 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     else:
         raise ValueError(f"Unsupported scoring function: {scoring_func}")
     logits = gating_output
+    with_grad = needs_gradient("fused_topk", logits)  # (of the caller's tensor, as it is)
     if logits.dtype not in (torch.float32, torch.bfloat16):
         logits = logits.float()
-    if needs_gradient("fused_topk", logits):
+    if with_grad:
         return _capi.host().topk_gating(logits, topk, scoring, renormalize)
     logits = logits.contiguous()
     M, E = logits.shape

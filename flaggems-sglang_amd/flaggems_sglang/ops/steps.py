@@ -96,10 +96,10 @@ def moe_unpermute(
     ``topk_weights`` (summed in fp32).
     """
     assert rows.shape[0] == order.slot_of_row.shape[0], "the order is one of other rows"
+    with_grad = needs_gradient("moe_unpermute", rows, topk_weights)  # (of the caller's tensors)
     if topk_weights is not None and topk_weights.dtype != torch.float32:
         topk_weights = topk_weights.float()
-    return _capi.host().unpermute(rows, order.row_of_slot, order.slot_of_row, topk_weights,
-                                  needs_gradient("moe_unpermute", rows, topk_weights))
+    return _capi.host().unpermute(rows, order.row_of_slot, order.slot_of_row, topk_weights, with_grad)
 
 
 __all__ = [
