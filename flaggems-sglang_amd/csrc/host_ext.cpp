@@ -479,7 +479,6 @@ PyMethodDef g_methods[] = {
     method<unpermute, 5>("unpermute"),
     method<topk_gating, 4>("topk_gating"),
     method<linear, 9>("linear"),
-    method<linear_grad, 11>("linear_grad"),
     method<foreign_leaf, 1>("foreign_leaf"),
     {nullptr, nullptr, 0, nullptr},
 };

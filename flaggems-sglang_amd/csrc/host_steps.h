@@ -182,24 +182,34 @@ std::array<at::Tensor, 2> topk_gating_of(const Arg& la, int64_t topk, int32_t sc
   return {weights, ids};
 }
 
-at::Tensor topk_gating_grad_of(const Arg& la, const Arg& wa, const Arg& ia, const Arg& da,
-                               int32_t scoring, bool renormalize) {
-  const int index = check_inputs({la, wa, ia, da});
-  const at::Tensor& l = *la.t;
-  check_logits(l, 0);
-  require(ia.t->dim() == 2 && ia.t->size(0) == l.size(0) && ia.t->scalar_type() == at::kInt,
-          "ids must be int32 [tokens, topk]");
+// The logits' gradient is one of the weights alone where they are the picks' own
+// softmax, or sigmoids that are not renormalised.
+bool topk_grad_reads_logits(int32_t scoring, bool renormalize) {
+  return (scoring == FGS_SCORING_SIGMOID) == renormalize;
+}
+
+// (la: not given where they are not read)
+at::Tensor topk_gating_grad_of(const Arg& wa, const Arg& ia, const Arg& da, const Arg& la,
+                               int64_t experts, at::ScalarType type, int32_t scoring,
+                               bool renormalize) {
+  const int index = check_inputs({wa, ia, da, la});
+  require(ia.t->dim() == 2 && ia.t->scalar_type() == at::kInt, "ids must be int32 [tokens, topk]");
   require(wa.t->sizes() == ia.t->sizes() && da.t->sizes() == ia.t->sizes() &&
               wa.t->scalar_type() == at::kFloat && da.t->scalar_type() == at::kFloat,
           "the weights and their gradient must be float32 [tokens, topk]");
-  const at::Tensor logits = contiguous(l), weights = contiguous(*wa.t), ids = contiguous(*ia.t),
-                   d = contiguous(*da.t);
-  const at::Tensor out = make(l.sizes(), l.scalar_type(), l);
+  require(la.t || !topk_grad_reads_logits(scoring, renormalize), "the logits are read");
+  require(!la.t || (la.t->dim() == 2 && la.t->size(0) == ia.t->size(0) && la.t->size(1) == experts &&
+                    la.t->scalar_type() == type),
+          "logits must be of the forward pass's shape and type");
+  const at::Tensor weights = contiguous(*wa.t), ids = contiguous(*ia.t), d = contiguous(*da.t),
+                   logits = la.t ? contiguous(*la.t) : at::Tensor();
+  const int64_t m = ids.size(0);
+  const at::Tensor out = make({m, experts}, type, ids);
   void* stream = stream_of(index);
   call(index, "fused_topk", g_steps.topk_gating_grad, ptr(logits),
-       static_cast<int32_t>(l.scalar_type() == at::kBFloat16), l.size(0),
-       static_cast<int32_t>(l.size(1)), static_cast<int32_t>(ids.size(1)), scoring,
-       static_cast<int32_t>(renormalize), floats(weights), ints(ids), floats(d), ptr(out), stream);
+       static_cast<int32_t>(type == at::kBFloat16), m, static_cast<int32_t>(experts),
+       static_cast<int32_t>(ids.size(1)), scoring, static_cast<int32_t>(renormalize),
+       floats(weights), ints(ids), floats(d), ptr(out), stream);
   return out;
 }
 
@@ -298,51 +308,66 @@ std::array<at::Tensor, 2> linear_of(const Arg& xa, const Arg& wa, const Arg& ca,
   return {out, z};
 }
 
-// (dx, dweight, dbias), those asked for
+// (dx, dweight, dbias), those asked for; w only for dx, x only for dweight.
 std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg& wa,
                                          const Arg& ca, const Arg& za, LinearHow how,
                                          bool with_dx, bool with_dw, bool with_db) {
   const int index = check_inputs({da, xa, wa, ca, za});
-  const at::Tensor &x = *xa.t, &w = *wa.t;
+  const at::Tensor& dout = *da.t;
   const char* what = ca.t ? "grouped_linear" : "fused_linear";
-  const LinearSizes s = check_product(x, w, ca);
-  require(!how.gated || s.wide % 2 == 0, "a gated weight must hold gate rows and up rows");
-  const int64_t n = how.gated ? s.wide / 2 : s.wide;
-  at::DimVector shape(x.sizes().begin(), x.sizes().end());
-  shape.back() = n;
-  require(da.t->sizes() == shape && da.t->scalar_type() == x.scalar_type(),
+  const int32_t type = static_cast<int32_t>(type_code(dout));
+  require((type == FGS_DTYPE_BF16 || type == FGS_DTYPE_FP16) && dout.dim() >= 1 && dout.size(-1) > 0,
           "dout must be of the output's shape and type");
+  const int64_t n = dout.size(-1);
+  LinearSizes s{ca.t ? ca.t->size(0) : 1, dout.numel() / n, how.gated ? 2 * n : n, 0, ca.t};
+  require(!ca.t || (ca.t->dim() == 1 && ca.t->scalar_type() == at::kInt), "counts must be int32 [groups]");
+  require((wa.t || !with_dx) && (xa.t || !with_dw), "dx needs the weight, dweight x");
+  if (with_dw) s.k = xa.t->size(-1);
+  if (with_dx) s.k = wa.t->size(-1);
+  require(!with_dx || (wa.t->dim() == (ca.t ? 3 : 2) && wa.t->size(-2) == s.wide &&
+                       wa.t->numel() == s.groups * s.wide * s.k &&
+                       wa.t->scalar_type() == dout.scalar_type()),
+          "weight must be of the forward pass's shape and type");
+  require(!with_dw || (xa.t->size(-1) == s.k && xa.t->numel() == s.rows * s.k &&
+                       xa.t->scalar_type() == dout.scalar_type()),
+          "x must be of the forward pass's shape and type");
   require(za.t || (how.act == FGS_ACT_NONE && !how.gated), "an activation's gradient needs z");
   require(!za.t || (za.t->dim() == 2 && za.t->size(0) == s.rows && za.t->size(1) == s.wide &&
                     za.t->scalar_type() == at::kFloat && za.t->is_contiguous()),
           "z must be float32 [rows, n], contiguous");
-  const int32_t type = static_cast<int32_t>(type_code(x)), groups = static_cast<int32_t>(s.groups);
+  const int32_t groups = static_cast<int32_t>(s.groups);
   const at::Tensor counts = ca.t ? contiguous(*ca.t) : at::Tensor();
   void* stream = stream_of(index);
-  Matrix dz = matrix(flat(*da.t, s.rows, n), s.rows, n, with_dw && !za.t ? n : 0);
+  Matrix dz = matrix(flat(dout, s.rows, n), s.rows, n, with_dw && !za.t ? n : 0);
   if (za.t) {
-    const at::Tensor t = make({s.rows, s.wide}, x.scalar_type(), x);
+    const at::Tensor t = make({s.rows, s.wide}, dout.scalar_type(), dout);
     call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, floats(*za.t), s.rows, n, type,
          how.act, static_cast<int32_t>(how.gated), ptr(t), stream);
     dz = {t, s.wide, 0};
   }
   at::Tensor dx, dw, db;
   if (with_dx) {
-    const Matrix wm = matrix(w, s.wide, s.k, s.k);
-    dx = make(x.sizes(), x.scalar_type(), x);
+    const Matrix wm = matrix(*wa.t, s.wide, s.k, s.k);
+    at::DimVector shape(dout.sizes().begin(), dout.sizes().end());
+    shape.back() = s.k;
+    dx = make(shape, dout.scalar_type(), dout);
     call(index, what, g_steps.linear_input_grad, ptr(dz.t), dz.row, ptr(wm.t), wm.row, wm.group,
          ints(counts), groups, s.rows, s.wide, s.k, type, how.of(1), ptr(dx), stream);
   }
   if (with_dw) {
-    const Matrix xm = matrix(flat(x, s.rows, s.k), s.rows, s.k, s.k);
-    dw = make(w.sizes(), x.scalar_type(), x);
+    const Matrix xm = matrix(flat(*xa.t, s.rows, s.k), s.rows, s.k, s.k);
+    at::DimVector shape{s.groups, s.wide, s.k};
+    if (!ca.t) shape.erase(shape.begin());
+    dw = make(shape, dout.scalar_type(), dout);
     call(index, what, g_steps.linear_weight_grad, ptr(dz.t), dz.row, ptr(xm.t), xm.row,
          ints(counts), groups, s.rows, s.wide, s.k, type, how.of(2), ptr(dw), stream);
   }
   if (with_db) {
     const int64_t need = g_steps.linear_bias_grad_workspace_bytes(groups, s.rows, s.wide);
-    const at::Tensor ws = bytes_for(need, x);
-    db = ca.t ? make({s.groups, s.wide}, x.scalar_type(), x) : make({s.wide}, x.scalar_type(), x);
+    const at::Tensor ws = bytes_for(need, dout);
+    at::DimVector shape{s.groups, s.wide};
+    if (!ca.t) shape.erase(shape.begin());
+    db = make(shape, dout.scalar_type(), dout);
     call(index, what, g_steps.linear_bias_grad, ptr(dz.t), dz.row, ints(counts), groups, s.rows,
          s.wide, type, ptr(ws), need, ptr(db), stream);
   }
@@ -425,7 +450,9 @@ struct UnpermuteFunction : torch::autograd::Function<UnpermuteFunction> {
                             bool with_dweights) {
     const at::Tensor weights = or_undefined(given_weights);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({with_dweights ? rows : at::Tensor(), weights, row_of_slot, slot_of_row});
+    const at::Tensor none;
+    ctx->save_for_backward({with_dweights ? rows : none, rows.requires_grad() ? weights : none,
+                            row_of_slot, slot_of_row});
     return unpermute_of({"rows", &rows}, {"row_of_slot", &row_of_slot},
                         optional_arg(weights, "topk_weights"));
   }
@@ -449,16 +476,19 @@ struct TopkFunction : torch::autograd::Function<TopkFunction> {
                                   renormalize);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({r[1]});
-    ctx->save_for_backward({logits, r[0], r[1]});
-    ctx->saved_data["how"] = scoring << 1 | int64_t{renormalize};
+    const bool read = topk_grad_reads_logits(static_cast<int32_t>(scoring), renormalize);
+    ctx->save_for_backward({read ? logits : at::Tensor(), r[0], r[1]});
+    ctx->saved_data["how"] = int64_t{renormalize} | scoring << 1 |
+                             int64_t{logits.scalar_type() == at::kBFloat16} << 2 | logits.size(1) << 3;
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     return backward_of("fused_topk", grads, 4, [&](variable_list& out) {
       const variable_list saved = ctx->get_saved_variables();
       const int64_t how = ctx->saved_data["how"].toInt();
-      out[0] = topk_gating_grad_of({"logits", &saved[0]}, {"weights", &saved[1]}, {"ids", &saved[2]},
-                                   {"dweights", &grads[0]}, static_cast<int32_t>(how >> 1), how & 1);
+      out[0] = topk_gating_grad_of({"weights", &saved[1]}, {"ids", &saved[2]}, {"dweights", &grads[0]},
+                                   optional_arg(saved[0], "logits"), how >> 3,
+                                   how & 4 ? at::kBFloat16 : at::kFloat, how >> 1 & 1, how & 1);
     });
   }
 };
@@ -476,7 +506,11 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                              optional_arg(bias, "bias"), optional_arg(residual, "residual"), how,
                              with_z);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({x, w, counts, r[1]});
+    // (what the gradients read that are asked for, and no more)
+    const bool dx = x.requires_grad(), dw = w.requires_grad(),
+               db = bias.defined() && bias.requires_grad();
+    const at::Tensor none;
+    ctx->save_for_backward({dw ? x : none, dx ? w : none, dx || dw || db ? counts : none, r[1]});
     // (one entry: each is a look-up by name, 0.4 us)
     ctx->saved_data["how"] = act | int64_t{gated} << 8 | int64_t{bias.defined()} << 9 |
                              int64_t{residual.defined()} << 10 | (flags & 0xffffff) << 16;
@@ -492,7 +526,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         const variable_list saved = ctx->get_saved_variables();
         const LinearHow how{static_cast<int32_t>(saved_how & 0xff), (saved_how >> 8 & 1) != 0,
                             static_cast<int32_t>(saved_how >> 16)};
-        const auto g = linear_grad_of({"dout", &grads[0]}, {"x", &saved[0]}, {"weight", &saved[1]},
+        const auto g = linear_grad_of({"dout", &grads[0]}, optional_arg(saved[0], "x"),
+                                      optional_arg(saved[1], "weight"),
                                       optional_arg(saved[2], "counts"), optional_arg(saved[3], "z"),
                                       how, dx, dw, db);
         for (int i = 0; i < 3; ++i) out[i] = g[i];
@@ -562,18 +597,6 @@ PyObject* linear(PyObject* const* args) {
   return wrap(LinearFunction::apply(*x.t, *w.t, given(bias), given(residual), given(counts),
                                     static_cast<int64_t>(how.act), how.gated,
                                     static_cast<int64_t>(how.flags), with_z));
-}
-
-// linear_grad(dout, x, weight, counts, z, act, gated, with_dx, with_dweight,
-// with_dbias, flags) -> (dx, dweight, dbias)
-PyObject* linear_grad(PyObject* const* args) {
-  const Arg dout = tensor_arg(args[0], "dout"), x = tensor_arg(args[1], "x"),
-            w = tensor_arg(args[2], "weight"), counts = tensor_arg(args[3], "counts", true),
-            z = tensor_arg(args[4], "z", true);
-  const LinearHow how{static_cast<int32_t>(whole(args[5])), truth(args[6]),
-                      static_cast<int32_t>(whole(args[10]))};
-  return wrap_all<3>(linear_grad_of(dout, x, w, counts, z, how, truth(args[7]), truth(args[8]),
-                                    truth(args[9])));
 }
 
 // foreign_leaf(tensor) -> whether autograd holds the tensor's gradient node for

@@ -90,7 +90,8 @@ int32_t fgs_moe_topk_gating_grad(const void* logits, int32_t logits_bf16, int64_
     return fail(FGS_EINVAL, "topk must be in [1, min(num_experts, 64)]");
   if (scoring != FGS_SCORING_SOFTMAX && scoring != FGS_SCORING_SIGMOID)
     return fail(FGS_EINVAL, "unknown scoring function");
-  if (m > 0 && (!logits || !topk_weights || !topk_ids || !dweights || !dlogits))
+  const bool reads_logits = (scoring == FGS_SCORING_SIGMOID) == (renormalize != 0);
+  if (m > 0 && ((reads_logits && !logits) || !topk_weights || !topk_ids || !dweights || !dlogits))
     return fail(FGS_EINVAL, "null pointer argument");
   return launch_topk_gating_grad(logits, logits_bf16 != 0, m, num_experts, topk,
                                  scoring == FGS_SCORING_SIGMOID, renormalize != 0, topk_weights,

@@ -469,7 +469,8 @@ int32_t fgs_moe_fp8_block_matmul_schedule(int64_t m, int64_t n, int64_t k, int32
 
 /* Gradient of fgs_moe_topk_gating's weights: dlogits [m, num_experts] (of
  * logits' type) from the weights and ids that it returned for these logits and
- * dweights f32 [m, topk]. (Ids outside [0, num_experts) have no gradient.) */
+ * dweights f32 [m, topk]. (Ids outside [0, num_experts) have no gradient.) logits may
+ * be null where they are not read: softmax renormalised, sigmoid not. */
 int32_t fgs_moe_topk_gating_grad(const void* logits, int32_t logits_bf16, int64_t m,
                                  int32_t num_experts, int32_t topk, int32_t scoring,
                                  int32_t renormalize, const float* topk_weights,

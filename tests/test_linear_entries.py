@@ -1,9 +1,9 @@
-"""Refusals of the products' gradients' entries: no GPU is touched."""
+"""Refusals of the steps' gradients' entries: no GPU is touched."""
 
 import pytest
 
 from flaggems_sglang import _capi
-from test_steps import DW, DX, call
+from test_steps import DW, DX, TOPK, call
 
 
 @pytest.mark.parametrize("name, defaults, which, forms", [
@@ -15,3 +15,9 @@ def test_rows_that_overlap(name, defaults, which, forms):
         for ld in (0, 8, defaults[which] - 8):
             rc, text = call(name, defaults, **{which: ld, "flags": form})
             assert rc == -2 and "overlap" in text, text
+
+
+@pytest.mark.parametrize("scoring, renorm", [(0, 0), (1, 1)])
+def test_logits_that_are_read(scoring, renorm):
+    rc, text = call("topk_gating_grad", TOPK, logits=None, scoring=scoring, renorm=renorm)
+    assert rc == -1 and "null pointer" in text, text

@@ -230,3 +230,58 @@ def test_gradients_reach_their_entries(steps_on_cpu):
             raise AssertionError
         assert locked.value == 0
     """)
+
+
+def test_only_what_a_gradient_needs_is_kept(steps_on_cpu):
+    """A tensor that no gradient asked for reads may be written before the backward pass;
+    one that is read may not."""
+    steps_on_cpu("""
+        leaf = lambda t: t.clone().requires_grad_()
+
+        def passes(out, of, dout, written, raises):
+            with torch.no_grad():
+                written.add_(1)
+            try:
+                g, = torch.autograd.grad(out, of, dout)
+            except RuntimeError as e:
+                assert raises and "modified by an inplace operation" in str(e), str(e)
+            else:
+                assert not raises and g.shape == of.shape and g.dtype == of.dtype
+
+        for kind in (None, "gelu"):
+            for call, w0, more in ((dense, w, {}), (grouped, ew, {"c": counts})):
+                b0 = bias if call is dense else torch.ones(3, 32).to(BF16)
+                for of in "xwbr":
+                    for write in "xwbrc":
+                        if write == "c" and call is dense:
+                            continue
+                        t = dict(x=a.clone(), w=w0.clone(), b=b0.clone(), r=res.clone(), c=counts.clone())
+                        t[of].requires_grad_()
+                        args = dict(x=t["x"], w=t["w"], b=t["b"], residual=t["r"], activation=kind)
+                        if call is grouped:
+                            args["c"] = t["c"]
+                        read = {"x": "wc", "w": "xc", "b": "c", "r": ""}[of]
+                        passes(call(**args), t[of], torch.ones_like(res), t[write], write in read)
+        # leading sizes, a vector
+        for shape in ((64,), (2, 3, 64), (0, 64)):
+            for of in (0, 1):
+                t = [torch.ones(shape).to(BF16), w.clone()]
+                t[of].requires_grad_()
+                out = dense(*t, activation="silu", gated=True)
+                passes(out, t[of], torch.ones_like(out), t[of], False)
+
+        for of in "rw":
+            for write in "rwo":
+                t = dict(r=rows.clone(), w=weights.clone(), o=order.row_of_slot.clone())
+                t[of].requires_grad_()
+                out = unpermute(t["r"], order._replace(row_of_slot=t["o"]), t["w"])
+                passes(out, t[of], torch.ones_like(out), t[write], write == "o" or write != of)
+
+        logits = torch.ones(4, 3)
+        for dtype in (torch.float32, BF16):
+            for scoring in (0, 1):
+                for renormalize in (False, True):
+                    t = logits.to(dtype).requires_grad_()
+                    out, _ = host.topk_gating(t, 2, scoring, renormalize)
+                    passes(out, t, torch.ones_like(out), t, scoring == int(renormalize))
+    """)
