@@ -264,7 +264,10 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
     renormalised to sum 1 when ``renormalize``. Returns ``(topk_weights f32
     [M, topk], topk_ids int32 [M, topk])`` -- the routing the reference's
     tests build with torch ops (tests/test_fused_moe.py:37-41). The weights'
-    gradient goes to ``gating_output``."""
+    gradient goes to ``gating_output``. Where it asks for one (and not under
+    ``torch.no_grad()``), a forward-mode tangent is refused, and while a stream is
+    captured a leaf that an earlier graph, recorded on another stream, keeps
+    alive."""
     _require_gpu("gating_output", gating_output)
     assert gating_output.ndim == 2, "gating_output must be [M, E]"
     assert hidden_states.shape[0] == gating_output.shape[0], "token count mismatch"
@@ -276,6 +279,8 @@ def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor,
         raise ValueError(f"Unsupported scoring function: {scoring_func}")
     logits = gating_output
     with_grad = needs_gradient("fused_topk", logits)  # (of the caller's tensor, as it is)
+    if logits.is_neg():  # (its memory holds the values' negatives)
+        logits = logits.resolve_neg()
     if logits.dtype not in (torch.float32, torch.bfloat16):
         logits = logits.float()
     if with_grad:

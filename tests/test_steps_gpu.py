@@ -472,3 +472,25 @@ def test_long_rows_and_offsets_past_32_bits(gpu):
     assert torch.equal(rows[:, -1], x[:, 0][slots // topk])
     out = fgs.moe_unpermute(rows, order, torch.full((m, topk), 1 / topk, device="cuda"))
     assert torch.equal(out[:, 0], x[:, 0]) and torch.equal(out[:, -1], x[:, 0])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("strided", [False, True])
+def test_router_takes_lazily_negated_logits(gpu, strided, dtype):
+    """With and without a gradient: the values, not what memory holds of them."""
+    gen = generator(31)
+    values = torch.randn(2, 9, 20, generator=gen, device="cuda").to(TYPES[dtype]).unbind(0)
+    d = torch.randn(9, 4, generator=gen, device="cuda")
+    hidden = torch.empty(9, 1, device="cuda")
+    base = torch.stack(values, -1)[..., 0] if strided else values[0]
+    assert base.is_contiguous() != strided
+    got, want = [], []
+    for to, make in ((got, lambda t: torch._neg_view(t)), (want, lambda t: -t)):
+        leaf = base.detach().requires_grad_()
+        assert make(leaf).is_neg() == (to is got)
+        w, ids = fgs.fused_topk(hidden, make(leaf), 4)
+        to.extend([w.detach(), ids, torch.autograd.grad(w, leaf, d)[0]])
+        with torch.no_grad():
+            to.extend(fgs.fused_topk(hidden, make(leaf), 4))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
