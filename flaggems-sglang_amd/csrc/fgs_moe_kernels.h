@@ -304,6 +304,7 @@ struct LinearActGradParams {
   int64_t ldd;
   const float* z;
   void* dz;
+  void* rest;  // bf16, what dz's rounding left, or null
   int64_t rows, n;
   int32_t act, gated;
 };
@@ -311,6 +312,7 @@ int launch_linear_act_grad(const LinearActGradParams& p, int dtype, hipStream_t 
 // Sums of dz's rows by group.
 struct LinearBiasGradParams {
   const void* dz;
+  const void* rest;  // bf16, likewise, or null
   int64_t ldd;
   const int32_t* counts;
   int32_t groups, rows;

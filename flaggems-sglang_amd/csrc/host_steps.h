@@ -340,9 +340,10 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
   void* stream = stream_of(index);
   Matrix dz = matrix(flat(dout, s.rows, n), s.rows, n, with_dw && !za.t ? n : 0);
   if (za.t) {
-    const at::Tensor t = make({s.rows, s.wide}, dout.scalar_type(), dout);
-    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, floats(*za.t), s.rows, n, type,
-         how.act, static_cast<int32_t>(how.gated), ptr(t), stream);
+    // (the products take dz rounded; the bias's sums with what that leaves, a matrix more)
+    const at::Tensor t = make({s.rows * (with_db ? 2 : 1), s.wide}, dout.scalar_type(), dout);
+    call(index, what, g_steps.linear_act_grad, ptr(dz.t), dz.row, floats(*za.t), s.rows, n,
+         with_db ? type | FGS_DZ_REST : type, how.act, static_cast<int32_t>(how.gated), ptr(t), stream);
     dz = {t, s.wide, 0};
   }
   at::Tensor dx, dw, db;
@@ -369,7 +370,7 @@ std::array<at::Tensor, 3> linear_grad_of(const Arg& da, const Arg& xa, const Arg
     if (!ca.t) shape.erase(shape.begin());
     db = make(shape, dout.scalar_type(), dout);
     call(index, what, g_steps.linear_bias_grad, ptr(dz.t), dz.row, ints(counts), groups, s.rows,
-         s.wide, type, ptr(ws), need, ptr(db), stream);
+         s.wide, za.t ? type | FGS_DZ_REST : type, ptr(ws), need, ptr(db), stream);
   }
   return {dx, dw, db};
 }

@@ -6,8 +6,11 @@ namespace fgs {
 
 // dz = dout act'(z), or for z = [gate | up] dgate = dout up act'(gate), dup = dout
 // act(gate): eight columns a thread, bound by its bytes (dout and z read, dz
-// written: 8192 x 14336 gated 304 us, 5.4 TB/s).
-template <int TY, int ACT, bool GATED>
+// written: 8192 x 14336 gated 304 us, 5.4 TB/s). REST: what dz's rounding leaves goes to
+// a second matrix, in bf16 whatever dz's type (fp16's range ends near the rests of small
+// values), so that the bias's sums are of values good to 16 bits and not of dz's 8
+// (366 us; dbias's error against 64 bits is then its last rounding's).
+template <int TY, int ACT, bool GATED, bool REST>
 __global__ __launch_bounds__(256) void linear_act_grad_kernel(const LinearActGradParams p,
                                                              int64_t vecs, int per_row) {
   const int64_t i = blockIdx.x * int64_t{256} + threadIdx.x;
@@ -32,8 +35,20 @@ __global__ __launch_bounds__(256) void linear_act_grad_kernel(const LinearActGra
       dg[j] = d[j] * slope;
     }
   }
-  store8<TY, true>(p.dz, r * wide + c, 8, dg);
-  if constexpr (GATED) store8<TY, true>(p.dz, r * wide + p.n + c, 8, du);
+  auto put = [&](int64_t at, const float (&v)[8]) {
+    store8<TY, true>(p.dz, at, 8, v);
+    if constexpr (REST) {
+      float rest[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float rounded = Elem<TY>::to_f32(Elem<TY>::from_f32(v[j]));
+        rest[j] = fabsf(rounded) < INFINITY ? v[j] - rounded : 0.f;  // (none of what is past the type)
+      }
+      store8<FGS_DTYPE_BF16, true>(p.rest, at, 8, rest);
+    }
+  };
+  put(r * wide + c, dg);
+  if constexpr (GATED) put(r * wide + p.n + c, du);
 }
 
 template <int TY>
@@ -44,8 +59,10 @@ static int act_grad_type(const LinearActGradParams& p, hipStream_t stream) {
   if (wgs > 0xffffffll) return fail(FGS_EUNSUPPORTED, "too many values for a grid");
   return with_act(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
-    auto kernel = p.gated ? linear_act_grad_kernel<TY, ACT, true>
-                          : linear_act_grad_kernel<TY, ACT, false>;
+    auto kernel = p.gated ? (p.rest ? linear_act_grad_kernel<TY, ACT, true, true>
+                                    : linear_act_grad_kernel<TY, ACT, true, false>)
+                          : (p.rest ? linear_act_grad_kernel<TY, ACT, false, true>
+                                    : linear_act_grad_kernel<TY, ACT, false, false>);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, stream, p, vecs,
                        per_row);
     return check_launch("linear_act_grad_kernel");
@@ -62,7 +79,8 @@ int launch_linear_act_grad(const LinearActGradParams& p, int dtype, hipStream_t 
 // added up in a fixed order. Bound by dz's bytes: 8192 x 28672 99 us, 4.7 TB/s (160
 // with 32 columns, whose lines two XCDs read); 65536 x 2048 56 (84 with one row in
 // flight), 128 groups of them 53.
-template <int TY>
+// REST: with what dz's rounding left (191 us, 4.9 TB/s; 128 groups 76).
+template <int TY, bool REST>
 __global__ __launch_bounds__(256) void linear_bias_grad_kernel(const LinearBiasGradParams p) {
   constexpr int AT_ONCE = 4;  // rows that a thread has in flight
   __shared__ float sums[32][65];
@@ -77,15 +95,19 @@ __global__ __launch_bounds__(256) void linear_bias_grad_kernel(const LinearBiasG
   if (col < p.n)
     for (int r = r0 + lr; r < r1; r += 32 * AT_ONCE) {
       Vec8<TY, true> v[AT_ONCE];
+      Vec8<FGS_DTYPE_BF16, true> rest[REST ? AT_ONCE : 1];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u)
+        if (r + 32 * u < r1) {
+          const int64_t at = (static_cast<int64_t>(first) + r + 32 * u) * p.ldd + col;
+          v[u].load(p.dz, at, 8);
+          if constexpr (REST) rest[u].load(p.rest, at, 8);
+        }
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u)
         if (r + 32 * u < r1)
-          v[u].load(p.dz, (static_cast<int64_t>(first) + r + 32 * u) * p.ldd + col, 8);
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u)
-        if (r + 32 * u < r1)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[j] += v[u][j];
+          for (int j = 0; j < 8; ++j) acc[j] += REST ? v[u][j] + rest[REST ? u : 0][j] : v[u][j];
     }
 #pragma unroll
   for (int j = 0; j < 8; ++j) sums[lr][lc + j] = acc[j];
@@ -125,7 +147,8 @@ template <int TY>
 static int bias_grad_type(const LinearBiasGradParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.n + 63) / 64), static_cast<unsigned>(p.groups),
                   static_cast<unsigned>(p.parts));
-  hipLaunchKernelGGL(linear_bias_grad_kernel<TY>, grid, dim3(256), 0, stream, p);
+  auto kernel = p.rest ? linear_bias_grad_kernel<TY, true> : linear_bias_grad_kernel<TY, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p);
   int rc = check_launch("linear_bias_grad_kernel");
   if (rc || p.parts == 1) return rc;
   const int64_t values = p.groups * p.n;

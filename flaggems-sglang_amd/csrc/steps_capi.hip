@@ -279,6 +279,8 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
 int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, int64_t rows,
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream) {
+  const bool with_rest = (dtype & FGS_DZ_REST) != 0;
+  dtype &= ~FGS_DZ_REST;
   int rc = check_linear(1, rows, n, 8, dtype);
   if (rc || (gated && (rc = check_linear(1, rows, 2 * n, 8, dtype)))) return rc;
   if ((rc = check_act(act))) return rc;
@@ -292,6 +294,7 @@ int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, i
   p.ldd = ldd;
   p.z = z;
   p.dz = dz;
+  if (with_rest) p.rest = static_cast<uint16_t*>(dz) + rows * (gated ? 2 * n : n);
   p.rows = rows;
   p.n = n;
   p.act = act;
@@ -372,6 +375,8 @@ int64_t fgs_moe_linear_bias_grad_workspace_bytes(int32_t groups, int64_t rows, i
 int32_t fgs_moe_linear_bias_grad(const void* dz, int64_t ldz, const int32_t* counts,
                                  int32_t groups, int64_t rows, int64_t wide, int32_t dtype,
                                  void* workspace, int64_t ws_bytes, void* dbias, void* stream) {
+  const bool with_rest = (dtype & FGS_DZ_REST) != 0;
+  dtype &= ~FGS_DZ_REST;
   int rc = check_linear(groups, rows, wide, 8, dtype);
   if (rc) return rc;
   if (!counts && groups != 1) return fail(FGS_EINVAL, "counts are needed for several groups");
@@ -381,8 +386,10 @@ int32_t fgs_moe_linear_bias_grad(const void* dz, int64_t ldz, const int32_t* cou
   if (need > 0 && (!workspace || ws_bytes < need)) return fail(FGS_EINVAL, "workspace too small");
   if (misaligned(dbias, 2) || misaligned(counts, 4) || misaligned(workspace, 4))
     return fail(FGS_EINVAL, "tensors must be aligned to their elements");
+  if (with_rest && rows > 1 && ldz != wide) return fail(FGS_EINVAL, "dz must be contiguous");
   LinearBiasGradParams p{};
   p.dz = dz;
+  if (with_rest) p.rest = static_cast<const uint16_t*>(dz) + rows * wide;
   p.ldd = rows > 1 ? ldz : wide;
   p.counts = counts;
   p.groups = groups;

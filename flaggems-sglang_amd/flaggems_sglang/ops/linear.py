@@ -57,7 +57,8 @@ def fused_linear(
 
     Gradients go to ``x``, ``weight``, ``bias`` and ``residual``. With an activation,
     what it is taken of is kept in fp32 for them, and its gradient is rounded to x's
-    type, in which the other gradients' products take it.
+    type, in which x's and the weight's products take it; the bias's sums take what
+    that rounding leaves as well.
     """
     return _linear("fused_linear", x, weight, None, bias, activation, gated, residual, _flags)
 

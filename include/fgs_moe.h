@@ -540,7 +540,10 @@ int32_t fgs_moe_linear(const void* x, int64_t ldx, const void* w, int64_t ldw,
                        int64_t n, int64_t k, int32_t dtype, int32_t act, int32_t gated,
                        int32_t flags, float* z, void* out, void* stream);
 /* Its gradients. dz [rows, wide] contiguous, of v, in dtype (rows behind the last group's: of
- * whatever z holds there; the two entries below leave them out): */
+ * whatever z holds there; the entries below leave them out). With dtype | FGS_DZ_REST a
+ * second matrix follows it, bf16 [rows, wide], of what its rounding left (0 where dz is not
+ * finite), for the bias's gradient: */
+#define FGS_DZ_REST 0x100
 int32_t fgs_moe_linear_act_grad(const void* dout, int64_t ldd, const float* z, int64_t rows,
                                 int64_t n, int32_t dtype, int32_t act, int32_t gated, void* dz,
                                 void* stream);
@@ -556,8 +559,9 @@ int32_t fgs_moe_linear_weight_grad(const void* dz, int64_t ldz, const void* x, i
                                    const int32_t* counts, int32_t groups, int64_t rows,
                                    int64_t wide, int64_t k, int32_t dtype, int32_t flags,
                                    void* dw, void* stream);
-/* dbias [groups, wide] = sum over the group's rows of dz[i]; workspace
- * fgs_moe_linear_bias_grad_workspace_bytes (0: none), 16-byte aligned. */
+/* dbias [groups, wide] = sum over the group's rows of dz[i] (dtype | FGS_DZ_REST: of both
+ * matrices, contiguous); workspace fgs_moe_linear_bias_grad_workspace_bytes (0: none),
+ * 16-byte aligned. */
 int64_t fgs_moe_linear_bias_grad_workspace_bytes(int32_t groups, int64_t rows, int64_t wide);
 int32_t fgs_moe_linear_bias_grad(const void* dz, int64_t ldz, const int32_t* counts,
                                  int32_t groups, int64_t rows, int64_t wide, int32_t dtype,

@@ -3,7 +3,7 @@
 import pytest
 
 from flaggems_sglang import _capi
-from test_steps import DW, DX, TOPK, call
+from test_steps import ACT, DB, DW, DX, TOPK, call
 
 
 @pytest.mark.parametrize("name, defaults, which, forms", [
@@ -21,3 +21,11 @@ def test_rows_that_overlap(name, defaults, which, forms):
 def test_logits_that_are_read(scoring, renorm):
     rc, text = call("topk_gating_grad", TOPK, logits=None, scoring=scoring, renorm=renorm)
     assert rc == -1 and "null pointer" in text, text
+
+
+def test_rests_lie_behind_contiguous_rows():
+    rc, text = call("linear_bias_grad", DB, ldz=40, dtype=0x100)
+    assert rc == -1 and "contiguous" in text, text
+    for name, defaults in (("linear_act_grad", ACT), ("linear_bias_grad", DB)):
+        rc, text = call(name, defaults, dtype=0x102)
+        assert rc == -2 and "bf16 or fp16" in text, text
